@@ -229,7 +229,7 @@ def _unpad(cu, n, total):
 def _plain_linear(s):
     x = s["x"].float()
     amax = x.abs().amax(1, keepdim=True)
-    q = (x * torch.where(amax > 0, 127.0 / amax, 0.0)).round()
+    q = (x * torch.where(amax > 0, torch.full_like(amax, 127.0) / amax, 0.0)).round()
     y = torch.matmul(q, s["w"].float().t()) * (amax / 127.0) * s["w_scale"]
     if s["bias"] is not None:
         y = y + s["bias"].float()
