@@ -252,6 +252,78 @@ LB_API int lb_decode_attention_noalloc(const void* qkv, const void* bias, const 
                                 void* k_cache, void* v_cache, void* out, int nh, int nkv, int hd, int64_t max_len,
                                 lb_stream_t stream);
 
+/*
+ * Chunks of new tokens (a prompt's, or one token each of many sequences) through a decoder layer. No counterpart in
+ * the reference. fp16 or bf16; every sum, statistic and rotation in fp32 or exact int32, rounded once per stored value.
+ */
+typedef enum lb_dtype { LB_F16 = 0, LB_BF16 = 1, LB_F32 = 2 } lb_dtype;
+
+/*
+ * Quantize rows to 8-bit integers: a = max_k |x[m, k]|, scales[m] = a / 127, q[m, k] = rint(x[m, k] * (127 / a)) in
+ * [-127, 127], half to even; a row of zeros gives zeros, a row with an infinity or a NaN a scale that is not finite.
+ * x [M, K] fp16, bf16 or fp32, rows ldx elements apart; q int8 [M, ldq], ldq a multiple of 16, columns K.. zeroed.
+ * Activations per token, and weights [N, K] per output channel. K <= 131072.
+ */
+LB_API int lb_w8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, void* q, int64_t ldq,
+                               float* scales, lb_stream_t stream);
+
+/*
+ * y[M, N] = (sum_k q[m, k] w[n, k]) s[m] w_scales[n] + bias[n], q and s the rows of x quantized as above, the sum
+ * exact in int32, the rest in fp32 with one rounding. x and y fp16 or bf16 (y contiguous), bias [N] of that type or
+ * NULL; w int8 [N, ldw] 16-byte aligned, ldw a multiple of 16, columns K.. zero; w and w_scales are model state: they
+ * may be read before the kernel waits on the previous one in the stream. workspace: lb_w8_workspace(m, n, ldw) bytes
+ * (0: none needed), 16-byte aligned, its content undefined before and after; calls that can overlap need distinct ones.
+ */
+LB_API int64_t lb_w8_workspace(int64_t m, int64_t n, int64_t ldw);
+LB_API int lb_w8_linear(const void* x, int dtype, int64_t ldx, const void* w, int64_t ldw, const float* w_scales,
+                        const void* bias, void* y, int64_t m, int64_t n, int64_t k, void* workspace,
+                        int64_t workspace_bytes, lb_stream_t stream);
+
+/*
+ * A paged KV cache: k and v [num_pages, nkv, page_size, hd], each page's block contiguous, pages k_page_stride /
+ * v_page_stride elements apart. page_size a multiple of 16. Token j of a sequence lies in row j % page_size of page
+ * table[j / page_size]; its slot is page * page_size + row.
+ */
+typedef struct lb_paged_cache {
+  void* k;
+  void* v;
+  int64_t k_page_stride, v_page_stride;
+  int64_t num_pages;
+  int dtype, nkv, hd, page_size;
+} lb_paged_cache;
+
+/*
+ * For each of `tokens` rows of qkv = [q (nh x hd) | k (nkv x hd) | v (nkv x hd)] (ld elements apart, a multiple of 8):
+ * q and k heads are normed (x * rsqrt(mean(x^2) + eps) * q_norm / k_norm, both [hd], or both NULL: no norm) and their
+ * first `rot` dimensions rotated (x[i], x[i + rot/2]) by positions[t] * inv_freq[i] (rot a multiple of 16 up to hd,
+ * inv_freq fp32 [rot/2]; 0: no rotation); q goes to q_out [tokens, nh, hd], k and v to the cache's slot slots[t]. A
+ * negative slot stores no k and v; one past the cache neither, and sets lb_device_error() to 3. Tokens of one call
+ * have distinct slots. hd a multiple of 16 up to 256. The norm weights (model state) are read before the kernel waits
+ * on the previous one in the stream.
+ */
+LB_API int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens, int nh, const void* q_norm,
+                                     const void* k_norm, float eps, const float* inv_freq, int rot,
+                                     const int64_t* positions, const int64_t* slots, const lb_paged_cache* cache,
+                                     void* q_out, lb_stream_t stream);
+
+/*
+ * out[t, h] = softmax over the visible keys j of scale * q[t, h] . K[j, h / (nh / nkv)], times V. Sequence s has the
+ * new tokens cu_new[s] .. cu_new[s + 1] - 1 (cu_new int32 [seqs + 1], not decreasing, from 0; tokens past its last
+ * value belong to no sequence and are left unwritten) and, them included, a context of seq_lens[s] tokens in the
+ * cache; its new token i of n sees keys 0 .. seq_lens[s] - n + i. A token that sees none gets zeros. seq_lens above
+ * table_width * page_size are cut to that. page_table int32 [seqs, table_width], rows table_stride apart; entries past
+ * a context are not read; an entry outside the cache sets lb_device_error() to 3 (its keys count as zeros or not at
+ * all). max_new / max_len: upper bounds of the new tokens and the context of any sequence (tokens and
+ * table_width * page_size if unknown): a smaller value than the truth is an error that leaves outputs undefined but
+ * stays inside every buffer. q's heads and tokens are strided (multiples of 8 elements), out's tokens too. hd 64 or
+ * 128. Rows of the cache past a context may hold anything, NaN included.
+ */
+LB_API int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
+                              const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride,
+                              int64_t table_width, const int32_t* seq_lens, const int32_t* cu_new, int seqs,
+                              int64_t max_new, int64_t max_len, float scale, void* out, int64_t out_token_stride,
+                              lb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -201,6 +201,8 @@ int lb_device_error(void) {
   if (!a) a = lb::gemm_tc_device_error();
   if (!a) a = lb::gemm_mma_device_error();
   if (!a) a = lb::allreduce_device_error();
+  if (!a) a = lb::w8_device_error();
+  if (!a) a = lb::paged_device_error();
   return a ? a : lb::decode_device_error();
 }
 
@@ -209,6 +211,8 @@ void lb_clear_device_error(void) {
   lb::gemm_tc_clear_device_error();
   lb::gemm_mma_clear_device_error();
   lb::allreduce_clear_device_error();
+  lb::w8_clear_device_error();
+  lb::paged_clear_device_error();
   lb::decode_clear_device_error();
 }
 
@@ -597,6 +601,124 @@ int lb_decode_silu_mul(const void* gu, void* a, int64_t I, lb_stream_t stream) {
   return launched(lb::launch_silu_mul(static_cast<const __half*>(gu), static_cast<__half*>(a), (int)I,
                                       reinterpret_cast<cudaStream_t>(stream)),
                   "decode_silu_mul");
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------- chunks of new tokens
+// (W8A8 linear, norm + rotation + paged append, attention over the paged cache)
+
+static int check_w8_quantize(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, const void* q, int64_t ldq,
+                             const void* scales) {
+  if (!x || !q || !scales) return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if (dtype < LB_F16 || dtype > LB_F32) return fail(LB_ERR_ARGUMENT, "dtype is 0 (fp16), 1 (bf16) or 2 (fp32)");
+  if (m < 1 || k < 1 || m > INT32_MAX) return fail(LB_ERR_ARGUMENT, "shape mismatch: M=%lld K=%lld", (long long)m, (long long)k);
+  if (k > 131072) return fail(LB_ERR_ARGUMENT, "K=%lld: at most 131072, so that the int32 sums are exact", (long long)k);
+  if (ldx < k) return fail(LB_ERR_ARGUMENT, "rows of x overlap: K=%lld, stride %lld", (long long)k, (long long)ldx);
+  if (ldq < k || ldq % 16) return fail(LB_ERR_ARGUMENT, "the quantized rows' stride must be a multiple of 16, at least K");
+  if ((reinterpret_cast<uintptr_t>(x) & (dtype == LB_F32 ? 3u : 1u)) || !aligned16(q) ||
+      (reinterpret_cast<uintptr_t>(scales) & 3u))
+    return fail(LB_ERR_ALIGNMENT, "x must be aligned to its type, q to 16 bytes, scales to 4");
+  return LB_OK;
+}
+
+static int check_cache(const lb_paged_cache* c) {
+  if (!c || !c->k || !c->v) return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if (c->dtype != LB_F16 && c->dtype != LB_BF16) return fail(LB_ERR_ARGUMENT, "the cache's dtype is 0 (fp16) or 1 (bf16)");
+  if (c->nkv < 1 || c->num_pages < 1) return fail(LB_ERR_ARGUMENT, "the cache has no pages or no heads");
+  if (c->page_size < 16 || c->page_size % 16 || c->page_size > 65536)
+    return fail(LB_ERR_ARGUMENT, "page_size=%d: a multiple of 16 up to 65536", c->page_size);
+  if (c->hd < 16 || c->hd % 16 || c->hd > 256) return fail(LB_ERR_ARGUMENT, "hd=%d: head dims are multiples of 16 up to 256", c->hd);
+  const int64_t block = (int64_t)c->nkv * c->page_size * c->hd;
+  if (c->k_page_stride < block || c->v_page_stride < block || c->k_page_stride % 8 || c->v_page_stride % 8)
+    return fail(LB_ERR_ARGUMENT, "page strides must be multiples of 8 elements, at least nkv * page_size * hd");
+  if (c->num_pages > INT32_MAX || (int64_t)c->nkv * c->page_size > INT32_MAX)
+    return fail(LB_ERR_ARGUMENT, "too many pages, or too many rows in a page");
+  if (!aligned16(c->k) || !aligned16(c->v)) return fail(LB_ERR_ALIGNMENT, "the cache must be 16-byte aligned");
+  return LB_OK;
+}
+
+extern "C" {
+
+int lb_w8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t ldx, void* q, int64_t ldq,
+                        float* scales, lb_stream_t stream) {
+  int rc = check_w8_quantize(x, dtype, m, k, ldx, q, ldq, scales);
+  if (rc || (rc = check_device())) return rc;
+  return launched(lb::launch_w8_quantize_rows(x, dtype, ldx, static_cast<int8_t*>(q), ldq, scales, m, k,
+                                              g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)),
+                  "w8_quantize_rows");
+}
+
+int64_t lb_w8_workspace(int64_t m, int64_t n, int64_t ldw) {
+  return m < 1 || n < 1 || ldw < 1 ? 0 : (int64_t)lb::w8_workspace_bytes(m, n, ldw);
+}
+
+int lb_w8_linear(const void* x, int dtype, int64_t ldx, const void* w, int64_t ldw, const float* w_scales,
+                 const void* bias, void* y, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes,
+                 lb_stream_t stream) {
+  if (!w || !w_scales || !y) return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if (dtype != LB_F16 && dtype != LB_BF16) return fail(LB_ERR_ARGUMENT, "dtype is 0 (fp16) or 1 (bf16)");
+  int rc = check_w8_quantize(x, dtype, m, k, ldx, w, ldw, w_scales);
+  if (rc) return rc;
+  if (n < 1 || n > (1 << 30)) return fail(LB_ERR_ARGUMENT, "shape mismatch: N=%lld", (long long)n);
+  if (!aligned2(bias) || !aligned2(y)) return fail(LB_ERR_ALIGNMENT, "bias and y must be 2-byte aligned");
+  const int64_t need = (int64_t)lb::w8_workspace_bytes(m, n, ldw);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(LB_ERR_ARGUMENT, "the workspace holds %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0),
+                (long long)need);
+  if (!aligned16(workspace)) return fail(LB_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
+  if ((rc = check_device())) return rc;
+  const lb::W8Params p{x, ldx, dtype, w, ldw, w_scales, bias, y, m, n, k, workspace};
+  return launched(lb::launch_w8_linear(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)), "w8_linear");
+}
+
+int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens, int nh, const void* q_norm,
+                              const void* k_norm, float eps, const float* inv_freq, int rot, const int64_t* positions,
+                              const int64_t* slots, const lb_paged_cache* cache, void* q_out, lb_stream_t stream) {
+  int rc = check_cache(cache);
+  if (rc) return rc;
+  if (!qkv || !positions || !slots || !q_out || (rot && !inv_freq)) return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if ((q_norm == nullptr) != (k_norm == nullptr)) return fail(LB_ERR_ARGUMENT, "q_norm and k_norm go together");
+  if (tokens < 1 || tokens > INT32_MAX || nh < 1 || nh > 65536 || cache->nkv > 65536)
+    return fail(LB_ERR_ARGUMENT, "tokens and heads must be positive");
+  if (rot < 0 || rot % 16 || rot > cache->hd) return fail(LB_ERR_ARGUMENT, "rot=%d: a multiple of 16 up to hd", rot);
+  if (ld % 8 || ld < (int64_t)(nh + 2 * cache->nkv) * cache->hd)
+    return fail(LB_ERR_ARGUMENT, "qkv rows are (nh + 2 nkv) * hd values, a multiple of 8 apart");
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned2(q_norm) || !aligned2(k_norm))
+    return fail(LB_ERR_ALIGNMENT, "qkv and q_out must be 16-byte aligned, the norm weights 2-byte");
+  if ((rc = check_device())) return rc;
+  const lb::PagedCacheView c{cache->k, cache->v, cache->k_page_stride, cache->v_page_stride, cache->num_pages,
+                             cache->dtype, cache->nkv, cache->hd, cache->page_size};
+  return launched(lb::launch_paged_append(qkv, ld, tokens, nh, q_norm, k_norm, eps, inv_freq, rot, positions, slots, c,
+                                          q_out, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)),
+                  "paged_norm_rope_append");
+}
+
+int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
+                       const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride, int64_t table_width,
+                       const int32_t* seq_lens, const int32_t* cu_new, int seqs, int64_t max_new, int64_t max_len,
+                       float scale, void* out, int64_t out_token_stride, lb_stream_t stream) {
+  int rc = check_cache(cache);
+  if (rc) return rc;
+  if (!q || !page_table || !seq_lens || !cu_new || !out) return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if (cache->hd != 64 && cache->hd != 128) return fail(LB_ERR_ARGUMENT, "hd=%d: the attention takes head dims 64 and 128", cache->hd);
+  if (nh < 1 || nh > 65536 || nh % cache->nkv) return fail(LB_ERR_ARGUMENT, "nh=%d must be a multiple of nkv=%d", nh, cache->nkv);
+  if (tokens < 1 || tokens * nh > INT32_MAX || seqs < 1) return fail(LB_ERR_ARGUMENT, "tokens and sequences must be positive, tokens * nh below 2^31");
+  if (table_width < 1 || table_stride < table_width || table_width * cache->page_size > INT32_MAX)
+    return fail(LB_ERR_ARGUMENT, "page table: at least one page a row, contexts below 2^31");
+  if (max_new < 1 || max_len < 1) return fail(LB_ERR_ARGUMENT, "max_new and max_len must be positive");
+  if (q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_token_stride < (int64_t)nh * cache->hd)
+    return fail(LB_ERR_ARGUMENT, "q and out strides must be multiples of 8 elements");
+  if (!aligned16(q) || !aligned16(out)) return fail(LB_ERR_ALIGNMENT, "q and out must be 16-byte aligned");
+  if ((rc = check_device())) return rc;
+  const int64_t width = table_width * cache->page_size;
+  const lb::PagedAttnParams p{q, q_token_stride, q_head_stride, (int)tokens, nh, cache->nkv, cache->hd, cache->dtype,
+                              cache->k, cache->v, cache->k_page_stride, cache->v_page_stride, cache->page_size,
+                              cache->num_pages, page_table, table_stride, (int)table_width, seq_lens, cu_new, seqs,
+                              (int)(max_new < tokens ? max_new : tokens), (int)(max_len < width ? max_len : width), scale,
+                              out, out_token_stride};
+  return launched(lb::launch_paged_attention(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)),
+                  "paged_attention");
 }
 
 }  // extern "C"

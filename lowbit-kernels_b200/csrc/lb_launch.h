@@ -129,4 +129,58 @@ cudaError_t launch_gemm_mma(const GemvParams& p, const MmaConfig& c, bool pdl, c
 int gemm_mma_device_error();   // synchronizes
 void gemm_mma_clear_device_error();
 
+// W8A8 linear layer (lb_w8.cu). dtype: 0 fp16, 1 bf16 (2 fp32, quantize only)
+struct W8Params {
+  const void* x;        // [M, K], rows ldx elements apart
+  int64_t ldx;
+  int dtype;
+  const void* w;        // int8 [N, ldw], bytes K.. of a row zero
+  int64_t ldw;
+  const float* w_scales;
+  const void* bias;     // [N] or null
+  void* y;              // [M, N]
+  int64_t M, N, K;
+  void* workspace;
+};
+size_t w8_workspace_bytes(int64_t M, int64_t N, int64_t ldw);
+cudaError_t launch_w8_linear(const W8Params& p, bool pdl, cudaStream_t st);
+cudaError_t launch_w8_quantize_rows(const void* x, int dtype, int64_t ldx, int8_t* q, int64_t ldq, float* s, int64_t M,
+                                    int64_t K, bool pdl, cudaStream_t st);
+int w8_device_error();   // synchronizes
+void w8_clear_device_error();
+
+// paged KV cache (lb_paged.cu): K and V [num_pages, nkv, page_size, hd], pages k_page / v_page elements apart
+struct PagedCacheView {
+  void* k;
+  void* v;
+  int64_t k_page, v_page;
+  int64_t num_pages;
+  int dtype, nkv, hd, page_size;
+};
+cudaError_t launch_paged_append(const void* qkv, int64_t ld, int64_t tokens, int nh, const void* q_norm,
+                                const void* k_norm, float eps, const float* inv_freq, int rot, const int64_t* pos,
+                                const int64_t* slots, const PagedCacheView& c, void* q_out, bool pdl, cudaStream_t st);
+struct PagedAttnParams {
+  const void* q;
+  int64_t q_token, q_head;   // element strides
+  int tokens, nh, nkv, hd, dtype;
+  const void* k;
+  const void* v;
+  int64_t k_page, v_page;
+  int page_size;
+  int64_t num_pages;
+  const int32_t* table;      // [seqs, table_width], rows table_stride apart
+  int64_t table_stride;
+  int table_width;
+  const int32_t* seq_lens;
+  const int32_t* cu_new;     // [seqs + 1]
+  int seqs, max_new, max_len;
+  float scale;
+  void* out;                 // [tokens, nh, hd], tokens out_token elements apart
+  int64_t out_token;
+};
+cudaError_t launch_paged_attention(const PagedAttnParams& p, bool pdl, cudaStream_t st);
+int paged_device_error();   // synchronizes
+void paged_clear_device_error();
+
 }  // namespace lb

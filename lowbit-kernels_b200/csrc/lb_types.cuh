@@ -1,0 +1,47 @@
+// fp16 / bf16 element types of the chunk operators: conversions to and from fp32, two values per 32-bit register.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+namespace lb {
+
+template <typename T>
+struct Elem;
+
+template <>
+struct Elem<__half> {
+  static constexpr bool kBf16 = false;
+  static __device__ __forceinline__ float2 unpack(uint32_t v) {
+    __half2 h;
+    *reinterpret_cast<uint32_t*>(&h) = v;
+    return __half22float2(h);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+};
+
+template <>
+struct Elem<__nv_bfloat16> {
+  static constexpr bool kBf16 = true;
+  static __device__ __forceinline__ float2 unpack(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+};
+
+template <>
+struct Elem<float> {
+  static __device__ __forceinline__ float to_float(float v) { return v; }
+};
+
+}  // namespace lb

@@ -49,7 +49,22 @@ SIGNATURES = {
     "lb_decode_gemv_residual_norm": ([_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, ctypes.c_float, _P, _P], _I),
     "lb_decode_norm_gemv": ([_P, _P, _P, _P, ctypes.c_float, _P, _P, _P, _I64, _I64, _I64, _P], _I),
     "lb_decode_swiglu_gemv": ([_P, _P, _P, _P, _I64, _I64, _I64, _P], _I),
+    "lb_w8_quantize_rows": ([_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P], _I),
+    "lb_w8_workspace": ([_I64, _I64, _I64], _I64),
+    "lb_w8_linear": ([_P, _I, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P], _I),
+    "lb_paged_norm_rope_append": ([_P, _I64, _I64, _I, _P, _P, ctypes.c_float, _P, _I, _P, _P, _P, _P, _P], _I),
+    "lb_paged_attention": ([_P, _I64, _I64, _I64, _I, _P, _P, _I64, _I64, _P, _P, _I, _I64, _I64, ctypes.c_float, _P,
+                            _I64, _P], _I),
 }
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """lb_paged_cache of include/lowbit_b200.h."""
+    _fields_ = [("k", _P), ("v", _P), ("k_page_stride", _I64), ("v_page_stride", _I64), ("num_pages", _I64),
+                ("dtype", _I), ("nkv", _I), ("hd", _I), ("page_size", _I)]
+
+
+DTYPE_IDS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
 def load_library(path=LIB_PATH):

@@ -18,7 +18,7 @@ import pathlib
 import torch
 
 from . import quant
-from ._lib import Ext
+from ._lib import DTYPE_IDS, Ext, _Device
 
 _EXT = None
 
@@ -349,3 +349,106 @@ def linear(x, wq, max_gemv_rows=8, version=0, out=None, bias=None):
     if out.shape != y.shape or out.dtype != y.dtype:
         raise RuntimeError(f"out must be a float16 {tuple(y.shape)} tensor")
     return out.copy_(y)
+
+
+# ------------------------------------------------------------------------------------------ 8-bit integer products
+#
+# W8A8: weights in 8-bit integers with one fp32 scale per output channel, activations quantized per token on the way
+# into the product, sums exact in int32 (lb_w8_linear). For prompts: twice the tensor-core rate of the dequantize +
+# fp16 path, and half its weight bytes. No counterpart in the reference.
+
+def quantize_w8_gpu(w):
+    """(int8 [N, K], scales fp32 [N]) of a float weight [N, K] (fp16, bf16 or fp32, on the GPU): per output channel
+    scale = max|w| / 127 and q = rint(w * (127 / max|w|)), half to even. The same rule per token is what linear_w8
+    applies to its activations."""
+    if not (isinstance(w, torch.Tensor) and w.is_cuda):
+        raise RuntimeError("quantize_w8_gpu takes GPU tensors")
+    if w.dim() != 2 or w.dtype not in DTYPE_IDS:
+        raise RuntimeError("w must be a float16, bfloat16 or float32 [N, K] tensor")
+    n, k = w.shape
+    if w.stride(1) != 1 or w.stride(0) < k:
+        w = w.contiguous()
+    q = torch.empty(n, -(-k // 16) * 16, dtype=torch.int8, device=w.device)
+    scales = torch.empty(n, dtype=torch.float32, device=w.device)
+    e = ext()
+    if n and k:
+        with _Device(w.device):
+            rc = e.lib.lb_w8_quantize_rows(w.data_ptr(), DTYPE_IDS[w.dtype], n, k, w.stride(0) if n > 1 else k,
+                                           q.data_ptr(), q.shape[1], scales.data_ptr(),
+                                           torch.cuda.current_stream().cuda_stream)
+        if rc:
+            e._raise(rc)
+    return q[:, :k], scales
+
+
+class W8Weight:
+    """One linear layer's weight in 8-bit integers on the GPU: q int8 [N, K], scales fp32 [N] (W = q * scale). Rows
+    are kept a multiple of 16 bytes apart with zeros behind K; a q that already lies so (every K that is a multiple of
+    16, and what quantize_w8_gpu returns) is kept without a copy."""
+
+    def __init__(self, q, scales):
+        if not (isinstance(q, torch.Tensor) and isinstance(scales, torch.Tensor) and q.is_cuda):
+            raise RuntimeError("W8Weight takes GPU tensors")
+        if q.dtype != torch.int8 or q.dim() != 2 or not q.numel():
+            raise RuntimeError("q must be an int8 [N, K] tensor")
+        self.n, self.k = q.shape
+        if scales.dtype != torch.float32 or scales.shape != (self.n,) or scales.device != q.device:
+            raise RuntimeError(f"scales must be a float32 [{self.n}] tensor on {q.device}")
+        if self.k > 131072:
+            raise ValueError(f"K={self.k}: at most 131072, so that the int32 sums are exact")
+        if (self.k % 16 == 0 and q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.stride(0) >= self.k
+                and q.data_ptr() % 16 == 0):
+            self.q = q
+        else:
+            pad = torch.zeros(self.n, -(-self.k // 16) * 16, dtype=torch.int8, device=q.device)
+            pad[:, :self.k] = q
+            self.q = pad[:, :self.k]
+        self.scales = scales.contiguous()
+        self._args = (self.q.data_ptr(), self.scales.data_ptr(), q.get_device(), self.n, self.k,
+                      self.q.stride(0) if self.n > 1 else -(-self.k // 16) * 16)
+
+    @classmethod
+    def from_float(cls, w):
+        return cls(*quantize_w8_gpu(w))
+
+    def nbytes(self):
+        return self.n * self.k + 4 * self.n
+
+
+def linear_w8(x, w8, bias=None, out=None):
+    """x [M, K] fp16 or bf16 (rows any stride apart) -> [M, N] of the same type: each row quantized to 8-bit integers
+    with its own scale, the product with w8 (W8Weight) exact in int32, then scaled, `bias` ([N], x's type) added and
+    rounded once. `out`: an optional contiguous [M, N] tensor that receives the result."""
+    tc = _tc if _tc is not None else _torchcall()
+    if tc:
+        p = w8._args
+        y = tc.linear_w8(x, p[0], p[1], p[2], p[3], p[4], p[5], out, bias)
+        if y is not None:
+            return y
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.device == w8.q.device):
+        raise RuntimeError(f"x must be on the weight's GPU, {w8.q.device}")
+    if x.dtype not in (torch.float16, torch.bfloat16) or x.dim() != 2 or x.shape[1] != w8.k:
+        raise RuntimeError(f"x must be a float16 or bfloat16 [M, {w8.k}] tensor")
+    m = x.shape[0]
+    if bias is not None and (not bias.is_cuda or bias.device != x.device or bias.dtype != x.dtype
+                             or bias.shape != (w8.n,) or not bias.is_contiguous()):
+        raise RuntimeError(f"bias must be a contiguous {x.dtype} [{w8.n}] tensor on {x.device}")
+    if out is None:
+        out = torch.empty(m, w8.n, dtype=x.dtype, device=x.device)
+    elif out.shape != (m, w8.n) or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
+        raise RuntimeError(f"out must be a contiguous {x.dtype} [{m}, {w8.n}] tensor on {x.device}")
+    if m == 0:
+        return out
+    if x.stride(1) != 1 or (m > 1 and x.stride(0) < w8.k):
+        x = x.contiguous()
+    e = ext()
+    w_ptr, s_ptr, _, n, k, ldw = w8._args
+    with _Device(x.device):
+        need = e.lib.lb_w8_workspace(m, n, ldw)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        rc = e.lib.lb_w8_linear(x.data_ptr(), DTYPE_IDS[x.dtype], x.stride(0) if m > 1 else k, w_ptr, ldw, s_ptr,
+                                None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, k,
+                                ws.data_ptr() if need else None, need, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        e._raise(rc)
+    return out
