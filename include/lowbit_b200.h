@@ -270,11 +270,12 @@ LB_API int lb_w8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, i
 /*
  * y[M, N] = (sum_k q[m, k] w[n, k]) s[m] w_scales[n] + bias[n], q and s the rows of x quantized as above, the sum
  * exact in int32, the rest in fp32 with one rounding. x and y fp16 or bf16 (y contiguous), bias [N] of that type or
- * NULL; w int8 [N, ldw] 16-byte aligned, ldw a multiple of 16, columns K.. zero; w and w_scales are model state: they
- * may be read before the kernel waits on the previous one in the stream. workspace: lb_w8_workspace(m, n, ldw) bytes
+ * NULL; w int8 [N, ldw] 16-byte aligned, ldw a multiple of 16, zeros from column K to the next multiple of 16; w and w_scales are model state: they
+ * may be read before the kernel waits on the previous one in the stream. workspace: lb_w8_workspace(m, n, k) bytes on the
+ * current device
  * (0: none needed), 16-byte aligned, its content undefined before and after; calls that can overlap need distinct ones.
  */
-LB_API int64_t lb_w8_workspace(int64_t m, int64_t n, int64_t ldw);
+LB_API int64_t lb_w8_workspace(int64_t m, int64_t n, int64_t k);
 LB_API int lb_w8_linear(const void* x, int dtype, int64_t ldx, const void* w, int64_t ldw, const float* w_scales,
                         const void* bias, void* y, int64_t m, int64_t n, int64_t k, void* workspace,
                         int64_t workspace_bytes, lb_stream_t stream);

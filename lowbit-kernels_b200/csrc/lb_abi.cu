@@ -649,8 +649,8 @@ int lb_w8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, int64_t 
                   "w8_quantize_rows");
 }
 
-int64_t lb_w8_workspace(int64_t m, int64_t n, int64_t ldw) {
-  return m < 1 || n < 1 || ldw < 1 ? 0 : (int64_t)lb::w8_workspace_bytes(m, n, ldw);
+int64_t lb_w8_workspace(int64_t m, int64_t n, int64_t k) {
+  return m < 1 || n < 1 || k < 1 ? 0 : (int64_t)lb::w8_workspace_bytes(m, n, k);
 }
 
 int lb_w8_linear(const void* x, int dtype, int64_t ldx, const void* w, int64_t ldw, const float* w_scales,
@@ -662,7 +662,7 @@ int lb_w8_linear(const void* x, int dtype, int64_t ldx, const void* w, int64_t l
   if (rc) return rc;
   if (n < 1 || n > (1 << 30)) return fail(LB_ERR_ARGUMENT, "shape mismatch: N=%lld", (long long)n);
   if (!aligned2(bias) || !aligned2(y)) return fail(LB_ERR_ALIGNMENT, "bias and y must be 2-byte aligned");
-  const int64_t need = (int64_t)lb::w8_workspace_bytes(m, n, ldw);
+  const int64_t need = (int64_t)lb::w8_workspace_bytes(m, n, k);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(LB_ERR_ARGUMENT, "the workspace holds %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0),
                 (long long)need);

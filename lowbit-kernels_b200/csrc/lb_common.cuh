@@ -77,6 +77,18 @@ __device__ __forceinline__ uint32_t ldg_cg_u32(const uint32_t* p) {
   return v;
 }
 
+// the same, 16 bytes
+__device__ __forceinline__ uint4 ldg_cg_u128(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.cg.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint16_t ldg_cg_u16(const void* p) {
+  uint16_t v;
+  asm volatile("ld.global.cg.u16 %0, [%1];" : "=h"(v) : "l"(p));
+  return v;
+}
+
 // Programmatic dependent launch: let the next kernel in the stream launch, and wait for the previous one.
 // Both are no-ops when the launch carries no programmatic dependency.
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

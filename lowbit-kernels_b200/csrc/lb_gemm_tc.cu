@@ -534,6 +534,12 @@ bool encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void
                 swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+int sm_count() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return device_sms(dev);
+}
+
 int gemm_tc05_splits(int M, int N, int K, int G, int forced) {
   if (M < 1 || M > 64 || K % 128 || G % 128 || K % G) return 0;
   int dev = 0;

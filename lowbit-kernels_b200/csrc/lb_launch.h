@@ -129,12 +129,14 @@ cudaError_t launch_gemm_mma(const GemvParams& p, const MmaConfig& c, bool pdl, c
 int gemm_mma_device_error();   // synchronizes
 void gemm_mma_clear_device_error();
 
+int sm_count();   // SMs of the current device (lb_gemm_tc.cu)
+
 // W8A8 linear layer (lb_w8.cu). dtype: 0 fp16, 1 bf16 (2 fp32, quantize only)
 struct W8Params {
   const void* x;        // [M, K], rows ldx elements apart
   int64_t ldx;
   int dtype;
-  const void* w;        // int8 [N, ldw], bytes K.. of a row zero
+  const void* w;        // int8 [N, ldw], zeros from K to the next multiple of 16
   int64_t ldw;
   const float* w_scales;
   const void* bias;     // [N] or null
@@ -142,7 +144,7 @@ struct W8Params {
   int64_t M, N, K;
   void* workspace;
 };
-size_t w8_workspace_bytes(int64_t M, int64_t N, int64_t ldw);
+size_t w8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 cudaError_t launch_w8_linear(const W8Params& p, bool pdl, cudaStream_t st);
 cudaError_t launch_w8_quantize_rows(const void* x, int dtype, int64_t ldx, int8_t* q, int64_t ldq, float* s, int64_t M,
                                     int64_t K, bool pdl, cudaStream_t st);

@@ -156,7 +156,7 @@ PyObject* linear_w8(PyObject* const* args) {
       Py_RETURN_NONE;
     y = *o;
   }
-  const int64_t need = lb_w8_workspace(m, n, ldw);
+  const int64_t need = lb_w8_workspace(m, n, k);
   at::Tensor ws;
   if (need > 0) ws = at::empty({need}, x->options().dtype(at::kByte));
   const int rc = lb_w8_linear(x->data_ptr(), type == at::kHalf ? LB_F16 : LB_BF16, ldx,

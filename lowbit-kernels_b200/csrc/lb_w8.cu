@@ -9,7 +9,7 @@
 #include <atomic>
 
 #include "lb_launch.h"
-#include "lb_tma.cuh"
+#include "lb_tc.cuh"
 #include "lb_types.cuh"
 
 namespace lb {
@@ -20,11 +20,7 @@ __device__ int g_w8_status;
 namespace {
 
 // ------------------------------------------------------------------------------------------- quantize rows
-// One CTA per row: |x| maximum over the row, then the quantized bytes. Memory bound: reads 2 K (4 K for fp32) and
-// writes K bytes a row; the row's second reading comes from L1 / L2.
-constexpr int kQThreads = 256;
-
-// q = rint(x * r), 127 / amax computed on amax * up so that the quotient of a row of subnormals stays finite
+// 127 / amax of a row of subnormals would overflow: such rows are scaled by `up`, a power of two, first
 struct RowScale {
   float up, r, s;
 };
@@ -35,122 +31,973 @@ __device__ __forceinline__ RowScale row_scale(float amax) {
   v.s = amax / 127.f;
   return v;
 }
-__device__ __forceinline__ int quant1(float x, const RowScale& v) {
-  return max(-127, min(127, __float2int_rn(x * v.up * v.r)));
+
+// rint(x r) in the low byte: adding 1.5 * 2^23 rounds to an integer, half to even (|x r| <= 127 but for rows that are
+// not finite, whose scale makes the outputs so)
+__device__ __forceinline__ uint32_t quant_bits(float x, float r) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(x, r), 12582912.f));   // two roundings: not to be fused
 }
 
-// the larger of |x| so far and |x|, keeping a NaN
-__device__ __forceinline__ float amax_nan(float a, float x) {
-  x = fabsf(x);
-  return (x > a || x != x) ? x : a;
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
+
+__device__ __forceinline__ uint2 quant8(const float (&f)[8], const RowScale& v) {
+  uint32_t q[8];
+  if (v.up == 1.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = quant_bits(f[i], v.r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = quant_bits(f[i] * v.up, v.r);
+  }
+  return make_uint2(low_bytes(q[0], q[1], q[2], q[3]), low_bytes(q[4], q[5], q[6], q[7]));
+}
+
+// Eight values of a row. Maxima of |x| are taken on the bits without the sign, which order like the magnitudes with NaN
+// above all: `amax` keeps them packed, `amax_float` gives the fp32 value.
+template <typename T>
+struct Vec8 {
+  uint32_t v[4];
+  // n: values left in the row, zeros behind them; through L2 only (the row may have been written while this kernel was
+  // already resident)
+  __device__ __forceinline__ void load(const T* p, int n, bool aligned) {
+    if (n >= 8 && aligned) {
+      const uint4 a = ldg_cg_u128(p);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+    } else {
+      uint16_t h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = i < n ? ldg_cg_u16(p + i) : (uint16_t)0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (uint32_t)h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
+    }
+  }
+  __device__ __forceinline__ uint32_t amax(uint32_t a) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a = __vmaxu2(a, v[i] & 0x7FFF7FFFu);
+    return a;
+  }
+  static __device__ __forceinline__ uint32_t amax_float(uint32_t a) {
+    return __float_as_uint(Elem<T>::unpack(max(a & 0xFFFFu, a >> 16)).x);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = Elem<T>::unpack(v[i]);
+      f[2 * i] = a.x;
+      f[2 * i + 1] = a.y;
+    }
+  }
+};
+template <>
+struct Vec8<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float* p, int n, bool) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? __uint_as_float(ldg_cg_u32(reinterpret_cast<const uint32_t*>(p + i))) : 0.f;
+  }
+  __device__ __forceinline__ uint32_t amax(uint32_t a) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return a;
+  }
+  static __device__ __forceinline__ uint32_t amax_float(uint32_t a) { return a; }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = v[i];
+  }
+};
+
+// GT threads take one row of up to 64 GT values: the row goes into registers once, the maximum is reduced over the
+// group, and the bytes are written 8 at a time. Memory bound: 2 K (4 K for fp32) bytes read and K written per row.
+constexpr int kQVecs = 8;
+
+template <typename T, int GT>
+__global__ void __launch_bounds__(256)
+    quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int ldq, float* __restrict__ s,
+                         int M, int K, bool early) {
+  constexpr int kRows = 256 / GT;
+  __shared__ uint32_t red[kRows][GT / 32];
+  if (early) pdl_launch_dependents();
+  pdl_wait();
+  const int g = threadIdx.x / GT, tid = threadIdx.x % GT;
+  const int64_t row = (int64_t)blockIdx.x * kRows + g;
+  const bool on = row < M;
+  const T* xr = x + (on ? row : 0) * ldx;
+  const int nv = on ? ldq / 8 : 0;
+  const bool aligned = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * sizeof(T))) & 15u) == 0;
+  Vec8<T> v[kQVecs];
+#pragma unroll
+  for (int i = 0; i < kQVecs; ++i) {
+    const int j = tid + i * GT;
+    if (j < nv) v[i].load(xr + 8 * j, K - 8 * j, aligned);
+  }
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < kQVecs; ++i)
+    if (tid + i * GT < nv) a = v[i].amax(a);
+  a = __reduce_max_sync(0xffffffffu, Vec8<T>::amax_float(a));
+  if (GT > 32) {
+    if ((tid & 31) == 0) red[g][tid >> 5] = a;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < GT / 32; ++w) a = max(a, red[g][w]);
+  }
+  const RowScale sc = row_scale(__uint_as_float(a));
+  if (on && tid == 0) s[row] = sc.s;
+  uint2* dst = reinterpret_cast<uint2*>(q + row * ldq);
+#pragma unroll
+  for (int i = 0; i < kQVecs; ++i) {
+    const int j = tid + i * GT;
+    if (j < nv) {
+      float f[8];
+      v[i].get(f);
+      dst[j] = quant8(f, sc);
+    }
+  }
+}
+
+// Longer rows, one CTA each: the row (its first `cap` values, if it is longer than that) is copied into shared memory
+// in one piece, so that several rows of an SM are in flight whatever the registers; both passes read it there.
+constexpr int kQLongThreads = 512;
+constexpr int kQLongBytes = 96 * 1024;
 
 template <typename T>
-__global__ void __launch_bounds__(kQThreads)
-    quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int ldq, float* __restrict__ s,
-                         int K) {
-  __shared__ float red[kQThreads / 32];
-  pdl_launch_dependents();
-  pdl_wait();
+__global__ void __launch_bounds__(kQLongThreads)
+    quantize_long_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int ldq, float* __restrict__ s,
+                         int K, int cap, bool early) {
+  extern __shared__ __align__(128) uint8_t row_bytes[];
+  __shared__ uint64_t bar;
+  __shared__ uint32_t red[kQLongThreads / 32];
+  if (early) pdl_launch_dependents();
+  const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ldx;
-  float a = 0.f;
-  for (int k = threadIdx.x; k < K; k += kQThreads) a = amax_nan(a, Elem<T>::to_float(xr[k]));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) a = amax_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+  const int nv = ldq / 8, held = min(K, cap) / 8;   // vectors in all, and in shared memory
+  const bool aligned = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * sizeof(T))) & 15u) == 0;
+  if (tid == 0) {
+    mbar_init(&bar, 1);
+    mbar_fence_init();
+  }
   __syncthreads();
-  a = red[0];
-#pragma unroll
-  for (int w = 1; w < kQThreads / 32; ++w) a = amax_nan(a, red[w]);
-  const RowScale v = row_scale(a);
-  if (threadIdx.x == 0) s[row] = v.s;
-  for (int k = threadIdx.x; k < ldq; k += kQThreads)
-    q[row * ldq + k] = k < K ? (int8_t)quant1(Elem<T>::to_float(xr[k]), v) : (int8_t)0;
-}
-
-// ------------------------------------------------------------------------------------------- the product
-constexpr int kTile = 64;
-
-template <typename T>
-__global__ void __launch_bounds__(256)
-    w8_gemm_kernel(const int8_t* __restrict__ q, const float* __restrict__ s, const int8_t* __restrict__ w,
-                   const float* __restrict__ t, const T* __restrict__ bias, T* __restrict__ y, int M, int N, int ld) {
-  __shared__ int qs[kTile][9], ws[kTile][9];   // 32 bytes of k per row, padded
-  pdl_launch_dependents();
   pdl_wait();
-  const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < ld; k0 += 32) {
-    for (int i = threadIdx.x; i < kTile * 8; i += 256) {
-      const int r = i >> 3, c = i & 7, k = k0 + 4 * c;
-      qs[r][c] = m0 + r < M && k < ld ? *reinterpret_cast<const int*>(q + (int64_t)(m0 + r) * ld + k) : 0;
-      ws[r][c] = n0 + r < N && k < ld ? *reinterpret_cast<const int*>(w + (int64_t)(n0 + r) * ld + k) : 0;
+  T* mine = reinterpret_cast<T*>(row_bytes);
+  if (aligned) {
+    if (tid == 0) {
+      mbar_arrive_expect_tx(&bar, (uint32_t)(8 * held * sizeof(T)));
+      bulk_copy_g2s(mine, xr, (uint32_t)(8 * held * sizeof(T)), &bar);
     }
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(qs[ty + 16 * i][c], ws[tx + 16 * j][c], acc[i][j]);
+    wait_bounded(&bar, 0, &g_w8_status);
+  } else {
+    for (int i = tid; i < 8 * held; i += kQLongThreads) mine[i] = xr[i];
     __syncthreads();
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m < M && n < N)
-        y[(int64_t)m * N + n] = Elem<T>::from_float(__int2float_rn(acc[i][j]) * s[m] * t[n] +
-                                                    (bias ? Elem<T>::to_float(bias[n]) : 0.f));
+  auto fetch = [&](int j, Vec8<T>& v) {
+    if (j < held) {
+      const uint4* src = reinterpret_cast<const uint4*>(mine + 8 * j);
+#pragma unroll
+      for (int h = 0; h < (int)sizeof(T) / 2; ++h) reinterpret_cast<uint4*>(&v.v[0])[h] = src[h];
+    } else {
+      v.load(xr + 8 * j, K - 8 * j, aligned);
     }
+  };
+  uint32_t a = 0;
+  for (int j = tid; j < nv; j += kQLongThreads) {
+    Vec8<T> v;
+    fetch(j, v);
+    a = v.amax(a);
+  }
+  a = __reduce_max_sync(0xffffffffu, Vec8<T>::amax_float(a));
+  if ((tid & 31) == 0) red[tid >> 5] = a;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kQLongThreads / 32; ++w) a = max(a, red[w]);
+  const RowScale sc = row_scale(__uint_as_float(a));
+  if (tid == 0) s[row] = sc.s;
+  uint2* dst = reinterpret_cast<uint2*>(q + row * ldq);
+  for (int j = tid; j < nv; j += kQLongThreads) {
+    Vec8<T> v;
+    fetch(j, v);
+    float f[8];
+    v.get(f);
+    dst[j] = quant8(f, sc);
+  }
 }
 
+// ------------------------------------------------------------------------------------------- the product, many rows
+// tcgen05.mma kind::i8 with the channels as the A side (128 rows a CTA) and a tile of BN tokens as the N side, int32
+// accumulators in tensor memory.
+//   * loader warp: one thread copies each 128-byte K chunk of the tile (channels, tokens; 128-byte swizzle, rows and
+//     columns past the edge read as zeros) into a stage ring; the first stages' weights before the wait on the previous
+//     kernel (the quantization), whose rows follow after it.
+//   * MMA warp: one thread issues four K = 32 MMAs per chunk; a commit per chunk releases the stage, one per tile hands
+//     the accumulator to the epilogue. Two accumulators: the next tile's MMAs run under this tile's epilogue.
+//   * 8 epilogue warps, two per 32-lane quarter of tensor memory: a lane holds one channel (its scale and bias in
+//     registers), a column one token; a warp stores 64 consecutive bytes of an output row at a time.
+// CTAs are persistent over tiles, tokens innermost, so that the CTAs of one moment share weights in L2.
+// PAIR: two CTAs work on one tile of 256 channels (cta_group::2): each loads its 128 channels and half of the tokens, and
+// the leader's MMAs read both. A chunk then costs each SM 16 + BN / 16 KB of loads instead of 16 + BN / 8, and it is the
+// L2-to-SM path that bounds the single-CTA form: at BN = 224 it wants 100 bytes a clock and SM.
+// Few tiles and long K: a cluster of S single CTAs splits K, each parks its int32 partial tile in its (then idle) ring
+// and all sum their share through distributed shared memory -- exact, so the bits do not depend on S.
+constexpr int kChunk = 128;               // bytes of K per stage
+constexpr int kWBytes = 128 * kChunk;
+constexpr int kMmaThreads = 10 * 32;      // loader, MMA, 8 epilogue warps
+constexpr int kMaxStages = 8;
+constexpr int kW8MaxSplits = 8;           // portable cluster size
+constexpr int kW8Smem = 227 * 1024;
+constexpr int kBarrierBytes = (2 * kMaxStages + 4) * 8 + 16 + 2 * 256 * 4;
+
+struct W8Gemm {
+  const float* s;       // token scales
+  const float* t;       // channel scales
+  const void* bias;
+  void* y;
+  int M, N, chunks;     // 128-byte chunks of K
+  int bn, tiles_m, tiles, splits, stages;
+  int columns;          // tensor memory: 2 accumulators (persistent), or 1 (split)
+  int acc_stride;       // columns between the accumulators
+  int park;             // byte offset behind the ring: barriers and scales
+};
+
+__device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// This CTA's share of a cluster's outputs: the int32 partial tiles [token][128 channels] at the same offset of every
+// CTA's shared memory, summed, scaled and stored. A thread's four channels are the same in every round.
+template <typename T>
+__device__ __forceinline__ void sum_partials(uint32_t red, const float* sc, const float* t, const T* bias, T* y, int n0,
+                                             int N, int rows, int rank, int S) {
+  const int r4 = (threadIdx.x & 31) * 4;
+  float tn[4], bn[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const bool on = n0 + r4 + j < N;
+    tn[j] = on ? t[n0 + r4 + j] : 0.f;
+    bn[j] = on && bias ? Elem<T>::to_float(bias[n0 + r4 + j]) : 0.f;
+  }
+  const int warps = blockDim.x >> 5;
+  for (int m = rank * warps + (threadIdx.x >> 5); m < rows; m += S * warps) {
+    const uint32_t off = red + (uint32_t)(m * 128 + r4) * 4u;
+    float4 f[kW8MaxSplits];
+#pragma unroll
+    for (int q = 0; q < kW8MaxSplits; ++q)
+      if (q < S) f[q] = ld_dsmem_f4(mapa_shared(off, (uint32_t)q));
+    int v[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int q = 0; q < kW8MaxSplits; ++q)
+      if (q < S) {
+        v[0] += __float_as_int(f[q].x);
+        v[1] += __float_as_int(f[q].y);
+        v[2] += __float_as_int(f[q].z);
+        v[3] += __float_as_int(f[q].w);
+      }
+    T* dst = y + (int64_t)m * N + n0 + r4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n0 + r4 + j < N) dst[j] = Elem<T>::from_float(fmaf(__int2float_rn(v[j]) * sc[m], tn[j], bn[j]));
+  }
+}
+
+template <typename T, bool PAIR>
+__global__ void __launch_bounds__(kMmaThreads)
+    w8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap, const W8Gemm p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + p.park);   // PAIR: the leader's, for both CTAs' copies
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* acc_full = empty + kMaxStages;
+  uint64_t* acc_empty = acc_full + 2;                            // PAIR: the leader's
+  uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  float* sc = reinterpret_cast<float*>(slot + 4);   // [2][256] token scales
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int own_bn = PAIR ? p.bn / 2 : p.bn;        // tokens this CTA loads
+  const int stage_bytes = kWBytes + own_bn * kChunk, S = PAIR ? 1 : p.splits, St = p.stages;
+  const int rank = PAIR || S > 1 ? (int)cluster_rank() : 0;
+  const int group = PAIR ? 2 : S;
+  const int first = blockIdx.x / group, step = gridDim.x / group;
+  const int c0 = PAIR ? 0 : p.chunks * rank / S, nc = PAIR ? p.chunks : p.chunks * (rank + 1) / S - c0;
+  constexpr int kTileN = PAIR ? 256 : 128;
+  const int n_off = PAIR ? 128 * rank : 0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < St; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], PAIR ? 16 : 8);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    if (PAIR)
+      tc::alloc_pair(slot, p.columns);
+    else
+      tc::alloc(slot, p.columns);
+  }
+  tc::fence_before();
+  if (PAIR)
+    cluster_sync_all();   // the peer's barriers exist before a copy or a commit reaches them
+  else
+    __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *slot;
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_map(&wmap);
+      tma_prefetch_map(&qmap);
+      const int mine = first < p.tiles ? (p.tiles - first + step - 1) / step : 0, total = mine * nc;
+      auto weights = [&](int i) {
+        const int n0 = (first + i / nc * step) / p.tiles_m * kTileN + n_off;
+        uint8_t* dst = ring + (i % St) * stage_bytes;
+        if (PAIR) {
+          if (rank == 0) mbar_arrive_expect_tx(&full[i % St], 2 * stage_bytes);
+          tc::tma_load_2d_pair(dst, &wmap, (i % nc) * kChunk, n0, mapa_shared(smem_addr(&full[i % St]), 0));
+        } else {
+          mbar_arrive_expect_tx(&full[i % St], stage_bytes);
+          tma_load_2d(dst, &wmap, (c0 + i % nc) * kChunk, n0, &full[i % St]);
+        }
+      };
+      auto tokens = [&](int i) {
+        const int m0 = (first + i / nc * step) % p.tiles_m * p.bn + (PAIR ? rank * own_bn : 0);
+        uint8_t* dst = ring + (i % St) * stage_bytes + kWBytes;
+        if (PAIR)
+          tc::tma_load_2d_pair(dst, &qmap, (i % nc) * kChunk, m0, mapa_shared(smem_addr(&full[i % St]), 0));
+        else
+          tma_load_2d(dst, &qmap, (c0 + i % nc) * kChunk, m0, &full[i % St]);
+      };
+      const int head = min(St, total);
+      for (int i = 0; i < head; ++i) weights(i);
+      pdl_wait();
+      for (int i = 0; i < head; ++i) tokens(i);
+      int issued = head;
+      for (int i = head; i < total; ++i) {
+        if (!wait_bounded(&empty[i % St], (i / St - 1) & 1, &g_w8_status)) break;
+        weights(i);
+        tokens(i);
+        issued = i + 1;
+      }
+      if (rank == 0 || !PAIR)   // no copy in flight past this point (the leader's barriers count the peer's too)
+        for (int i = max(0, issued - St); i < issued; ++i) wait_bounded(&full[i % St], (i / St) & 1, &g_w8_status);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && (!PAIR || rank == 0)) {
+      // int32 accumulator, signed 8-bit A and B, both K-major
+      const uint32_t idesc =
+          (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kTileN >> 4) << 24);
+      int i = 0, a = 0;
+      bool ok = true;
+      for (int tile = first; tile < p.tiles && ok; tile += step, ++a) {
+        if (a >= 2) ok = wait_bounded(&acc_empty[a & 1], ((a >> 1) - 1) & 1, &g_w8_status);
+        tc::fence_after();
+        const uint32_t d = tmem + (a & 1) * p.acc_stride;
+        for (int c = 0; c < nc && ok; ++c, ++i) {
+          ok = wait_bounded(&full[i % St], (i / St) & 1, &g_w8_status);
+          if (!ok) break;
+          tc::fence_after();
+          const uint32_t at = smem_addr(ring + (i % St) * stage_bytes);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t ad = tc::desc_sw128(at + 32 * k, 16, 1024), bd = tc::desc_sw128(at + kWBytes + 32 * k, 16, 1024);
+            if (PAIR)
+              tc::mma_i8_ss_pair(d, ad, bd, idesc, c > 0 || k > 0);
+            else
+              tc::mma_i8_ss(d, ad, bd, idesc, c > 0 || k > 0);
+          }
+          if (PAIR)
+            tc::commit_pair(&empty[i % St]);
+          else
+            tc::commit(&empty[i % St]);
+        }
+        if (PAIR)
+          tc::commit_pair(&acc_full[a & 1]);
+        else
+          tc::commit(&acc_full[a & 1]);
+      }
+      // no MMA in flight past this point
+      for (int b = max(0, a - 2); b < a; ++b) wait_bounded(&acc_full[b & 1], (b >> 1) & 1, &g_w8_status);
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, half = warp >= 6, row = 32 * quarter + lane, et = threadIdx.x - 64;
+    const uint32_t tlane = (uint32_t)(32 * quarter) << 16;
+    const T* bias = static_cast<const T*>(p.bias);
+    T* y = static_cast<T*>(p.y);
+    pdl_wait();
+    int a = 0;
+    bool ok = true;
+    for (int tile = first; tile < p.tiles && ok; tile += step, ++a) {
+      const int m0 = tile % p.tiles_m * p.bn, n = tile / p.tiles_m * kTileN + n_off + row;
+      const bool on = n < p.N;
+      float* scale = sc + (a & 1) * 256;
+      if (et < p.bn)
+        scale[et] = m0 + et < p.M ? __uint_as_float(ldg_cg_u32(reinterpret_cast<const uint32_t*>(p.s + m0 + et))) : 0.f;
+      const float tn = on ? p.t[n] : 0.f, bn = on && bias ? Elem<T>::to_float(bias[n]) : 0.f;
+      named_barrier(1, 256);
+      ok = wait_bounded(&acc_full[a & 1], (a >> 1) & 1, &g_w8_status);
+      __syncwarp();
+      tc::fence_after();
+      for (int j0 = 16 * half; j0 < p.bn; j0 += 32) {
+        uint32_t v[16];
+        tc::ld16(tmem + tlane + (uint32_t)((a & 1) * p.acc_stride + j0), v);
+        tc::wait_ld();
+        if (S == 1) {
+          T* dst = y + (int64_t)(m0 + j0) * p.N + n;
+          if (on && m0 + j0 + 16 <= p.M) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j, dst += p.N)
+              *dst = Elem<T>::from_float(fmaf(__int2float_rn((int)v[j]) * scale[j0 + j], tn, bn));
+          } else if (on) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j, dst += p.N)
+              if (m0 + j0 + j < p.M) *dst = Elem<T>::from_float(fmaf(__int2float_rn((int)v[j]) * scale[j0 + j], tn, bn));
+          }
+        } else {
+          int* red = reinterpret_cast<int*>(ring);   // [token][128 channels]
+#pragma unroll
+          for (int j = 0; j < 16; ++j) red[(j0 + j) * 128 + row] = (int)v[j];
+        }
+      }
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (PAIR)
+          tc::arrive_cluster(mapa_shared(smem_addr(&acc_empty[a & 1]), 0));
+        else
+          mbar_arrive(&acc_empty[a & 1]);
+      }
+    }
+  }
+  __syncwarp();
+  if (!PAIR && S > 1) {
+    cluster_sync_all();
+    const int n0 = first / p.tiles_m * 128, m0 = first % p.tiles_m * p.bn;
+    sum_partials<T>(smem_addr(ring), sc, p.t, static_cast<const T*>(p.bias),
+                    static_cast<T*>(p.y) + (int64_t)m0 * p.N, n0, p.N, min(p.bn, p.M - m0), rank, S);
+  }
+  tc::fence_before();
+  if (PAIR || S > 1)
+    cluster_sync_all();   // no CTA leaves while its partner still reads, or signals, its shared memory
+  else
+    __syncthreads();
+  if (warp == 1) {
+    tc::fence_after();
+    if (PAIR)
+      tc::dealloc_pair(tmem, p.columns);
+    else
+      tc::dealloc(tmem, p.columns);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- the product, few rows
+// Up to 64 tokens in one launch: a decode batch is bound by the weights' way from memory and by latency, so the
+// quantization is done inside. The S CTAs of a cluster split K of one 128-channel tile; each
+//   * streams its K range of the weights into a stage ring from the start (weights do not wait for the activations),
+//   * reads its K range of the token rows, whose maxima the cluster exchanges through distributed shared memory,
+//   * writes the quantized bytes straight into the MMAs' swizzled B tiles (all of its K range stays resident),
+//   * multiplies, and sums the int32 partial tiles over the cluster.
+// Rows past the last token hold whatever was there: integers, and their columns are not stored.
+constexpr int kSkinnyRows = 64;
+constexpr int kSkinnyVecs = 12;
+
+struct W8Skinny {
+  const void* x;
+  int64_t ldx;
+  const float* t;
+  const void* bias;
+  void* y;
+  int M, N, K, chunks, bn, splits, stages;
+  int columns;
+  int b_off;        // bytes: the B tiles behind the ring
+  int park;         // barriers, maxima and scales behind those
+};
+constexpr int kSkinnyPark = (2 * kMaxStages + 2) * 8 + 16 + 2 * kSkinnyRows * 4;
+
+template <typename T>
+__global__ void __launch_bounds__(kMmaThreads) w8_skinny_kernel(const __grid_constant__ CUtensorMap wmap, const W8Skinny p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + p.park);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* tokens_ready = empty + kMaxStages;
+  uint64_t* acc_full = tokens_ready + 1;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint32_t* maxima = slot + 4;                                   // [64], this CTA's K range
+  float* sc = reinterpret_cast<float*>(maxima + kSkinnyRows);    // [64] token scales
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = p.splits, St = p.stages, rank = S > 1 ? (int)cluster_rank() : 0;
+  const int n0 = blockIdx.x / S * 128;
+  const int c0 = p.chunks * rank / S, nc = p.chunks * (rank + 1) / S - c0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < St; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(tokens_ready, 8);
+    mbar_init(acc_full, 1);
+    mbar_fence_init();
+  }
+  if (threadIdx.x < kSkinnyRows) maxima[threadIdx.x] = 0u;
+  if (warp == 1) tc::alloc(slot, p.columns);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *slot;
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    // (the loader and the MMA warp have no maxima to give: they arrive for the exchange here and wait for it at their end)
+    if (S > 1) cluster_arrive();
+    if (lane == 0) {
+      tma_prefetch_map(&wmap);
+      run_loader(nc, St, full, empty, kWBytes, &g_w8_status, [&](int i, int st) {
+        tma_load_2d(ring + st * kWBytes, &wmap, (c0 + i) * kChunk, n0, &full[st]);
+      });
+    }
+    __syncwarp();
+    if (S > 1) cluster_wait();
+  } else if (warp == 1) {
+    if (S > 1) cluster_arrive();
+    if (lane == 0) {
+      const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((128u >> 4) << 24);
+      bool ok = wait_bounded(tokens_ready, 0, &g_w8_status);
+      for (int c = 0; c < nc && ok; ++c) {
+        ok = wait_bounded(&full[c % St], (c / St) & 1, &g_w8_status);
+        if (!ok) break;
+        tc::fence_after();
+        const uint32_t at = smem_addr(ring + (c % St) * kWBytes), bt = smem_addr(ring + p.b_off + c * p.bn * kChunk);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          tc::mma_i8_ss(tmem, tc::desc_sw128(at + 32 * k, 16, 1024), tc::desc_sw128(bt + 32 * k, 16, 1024), idesc,
+                        c > 0 || k > 0);
+        tc::commit(&empty[c % St]);
+      }
+      tc::commit(acc_full);
+      wait_bounded(acc_full, 0, &g_w8_status);   // no MMA in flight past this point
+    }
+    __syncwarp();
+    if (S > 1) cluster_wait();
+  } else {
+    const int quarter = warp & 3, half = warp >= 6, row = 32 * quarter + lane, n = n0 + row;
+    const T* bias = static_cast<const T*>(p.bias);
+    const bool on = n < p.N;
+    const float tn = on ? p.t[n] : 0.f, bn = on && bias ? Elem<T>::to_float(bias[n]) : 0.f;
+    const int k0 = c0 * kChunk, nv = nc * (kChunk / 8), left = p.K - k0;   // this CTA's vectors, and values left in a row
+    const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * sizeof(T))) & 15u) == 0;
+    const T* x = static_cast<const T*>(p.x) + k0;
+    pdl_wait();
+    // the M x nv vectors of 8 values, 256 neighbours at a time, 12 of a thread in flight; nv is a multiple of 16, so half
+    // a warp holds one row's. What fits in one round stays in registers until the maxima are known.
+    const int total = p.M * nv, et = threadIdx.x - 64;
+    Vec8<T> v[kSkinnyVecs];
+    auto fetch = [&](int base) {
+#pragma unroll
+      for (int i = 0; i < kSkinnyVecs; ++i) {
+        const int u = base + 256 * i + et;
+        if (u < total) v[i].load(x + u / nv * p.ldx + 8 * (u % nv), left - 8 * (u % nv), aligned);
+      }
+    };
+    for (int base = 0; base < total; base += 256 * kSkinnyVecs) {
+      fetch(base);
+#pragma unroll
+      for (int i = 0; i < kSkinnyVecs; ++i) {
+        const int u = base + 256 * i + et;
+        if (base + 256 * i >= total) break;
+        uint32_t a = u < total ? Vec8<T>::amax_float(v[i].amax(0u)) : 0u;
+        a = __reduce_max_sync(lane < 16 ? 0x0000ffffu : 0xffff0000u, a);
+        if ((lane & 15) == 0 && u < total) atomicMax(&maxima[u / nv], a);
+      }
+    }
+    __syncwarp();
+    if (S > 1)
+      cluster_sync_all();
+    else
+      named_barrier(1, 256);
+    if (et < p.M) {
+      uint32_t a = maxima[et];
+      for (int q = 0; q < S; ++q)
+        if (q != rank) a = max(a, ld_dsmem_u32(mapa_shared(smem_addr(maxima + et), (uint32_t)q)));
+      sc[et] = __uint_as_float(a);   // the maximum first; the scale takes its place below
+    }
+    named_barrier(1, 256);
+    for (int base = 0; base < total; base += 256 * kSkinnyVecs) {
+      if (total > 256 * kSkinnyVecs) fetch(base);
+#pragma unroll
+      for (int i = 0; i < kSkinnyVecs; ++i) {
+        const int u = base + 256 * i + et;
+        if (u < total) {
+          const int m = u / nv, j = u % nv, c = j >> 4, b = j & 15;   // row, chunk, 8-byte piece of its 128 bytes
+          float f[8];
+          v[i].get(f);
+          uint8_t* tile = ring + p.b_off + c * p.bn * kChunk;
+          *reinterpret_cast<uint2*>(tile + m * kChunk + (((b >> 1) ^ (m & 7)) << 4) + (b & 1) * 8) = quant8(f, row_scale(sc[m]));
+        }
+      }
+    }
+    tc::fence_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(tokens_ready);
+    named_barrier(1, 256);   // every maximum has been read
+    if (et < p.M) sc[et] = row_scale(sc[et]).s;
+    named_barrier(1, 256);
+    wait_bounded(acc_full, 0, &g_w8_status);
+    __syncwarp();
+    tc::fence_after();
+    for (int j0 = 16 * half; j0 < p.bn; j0 += 32) {
+      uint32_t v[16];
+      tc::ld16(tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)j0, v);
+      tc::wait_ld();
+      if (S == 1) {
+        T* dst = static_cast<T*>(p.y) + (int64_t)j0 * p.N + n;
+#pragma unroll
+        for (int j = 0; j < 16; ++j, dst += p.N)
+          if (on && j0 + j < p.M) *dst = Elem<T>::from_float(fmaf(__int2float_rn((int)v[j]) * sc[j0 + j], tn, bn));
+      } else {
+        int* red = reinterpret_cast<int*>(ring);   // [token][128 channels]
+#pragma unroll
+        for (int j = 0; j < 16; ++j) red[(j0 + j) * 128 + row] = (int)v[j];
+      }
+    }
+  }
+  __syncwarp();
+  if (S > 1) {
+    cluster_sync_all();
+    sum_partials<T>(smem_addr(ring), sc, p.t, static_cast<const T*>(p.bias), static_cast<T*>(p.y), n0, p.N, p.M, rank, S);
+  }
+  tc::fence_before();
+  if (S > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  if (warp == 1) {
+    tc::fence_after();
+    tc::dealloc(tmem, p.columns);
+  }
+}
+
+// ------------------------------------------------------------------------------------------- the product, one to eight rows
+// A CTA takes 16 channels and all of K: mma.sync m16n8k32 with the weights' fragments loaded straight into registers,
+// 64 bytes of K of a row per four lanes and 16-byte load (the order of k inside a fragment is free as long as both
+// operands share it). The first loads -- all there are, up to 64 kGemvRound NW values of K -- are issued before the wait
+// on the previous kernel; the CTA quantizes the token rows while they are under way. Bound by the weights' way from
+// memory; a cluster, tensor memory or a second launch would each add about a microsecond of latency to some four.
+constexpr int kGemvRows = 8;
+constexpr int kGemvRound = 4;    // 64-byte pieces of K of a warp in flight
+constexpr int kGemvVecs = 4;     // vectors of a token row that a thread keeps between the maximum and the quantization
+
+struct W8Gemv {
+  const void* x;
+  int64_t ldx;
+  const int8_t* w;
+  int64_t ldw;
+  const float* t;
+  const void* bias;
+  void* y;
+  int M, N, K, pieces;   // 64-byte pieces of K
+  int pitch;             // bytes between the quantized rows: 64 modulo 128, so that two rows' reads do not share banks
+};
+
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename T, int NW>
+__global__ void __launch_bounds__(32 * NW) w8_gemv_kernel(const W8Gemv p, int guard) {
+  extern __shared__ __align__(16) uint8_t rows[];   // [M][pitch] quantized tokens
+  __shared__ int part[NW][128];
+  __shared__ uint32_t maxima[kGemvRows];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16;
+  pdl_launch_dependents();
+  // rows past N repeat the last one; pieces past K read as zeros (K is padded to 16, a lane's share of a piece)
+  const int8_t* w0 = p.w + (int64_t)min(n0 + g, p.N - 1) * p.ldw + 16 * t;
+  const int8_t* w1 = p.w + (int64_t)min(n0 + g + 8, p.N - 1) * p.ldw + 16 * t;
+  uint4 a[kGemvRound][2];
+  auto fetch = [&](int i, int c) {
+    const bool on = 64 * c + 16 * t < p.K;
+    a[i][0] = on ? ldg_stream(reinterpret_cast<const uint4*>(w0 + 64 * c)) : make_uint4(0, 0, 0, 0);
+    a[i][1] = on ? ldg_stream(reinterpret_cast<const uint4*>(w1 + 64 * c)) : make_uint4(0, 0, 0, 0);
+  };
+#pragma unroll
+  for (int i = 0; i < kGemvRound; ++i) fetch(i, warp + i * NW);
+  const int out_n = n0 + (tid & 15), out_m = tid >> 4;   // the output this thread sums, of 16 x 8
+  const bool out_on = tid < 128 && out_n < p.N && out_m < p.M;
+  const float tn = out_on ? p.t[out_n] : 0.f;
+  const float bn = out_on && p.bias ? Elem<T>::to_float(static_cast<const T*>(p.bias)[out_n]) : 0.f;
+  if (tid < kGemvRows) maxima[tid] = 0u;
+  __syncthreads();
+  pdl_wait_after_loads(guard);
+  const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * sizeof(T))) & 15u) == 0;
+  const T* x = static_cast<const T*>(p.x);
+  const int nv = p.pieces * 8, total = p.M * nv;   // vectors of 8 values; eight lanes share a row
+  Vec8<T> v[kGemvVecs];
+  auto tokens = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < kGemvVecs; ++i) {
+      const int u = base + 32 * NW * i + tid;
+      if (u < total) v[i].load(x + u / nv * p.ldx + 8 * (u % nv), p.K - 8 * (u % nv), aligned);
+    }
+  };
+  for (int base = 0; base < total; base += 32 * NW * kGemvVecs) {
+    tokens(base);
+#pragma unroll
+    for (int i = 0; i < kGemvVecs; ++i) {
+      const int u = base + 32 * NW * i + tid;
+      if (base + 32 * NW * i >= total) break;
+      uint32_t am = u < total ? Vec8<T>::amax_float(v[i].amax(0u)) : 0u;
+      am = __reduce_max_sync(0xffu << (lane & 24), am);
+      if ((lane & 7) == 0 && u < total) atomicMax(&maxima[u / nv], am);
+    }
+  }
+  __syncthreads();
+  for (int base = 0; base < total; base += 32 * NW * kGemvVecs) {
+    if (total > 32 * NW * kGemvVecs) tokens(base);
+#pragma unroll
+    for (int i = 0; i < kGemvVecs; ++i) {
+      const int u = base + 32 * NW * i + tid;
+      if (u < total) {
+        const int m = u / nv;
+        float f[8];
+        v[i].get(f);
+        *reinterpret_cast<uint2*>(rows + m * p.pitch + 8 * (u % nv)) = quant8(f, row_scale(__uint_as_float(maxima[m])));
+      }
+    }
+  }
+  __syncthreads();
+  int d[4] = {0, 0, 0, 0};
+  const uint32_t own = smem_addr(rows) + (uint32_t)(min(g, p.M - 1) * p.pitch + 16 * t);   // unused columns repeat a row
+  for (int c0 = warp; c0 < p.pieces; c0 += NW * kGemvRound) {
+#pragma unroll
+    for (int i = 0; i < kGemvRound; ++i) {
+      const int c = c0 + i * NW;
+      if (c < p.pieces) {
+        const uint4 b = lds128(own + 64 * c);
+        mma_s8(d, a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b.x, b.y);
+        mma_s8(d, a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b.z, b.w);
+        fetch(i, c + NW * kGemvRound);
+      }
+    }
+  }
+  // D[g][2t], D[g][2t + 1], D[g + 8][..]: channel x token
+  part[warp][(2 * t) * 16 + g] = d[0];
+  part[warp][(2 * t + 1) * 16 + g] = d[1];
+  part[warp][(2 * t) * 16 + g + 8] = d[2];
+  part[warp][(2 * t + 1) * 16 + g + 8] = d[3];
+  __syncthreads();
+  if (out_on) {
+    int sum = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) sum += part[w][tid];
+    static_cast<T*>(p.y)[(int64_t)out_m * p.N + out_n] = Elem<T>::from_float(
+        fmaf(__int2float_rn(sum) * row_scale(__uint_as_float(maxima[out_m])).s, tn, bn));
+  }
+}
+
+// ------------------------------------------------------------------------------------------- launches
 template <typename Kern, typename... Args>
-cudaError_t launch_w8(Kern kern, dim3 grid, dim3 block, size_t smem, bool pdl, cudaStream_t st, Args... args) {
+cudaError_t launch_w8(Kern kern, unsigned grid, int threads, size_t smem, int cluster, bool pdl, cudaStream_t st,
+                      Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  if (pdl) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// Lets a kernel use that much dynamic shared memory, once per device
+template <typename Kern>
+cudaError_t allow_smem(Kern kern, std::atomic<uint64_t>& done, int bytes = kW8Smem) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+// a warp or 128 threads a row where the registers hold it, else a CTA. With few rows the next kernel is let in at once;
+// with many it would take the registers of CTAs still to come (measured at 8192 rows of 18944: the quantization ran at
+// half its speed under the product's resident CTAs).
+template <typename T>
+cudaError_t quantize_t(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* s, int64_t M, int64_t K, bool pdl,
+                       cudaStream_t st) {
+  const int64_t nv = ldq / 8;
+  const bool early = M <= 296;
+  const T* xt = static_cast<const T*>(x);
+  if (nv <= 128 * kQVecs) {
+    const int GT = nv <= 32 * kQVecs && M > 512 ? 32 : 128, rows = 256 / GT;
+    return launch_w8(GT == 32 ? quantize_rows_kernel<T, 32> : quantize_rows_kernel<T, 128>,
+                     (unsigned)((M + rows - 1) / rows), 256, 0, 1, pdl, st, xt, ldx, q, (int)ldq, s, (int)M, (int)K, early);
+  }
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(quantize_long_kernel<T>, done, kQLongBytes + 16);
+  if (e != cudaSuccess) return e;
+  const int cap = (int)min(K, (int64_t)(kQLongBytes / sizeof(T)));
+  return launch_w8(quantize_long_kernel<T>, (unsigned)M, kQLongThreads, (size_t)cap * sizeof(T) + 16, 1, pdl, st, xt, ldx,
+                   q, (int)ldq, s, (int)K, cap, early);
+}
+
+int64_t padded(int64_t k) { return (k + 15) / 16 * 16; }
+
+bool encode_rows(CUtensorMap* map, const void* base, int64_t width, int64_t ld, int64_t rows, int box_rows) {
+  return encode_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, (uint64_t)width, (uint64_t)rows, (uint64_t)ld, kChunk,
+                              (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int tmem_columns(int bn) { return bn <= 32 ? 32 : bn <= 64 ? 64 : bn <= 128 ? 128 : 256; }
+
+// Few rows: K split while the CTAs do not exceed two an SM and each keeps two chunks. Stages fill what shared memory a
+// second CTA of the SM leaves. splits 0: the token tiles do not fit.
+W8Skinny skinny_plan(int64_t M, int64_t N, int chunks, int sms) {
+  W8Skinny g = {};
+  g.bn = (int)(M + 15) / 16 * 16;
+  g.chunks = chunks;
+  const int tiles = (int)((N + 127) / 128);
+  int S = 1;
+  while (S < kW8MaxSplits && (int64_t)tiles * (S + 1) <= 2 * sms && chunks >= 2 * (S + 1)) ++S;
+  for (; S <= kW8MaxSplits && S <= chunks; ++S) {
+    const int nc = (chunks + S - 1) / S, b = nc * g.bn * kChunk, fixed = b + kSkinnyPark + 1024;
+    const int room = fixed + 3 * kWBytes <= kW8Smem / 2 ? kW8Smem / 2 - 1024 : kW8Smem;
+    g.stages = min(min(kMaxStages, nc), (room - fixed) / kWBytes);
+    if (g.stages < min(nc, 3)) continue;
+    if (S > 1 && g.stages * kWBytes < g.bn * 512) continue;   // the partial tile is parked in the ring
+    g.splits = S;
+    g.b_off = g.stages * kWBytes;
+    g.park = g.b_off + b;
+    g.columns = tmem_columns(g.bn);
+    return g;
+  }
+  return g;
+}
+
+// Tokens per tile, K split and stages of a product with many rows. The tile width whose waves over the SMs (or pairs)
+// cost least, a wave counted as its tokens plus a constant for the channels' side of a chunk; ties go to the wider tile.
+// Pairs of CTAs where they fill the SMs; else single ones, K split over a cluster while that fills idle SMs.
+struct W8Plan {
+  int bn, splits, stages;
+  bool pair;
+};
+W8Plan w8_plan(int64_t M, int64_t N, int chunks, int sms) {
+  W8Plan best{256, 1, 4, false};
+  for (int pair = 1; pair >= 0; --pair) {
+    const int64_t tn = pair ? (N + 255) / 256 : (N + 127) / 128, slots = pair ? sms / 2 : sms;
+    int64_t cost = INT64_MAX, tiles = 0;
+    for (int bn = 256; bn >= 32; bn -= 32) {
+      const int64_t t = (M + bn - 1) / bn * tn, c = (t + slots - 1) / slots * (bn + 32);
+      if (c < cost) {
+        cost = c;
+        best.bn = bn;
+        tiles = t;
+      }
+    }
+    best.pair = pair != 0;
+    if (tiles >= slots) break;
+    if (!pair)
+      while (best.splits < kW8MaxSplits && tiles * (best.splits + 1) <= sms && chunks >= 2 * (best.splits + 1)) ++best.splits;
+  }
+  best.stages = min(kMaxStages, (kW8Smem - 1024 - kBarrierBytes) / (kWBytes + (best.pair ? best.bn / 2 : best.bn) * kChunk));
+  return best;
+}
+
+// One to eight rows that fit a CTA's shared memory beside others: every CTA quantizes all of them, so the rows' values
+// are bounded too
+bool gemv_takes(int64_t M, int64_t K) { return M <= kGemvRows && M * K <= 32768; }
+
+template <typename T>
+cudaError_t gemv_t(const W8Params& p, bool pdl, cudaStream_t st) {
+  const int pieces = (int)((p.K + 63) / 64), pitch = (pieces * 64 + 127) / 128 * 128 + 64;
+  const W8Gemv g{p.x, p.ldx, static_cast<const int8_t*>(p.w), p.ldw, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, (int)p.K,
+                 pieces, pitch};
+  const bool wide = pieces > 8 * kGemvRound || p.N < 4096;
+  return launch_w8(wide ? w8_gemv_kernel<T, 16> : w8_gemv_kernel<T, 8>, (unsigned)((p.N + 15) / 16), wide ? 512 : 256,
+                   (size_t)p.M * pitch, 1, pdl, st, g, 1);
 }
 
 template <typename T>
 cudaError_t linear_t(const W8Params& p, bool pdl, cudaStream_t st) {
+  if (gemv_takes(p.M, p.K)) return gemv_t<T>(p, pdl, st);
+  const int sms = sm_count();
+  const int64_t kp = padded(p.K);
+  const int chunks = (int)((kp + kChunk - 1) / kChunk);
+  CUtensorMap wmap, qmap;
+  if (!encode_rows(&wmap, p.w, kp, p.ldw, p.N, 128)) return cudaErrorInvalidValue;
+  if (p.M <= kSkinnyRows) {
+    W8Skinny g = skinny_plan(p.M, p.N, chunks, sms);
+    if (g.splits > 0) {
+      g.x = p.x, g.ldx = p.ldx, g.t = p.w_scales, g.bias = p.bias, g.y = p.y;
+      g.M = (int)p.M, g.N = (int)p.N, g.K = (int)p.K;
+      static std::atomic<uint64_t> done{0};
+      const cudaError_t e = allow_smem(w8_skinny_kernel<T>, done);
+      if (e != cudaSuccess) return e;
+      return launch_w8(w8_skinny_kernel<T>, (unsigned)((p.N + 127) / 128 * g.splits), kMmaThreads,
+                       (size_t)g.park + kSkinnyPark + 1024, g.splits, pdl, st, wmap, g);
+    }
+  }
   int8_t* q = static_cast<int8_t*>(p.workspace);
-  float* s = reinterpret_cast<float*>(q + p.M * p.ldw);
-  cudaError_t e = launch_w8(quantize_rows_kernel<T>, dim3((unsigned)p.M), dim3(kQThreads), 0, pdl, st,
-                            static_cast<const T*>(p.x), p.ldx, q, (int)p.ldw, s, (int)p.K);
+  float* s = reinterpret_cast<float*>(q + p.M * kp);
+  cudaError_t e = quantize_t<T>(p.x, p.ldx, q, kp, s, p.M, p.K, pdl, st);
   if (e != cudaSuccess) return e;
-  return launch_w8(w8_gemm_kernel<T>, dim3((unsigned)((p.N + 63) / 64), (unsigned)((p.M + 63) / 64)), dim3(256), 0,
-                   pdl, st, (const int8_t*)q, (const float*)s, static_cast<const int8_t*>(p.w), p.w_scales,
-                   static_cast<const T*>(p.bias), static_cast<T*>(p.y), (int)p.M, (int)p.N, (int)p.ldw);
+  const W8Plan plan = w8_plan(p.M, p.N, chunks, sms);
+  const int own_bn = plan.pair ? plan.bn / 2 : plan.bn, tile_n = plan.pair ? 256 : 128;
+  const int tiles_m = (int)((p.M + plan.bn - 1) / plan.bn), tiles = (int)((p.N + tile_n - 1) / tile_n) * tiles_m;
+  const int stride = tmem_columns(plan.bn), park = plan.stages * (kWBytes + own_bn * kChunk);
+  const W8Gemm g{s, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, chunks, plan.bn, tiles_m, tiles, plan.splits,
+                 plan.stages, plan.splits > 1 ? stride : 2 * stride, stride, park};
+  if (!encode_rows(&qmap, q, kp, kp, p.M, own_bn)) return cudaErrorInvalidValue;
+  const size_t smem = (size_t)park + kBarrierBytes + 1024;
+  if (plan.pair) {
+    static std::atomic<uint64_t> done{0};
+    if ((e = allow_smem(w8_gemm_kernel<T, true>, done)) != cudaSuccess) return e;
+    return launch_w8(w8_gemm_kernel<T, true>, (unsigned)(2 * min(tiles, sms / 2)), kMmaThreads, smem, 2, pdl, st, wmap, qmap, g);
+  }
+  static std::atomic<uint64_t> done{0};
+  if ((e = allow_smem(w8_gemm_kernel<T, false>, done)) != cudaSuccess) return e;
+  return launch_w8(w8_gemm_kernel<T, false>, (unsigned)(plan.splits > 1 ? tiles * plan.splits : min(tiles, sms)), kMmaThreads,
+                   smem, plan.splits, pdl, st, wmap, qmap, g);
 }
 
 }  // namespace
 
-size_t w8_workspace_bytes(int64_t M, int64_t N, int64_t ldw) { return (size_t)M * (size_t)ldw + (size_t)M * 4; }
+// none where the few-rows kernels quantize by themselves
+size_t w8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (gemv_takes(M, K)) return 0;
+  const int64_t kp = padded(K);
+  if (M <= kSkinnyRows && skinny_plan(M, N, (int)((kp + kChunk - 1) / kChunk), sm_count()).splits > 0) return 0;
+  return (size_t)M * (size_t)kp + (size_t)M * 4;
+}
 
 cudaError_t launch_w8_quantize_rows(const void* x, int dtype, int64_t ldx, int8_t* q, int64_t ldq, float* s, int64_t M,
                                     int64_t K, bool pdl, cudaStream_t st) {
-  const dim3 grid((unsigned)M), block(kQThreads);
-  switch (dtype) {
-    case 0:
-      return launch_w8(quantize_rows_kernel<__half>, grid, block, 0, pdl, st, static_cast<const __half*>(x), ldx, q,
-                       (int)ldq, s, (int)K);
-    case 1:
-      return launch_w8(quantize_rows_kernel<__nv_bfloat16>, grid, block, 0, pdl, st,
-                       static_cast<const __nv_bfloat16*>(x), ldx, q, (int)ldq, s, (int)K);
-    default:
-      return launch_w8(quantize_rows_kernel<float>, grid, block, 0, pdl, st, static_cast<const float*>(x), ldx, q,
-                       (int)ldq, s, (int)K);
-  }
+  return dtype == 0   ? quantize_t<__half>(x, ldx, q, ldq, s, M, K, pdl, st)
+         : dtype == 1 ? quantize_t<__nv_bfloat16>(x, ldx, q, ldq, s, M, K, pdl, st)
+                      : quantize_t<float>(x, ldx, q, ldq, s, M, K, pdl, st);
 }
 
 cudaError_t launch_w8_linear(const W8Params& p, bool pdl, cudaStream_t st) {

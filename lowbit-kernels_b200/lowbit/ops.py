@@ -382,9 +382,8 @@ def quantize_w8_gpu(w):
 
 
 class W8Weight:
-    """One linear layer's weight in 8-bit integers on the GPU: q int8 [N, K], scales fp32 [N] (W = q * scale). Rows
-    are kept a multiple of 16 bytes apart with zeros behind K; a q that already lies so (every K that is a multiple of
-    16, and what quantize_w8_gpu returns) is kept without a copy."""
+    """One linear layer's weight in 8-bit integers on the GPU: q int8 [N, K], scales fp32 [N] (W = q * scale). A q
+    whose K and row stride are multiples of 16 is kept without a copy, any other is laid out once with zeros behind K."""
 
     def __init__(self, q, scales):
         if not (isinstance(q, torch.Tensor) and isinstance(scales, torch.Tensor) and q.is_cuda):
@@ -444,7 +443,7 @@ def linear_w8(x, w8, bias=None, out=None):
     e = ext()
     w_ptr, s_ptr, _, n, k, ldw = w8._args
     with _Device(x.device):
-        need = e.lib.lb_w8_workspace(m, n, ldw)
+        need = e.lib.lb_w8_workspace(m, n, k)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
         rc = e.lib.lb_w8_linear(x.data_ptr(), DTYPE_IDS[x.dtype], x.stride(0) if m > 1 else k, w_ptr, ldw, s_ptr,
                                 None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, k,
