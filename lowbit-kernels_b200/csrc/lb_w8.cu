@@ -233,17 +233,21 @@ __global__ void __launch_bounds__(kQLongThreads)
 //     kernel (the quantization), whose rows follow after it.
 //   * MMA warp: one thread issues four K = 32 MMAs per chunk; a commit per chunk releases the stage, one per tile hands
 //     the accumulator to the epilogue. Two accumulators: the next tile's MMAs run under this tile's epilogue.
-//   * 8 epilogue warps, two per 32-lane quarter of tensor memory: a lane holds one channel (its scale and bias in
+//   * 16 epilogue warps, four per 32-lane quarter of tensor memory: a lane holds one channel (its scale and bias in
 //     registers), a column one token; a warp stores 64 consecutive bytes of an output row at a time.
 // CTAs are persistent over tiles, tokens innermost, so that the CTAs of one moment share weights in L2.
 // PAIR: two CTAs work on one tile of 256 channels (cta_group::2): each loads its 128 channels and half of the tokens, and
 // the leader's MMAs read both. A chunk then costs each SM 16 + BN / 16 KB of loads instead of 16 + BN / 8, and it is the
 // L2-to-SM path that bounds the single-CTA form: at BN = 224 it wants 100 bytes a clock and SM.
+// With `halves` = 2 a pair's tile is up to 512 tokens wide, in two accumulators that fill the tensor memory: 48 bytes a
+// clock and SM instead of 64 for 256 x 256, and the epilogue, which then only the next tile's loads run under, is short
+// beside a long K.
 // Few tiles and long K: a cluster of S single CTAs splits K, each parks its int32 partial tile in its (then idle) ring
 // and all sum their share through distributed shared memory -- exact, so the bits do not depend on S.
 constexpr int kChunk = 128;               // bytes of K per stage
 constexpr int kWBytes = 128 * kChunk;
-constexpr int kMmaThreads = 10 * 32;      // loader, MMA, 8 epilogue warps
+constexpr int kEpiWarps = 16;
+constexpr int kMmaThreads = (2 + kEpiWarps) * 32;   // loader, MMA, epilogue warps
 constexpr int kMaxStages = 8;
 constexpr int kW8MaxSplits = 8;           // portable cluster size
 constexpr int kW8Smem = 227 * 1024;
@@ -255,17 +259,11 @@ struct W8Gemm {
   const void* bias;
   void* y;
   int M, N, chunks;     // 128-byte chunks of K
-  int bn, tiles_m, tiles, splits, stages;
+  int bn, halves, tiles_m, tiles, splits, stages;
   int columns;          // tensor memory: 2 accumulators (persistent), or 1 (split)
   int acc_stride;       // columns between the accumulators
   int park;             // byte offset behind the ring: barriers and scales
 };
-
-__device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
 
 // This CTA's share of a cluster's outputs: the int32 partial tiles [token][128 channels] at the same offset of every
 // CTA's shared memory, summed, scaled and stored. A thread's four channels are the same in every round.
@@ -304,7 +302,7 @@ __device__ __forceinline__ void sum_partials(uint32_t red, const float* sc, cons
 }
 
 template <typename T, bool PAIR>
-__global__ void __launch_bounds__(kMmaThreads)
+__global__ void __launch_bounds__(kMmaThreads, 1)
     w8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap, const W8Gemm p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -316,6 +314,7 @@ __global__ void __launch_bounds__(kMmaThreads)
   float* sc = reinterpret_cast<float*>(slot + 4);   // [2][256] token scales
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int own_bn = PAIR ? p.bn / 2 : p.bn;        // tokens this CTA loads
+  const int H = PAIR ? p.halves : 1, acc_bn = p.bn / H, box = own_bn / H;
   const int stage_bytes = kWBytes + own_bn * kChunk, S = PAIR ? 1 : p.splits, St = p.stages;
   const int rank = PAIR || S > 1 ? (int)cluster_rank() : 0;
   const int group = PAIR ? 2 : S;
@@ -331,7 +330,7 @@ __global__ void __launch_bounds__(kMmaThreads)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], PAIR ? 16 : 8);
+      mbar_init(&acc_empty[i], PAIR ? 2 * kEpiWarps : kEpiWarps);
     }
     mbar_fence_init();
   }
@@ -354,117 +353,175 @@ __global__ void __launch_bounds__(kMmaThreads)
     if (lane == 0) {
       tma_prefetch_map(&wmap);
       tma_prefetch_map(&qmap);
-      const int mine = first < p.tiles ? (p.tiles - first + step - 1) / step : 0, total = mine * nc;
-      auto weights = [&](int i) {
-        const int n0 = (first + i / nc * step) / p.tiles_m * kTileN + n_off;
-        uint8_t* dst = ring + (i % St) * stage_bytes;
+      // counters instead of quotients: with the integer divisions of a running index this one thread took some 450
+      // clocks a chunk and bounded every shape
+      struct Place {
+        int tile, c, m0, n0;
+      };
+      auto at = [&](int tile) {
+        const int n = tile / p.tiles_m, m = tile - n * p.tiles_m;
+        return Place{tile, 0, m * p.bn + (PAIR ? rank * box : 0), n * kTileN + n_off};
+      };
+      auto next = [&](Place& q) {
+        if (++q.c == nc) q = at(q.tile + step);
+      };
+      auto weights = [&](const Place& q, int s) {
+        uint8_t* dst = ring + s * stage_bytes;
         if (PAIR) {
-          if (rank == 0) mbar_arrive_expect_tx(&full[i % St], 2 * stage_bytes);
-          tc::tma_load_2d_pair(dst, &wmap, (i % nc) * kChunk, n0, mapa_shared(smem_addr(&full[i % St]), 0));
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * stage_bytes);
+          tc::tma_load_2d_pair(dst, &wmap, q.c * kChunk, q.n0, mapa_shared(smem_addr(&full[s]), 0));
         } else {
-          mbar_arrive_expect_tx(&full[i % St], stage_bytes);
-          tma_load_2d(dst, &wmap, (c0 + i % nc) * kChunk, n0, &full[i % St]);
+          mbar_arrive_expect_tx(&full[s], stage_bytes);
+          tma_load_2d(dst, &wmap, (c0 + q.c) * kChunk, q.n0, &full[s]);
         }
       };
-      auto tokens = [&](int i) {
-        const int m0 = (first + i / nc * step) % p.tiles_m * p.bn + (PAIR ? rank * own_bn : 0);
-        uint8_t* dst = ring + (i % St) * stage_bytes + kWBytes;
+      auto tokens = [&](const Place& q, int s) {
+        uint8_t* dst = ring + s * stage_bytes + kWBytes;
         if (PAIR)
-          tc::tma_load_2d_pair(dst, &qmap, (i % nc) * kChunk, m0, mapa_shared(smem_addr(&full[i % St]), 0));
+          for (int h = 0; h < H; ++h)
+            tc::tma_load_2d_pair(dst + h * box * kChunk, &qmap, q.c * kChunk, q.m0 + h * acc_bn,
+                                 mapa_shared(smem_addr(&full[s]), 0));
         else
-          tma_load_2d(dst, &qmap, (c0 + i % nc) * kChunk, m0, &full[i % St]);
+          tma_load_2d(dst, &qmap, (c0 + q.c) * kChunk, q.m0, &full[s]);
       };
-      const int head = min(St, total);
-      for (int i = 0; i < head; ++i) weights(i);
+      Place w = at(first), q = w;
+      int head = 0;
+      for (; head < St && w.tile < p.tiles; ++head, next(w)) weights(w, head);
       pdl_wait();
-      for (int i = 0; i < head; ++i) tokens(i);
-      int issued = head;
-      for (int i = head; i < total; ++i) {
-        if (!wait_bounded(&empty[i % St], (i / St - 1) & 1, &g_w8_status)) break;
-        weights(i);
-        tokens(i);
-        issued = i + 1;
+      for (int s = 0; s < head; ++s, next(q)) tokens(q, s);
+      int s = 0, phase = 0;   // the stage to fill next, and the parity of its release
+      bool ok = true;
+      for (; q.tile < p.tiles; next(q)) {
+        ok = wait_bounded(&empty[s], phase, &g_w8_status);
+        if (!ok) break;
+        weights(q, s);
+        tokens(q, s);
+        if (++s == St) s = 0, phase ^= 1;
       }
-      if (rank == 0 || !PAIR)   // no copy in flight past this point (the leader's barriers count the peer's too)
-        for (int i = max(0, issued - St); i < issued; ++i) wait_bounded(&full[i % St], (i / St) & 1, &g_w8_status);
+      // no copy in flight past this point (a pair's leader's barriers count its peer's copies too): stage s holds the
+      // oldest of the last `head` copies, its parity is that of the release before it
+      if (rank == 0 || !PAIR)
+        for (int i = 0; i < head; ++i) {
+          wait_bounded(&full[s], phase, &g_w8_status);
+          if (++s == head) s = 0, phase ^= 1;
+        }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && (!PAIR || rank == 0)) {
+    // the whole warp runs the loop and one lane issues: in a loop of a single thread the descriptors' way into uniform
+    // registers made four MMAs and their waits cost 560 clocks, more than the 512 that they take at 256 tokens
+    if (!PAIR || rank == 0) {
       // int32 accumulator, signed 8-bit A and B, both K-major
       const uint32_t idesc =
-          (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kTileN >> 4) << 24);
-      int i = 0, a = 0;
+          (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(acc_bn >> 3) << 17) | ((uint32_t)(kTileN >> 4) << 24);
+      const uint64_t desc0 = tc::desc_sw128(smem_addr(ring), 16, 1024);   // the address field counts 16 bytes
+      const uint32_t hi = (uint32_t)(desc0 >> 32), lo0 = (uint32_t)desc0, half_step = (uint32_t)(box * kChunk) >> 4;
+      uint32_t lo = lo0;
+      int s = 0, phase = 0, a = 0;   // stage, its parity, accumulators used so far
       bool ok = true;
-      for (int tile = first; tile < p.tiles && ok; tile += step, ++a) {
-        if (a >= 2) ok = wait_bounded(&acc_empty[a & 1], ((a >> 1) - 1) & 1, &g_w8_status);
-        tc::fence_after();
-        const uint32_t d = tmem + (a & 1) * p.acc_stride;
-        for (int c = 0; c < nc && ok; ++c, ++i) {
-          ok = wait_bounded(&full[i % St], (i / St) & 1, &g_w8_status);
-          if (!ok) break;
-          tc::fence_after();
-          const uint32_t at = smem_addr(ring + (i % St) * stage_bytes);
+      for (int tile = first; tile < p.tiles && ok; tile += step, a += H) {
+        for (int c = 0; c < nc && ok; ++c) {
+          ok = wait_bounded(&full[s], phase, &g_w8_status);
+          for (int h = 0; h < H && ok; ++h) {
+            const int u = a + h;
+            if (c == 0 && u >= 2) ok = wait_bounded(&acc_empty[u & 1], ((u >> 1) - 1) & 1, &g_w8_status);
+            if (!ok) break;
+            tc::fence_after();
+            const uint32_t d = tmem + (u & 1) * p.acc_stride, lo_b = lo + (kWBytes >> 4) + h * half_step;
+            if (tc::elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint64_t ad = tc::desc_sw128(at + 32 * k, 16, 1024), bd = tc::desc_sw128(at + kWBytes + 32 * k, 16, 1024);
-            if (PAIR)
-              tc::mma_i8_ss_pair(d, ad, bd, idesc, c > 0 || k > 0);
-            else
-              tc::mma_i8_ss(d, ad, bd, idesc, c > 0 || k > 0);
+              for (int k = 0; k < 4; ++k) {
+                const uint64_t ad = (uint64_t)hi << 32 | (lo + 2 * k), bd = (uint64_t)hi << 32 | (lo_b + 2 * k);
+                if (PAIR)
+                  tc::mma_i8_ss_pair(d, ad, bd, idesc, c > 0 || k > 0);
+                else
+                  tc::mma_i8_ss(d, ad, bd, idesc, c > 0 || k > 0);
+              }
+              if (h == H - 1) {
+                if (PAIR)
+                  tc::commit_pair(&empty[s]);
+                else
+                  tc::commit(&empty[s]);
+                if (c == nc - 1)
+                  for (int e = 0; e < H; ++e) {
+                    if (PAIR)
+                      tc::commit_pair(&acc_full[(a + e) & 1]);
+                    else
+                      tc::commit(&acc_full[(a + e) & 1]);
+                  }
+              }
+            }
+            __syncwarp();
           }
-          if (PAIR)
-            tc::commit_pair(&empty[i % St]);
-          else
-            tc::commit(&empty[i % St]);
+          lo += (uint32_t)stage_bytes >> 4;
+          if (++s == St) s = 0, phase ^= 1, lo = lo0;
         }
-        if (PAIR)
-          tc::commit_pair(&acc_full[a & 1]);
-        else
-          tc::commit(&acc_full[a & 1]);
       }
       // no MMA in flight past this point
-      for (int b = max(0, a - 2); b < a; ++b) wait_bounded(&acc_full[b & 1], (b >> 1) & 1, &g_w8_status);
+      if (!ok) {   // a wait gave up: what has been issued hands its tile over as it is
+        if (tc::elect_one()) {
+          if (PAIR)
+            tc::commit_pair(&acc_full[a & 1]);
+          else
+            tc::commit(&acc_full[a & 1]);
+        }
+        __syncwarp();
+        wait_bounded(&acc_full[a & 1], (a >> 1) & 1, &g_w8_status);
+      } else
+        for (int b = max(0, a - 2); b < a; ++b) wait_bounded(&acc_full[b & 1], (b >> 1) & 1, &g_w8_status);
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = warp >= 6, row = 32 * quarter + lane, et = threadIdx.x - 64;
+    const int quarter = warp & 3, part = (warp - 2) >> 2, row = 32 * quarter + lane, et = threadIdx.x - 64;
     const uint32_t tlane = (uint32_t)(32 * quarter) << 16;
     const T* bias = static_cast<const T*>(p.bias);
     T* y = static_cast<T*>(p.y);
     pdl_wait();
-    int a = 0;
     bool ok = true;
-    for (int tile = first; tile < p.tiles && ok; tile += step, ++a) {
-      const int m0 = tile % p.tiles_m * p.bn, n = tile / p.tiles_m * kTileN + n_off + row;
+    const int mine = first < p.tiles ? (p.tiles - first + step - 1) / step : 0;
+    for (int a = 0; a < mine * H && ok; ++a) {
+      const int tile = first + a / H * step;
+      const int m0 = tile % p.tiles_m * p.bn + a % H * acc_bn, n = tile / p.tiles_m * kTileN + n_off + row;
       const bool on = n < p.N;
       float* scale = sc + (a & 1) * 256;
-      if (et < p.bn)
+      if (et < acc_bn)
         scale[et] = m0 + et < p.M ? __uint_as_float(ldg_cg_u32(reinterpret_cast<const uint32_t*>(p.s + m0 + et))) : 0.f;
       const float tn = on ? p.t[n] : 0.f, bn = on && bias ? Elem<T>::to_float(bias[n]) : 0.f;
-      named_barrier(1, 256);
+      named_barrier(1, 32 * kEpiWarps);
       ok = wait_bounded(&acc_full[a & 1], (a >> 1) & 1, &g_w8_status);
       __syncwarp();
       tc::fence_after();
-      for (int j0 = 16 * half; j0 < p.bn; j0 += 32) {
-        uint32_t v[16];
-        tc::ld16(tmem + tlane + (uint32_t)((a & 1) * p.acc_stride + j0), v);
-        tc::wait_ld();
+      // 16 columns at a time, the next ones on their way from tensor memory under this block's stores
+      const uint32_t acc = tmem + tlane + (uint32_t)((a & 1) * p.acc_stride);
+      constexpr int kStep = 4 * kEpiWarps;   // columns between a warp's blocks
+      uint32_t v[2][16];
+      if (16 * part < acc_bn) tc::ld16(acc + 16 * part, v[0]);
+      auto block = [&](int j0, const uint32_t (&w)[16]) {
         if (S == 1) {
           T* dst = y + (int64_t)(m0 + j0) * p.N + n;
           if (on && m0 + j0 + 16 <= p.M) {
 #pragma unroll
             for (int j = 0; j < 16; ++j, dst += p.N)
-              *dst = Elem<T>::from_float(fmaf(__int2float_rn((int)v[j]) * scale[j0 + j], tn, bn));
+              *dst = Elem<T>::from_float(fmaf(__int2float_rn((int)w[j]) * scale[j0 + j], tn, bn));
           } else if (on) {
 #pragma unroll
             for (int j = 0; j < 16; ++j, dst += p.N)
-              if (m0 + j0 + j < p.M) *dst = Elem<T>::from_float(fmaf(__int2float_rn((int)v[j]) * scale[j0 + j], tn, bn));
+              if (m0 + j0 + j < p.M) *dst = Elem<T>::from_float(fmaf(__int2float_rn((int)w[j]) * scale[j0 + j], tn, bn));
           }
         } else {
           int* red = reinterpret_cast<int*>(ring);   // [token][128 channels]
 #pragma unroll
-          for (int j = 0; j < 16; ++j) red[(j0 + j) * 128 + row] = (int)v[j];
+          for (int j = 0; j < 16; ++j) red[(j0 + j) * 128 + row] = (int)w[j];
+        }
+      };
+      for (int j0 = 16 * part; j0 < acc_bn; j0 += 2 * kStep) {
+        tc::wait_ld();
+        if (j0 + kStep < acc_bn) tc::ld16(acc + j0 + kStep, v[1]);
+        block(j0, v[0]);
+        if (j0 + kStep < acc_bn) {
+          tc::wait_ld();
+          if (j0 + 2 * kStep < acc_bn) tc::ld16(acc + j0 + 2 * kStep, v[0]);
+          block(j0 + kStep, v[1]);
         }
       }
       tc::fence_before();
@@ -498,193 +555,6 @@ __global__ void __launch_bounds__(kMmaThreads)
   }
 }
 
-// ------------------------------------------------------------------------------------------- the product, few rows
-// Up to 64 tokens in one launch: a decode batch is bound by the weights' way from memory and by latency, so the
-// quantization is done inside. The S CTAs of a cluster split K of one 128-channel tile; each
-//   * streams its K range of the weights into a stage ring from the start (weights do not wait for the activations),
-//   * reads its K range of the token rows, whose maxima the cluster exchanges through distributed shared memory,
-//   * writes the quantized bytes straight into the MMAs' swizzled B tiles (all of its K range stays resident),
-//   * multiplies, and sums the int32 partial tiles over the cluster.
-// Rows past the last token hold whatever was there: integers, and their columns are not stored.
-constexpr int kSkinnyRows = 64;
-constexpr int kSkinnyVecs = 12;
-
-struct W8Skinny {
-  const void* x;
-  int64_t ldx;
-  const float* t;
-  const void* bias;
-  void* y;
-  int M, N, K, chunks, bn, splits, stages;
-  int columns;
-  int b_off;        // bytes: the B tiles behind the ring
-  int park;         // barriers, maxima and scales behind those
-};
-constexpr int kSkinnyPark = (2 * kMaxStages + 2) * 8 + 16 + 2 * kSkinnyRows * 4;
-
-template <typename T>
-__global__ void __launch_bounds__(kMmaThreads) w8_skinny_kernel(const __grid_constant__ CUtensorMap wmap, const W8Skinny p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + p.park);
-  uint64_t* empty = full + kMaxStages;
-  uint64_t* tokens_ready = empty + kMaxStages;
-  uint64_t* acc_full = tokens_ready + 1;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(acc_full + 1);
-  uint32_t* maxima = slot + 4;                                   // [64], this CTA's K range
-  float* sc = reinterpret_cast<float*>(maxima + kSkinnyRows);    // [64] token scales
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int S = p.splits, St = p.stages, rank = S > 1 ? (int)cluster_rank() : 0;
-  const int n0 = blockIdx.x / S * 128;
-  const int c0 = p.chunks * rank / S, nc = p.chunks * (rank + 1) / S - c0;
-
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < St; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    mbar_init(tokens_ready, 8);
-    mbar_init(acc_full, 1);
-    mbar_fence_init();
-  }
-  if (threadIdx.x < kSkinnyRows) maxima[threadIdx.x] = 0u;
-  if (warp == 1) tc::alloc(slot, p.columns);
-  tc::fence_before();
-  __syncthreads();
-  tc::fence_after();
-  const uint32_t tmem = *slot;
-  pdl_launch_dependents();
-
-  if (warp == 0) {
-    // (the loader and the MMA warp have no maxima to give: they arrive for the exchange here and wait for it at their end)
-    if (S > 1) cluster_arrive();
-    if (lane == 0) {
-      tma_prefetch_map(&wmap);
-      run_loader(nc, St, full, empty, kWBytes, &g_w8_status, [&](int i, int st) {
-        tma_load_2d(ring + st * kWBytes, &wmap, (c0 + i) * kChunk, n0, &full[st]);
-      });
-    }
-    __syncwarp();
-    if (S > 1) cluster_wait();
-  } else if (warp == 1) {
-    if (S > 1) cluster_arrive();
-    if (lane == 0) {
-      const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | ((128u >> 4) << 24);
-      bool ok = wait_bounded(tokens_ready, 0, &g_w8_status);
-      for (int c = 0; c < nc && ok; ++c) {
-        ok = wait_bounded(&full[c % St], (c / St) & 1, &g_w8_status);
-        if (!ok) break;
-        tc::fence_after();
-        const uint32_t at = smem_addr(ring + (c % St) * kWBytes), bt = smem_addr(ring + p.b_off + c * p.bn * kChunk);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          tc::mma_i8_ss(tmem, tc::desc_sw128(at + 32 * k, 16, 1024), tc::desc_sw128(bt + 32 * k, 16, 1024), idesc,
-                        c > 0 || k > 0);
-        tc::commit(&empty[c % St]);
-      }
-      tc::commit(acc_full);
-      wait_bounded(acc_full, 0, &g_w8_status);   // no MMA in flight past this point
-    }
-    __syncwarp();
-    if (S > 1) cluster_wait();
-  } else {
-    const int quarter = warp & 3, half = warp >= 6, row = 32 * quarter + lane, n = n0 + row;
-    const T* bias = static_cast<const T*>(p.bias);
-    const bool on = n < p.N;
-    const float tn = on ? p.t[n] : 0.f, bn = on && bias ? Elem<T>::to_float(bias[n]) : 0.f;
-    const int k0 = c0 * kChunk, nv = nc * (kChunk / 8), left = p.K - k0;   // this CTA's vectors, and values left in a row
-    const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * sizeof(T))) & 15u) == 0;
-    const T* x = static_cast<const T*>(p.x) + k0;
-    pdl_wait();
-    // the M x nv vectors of 8 values, 256 neighbours at a time, 12 of a thread in flight; nv is a multiple of 16, so half
-    // a warp holds one row's. What fits in one round stays in registers until the maxima are known.
-    const int total = p.M * nv, et = threadIdx.x - 64;
-    Vec8<T> v[kSkinnyVecs];
-    auto fetch = [&](int base) {
-#pragma unroll
-      for (int i = 0; i < kSkinnyVecs; ++i) {
-        const int u = base + 256 * i + et;
-        if (u < total) v[i].load(x + u / nv * p.ldx + 8 * (u % nv), left - 8 * (u % nv), aligned);
-      }
-    };
-    for (int base = 0; base < total; base += 256 * kSkinnyVecs) {
-      fetch(base);
-#pragma unroll
-      for (int i = 0; i < kSkinnyVecs; ++i) {
-        const int u = base + 256 * i + et;
-        if (base + 256 * i >= total) break;
-        uint32_t a = u < total ? Vec8<T>::amax_float(v[i].amax(0u)) : 0u;
-        a = __reduce_max_sync(lane < 16 ? 0x0000ffffu : 0xffff0000u, a);
-        if ((lane & 15) == 0 && u < total) atomicMax(&maxima[u / nv], a);
-      }
-    }
-    __syncwarp();
-    if (S > 1)
-      cluster_sync_all();
-    else
-      named_barrier(1, 256);
-    if (et < p.M) {
-      uint32_t a = maxima[et];
-      for (int q = 0; q < S; ++q)
-        if (q != rank) a = max(a, ld_dsmem_u32(mapa_shared(smem_addr(maxima + et), (uint32_t)q)));
-      sc[et] = __uint_as_float(a);   // the maximum first; the scale takes its place below
-    }
-    named_barrier(1, 256);
-    for (int base = 0; base < total; base += 256 * kSkinnyVecs) {
-      if (total > 256 * kSkinnyVecs) fetch(base);
-#pragma unroll
-      for (int i = 0; i < kSkinnyVecs; ++i) {
-        const int u = base + 256 * i + et;
-        if (u < total) {
-          const int m = u / nv, j = u % nv, c = j >> 4, b = j & 15;   // row, chunk, 8-byte piece of its 128 bytes
-          float f[8];
-          v[i].get(f);
-          uint8_t* tile = ring + p.b_off + c * p.bn * kChunk;
-          *reinterpret_cast<uint2*>(tile + m * kChunk + (((b >> 1) ^ (m & 7)) << 4) + (b & 1) * 8) = quant8(f, row_scale(sc[m]));
-        }
-      }
-    }
-    tc::fence_async();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(tokens_ready);
-    named_barrier(1, 256);   // every maximum has been read
-    if (et < p.M) sc[et] = row_scale(sc[et]).s;
-    named_barrier(1, 256);
-    wait_bounded(acc_full, 0, &g_w8_status);
-    __syncwarp();
-    tc::fence_after();
-    for (int j0 = 16 * half; j0 < p.bn; j0 += 32) {
-      uint32_t v[16];
-      tc::ld16(tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)j0, v);
-      tc::wait_ld();
-      if (S == 1) {
-        T* dst = static_cast<T*>(p.y) + (int64_t)j0 * p.N + n;
-#pragma unroll
-        for (int j = 0; j < 16; ++j, dst += p.N)
-          if (on && j0 + j < p.M) *dst = Elem<T>::from_float(fmaf(__int2float_rn((int)v[j]) * sc[j0 + j], tn, bn));
-      } else {
-        int* red = reinterpret_cast<int*>(ring);   // [token][128 channels]
-#pragma unroll
-        for (int j = 0; j < 16; ++j) red[(j0 + j) * 128 + row] = (int)v[j];
-      }
-    }
-  }
-  __syncwarp();
-  if (S > 1) {
-    cluster_sync_all();
-    sum_partials<T>(smem_addr(ring), sc, p.t, static_cast<const T*>(p.bias), static_cast<T*>(p.y), n0, p.N, p.M, rank, S);
-  }
-  tc::fence_before();
-  if (S > 1)
-    cluster_sync_all();
-  else
-    __syncthreads();
-  if (warp == 1) {
-    tc::fence_after();
-    tc::dealloc(tmem, p.columns);
-  }
-}
-
 // ------------------------------------------------------------------------------------------- the product, one to eight rows
 // A CTA takes 16 channels and all of K: mma.sync m16n8k32 with the weights' fragments loaded straight into registers,
 // 64 bytes of K of a row per four lanes and 16-byte load (the order of k inside a fragment is free as long as both
@@ -693,7 +563,6 @@ __global__ void __launch_bounds__(kMmaThreads) w8_skinny_kernel(const __grid_con
 // memory; a cluster, tensor memory or a second launch would each add about a microsecond of latency to some four.
 constexpr int kGemvRows = 8;
 constexpr int kGemvRound = 4;    // 64-byte pieces of K of a warp in flight
-constexpr int kGemvVecs = 4;     // vectors of a token row that a thread keeps between the maximum and the quantization
 
 struct W8Gemv {
   const void* x;
@@ -714,7 +583,7 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <typename T, int NW>
+template <typename T, int NW, int MR>   // MR: the most rows, 1, 4 or 8
 __global__ void __launch_bounds__(32 * NW) w8_gemv_kernel(const W8Gemv p, int guard) {
   extern __shared__ __align__(16) uint8_t rows[];   // [M][pitch] quantized tokens
   __shared__ int part[NW][128];
@@ -742,39 +611,41 @@ __global__ void __launch_bounds__(32 * NW) w8_gemv_kernel(const W8Gemv p, int gu
   pdl_wait_after_loads(guard);
   const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * sizeof(T))) & 15u) == 0;
   const T* x = static_cast<const T*>(p.x);
-  const int nv = p.pieces * 8, total = p.M * nv;   // vectors of 8 values; eight lanes share a row
-  Vec8<T> v[kGemvVecs];
-  auto tokens = [&](int base) {
+  const int nv = p.pieces * 8;   // vectors of 8 values of a row
+  Vec8<T> v[MR];
+  auto tokens = [&](int j) {
 #pragma unroll
-    for (int i = 0; i < kGemvVecs; ++i) {
-      const int u = base + 32 * NW * i + tid;
-      if (u < total) v[i].load(x + u / nv * p.ldx + 8 * (u % nv), p.K - 8 * (u % nv), aligned);
-    }
+    for (int m = 0; m < MR; ++m)
+      if (m < p.M && j < nv) v[m].load(x + m * p.ldx + 8 * j, p.K - 8 * j, aligned);
   };
-  for (int base = 0; base < total; base += 32 * NW * kGemvVecs) {
-    tokens(base);
+  uint32_t mx[MR] = {};
+  for (int j = tid; j < nv; j += 32 * NW) {
+    tokens(j);
 #pragma unroll
-    for (int i = 0; i < kGemvVecs; ++i) {
-      const int u = base + 32 * NW * i + tid;
-      if (base + 32 * NW * i >= total) break;
-      uint32_t am = u < total ? Vec8<T>::amax_float(v[i].amax(0u)) : 0u;
-      am = __reduce_max_sync(0xffu << (lane & 24), am);
-      if ((lane & 7) == 0 && u < total) atomicMax(&maxima[u / nv], am);
-    }
+    for (int m = 0; m < MR; ++m)
+      if (m < p.M) mx[m] = v[m].amax(mx[m]);
   }
-  __syncthreads();
-  for (int base = 0; base < total; base += 32 * NW * kGemvVecs) {
-    if (total > 32 * NW * kGemvVecs) tokens(base);
 #pragma unroll
-    for (int i = 0; i < kGemvVecs; ++i) {
-      const int u = base + 32 * NW * i + tid;
-      if (u < total) {
-        const int m = u / nv;
-        float f[8];
-        v[i].get(f);
-        *reinterpret_cast<uint2*>(rows + m * p.pitch + 8 * (u % nv)) = quant8(f, row_scale(__uint_as_float(maxima[m])));
-      }
+  for (int m = 0; m < MR; ++m)
+    if (m < p.M) {
+      const uint32_t am = __reduce_max_sync(0xffffffffu, Vec8<T>::amax_float(mx[m]));
+      if (lane == 0) atomicMax(&maxima[m], am);
     }
+  __syncthreads();
+  const RowScale mine = row_scale(__uint_as_float(maxima[lane & 7]));
+  for (int j0 = 0; j0 < nv; j0 += 32 * NW) {
+    const int j = j0 + tid;
+    if (nv > 32 * NW) tokens(j);
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+      if (m < p.M) {
+        const RowScale rs{__shfl_sync(0xffffffffu, mine.up, m), __shfl_sync(0xffffffffu, mine.r, m), 0.f};
+        if (j < nv) {
+          float f[8];
+          v[m].get(f);
+          *reinterpret_cast<uint2*>(rows + m * p.pitch + 8 * j) = quant8(f, rs);
+        }
+      }
   }
   __syncthreads();
   int d[4] = {0, 0, 0, 0};
@@ -873,62 +744,75 @@ bool encode_rows(CUtensorMap* map, const void* base, int64_t width, int64_t ld, 
 
 int tmem_columns(int bn) { return bn <= 32 ? 32 : bn <= 64 ? 64 : bn <= 128 ? 128 : 256; }
 
-// Few rows: K split while the CTAs do not exceed two an SM and each keeps two chunks. Stages fill what shared memory a
-// second CTA of the SM leaves. splits 0: the token tiles do not fit.
-W8Skinny skinny_plan(int64_t M, int64_t N, int chunks, int sms) {
-  W8Skinny g = {};
-  g.bn = (int)(M + 15) / 16 * 16;
-  g.chunks = chunks;
-  const int tiles = (int)((N + 127) / 128);
-  int S = 1;
-  while (S < kW8MaxSplits && (int64_t)tiles * (S + 1) <= 2 * sms && chunks >= 2 * (S + 1)) ++S;
-  for (; S <= kW8MaxSplits && S <= chunks; ++S) {
-    const int nc = (chunks + S - 1) / S, b = nc * g.bn * kChunk, fixed = b + kSkinnyPark + 1024;
-    const int room = fixed + 3 * kWBytes <= kW8Smem / 2 ? kW8Smem / 2 - 1024 : kW8Smem;
-    g.stages = min(min(kMaxStages, nc), (room - fixed) / kWBytes);
-    if (g.stages < min(nc, 3)) continue;
-    if (S > 1 && g.stages * kWBytes < g.bn * 512) continue;   // the partial tile is parked in the ring
-    g.splits = S;
-    g.b_off = g.stages * kWBytes;
-    g.park = g.b_off + b;
-    g.columns = tmem_columns(g.bn);
-    return g;
-  }
-  return g;
-}
-
-// Tokens per tile, K split and stages of a product with many rows. The tile width whose waves over the SMs (or pairs)
-// cost least, a wave counted as its tokens plus a constant for the channels' side of a chunk; ties go to the wider tile.
-// Pairs of CTAs where they fill the SMs; else single ones, K split over a cluster while that fills idle SMs.
+// Tokens per tile, pairs or single CTAs, K split and stages: the candidate whose estimated time is least, in clocks per
+// CTA. A start and an end (measured 2.5 us of setup, first loads and last stores); per wave and 128-byte chunk the MMAs
+// (two clocks a token, but 450 at least, the issue's own time) and the loads at 64 bytes a clock -- both, since at large
+// sizes the power cap makes either cost the other's clock; the epilogue that nothing runs under; and a cluster's sum,
+// 1.5 us, where the cluster's CTAs can all be resident.
 struct W8Plan {
-  int bn, splits, stages;
+  int bn, halves, splits, stages;
   bool pair;
 };
-W8Plan w8_plan(int64_t M, int64_t N, int chunks, int sms) {
-  W8Plan best{256, 1, 4, false};
-  for (int pair = 1; pair >= 0; --pair) {
-    const int64_t tn = pair ? (N + 255) / 256 : (N + 127) / 128, slots = pair ? sms / 2 : sms;
-    int64_t cost = INT64_MAX, tiles = 0;
-    for (int bn = 256; bn >= 32; bn -= 32) {
-      const int64_t t = (M + bn - 1) / bn * tn, c = (t + slots - 1) / slots * (bn + 32);
-      if (c < cost) {
-        cost = c;
-        best.bn = bn;
-        tiles = t;
-      }
+
+template <typename T>
+int resident_clusters(int S) {   // of S single CTAs with the whole shared memory each, on the current device
+  static std::atomic<int> known[64][kW8MaxSplits + 1];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::atomic<int>& k = known[dev & 63][S];
+  int v = k.load(std::memory_order_relaxed);
+  if (v == 0) {
+    static std::atomic<uint64_t> done{0};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S);
+    cfg.blockDim = dim3(kMmaThreads);
+    cfg.dynamicSmemBytes = kW8Smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = S;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (allow_smem(w8_gemm_kernel<T, false>, done) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, w8_gemm_kernel<T, false>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
     }
-    best.pair = pair != 0;
-    if (tiles >= slots) break;
-    if (!pair)
-      while (best.splits < kW8MaxSplits && tiles * (best.splits + 1) <= sms && chunks >= 2 * (best.splits + 1)) ++best.splits;
+    v = n + 1;
+    k.store(v, std::memory_order_relaxed);
+  }
+  return v - 1;
+}
+
+template <typename T>
+W8Plan w8_plan(int64_t M, int64_t N, int chunks, int sms) {
+  W8Plan best{0, 1, 1, 0, false};
+  int64_t least = INT64_MAX;
+  auto consider = [&](int bn, bool pair, int S) {
+    const int64_t tiles = (M + bn - 1) / bn * (pair ? (N + 255) / 256 : (N + 127) / 128);
+    if (S > 1 && tiles > resident_clusters<T>(S)) return;
+    const int64_t ctas = tiles * (pair ? 2 : S), waves = (ctas + sms - 1) / sms;
+    const int64_t chunk = max(450, 2 * bn) + (kWBytes + (pair ? bn / 2 : bn) * kChunk) / 64;
+    const int64_t c = 4700 + waves * ((chunks + S - 1) / S) * chunk + (bn > 256 ? waves * 6 * bn : 6 * bn) + (S > 1 ? 2800 : 0);
+    if (c < least) {
+      least = c;
+      best.bn = bn, best.pair = pair, best.splits = S, best.halves = bn > 256 ? 2 : 1;
+    }
+  };
+  for (int bn = 512; bn >= 64; bn -= bn > 256 ? 64 : 32) consider(bn, true, 1);
+  for (int bn = 256; bn >= 16; bn -= 16) {
+    if (bn - 16 >= M) continue;   // wider than the tokens
+    for (int S = 1; S <= kW8MaxSplits && (S == 1 || chunks >= 2 * S); ++S) consider(bn, false, S);
   }
   best.stages = min(kMaxStages, (kW8Smem - 1024 - kBarrierBytes) / (kWBytes + (best.pair ? best.bn / 2 : best.bn) * kChunk));
   return best;
 }
 
-// One to eight rows that fit a CTA's shared memory beside others: every CTA quantizes all of them, so the rows' values
-// are bounded too
-bool gemv_takes(int64_t M, int64_t K) { return M <= kGemvRows && M * K <= 32768; }
+// One to eight rows, while their values are few: every CTA quantizes all of them. Measured, the GEMV against the two
+// launches: 11008 x 2048 M = 4 8.2 / 9.0 us, M = 8 13.5 / 9.0; 2048 x 11008 M = 1 8.0 / 8.9, M = 2 9.6 / 8.9;
+// 3584 x 18944 M = 1 25.7 / 15.5; 896 x 896 M = 8 3.7 / 5.5.
+bool gemv_takes(int64_t M, int64_t K) { return M <= kGemvRows && M * K <= 12288; }
 
 template <typename T>
 cudaError_t gemv_t(const W8Params& p, bool pdl, cudaStream_t st) {
@@ -936,8 +820,10 @@ cudaError_t gemv_t(const W8Params& p, bool pdl, cudaStream_t st) {
   const W8Gemv g{p.x, p.ldx, static_cast<const int8_t*>(p.w), p.ldw, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, (int)p.K,
                  pieces, pitch};
   const bool wide = pieces > 8 * kGemvRound || p.N < 4096;
-  return launch_w8(wide ? w8_gemv_kernel<T, 16> : w8_gemv_kernel<T, 8>, (unsigned)((p.N + 15) / 16), wide ? 512 : 256,
-                   (size_t)p.M * pitch, 1, pdl, st, g, 1);
+  auto kern = p.M == 1  ? (wide ? w8_gemv_kernel<T, 16, 1> : w8_gemv_kernel<T, 8, 1>)
+              : p.M <= 4 ? (wide ? w8_gemv_kernel<T, 16, 4> : w8_gemv_kernel<T, 8, 4>)
+                         : (wide ? w8_gemv_kernel<T, 16, 8> : w8_gemv_kernel<T, 8, 8>);
+  return launch_w8(kern, (unsigned)((p.N + 15) / 16), wide ? 512 : 256, (size_t)p.M * pitch, 1, pdl, st, g, 1);
 }
 
 template <typename T>
@@ -948,29 +834,24 @@ cudaError_t linear_t(const W8Params& p, bool pdl, cudaStream_t st) {
   const int chunks = (int)((kp + kChunk - 1) / kChunk);
   CUtensorMap wmap, qmap;
   if (!encode_rows(&wmap, p.w, kp, p.ldw, p.N, 128)) return cudaErrorInvalidValue;
-  if (p.M <= kSkinnyRows) {
-    W8Skinny g = skinny_plan(p.M, p.N, chunks, sms);
-    if (g.splits > 0) {
-      g.x = p.x, g.ldx = p.ldx, g.t = p.w_scales, g.bias = p.bias, g.y = p.y;
-      g.M = (int)p.M, g.N = (int)p.N, g.K = (int)p.K;
-      static std::atomic<uint64_t> done{0};
-      const cudaError_t e = allow_smem(w8_skinny_kernel<T>, done);
-      if (e != cudaSuccess) return e;
-      return launch_w8(w8_skinny_kernel<T>, (unsigned)((p.N + 127) / 128 * g.splits), kMmaThreads,
-                       (size_t)g.park + kSkinnyPark + 1024, g.splits, pdl, st, wmap, g);
-    }
-  }
   int8_t* q = static_cast<int8_t*>(p.workspace);
   float* s = reinterpret_cast<float*>(q + p.M * kp);
   cudaError_t e = quantize_t<T>(p.x, p.ldx, q, kp, s, p.M, p.K, pdl, st);
   if (e != cudaSuccess) return e;
-  const W8Plan plan = w8_plan(p.M, p.N, chunks, sms);
+  static thread_local struct {   // the last plan of this host thread: a layer's calls follow one another
+    int64_t M, N, chunks;
+    int sms;
+    W8Plan plan;
+  } last = {};
+  if (last.M != p.M || last.N != p.N || last.chunks != chunks || last.sms != sms)
+    last = {p.M, p.N, chunks, sms, w8_plan<T>(p.M, p.N, chunks, sms)};
+  const W8Plan plan = last.plan;
   const int own_bn = plan.pair ? plan.bn / 2 : plan.bn, tile_n = plan.pair ? 256 : 128;
   const int tiles_m = (int)((p.M + plan.bn - 1) / plan.bn), tiles = (int)((p.N + tile_n - 1) / tile_n) * tiles_m;
-  const int stride = tmem_columns(plan.bn), park = plan.stages * (kWBytes + own_bn * kChunk);
-  const W8Gemm g{s, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, chunks, plan.bn, tiles_m, tiles, plan.splits,
+  const int stride = tmem_columns(plan.bn / plan.halves), park = plan.stages * (kWBytes + own_bn * kChunk);
+  const W8Gemm g{s, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, chunks, plan.bn, plan.halves, tiles_m, tiles, plan.splits,
                  plan.stages, plan.splits > 1 ? stride : 2 * stride, stride, park};
-  if (!encode_rows(&qmap, q, kp, kp, p.M, own_bn)) return cudaErrorInvalidValue;
+  if (!encode_rows(&qmap, q, kp, kp, p.M, own_bn / plan.halves)) return cudaErrorInvalidValue;
   const size_t smem = (size_t)park + kBarrierBytes + 1024;
   if (plan.pair) {
     static std::atomic<uint64_t> done{0};
@@ -985,11 +866,10 @@ cudaError_t linear_t(const W8Params& p, bool pdl, cudaStream_t st) {
 
 }  // namespace
 
-// none where the few-rows kernels quantize by themselves
+// none where the product quantizes by itself
 size_t w8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   if (gemv_takes(M, K)) return 0;
   const int64_t kp = padded(K);
-  if (M <= kSkinnyRows && skinny_plan(M, N, (int)((kp + kChunk - 1) / kChunk), sm_count()).splits > 0) return 0;
   return (size_t)M * (size_t)kp + (size_t)M * 4;
 }
 
