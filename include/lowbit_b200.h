@@ -317,13 +317,17 @@ LB_API int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens
  * all). max_new / max_len: upper bounds of the new tokens and the context of any sequence (tokens and
  * table_width * page_size if unknown): a smaller value than the truth is an error that leaves outputs undefined but
  * stays inside every buffer. q's heads and tokens are strided (multiples of 8 elements), out's tokens too. hd 64 or
- * 128. Rows of the cache past a context may hold anything, NaN included.
+ * 128. Rows of the cache past a context may hold anything, NaN included. workspace:
+ * lb_paged_attention_workspace(...) bytes on the current device (0: none needed), 16-byte aligned, its content
+ * undefined before and after; calls that can overlap need distinct ones.
  */
+LB_API int64_t lb_paged_attention_workspace(int64_t tokens, int nh, const lb_paged_cache* cache, int64_t table_width,
+                                            int seqs, int64_t max_new, int64_t max_len);
 LB_API int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
                               const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride,
                               int64_t table_width, const int32_t* seq_lens, const int32_t* cu_new, int seqs,
                               int64_t max_new, int64_t max_len, float scale, void* out, int64_t out_token_stride,
-                              lb_stream_t stream);
+                              void* workspace, int64_t workspace_bytes, lb_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -694,10 +694,21 @@ int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens, int n
                   "paged_norm_rope_append");
 }
 
+int64_t lb_paged_attention_workspace(int64_t tokens, int nh, const lb_paged_cache* cache, int64_t table_width, int seqs,
+                                     int64_t max_new, int64_t max_len) {
+  if (!cache || tokens < 1 || nh < 1 || cache->nkv < 1 || nh % cache->nkv || table_width < 1 || seqs < 1 || max_new < 1 ||
+      max_len < 1)
+    return 0;
+  const int64_t width = table_width * cache->page_size;
+  return (int64_t)lb::paged_attention_workspace(seqs, nh, cache->nkv, cache->hd, max_new < tokens ? max_new : tokens,
+                                                max_len < width ? max_len : width);
+}
+
 int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
                        const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride, int64_t table_width,
                        const int32_t* seq_lens, const int32_t* cu_new, int seqs, int64_t max_new, int64_t max_len,
-                       float scale, void* out, int64_t out_token_stride, lb_stream_t stream) {
+                       float scale, void* out, int64_t out_token_stride, void* workspace,
+                       int64_t workspace_bytes, lb_stream_t stream) {
   int rc = check_cache(cache);
   if (rc) return rc;
   if (!q || !page_table || !seq_lens || !cu_new || !out) return fail(LB_ERR_ARGUMENT, "null pointer argument");
@@ -710,13 +721,18 @@ int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_str
   if (q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_token_stride < (int64_t)nh * cache->hd)
     return fail(LB_ERR_ARGUMENT, "q and out strides must be multiples of 8 elements");
   if (!aligned16(q) || !aligned16(out)) return fail(LB_ERR_ALIGNMENT, "q and out must be 16-byte aligned");
+  const int64_t need = lb_paged_attention_workspace(tokens, nh, cache, table_width, seqs, max_new, max_len);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(LB_ERR_ARGUMENT, "the workspace holds %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0),
+                (long long)need);
+  if (!aligned16(workspace)) return fail(LB_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
   if ((rc = check_device())) return rc;
   const int64_t width = table_width * cache->page_size;
   const lb::PagedAttnParams p{q, q_token_stride, q_head_stride, (int)tokens, nh, cache->nkv, cache->hd, cache->dtype,
                               cache->k, cache->v, cache->k_page_stride, cache->v_page_stride, cache->page_size,
                               cache->num_pages, page_table, table_stride, (int)table_width, seq_lens, cu_new, seqs,
                               (int)(max_new < tokens ? max_new : tokens), (int)(max_len < width ? max_len : width), scale,
-                              out, out_token_stride};
+                              out, out_token_stride, workspace};
   return launched(lb::launch_paged_attention(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)),
                   "paged_attention");
 }

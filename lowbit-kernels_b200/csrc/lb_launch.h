@@ -180,7 +180,11 @@ struct PagedAttnParams {
   float scale;
   void* out;                 // [tokens, nh, hd], tokens out_token elements apart
   int64_t out_token;
+  void* workspace;
+  float* work_ml = nullptr;  // parts of the workspace (lb_paged.cu)
+  float* work_o = nullptr;
 };
+size_t paged_attention_workspace(int64_t seqs, int nh, int nkv, int hd, int64_t max_new, int64_t max_len);
 cudaError_t launch_paged_attention(const PagedAttnParams& p, bool pdl, cudaStream_t st);
 int paged_device_error();   // synchronizes
 void paged_clear_device_error();

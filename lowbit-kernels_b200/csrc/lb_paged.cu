@@ -162,9 +162,11 @@ __global__ void __launch_bounds__(kAppendMaxThreads) append_kernel(const AppendP
 //     2^8 and most blocks cost one vote instead of shuffles and a rescale. Sums stay with their lane until the end.
 //   * keys no row sees are masked by selection and their V rows replaced by zeros: cache rows past a context may hold NaN.
 // The warps' (maximum, sum, O) are joined in shared memory, the CTAs' through distributed shared memory, in one fixed
-// order.
+// order. Few long contexts leave most SMs idle even so: then Z clusters share a context, and a second kernel joins their
+// parts from a workspace.
 constexpr int kFewWarps = 4;
-constexpr int kFewRows = 64;   // rows of a key head that go this way
+constexpr int kFewRows = 64;     // rows of a key head that go this way
+constexpr int kFewCluster = 8;
 
 template <typename T>
 __device__ __forceinline__ void mma_rows(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -209,25 +211,31 @@ __device__ __forceinline__ SeqSpan seq_span(const PagedAttnParams& p, int seq) {
 }
 
 template <typename T, int HD, int NT>   // NT: n-tiles of 8 query rows
-__global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const PagedAttnParams p, int row_tiles, int C) {
+__global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const PagedAttnParams p, int row_tiles, int C, int Z) {
   constexpr int kRows = 8 * NT, KI = HD / 32, VH = HD / 64;
-  __shared__ float part[kFewWarps][kRows][HD + 4];
-  __shared__ float part_m[kFewWarps][kRows], part_l[kFewWarps][kRows];
+  __shared__ __align__(16) float part[kFewWarps][kRows][HD + 4];
+  __shared__ float part_m[kFewWarps][kRows], part_l[kFewWarps][kRows], cta_m[kRows], cta_l[kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = C > 1 ? (int)cluster_rank() : 0;
   int item = blockIdx.x / C;
+  const int z = item % Z;
+  item /= Z;
+  const int work_row = item * kRows;   // this item's rows in the workspace
   const int rt = item % row_tiles;
   item /= row_tiles;
   const int kvh = item % p.nkv, seq = item / p.nkv, grp = p.nh / p.nkv;
   pdl_launch_dependents();
   pdl_wait();
+  const int32_t* table = p.table + (int64_t)seq * p.table_stride;
+  const int pages0 = lane < p.table_width ? table[lane] : 0;   // on its way together with the lengths
   const SeqSpan sp = seq_span(p, seq);
   const int rows = min(kRows, sp.n * grp - rt * kRows);   // of this tile (all the CTAs of a cluster agree)
   if (rows <= 0) return;
   const int row0 = rt * kRows;
   const int keys = min(sp.len, sp.len - sp.n + (row0 + rows - 1) / grp + 1);   // the last row's
   const int blocks = keys > 0 ? (keys + 15) / 16 : 0;
-  const int u0 = (int)((int64_t)blocks * rank / C), u1 = (int)((int64_t)blocks * (rank + 1) / C);
+  const int share = z * C + rank, shares = Z * C;
+  const int u0 = (int)((int64_t)blocks * share / shares), u1 = (int)((int64_t)blocks * (share + 1) / shares);
 
   // Q as the n-side operand, rows past the tile as zeros; the last key each of this lane's two rows per n-tile sees
   uint4 q[NT][KI];
@@ -253,12 +261,13 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
   first_masked = sp.len - sp.n + row0 / grp + 1;   // the first row's count of keys
   const float scale = p.scale * 1.44269504088896340736f;   // scores in powers of two
 
-  const int32_t* table = p.table + (int64_t)seq * p.table_stride;
   const int per_page = p.page_size / 16;
   const T* kbase = static_cast<const T*>(p.k) + (int64_t)kvh * p.page_size * HD;
   const T* vbase = static_cast<const T*>(p.v) + (int64_t)kvh * p.page_size * HD;
-  auto page_of = [&](int u) {
-    int pg = u < u1 ? table[u / per_page] : 0;
+  auto page_of = [&](int u, bool start) {   // start: the first lookups, which `pages0` may answer
+    const int at = u / per_page;
+    int pg = 0;
+    if (u < u1) pg = start && at < 32 ? __shfl_sync(0xffffffffu, pages0, at) : table[at];
     if (pg < 0 || pg >= p.num_pages) {
       atomicExch(&g_paged_status, kErrBadPosition);
       pg = 0;
@@ -291,7 +300,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
   for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
 
   int u = u0 + warp;
-  int page = page_of(u), page_next = page_of(u + kFewWarps);
+  int page = page_of(u, true), page_next = page_of(u + kFewWarps, true);
   if (u < u1) load_k(u, page);
   for (; u < u1; u += kFewWarps) {
     load_v(u, page);
@@ -307,7 +316,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
     }
     const int un = u + kFewWarps;
     page = page_next;
-    page_next = page_of(un + kFewWarps);
+    page_next = page_of(un + kFewWarps, false);
     if (un < u1) load_k(un, page);
     // scores in powers of two, unseen keys -inf; s[.][e] key g, row 2t + e; s[.][2 + e] key g + 8
     const bool masked = 16 * u + 16 > first_masked;
@@ -392,55 +401,124 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
     }
   __syncthreads();
   T* out = static_cast<T*>(p.out);
-  auto store = [&](int r, int d, float v) {
+  auto store = [&](int r, int d, const float4& v, float sum) {
     const int row = row0 + r;
-    out[(int64_t)(sp.t0 + row / grp) * p.out_token + (int64_t)(kvh * grp + row % grp) * HD + d] = Elem<T>::from_float(v);
+    const float c = sum > 0.f ? 1.f / sum : 0.f;
+    *reinterpret_cast<uint2*>(out + (int64_t)(sp.t0 + row / grp) * p.out_token + (int64_t)(kvh * grp + row % grp) * HD + d) =
+        make_uint2(Elem<T>::pack(v.x * c, v.y * c), Elem<T>::pack(v.z * c, v.w * c));
   };
-  // a thread takes the dims d, d + 128 mod HD of a row; the CTA's sum replaces warp 0's part
-  for (int e = threadIdx.x; e < rows * HD; e += 32 * kFewWarps) {
-    const int r = e / HD, d = e % HD;
+  // four dims of a row a thread; the CTA's sum replaces warp 0's part
+  for (int e = threadIdx.x; e < rows * (HD / 4); e += 32 * kFewWarps) {
+    const int r = e / (HD / 4), d = e % (HD / 4) * 4;
     float mx = part_m[0][r];
 #pragma unroll
     for (int w = 1; w < kFewWarps; ++w) mx = fmaxf(mx, part_m[w][r]);
-    float acc = 0.f, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kFewWarps; ++w) {
       const float c = part_m[w][r] == -INFINITY ? 0.f : exp2_fast(part_m[w][r] - mx);
-      acc += c * part[w][r][d];
+      const float4 x = *reinterpret_cast<const float4*>(&part[w][r][d]);
+      acc.x += c * x.x, acc.y += c * x.y, acc.z += c * x.z, acc.w += c * x.w;
       sum += c * part_l[w][r];
     }
-    if (C == 1)
-      store(r, d, sum > 0.f ? acc / sum : 0.f);
-    else
-      part[0][r][d] = acc;
+    if (C == 1) {
+      store(r, d, acc, sum);
+    } else {
+      *reinterpret_cast<float4*>(&part[0][r][d]) = acc;
+      if (d == 0) cta_m[r] = mx, cta_l[r] = sum;
+    }
   }
   if (C == 1) return;
-  __shared__ float cta_m[kRows], cta_l[kRows];
-  if (threadIdx.x < rows) {
-    const int r = threadIdx.x;
-    float mx = part_m[0][r], sum = 0.f;
-    for (int w = 1; w < kFewWarps; ++w) mx = fmaxf(mx, part_m[w][r]);
-    for (int w = 0; w < kFewWarps; ++w) sum += part_m[w][r] == -INFINITY ? 0.f : exp2_fast(part_m[w][r] - mx) * part_l[w][r];
-    cta_m[r] = mx;
-    cta_l[r] = sum;
-  }
   cluster_sync_all();
-  for (int e = rank * 32 * kFewWarps + threadIdx.x; e < rows * HD; e += C * 32 * kFewWarps) {
-    const int r = e / HD, d = e % HD;
+  for (int e = rank * 32 * kFewWarps + threadIdx.x; e < rows * (HD / 4); e += C * 32 * kFewWarps) {
+    const int r = e / (HD / 4), d = e % (HD / 4) * 4;
     const uint32_t am = smem_addr(&cta_m[r]), al = smem_addr(&cta_l[r]), ao = smem_addr(&part[0][r][d]);
-    float mx = -INFINITY, acc = 0.f, sum = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < C; ++k) mx = fmaxf(mx, ld_dsmem_f1(mapa_shared(am, k)));
-#pragma unroll 4
-    for (int k = 0; k < C; ++k) {
-      const float mk = ld_dsmem_f1(mapa_shared(am, k));
-      const float c = mk == -INFINITY ? 0.f : exp2_fast(mk - mx);
-      acc += c * ld_dsmem_f1(mapa_shared(ao, k));
-      sum += c * ld_dsmem_f1(mapa_shared(al, k));
+    float mk[kFewCluster], lk[kFewCluster];
+    float4 x[kFewCluster];
+#pragma unroll
+    for (int k = 0; k < kFewCluster; ++k)   // (all of them under way together)
+      if (k < C) {
+        mk[k] = ld_dsmem_f1(mapa_shared(am, k));
+        lk[k] = ld_dsmem_f1(mapa_shared(al, k));
+        x[k] = ld_dsmem_f4(mapa_shared(ao, k));
+      }
+    float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < kFewCluster; ++k)
+      if (k < C) mx = fmaxf(mx, mk[k]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kFewCluster; ++k)
+      if (k < C) {
+        const float c = mk[k] == -INFINITY ? 0.f : exp2_fast(mk[k] - mx);
+        acc.x += c * x[k].x, acc.y += c * x[k].y, acc.z += c * x[k].z, acc.w += c * x[k].w;
+        sum += c * lk[k];
+      }
+    if (Z == 1) {
+      store(r, d, acc, sum);
+    } else {
+      const int64_t at = (int64_t)(work_row + r) * Z + z;
+      *reinterpret_cast<float4*>(p.work_o + at * HD + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(p.work_ml + 2 * at) = make_float2(mx, sum);
     }
-    store(r, d, sum > 0.f ? acc / sum : 0.f);
   }
   cluster_sync_all();   // no CTA leaves while another still reads its part
+}
+
+// Joins the Z <= 32 parts of each row: work_o [item rows][Z][HD], work_ml [item rows][Z][2]. A CTA takes a row; its
+// threads hold four dims of every 512 / HD-th part, all loads under way at once.
+constexpr int kFewParts = 32;
+
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnParams p, int row_tiles, int Z) {
+  constexpr int kRows = 8 * NT, kGroups = 512 / HD, kHeld = kFewParts / kGroups;
+  __shared__ float4 sums[kGroups][HD / 4];
+  __shared__ float weights[kGroups];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t work_row = blockIdx.x;
+  const int group = threadIdx.x / (HD / 4), d = threadIdx.x % (HD / 4) * 4;
+  float2 ml[kHeld];
+  float4 x[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int k = group + i * kGroups;
+    if (k < Z) {
+      ml[i] = __ldcg(reinterpret_cast<const float2*>(p.work_ml + 2 * (work_row * Z + k)));
+      x[i] = __ldcg(reinterpret_cast<const float4*>(p.work_o + (work_row * Z + k) * HD + d));
+    }
+  }
+  float mx = (threadIdx.x & 31) < Z ? __ldcg(p.work_ml + 2 * (work_row * Z + (threadIdx.x & 31))) : -INFINITY;
+  int item = (int)(work_row / kRows);
+  const int row = item % row_tiles * kRows + (int)(work_row % kRows);
+  item /= row_tiles;
+  const int kvh = item % p.nkv, seq = item / p.nkv, grp = p.nh / p.nkv;
+  const SeqSpan sp = seq_span(p, seq);
+  if (row >= sp.n * grp) return;
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (group + i * kGroups < Z) {
+      const float c = ml[i].x == -INFINITY ? 0.f : exp2_fast(ml[i].x - mx);
+      acc.x += c * x[i].x, acc.y += c * x[i].y, acc.z += c * x[i].z, acc.w += c * x[i].w;
+      sum += c * ml[i].y;
+    }
+  sums[group][d / 4] = acc;
+  if (d == 0) weights[group] = sum;
+  __syncthreads();
+  if (group) return;
+  for (int k = 1; k < kGroups; ++k) {
+    const float4 v = sums[k][d / 4];
+    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+    sum += weights[k];
+  }
+  const float c = sum > 0.f ? 1.f / sum : 0.f;
+  T* dst = static_cast<T*>(p.out) + (int64_t)(sp.t0 + row / grp) * p.out_token + (int64_t)(kvh * grp + row % grp) * HD + d;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * c, acc.y * c), Elem<T>::pack(acc.z * c, acc.w * c));
 }
 
 // ---------------------------------------------------------------------------------------------------- attention
@@ -528,28 +606,74 @@ cudaError_t append_t(const AppendParams& p, bool pdl, cudaStream_t st) {
                       (size_t)a.tpb * p.F * sizeof(float2), pdl, st, a);
 }
 
-template <typename T, int HD, int NT>
-cudaError_t few_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
-  const int row_tiles = (int)(((int64_t)p.max_new * (p.nh / p.nkv) + 8 * NT - 1) / (8 * NT));
-  const int64_t items = (int64_t)p.seqs * p.nkv * row_tiles;
-  const int sms = sm_count(), blocks = (p.max_len + 15) / 16;
-  int C = 1;
-  while (C < 8 && items * C < 6 * sms && blocks > C * 2 * kFewWarps) C *= 2;
-  auto kern = attention_few_kernel<T, HD, NT>;
-  if (items * C < sms && blocks > 32 * kFewWarps) {   // few long contexts: a cluster beyond the portable size
-    static std::atomic<uint64_t> done{0};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const uint64_t bit = 1ull << (dev & 63);
-    if (!(done.load(std::memory_order_relaxed) & bit)) {
-      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return e;
-      done.fetch_or(bit, std::memory_order_relaxed);
+// CTAs of the few-rows kernel that can be resident at once in clusters of C, on the current device
+template <int HD, int NT>
+int few_resident(int C) {
+  static std::atomic<int> known[64][kFewCluster + 1];   // + 1; 0: not asked yet
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int v = known[dev & 63][C].load(std::memory_order_relaxed);
+  if (v == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(C);
+    cfg.blockDim = dim3(32 * kFewWarps);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, attention_few_kernel<__half, HD, NT>, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 2 * sm_count() / C;
     }
-    C = 16;
+    v = n * C + 1;
+    known[dev & 63][C].store(v, std::memory_order_relaxed);
   }
+  return v - 1;
+}
+
+// How few rows are laid out: tiles of 8 or 16 rows, clusters of C CTAs, Z clusters a context -- the choice whose estimated
+// time is least, in microseconds as measured: 4 to start and end a CTA, 1 a block of keys and warp, more where memory
+// bounds all CTAs' blocks together, 1 to join a cluster, 4 for the second kernel; CTAs past those resident at once come
+// in further rounds, with a quarter of a round of tail. A warp takes at most 48 blocks where a split can help it: contexts differ,
+// and the longest ends last.
+struct FewPlan {
+  int nt, row_tiles, C, Z;
+  int64_t items;
+};
+FewPlan few_plan(int64_t rows, int64_t seqs, int nkv, int hd, int64_t max_len) {
+  FewPlan f;
+  f.nt = rows <= 8 ? 1 : 2;
+  f.row_tiles = (int)((rows + 8 * f.nt - 1) / (8 * f.nt));
+  f.items = seqs * nkv * f.row_tiles;
+  const int64_t blocks = (max_len + 15) / 16;
+  double least = 1e30;
+  f.C = f.Z = 1;
+  for (int C = 1; C <= kFewCluster; ++C) {
+    const double resident = hd == 128 ? (f.nt == 1 ? few_resident<128, 1>(C) : few_resident<128, 2>(C))
+                                      : (f.nt == 1 ? few_resident<64, 1>(C) : few_resident<64, 2>(C));
+    for (int Z = 1; Z <= (C == kFewCluster ? kFewParts : 1); ++Z) {
+      if (C * Z > 1 && blocks < 2 * C * Z) break;
+      const int64_t turns = (blocks + C * Z * kFewWarps - 1) / (C * Z * kFewWarps);
+      const double ctas = (double)(f.items * C * Z), full = ctas / resident;
+      const double turn = max(1.0, min(ctas, resident) * kFewWarps * 16 * hd * 4 / 6.2e6);
+      double t = (full <= 1 ? 1 : full + 0.25) * (4 + turns * turn) + (C > 1) + (Z > 1 ? 4 : 0);
+      if (turns > 48) t += turns;
+      if (t < least) least = t, f.C = C, f.Z = Z;
+    }
+  }
+  return f;
+}
+
+template <typename T, int HD, int NT>
+cudaError_t few_t(PagedAttnParams p, const FewPlan& f, bool pdl, cudaStream_t st) {
+  const int64_t rows = f.items * 8 * NT;
+  p.work_ml = static_cast<float*>(p.workspace);
+  p.work_o = p.work_ml + (2 * rows * f.Z + 3) / 4 * 4;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(items * C));
+  cfg.gridDim = dim3((unsigned)(f.items * f.Z * f.C));
   cfg.blockDim = dim3(32 * kFewWarps);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -557,22 +681,30 @@ cudaError_t few_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
-  if (C > 1) {
+  const int joined_attrs = cfg.numAttrs;
+  if (f.C > 1) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[cfg.numAttrs].val.clusterDim.x = C;
+    attr[cfg.numAttrs].val.clusterDim.x = f.C;
     attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
   }
   cfg.attrs = attr;
-  return cudaLaunchKernelEx(&cfg, kern, p, row_tiles, C);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attention_few_kernel<T, HD, NT>, (const PagedAttnParams)p, f.row_tiles, f.C, f.Z);
+  if (e != cudaSuccess || f.Z == 1) return e;
+  cfg.gridDim = dim3((unsigned)rows);
+  cfg.blockDim = dim3(128);
+  cfg.numAttrs = joined_attrs;
+  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, HD, NT>, (const PagedAttnParams)p, f.row_tiles, f.Z);
 }
 
 template <typename T>
 cudaError_t attention_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   const int64_t most_rows = (int64_t)p.max_new * (p.nh / p.nkv);
-  if (most_rows <= kFewRows)
-    return p.hd == 128 ? (most_rows <= 8 ? few_t<T, 128, 1>(p, pdl, st) : few_t<T, 128, 2>(p, pdl, st))
-                       : (most_rows <= 8 ? few_t<T, 64, 1>(p, pdl, st) : few_t<T, 64, 2>(p, pdl, st));
+  if (most_rows <= kFewRows) {
+    const FewPlan f = few_plan(most_rows, p.seqs, p.nkv, p.hd, p.max_len);
+    return p.hd == 128 ? (f.nt == 1 ? few_t<T, 128, 1>(p, f, pdl, st) : few_t<T, 128, 2>(p, f, pdl, st))
+                       : (f.nt == 1 ? few_t<T, 64, 1>(p, f, pdl, st) : few_t<T, 64, 2>(p, f, pdl, st));
+  }
   const int64_t items = (int64_t)p.tokens * p.nh;
   return launch_paged(p.hd == 128 ? attention_kernel<T, 128> : attention_kernel<T, 64>,
                       dim3((unsigned)((items + 3) / 4)), dim3(128), 0, pdl, st, p);
@@ -586,6 +718,14 @@ cudaError_t launch_paged_append(const void* qkv, int64_t ld, int64_t tokens, int
   AppendParams p{qkv, ld, (int)tokens, nh, c.nkv, c.hd, rot / 2, q_norm, k_norm, eps, inv_freq, pos, slots, q_out,
                  c.k, c.v, c.k_page, c.v_page, c.num_pages * c.page_size, c.page_size, 1};
   return c.dtype == 0 ? append_t<__half>(p, pdl, st) : append_t<__nv_bfloat16>(p, pdl, st);
+}
+
+size_t paged_attention_workspace(int64_t seqs, int nh, int nkv, int hd, int64_t max_new, int64_t max_len) {
+  const int64_t rows = max_new * (nh / nkv);
+  if (rows > kFewRows) return 0;
+  const FewPlan f = few_plan(rows, seqs, nkv, hd, max_len);
+  if (f.Z == 1) return 0;
+  return (size_t)((2 * f.items * 8 * f.nt * f.Z + 3) / 4 * 4 + f.items * 8 * f.nt * f.Z * hd) * sizeof(float);
 }
 
 cudaError_t launch_paged_attention(const PagedAttnParams& p, bool pdl, cudaStream_t st) {

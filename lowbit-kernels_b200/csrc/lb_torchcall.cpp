@@ -247,9 +247,13 @@ PyObject* paged_attention(PyObject* const* args) {
   }
   at::Tensor y;
   if (!heads_out(args[9], dev, *q, t, nh, c->hd, &y)) Py_RETURN_NONE;
+  const int64_t need = lb_paged_attention_workspace(t, (int)nh, c, w, (int)s, bound[0], bound[1]);
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({need}, q->options().dtype(at::kByte));
   const int rc = lb_paged_attention(q->data_ptr(), t > 1 ? q->stride(0) : 0, nh > 1 ? q->stride(1) : 0, t, (int)nh, c, table->data_ptr<int32_t>(),
                                     s > 1 ? table->stride(0) : w, w, lens->data_ptr<int32_t>(), cu->data_ptr<int32_t>(),
-                                    (int)s, bound[0], bound[1], (float)scale, y.data_ptr(), nh * c->hd, stream_of(dev));
+                                    (int)s, bound[0], bound[1], (float)scale, y.data_ptr(), nh * c->hd,
+                                    need > 0 ? ws.data_ptr() : nullptr, need, stream_of(dev));
   return rc ? refused(rc) : result(args[9], y);
 }
 

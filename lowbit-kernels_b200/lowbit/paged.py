@@ -162,9 +162,12 @@ def attention(q, cache, page_table, seq_lens, cu_new, max_new=None, max_len=None
         return out
     e = ops.ext()
     with _Device(q.device):
+        need = e.lib.lb_paged_attention_workspace(t, nh, cache._ptr, width, s, max_new, max_len)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         rc = e.lib.lb_paged_attention(q.data_ptr(), t_stride, h_stride, t, nh, cache._ptr, page_table.data_ptr(),
                                       page_table.stride(0) if s > 1 else width, width, lens, cu, s, max_new, max_len,
                                       1 / math.sqrt(hd) if scale is None else scale, out.data_ptr(), nh * hd,
+                                      ws.data_ptr() if need else None, need,
                                       torch.cuda.current_stream().cuda_stream)
     if rc:
         e._raise(rc)

@@ -543,11 +543,14 @@ def test_paged_abi_refusals():
         assert append(**kw) == 1, kw
     assert append(k=A + 8) == 2
 
-    def attend(q=A, ts=256, hs=64, t=4, nh=4, width=3, stride=3, seqs=2, max_new=1, max_len=9, out=A, ots=256, **kw):
+    def attend(q=A, ts=256, hs=64, t=4, nh=4, width=3, stride=3, seqs=2, max_new=1, max_len=9, out=A, ots=256, ws=A,
+               wsb=1 << 40, **kw):
         return lib.lb_paged_attention(q, ts, hs, t, nh, cache(**kw), A, stride, width, A, A, seqs, max_new, max_len, 0.1, out,
-                                      ots, None)
+                                      ots, ws, wsb, None)
 
     for kw in (dict(q=None), dict(hd=32, k_page_stride=2 * 16 * 64), dict(nh=3), dict(nh=0), dict(t=0), dict(seqs=0), dict(width=0),
                dict(stride=2), dict(max_new=0), dict(max_len=0), dict(ts=100), dict(hs=60), dict(ots=128), dict(width=2 ** 30, stride=2 ** 30)):
         assert attend(**kw) == 1, kw
-    assert attend(q=A + 8) == 2 and attend(out=MIS) == 2
+    assert attend(q=A + 8) == 2 and attend(out=MIS) == 2 and attend(ws=A + 8) == 2
+    long = dict(seqs=1, width=4096, stride=4096, max_len=65536)
+    assert attend(wsb=0, **long) == 1 and "workspace" in message(lib)
