@@ -308,7 +308,7 @@ LB_API int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens
                                      void* q_out, lb_stream_t stream);
 
 /*
- * out[t, h] = softmax over the visible keys j of scale * q[t, h] . K[j, h / (nh / nkv)], times V. Sequence s has the
+ * out[t, h] = softmax over the visible keys j of scale * q[t, h] . K[j, h / (nh / nkv)], times V; scale > 0. Sequence s has the
  * new tokens cu_new[s] .. cu_new[s + 1] - 1 (cu_new int32 [seqs + 1], not decreasing, from 0; tokens past its last
  * value belong to no sequence and are left unwritten) and, them included, a context of seq_lens[s] tokens in the
  * cache; its new token i of n sees keys 0 .. seq_lens[s] - n + i. A token that sees none gets zeros. seq_lens above

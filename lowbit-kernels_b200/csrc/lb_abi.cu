@@ -718,6 +718,7 @@ int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_str
   if (table_width < 1 || table_stride < table_width || table_width * cache->page_size > INT32_MAX)
     return fail(LB_ERR_ARGUMENT, "page table: at least one page a row, contexts below 2^31");
   if (max_new < 1 || max_len < 1) return fail(LB_ERR_ARGUMENT, "max_new and max_len must be positive");
+  if (!(scale > 0.f) || scale > 1e30f) return fail(LB_ERR_ARGUMENT, "scale must be positive and finite");
   if (q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_token_stride < (int64_t)nh * cache->hd)
     return fail(LB_ERR_ARGUMENT, "q and out strides must be multiples of 8 elements");
   if (!aligned16(q) || !aligned16(out)) return fail(LB_ERR_ALIGNMENT, "q and out must be 16-byte aligned");

@@ -540,6 +540,18 @@ int sm_count() {
   return device_sms(dev);
 }
 
+bool encode_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const uint64_t (&extent)[3],
+                          const uint64_t (&stride_bytes)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swizzle) {
+  auto encode = tensor_map_encoder();
+  if (!encode) return false;
+  const cuuint64_t dims[3] = {extent[0], extent[1], extent[2]};
+  const cuuint64_t strides[2] = {stride_bytes[0], stride_bytes[1]};
+  const cuuint32_t boxes[3] = {box[0], box[1], box[2]};
+  const cuuint32_t estride[3] = {1, 1, 1};
+  return encode(map, type, 3, const_cast<void*>(base), dims, strides, boxes, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int gemm_tc05_splits(int M, int N, int K, int G, int forced) {
   if (M < 1 || M > 64 || K % 128 || G % 128 || K % G) return 0;
   int dev = 0;

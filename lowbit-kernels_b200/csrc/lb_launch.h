@@ -108,6 +108,10 @@ float* noalloc_attn_scratch();   // this device's scratch address (cudaGetSymbol
 bool encode_tensor_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
                           uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle);
 
+// the same in three dimensions
+bool encode_tensor_map_3d(CUtensorMap* map, CUtensorMapDataType type, const void* base, const uint64_t (&extent)[3],
+                          const uint64_t (&stride_bytes)[2], const uint32_t (&box)[3], CUtensorMapSwizzle swizzle);
+
 // tcgen05 skinny GEMM (lb_gemm_tc.cu), M <= 64: per 128-row tile a cluster of `splits` CTAs splitting K.
 // gemm_tc05_splits picks the split for a shape on the current device (forced > 0: that split, capped by the
 // cluster limit and the number of K chunks), 0 if the shape does not fit the kernel.

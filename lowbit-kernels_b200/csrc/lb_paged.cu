@@ -7,7 +7,7 @@
 #include <climits>
 
 #include "lb_launch.h"
-#include "lb_tma.cuh"
+#include "lb_tc.cuh"
 #include "lb_types.cuh"
 
 namespace lb {
@@ -521,62 +521,450 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnPara
   *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * c, acc.y * c), Elem<T>::pack(acc.z * c, acc.w * c));
 }
 
-// ---------------------------------------------------------------------------------------------------- attention
-// One warp per new token and query head: the keys in blocks of 32, one a lane; running maximum and sum.
+// ---------------------------------------------------------------------------------------- attention, chunks of tokens
+// tcgen05 with two 128-row tiles of one key head's queries (new tokens x heads that share it) a CTA, over 128 keys at a
+// time; one pass, running maximum and sum in registers, a query row per thread.
+//   * loader warp: K and V tiles alternate in one ring of stages; a tile is put together from its pages, one tensor copy
+//     per page (or part of a page: gcd(page size, 128) rows) and 128-byte half of a row, a lane each.
+//   * MMA warp: S_t = Q_t K^T (K-major operands) into tensor memory, O_t += P_t V with P_t, the A operand, in tensor memory
+//     over S_t's columns and V taken as it lies (MN-major B). PV of one tile and the next QK^T of the same tile are issued
+//     together, so that while one tile's softmax runs the tensor core works for the other.
+//   * two softmax warpgroups, one a tile: a thread reads its row's 128 scores at once, moves its running maximum only
+//     when one exceeds it by 8 in powers of two (weights stay below 2^8; else O would be rescaled in tensor memory every
+//     tile), writes the weights back as 16-bit pairs, and keeps their fp32 sum unrounded.
+// Masks are applied by selection and only in tiles that reach past the first row's last key. V rows past the context may
+// hold NaN, and 0 x NaN is NaN: the MMA warp zeroes them in shared memory before the last product.
+// Weights are rounded to the 16-bit type for the second product, as tensor cores take it; scores, maxima, sums and O are
+// fp32.
+// Few tiles: a cluster of C CTAs splits the keys; each parks O, maxima and sums in its idle ring and all join their share
+// of the rows through distributed shared memory, in one fixed order.
+constexpr int kTileKeys = 128;
+constexpr int kTileRows = 256;
+constexpr int kChunkThreads = 12 * 32;   // loader, MMA, two idle warps (a warpgroup boundary), 8 softmax warps
+constexpr int kChunkCluster = 8;
+
+template <int HD>
+struct ChunkSmem {
+  static constexpr int kHalves = HD / 64;
+  static constexpr int kStageBytes = kTileKeys * HD * 2;
+  static constexpr int kStages = HD == 128 ? 5 : 8;
+  static constexpr int kQ = kTileRows * HD * 2;
+  static constexpr int kBars = kQ + kStages * kStageBytes;                  // offset of the barriers
+  static constexpr int kSlot = kBars + (2 * kStages + 8) * 8;
+  static constexpr int kTotal = kSlot + 16 + 1024;                          // + alignment
+};
+
+struct ChunkParams {
+  PagedAttnParams a;
+  int piece;     // keys of one tensor copy
+  int tiles;     // row tiles of the grid per key head
+  int C;
+};
+
+// The grid's row tile x, counted over the sequences: its sequence and the tile in it (seq = -1: past the last). All
+// lanes of a warp call it.
+__device__ __forceinline__ int2 find_tile(const PagedAttnParams& p, int x, int grp) {
+  const int lane = threadIdx.x & 31;
+  for (int s0 = 0; s0 < p.seqs; s0 += 32) {
+    const int s = s0 + lane;
+    int n = 0;
+    if (s < p.seqs) {
+      const int t0 = max(0, p.cu_new[s]);
+      n = max(0, min(p.cu_new[s + 1], p.tokens) - t0);
+    }
+    const int mine = (int)(((int64_t)n * grp + kTileRows - 1) / kTileRows);
+    int sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, sum > x);
+    if (past) {
+      const int at = __ffs(past) - 1;
+      return make_int2(s0 + at, x - __shfl_sync(0xffffffffu, sum - mine, at));
+    }
+    x -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return make_int2(-1, 0);
+}
+
 template <typename T, int HD>
-__global__ void __launch_bounds__(128) attention_kernel(const PagedAttnParams p) {
-  __shared__ float qs[4][HD];
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                           const ChunkParams cp) {
+  using L = ChunkSmem<HD>;
+  constexpr int kHalves = L::kHalves, St = L::kStages;
+  constexpr uint32_t kHalfK = kTileKeys * 128, kHalfQ = 128 * 128;   // bytes of a 64-dim half of a tile
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  uint8_t* ring = smem + L::kQ;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* empty = full + St;
+  uint64_t* q_ready = empty + St;
+  uint64_t* s_full = q_ready + 1;
+  uint64_t* p_ready = s_full + 2;
+  uint64_t* o_done = p_ready + 2;
+  uint64_t* drain = o_done + 2;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kSlot);
+  float* row_m = reinterpret_cast<float*>(smem);   // [256] each, over Q, which no product reads any more by then
+  float* row_l = row_m + kTileRows;
+  const PagedAttnParams& p = cp.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int C = cp.C, rank = C > 1 ? (int)cluster_rank() : 0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < St; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(q_ready, 8);
+    mbar_init(drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) tc::alloc(slot, 512);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = *slot;
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + warp;
-  if (item >= (int64_t)p.tokens * p.nh) return;
-  const int t = (int)(item / p.nh), head = (int)(item % p.nh), kvh = head / (p.nh / p.nkv);
-  int seq = 0;
-  while (seq < p.seqs && p.cu_new[seq + 1] <= t) ++seq;
-  if (seq == p.seqs) return;
-  T* out = static_cast<T*>(p.out) + (int64_t)t * p.out_token + (int64_t)head * HD;
-  int len = 0;
-  if (t >= p.cu_new[seq]) len = min(p.seq_lens[seq], p.table_width * p.page_size) - (p.cu_new[seq + 1] - 1 - t);
-  const T* q = static_cast<const T*>(p.q) + t * p.q_token + head * p.q_head;
-  for (int d = lane; d < HD; d += 32) qs[warp][d] = Elem<T>::to_float(q[d]) * p.scale;
-  __syncwarp();
-  float m = -INFINITY, l = 0.f, o[HD / 32] = {};
-  for (int j0 = 0; j0 < len; j0 += 32) {
-    const int j = j0 + lane;
-    int64_t at = -1;
-    float sc = -INFINITY;
-    if (j < len) {
-      const int page = p.table[(int64_t)seq * p.table_stride + j / p.page_size];
-      if (page < 0 || page >= p.num_pages) {
-        atomicExch(&g_paged_status, kErrBadPosition);
-      } else {
-        at = ((int64_t)kvh * p.page_size + j % p.page_size) * HD;
-        const T* k = static_cast<const T*>(p.k) + page * p.k_page + at;
-        sc = 0.f;
-        for (int d = 0; d < HD; ++d) sc += qs[warp][d] * Elem<T>::to_float(k[d]);
-        at += page * p.v_page;
+
+  // heaviest tiles first: a sequence's later rows see more keys
+  const int grp = p.nh / p.nkv, item = blockIdx.x / C;
+  const int kvh = item % p.nkv;
+  const int2 at = find_tile(p, cp.tiles - 1 - item / p.nkv, grp);
+  const int seq = at.x, row0 = at.y * kTileRows;
+  SeqSpan sp = {0, 0, 0};
+  int rows = 0, keys = 0;
+  if (seq >= 0) {
+    sp = seq_span(p, seq);
+    rows = min(kTileRows, sp.n * grp - row0);
+    keys = max(0, min(sp.len, sp.len - sp.n + (row0 + rows - 1) / grp + 1));   // the last row's
+  }
+  const int key_tiles = (keys + kTileKeys - 1) / kTileKeys;
+  const int j0 = (int)((int64_t)key_tiles * rank / C), nt = (int)((int64_t)key_tiles * (rank + 1) / C) - j0;
+
+  if (warp == 0) {
+    if (seq >= 0 && nt > 0) {
+      if (lane == 0) {
+        tma_prefetch_map(&kmap);
+        tma_prefetch_map(&vmap);
+      }
+      // lane -> (piece, half); table entries one tile ahead
+      const int pieces = kTileKeys / cp.piece, piece = lane / kHalves, half = lane % kHalves;
+      const bool mine = piece < pieces;
+      const int32_t* table = p.table + (int64_t)seq * p.table_stride;
+      const int per_page = p.page_size / cp.piece;
+      const uint32_t dst0 = half * kHalfK + piece * cp.piece * 128;
+      auto lookup = [&](int j, int& page, int& row) {   // this lane's piece of key tile j
+        const int key = (j0 + j) * kTileKeys + piece * cp.piece;
+        page = -1;
+        if (mine && j < nt && key < keys) {
+          const int idx = key / cp.piece, tp = idx / per_page;
+          row = kvh * p.page_size + (idx - tp * per_page) * cp.piece;
+          page = table[tp];
+          if (page < 0 || page >= p.num_pages) {
+            if (half == 0) atomicExch(&g_paged_status, kErrBadPosition);
+            page = 0;
+          }
+        }
+      };
+      int page, row = 0, page_next, row_next = 0;
+      lookup(0, page, row);
+      int s = 0, phase = 0, filled = 0;
+      bool ok = true;
+      for (int j = 0; j < nt && ok; ++j) {
+        lookup(j + 1, page_next, row_next);
+        const int live = __popc(__ballot_sync(0xffffffffu, page >= 0));
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (filled >= St) ok = wait_bounded(&empty[s], phase, &g_paged_status);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&full[s], live * cp.piece * 128);
+          __syncwarp();
+          if (page >= 0)
+            tc::tma_load_3d(smem_addr(ring) + s * L::kStageBytes + dst0, kv ? &vmap : &kmap, 64 * half, row, page, &full[s]);
+          ++filled;
+          if (++s == St) s = 0, phase ^= filled > St;
+        }
+        page = page_next, row = row_next;
+      }
+      // no copy in flight past this point
+      const int last = min(filled, St);
+      for (int i = 0; i < last; ++i) {
+        const int f = filled - last + i;
+        wait_bounded(&full[f % St], (f / St) & 1, &g_paged_status);
       }
     }
-    float mx = sc;
+    __syncwarp();
+  } else if (warp == 1) {
+    if (seq >= 0 && nt > 0) {
+      constexpr uint32_t kType = Elem<T>::kBf16 ? (1u << 7) | (1u << 10) : 0u;
+      constexpr uint32_t kQK = (1u << 4) | kType | ((kTileKeys >> 3) << 17) | ((128u >> 4) << 24);
+      constexpr uint32_t kPV = (1u << 4) | kType | (1u << 16) | ((HD >> 3) << 17) | ((128u >> 4) << 24);   // B MN-major
+      const uint64_t kd = tc::desc_sw128(smem_addr(ring), 16, 1024), vd = tc::desc_sw128(smem_addr(ring), kHalfK, 1024);
+      const uint64_t qd = tc::desc_sw128(smem_addr(smem), 16, 1024);
+      constexpr uint32_t kStep = L::kStageBytes >> 4;
+      auto qk = [&](int t, int s) {
+        if (tc::elect_one()) {
 #pragma unroll
-    for (int o2 = 16; o2 > 0; o2 >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o2));
-    mx = fmaxf(mx, m);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    const float c = expf(m - base), pr = expf(sc - base);
-    l = l * c + warp_sum(pr);
-    m = mx;
+          for (int k = 0; k < HD / 16; ++k)
+            tc::mma_f16_ss(tmem + 128 * t, qd + ((t * kHalves * kHalfQ + (k / 4) * kHalfQ + (k % 4) * 32) >> 4),
+                           kd + s * kStep + (((k / 4) * kHalfK + (k % 4) * 32) >> 4), kQK, k > 0);
+          tc::commit(&s_full[t]);
+        }
+        __syncwarp();
+      };
+      bool ok = wait_bounded(q_ready, 0, &g_paged_status);
+      int s = 0, phase = 0;
+      auto next = [&] {
+        if (++s == St) s = 0, phase ^= 1;
+      };
+      if (ok) ok = wait_bounded(&full[0], 0, &g_paged_status);
+      tc::fence_after();
+      if (ok) {
+        qk(0, 0);
+        qk(1, 0);
+        if (tc::elect_one()) tc::commit(&empty[0]);
+        __syncwarp();
+        next();
+      }
+      for (int j = 0; j < nt && ok; ++j) {
+        const int sv = s, pv_phase = phase;
+        next();
+        const int sk = s, k_phase = phase;
+        const bool more = j + 1 < nt;
+        if (more) next();
+        ok = wait_bounded(&full[sv], pv_phase, &g_paged_status);
+        if (!ok) break;
+        const int tail = keys - (j0 + j) * kTileKeys;   // V rows of this tile that exist
+        if (tail < kTileKeys) {
+          for (int i = lane; i < (kTileKeys - tail) * 8 * kHalves; i += 32) {
+            const int half = i / ((kTileKeys - tail) * 8), e = i - half * (kTileKeys - tail) * 8;
+            *reinterpret_cast<uint4*>(ring + sv * L::kStageBytes + half * kHalfK + tail * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+          }
+          tc::fence_async();
+          __syncwarp();
+        }
 #pragma unroll
-    for (int i = 0; i < HD / 32; ++i) o[i] *= c;
-    for (int jj = 0; jj < 32; ++jj) {
-      const float pj = __shfl_sync(0xffffffffu, pr, jj);
-      const int64_t aj = __shfl_sync(0xffffffffu, at, jj);
-      if (aj < 0) continue;
+        for (int t = 0; t < 2; ++t) {
+          ok = wait_bounded(&p_ready[t], j & 1, &g_paged_status);
+          if (!ok) break;
+          tc::fence_after();
+          if (tc::elect_one()) {
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) o[i] += pj * Elem<T>::to_float(static_cast<const T*>(p.v)[aj + lane + 32 * i]);
+            for (int k = 0; k < kTileKeys / 16; ++k)
+              tc::mma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, vd + sv * kStep + ((k * 2048) >> 4), kPV,
+                             j > 0 || k > 0);
+            tc::commit(&o_done[t]);
+            if (t == 1) tc::commit(&empty[sv]);
+          }
+          __syncwarp();
+          if (more) {
+            if (t == 0) {
+              ok = wait_bounded(&full[sk], k_phase, &g_paged_status);
+              if (!ok) break;
+              tc::fence_after();
+            }
+            qk(t, sk);
+            if (t == 1) {
+              if (tc::elect_one()) tc::commit(&empty[sk]);
+              __syncwarp();
+            }
+          }
+        }
+      }
+      // no MMA in flight past this point
+      if (tc::elect_one()) tc::commit(drain);
+      __syncwarp();
+      wait_bounded(drain, 0, &g_paged_status);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int t = (warp - 4) >> 2, quarter = warp & 3, r = 128 * t + 32 * quarter + lane, row = row0 + r;
+    const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
+    const uint32_t ts = lane_base + 128 * t, to = lane_base + 256 + 128 * t;
+    const bool on = r < rows;
+    float m = -INFINITY, l = 0.f;
+    const float scale = p.scale * 1.44269504088896340736f;
+    const int last = on ? sp.len - sp.n + row / grp : -1;
+    const int64_t token = sp.t0 + row / grp, head = (int64_t)kvh * grp + row % grp;
+    if (seq >= 0 && nt > 0) {
+      const T* src = static_cast<const T*>(p.q) + token * p.q_token + head * p.q_head;
+      uint8_t* dst = smem + t * kHalves * kHalfQ + (32 * quarter + lane) * 128;
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) {
+        const uint4 v = on ? ldg_cg_u128(src + 8 * c) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst + (c / 8) * kHalfQ + (((c % 8) ^ (lane & 7)) << 4)) = v;
+      }
+      tc::fence_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+      const int first_last = sp.len - sp.n + row0 / grp;   // the CTA's first row's last key
+      bool ok = true;
+      for (int j = 0; j < nt && ok; ++j) {
+        ok = wait_bounded(&s_full[t], j & 1, &g_paged_status);
+        __syncwarp();
+        tc::fence_after();
+        uint32_t v[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc::ld32(ts + 32 * c, v[c]);
+        tc::wait_ld();
+        const int k0 = (j0 + j) * kTileKeys;
+        if (k0 + kTileKeys - 1 > first_last) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (k0 + 32 * c + i > last) v[c][i] = 0xFF800000u;   // -inf
+        }
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          mx[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+          for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][i]));
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+        if (__any_sync(0xffffffffu, top > m + 8.f)) {
+          const float mn = fmaxf(m, top);
+          const float c = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
+          m = mn;
+          l *= c;
+          if (j > 0) {   // the last product of this tile is complete before O is touched
+            wait_bounded(&o_done[t], (j - 1) & 1, &g_paged_status);
+            __syncwarp();
+            tc::fence_after();
+#pragma unroll
+            for (int h = 0; h < HD / 32; ++h) {
+              uint32_t o[32];
+              tc::ld32(to + 32 * h, o);
+              tc::wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
+              tc::st32(to + 32 * h, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t w[64];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float a = exp2_fast(fmaf(__uint_as_float(v[c][i]), scale, -base));
+            const float b = exp2_fast(fmaf(__uint_as_float(v[c][i + 1]), scale, -base));
+            sum[c] += a + b;
+            w[16 * c + i / 2] = Elem<T>::pack(a, b);
+          }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc::st32(ts, w);
+        tc::st32(ts + 32, w + 32);
+        tc::wait_st();
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[t]);
+      }
+      wait_bounded(&o_done[t], (nt - 1) & 1, &g_paged_status);
+      __syncwarp();
+      tc::fence_after();
+    }
+    if (C == 1) {
+      if (seq >= 0) {
+        T* dst = static_cast<T*>(p.out) + token * p.out_token + head * HD;
+        const float c = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+        for (int h = 0; h < HD / 32; ++h) {
+          uint32_t o[32];
+          if (nt > 0) {
+            tc::ld32(to + 32 * h, o);
+            tc::wait_ld();
+          }
+          if (on)
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = l > 0.f ? Elem<T>::pack(__uint_as_float(o[i + 2 * e]) * c, __uint_as_float(o[i + 2 * e + 1]) * c) : 0u;
+              *reinterpret_cast<uint4*>(dst + 32 * h + i) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+      }
+    } else {
+      // the second tile's last product is the last to read the ring
+      if (seq >= 0 && nt > 0) wait_bounded(&o_done[1], (nt - 1) & 1, &g_paged_status);
+      __syncwarp();
+      tc::fence_after();
+      // parked at ring + row * HD * 4, 16-byte pieces permuted by the row so that eight lanes' stores take all banks
+      row_m[r] = nt > 0 ? m : -INFINITY;
+      row_l[r] = nt > 0 ? l : 0.f;
+      if (seq >= 0 && nt > 0) {
+#pragma unroll
+        for (int h = 0; h < HD / 32; ++h) {
+          uint32_t o[32];
+          tc::ld32(to + 32 * h, o);
+          tc::wait_ld();
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(ring + r * HD * 4 + (((8 * h + i) ^ (r & 7)) << 4)) =
+                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
     }
   }
-  for (int i = 0; i < HD / 32; ++i) out[lane + 32 * i] = Elem<T>::from_float(l > 0.f ? o[i] / l : 0.f);
+  __syncwarp();
+  if (C > 1) {
+    cluster_sync_all();
+    if (warp >= 4 && seq >= 0) {
+      // a share of the rows a CTA, HD / 4 lanes a row
+      constexpr int kLanes = HD / 4;
+      const int c4 = (threadIdx.x - 128) % kLanes;
+      for (int r = rank * (256 / kLanes) + (threadIdx.x - 128) / kLanes; r < rows; r += C * (256 / kLanes)) {
+        float mk[kChunkCluster], lk[kChunkCluster];
+        float4 x[kChunkCluster];
+        const uint32_t am = smem_addr(row_m + r), al = smem_addr(row_l + r);
+        const uint32_t ao = smem_addr(ring) + r * HD * 4 + ((c4 ^ (r & 7)) << 4);
+#pragma unroll
+        for (int k = 0; k < kChunkCluster; ++k)
+          if (k < C) {
+            mk[k] = ld_dsmem_f1(mapa_shared(am, k));
+            lk[k] = ld_dsmem_f1(mapa_shared(al, k));
+            x[k] = ld_dsmem_f4(mapa_shared(ao, k));
+          }
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kChunkCluster; ++k)
+          if (k < C) mx = fmaxf(mx, mk[k]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kChunkCluster; ++k)
+          if (k < C && mk[k] != -INFINITY) {   // (a part without keys holds whatever its ring held)
+            const float c = exp2_fast(mk[k] - mx);
+            acc.x += c * x[k].x, acc.y += c * x[k].y, acc.z += c * x[k].z, acc.w += c * x[k].w;
+            sum += c * lk[k];
+          }
+        const float c = sum > 0.f ? 1.f / sum : 0.f;
+        const int row = row0 + r;
+        T* dst = static_cast<T*>(p.out) + (int64_t)(sp.t0 + row / grp) * p.out_token + ((int64_t)kvh * grp + row % grp) * HD + 4 * c4;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * c, acc.y * c), Elem<T>::pack(acc.z * c, acc.w * c));
+      }
+    }
+    cluster_sync_all();
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after();
+    tc::dealloc(tmem, 512);
+  }
 }
 
 template <typename Kern, typename P>
@@ -697,6 +1085,95 @@ cudaError_t few_t(PagedAttnParams p, const FewPlan& f, bool pdl, cudaStream_t st
   return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, HD, NT>, (const PagedAttnParams)p, f.row_tiles, f.Z);
 }
 
+int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+// Clusters of C CTAs of the chunk kernel that can be resident at once
+template <int HD>
+int chunk_resident(int C) {
+  static std::atomic<int> known[64][kChunkCluster + 1];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int v = known[dev & 63][C].load(std::memory_order_relaxed);
+  if (v == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(C);
+    cfg.blockDim = dim3(kChunkThreads);
+    cfg.dynamicSmemBytes = ChunkSmem<HD>::kTotal;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, attention_chunk_kernel<__half, HD>, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = max(1, (sm_count() - 16) / C);
+    }
+    v = n;
+    known[dev & 63][C].store(v, std::memory_order_relaxed);
+  }
+  return v;
+}
+
+template <typename T, int HD>
+cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
+  using L = ChunkSmem<HD>;
+  auto kern = attention_chunk_kernel<T, HD>;
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(done.load(std::memory_order_relaxed) & bit)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_chunk_kernel<__half, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
+    if (e != cudaSuccess) return e;
+    done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  ChunkParams cp;
+  cp.a = p;
+  cp.piece = gcd(p.page_size, kTileKeys);
+  const int64_t grp = p.nh / p.nkv;
+  // every sequence's last tile may be partial
+  cp.tiles = (int)min(p.seqs * ((p.max_new * grp + kTileRows - 1) / kTileRows), (p.tokens * grp + kTileRows - 1) / kTileRows + p.seqs);
+  const int64_t items = (int64_t)cp.tiles * p.nkv, key_tiles = (p.max_len + kTileKeys - 1) / kTileKeys;
+  // The cluster that costs least: rounds of CTAs times their key tiles (1.2 us each, measured) and 6 us to start and end,
+  // 3 more to join a cluster
+  double least = 1e30;
+  cp.C = 1;
+  for (int C = 1; C <= kChunkCluster && (C == 1 || key_tiles >= 2 * C); ++C) {
+    const int64_t resident = C == 1 ? sm_count() : chunk_resident<HD>(C), rounds = (items + resident - 1) / resident;
+    const double t = (double)rounds * (6 + (C > 1 ? 3 : 0) + 1.2 * (double)((key_tiles + C - 1) / C));
+    if (t < least) least = t, cp.C = C;
+  }
+  CUtensorMap kmap, vmap;
+  const CUtensorMapDataType type = Elem<T>::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const uint64_t extent[3] = {(uint64_t)HD, (uint64_t)p.nkv * p.page_size, (uint64_t)p.num_pages};
+  const uint32_t box[3] = {64, (uint32_t)cp.piece, 1};
+  const uint64_t ks[2] = {(uint64_t)HD * 2, (uint64_t)p.k_page * 2}, vs[2] = {(uint64_t)HD * 2, (uint64_t)p.v_page * 2};
+  if (!encode_tensor_map_3d(&kmap, type, p.k, extent, ks, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !encode_tensor_map_3d(&vmap, type, p.v, extent, vs, box, CU_TENSOR_MAP_SWIZZLE_128B))
+    return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(items * cp.C));
+  cfg.blockDim = dim3(kChunkThreads);
+  cfg.dynamicSmemBytes = L::kTotal;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  if (pdl) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cp.C > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cp.C;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.attrs = attr;
+  return cudaLaunchKernelEx(&cfg, kern, kmap, vmap, cp);
+}
+
 template <typename T>
 cudaError_t attention_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   const int64_t most_rows = (int64_t)p.max_new * (p.nh / p.nkv);
@@ -705,9 +1182,7 @@ cudaError_t attention_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
     return p.hd == 128 ? (f.nt == 1 ? few_t<T, 128, 1>(p, f, pdl, st) : few_t<T, 128, 2>(p, f, pdl, st))
                        : (f.nt == 1 ? few_t<T, 64, 1>(p, f, pdl, st) : few_t<T, 64, 2>(p, f, pdl, st));
   }
-  const int64_t items = (int64_t)p.tokens * p.nh;
-  return launch_paged(p.hd == 128 ? attention_kernel<T, 128> : attention_kernel<T, 64>,
-                      dim3((unsigned)((items + 3) / 4)), dim3(128), 0, pdl, st, p);
+  return p.hd == 128 ? chunk_t<T, 128>(p, pdl, st) : chunk_t<T, 64>(p, pdl, st);
 }
 
 }  // namespace

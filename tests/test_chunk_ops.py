@@ -486,7 +486,7 @@ def test_attention_refusals():
     for kw in (dict(q=q.bfloat16()), dict(q=q[..., :32]), dict(q=q[:, :3]), dict(q=q.cpu()), dict(q=q[0]),
                dict(page_table=table.long()), dict(page_table=table[0]), dict(page_table=table[:1]),
                dict(seq_lens=lens.long()), dict(seq_lens=lens[:1]), dict(cu_new=cu[:2]), dict(max_new=0), dict(max_len=0),
-               dict(out=torch.zeros(3, 4, 32, device="cuda", dtype=torch.float16))):
+               dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(out=torch.zeros(3, 4, 32, device="cuda", dtype=torch.float16))):
         with pytest.raises(RuntimeError):
             paged.attention(**{**ok, **kw})
     big = paged.PagedCache(2, 16, 1, 96)
