@@ -650,6 +650,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int key_tiles = (keys + kTileKeys - 1) / kTileKeys;
   const int j0 = (int)((int64_t)key_tiles * rank / C), nt = (int)((int64_t)key_tiles * (rank + 1) / C) - j0;
 
+  // 128 x 56 + 256 x 224 registers are the launch's 384 x 168: a softmax thread holds its row's 128 scores. (The
+  // warpgroups' paths do not meet again before the end: what follows a meeting has the fewer registers.)
+  if (warp < 4) {
+  tc::regs_dec<56>();
   if (warp == 0) {
     if (seq >= 0 && nt > 0) {
       if (lane == 0) {
@@ -786,7 +790,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       wait_bounded(drain, 0, &g_paged_status);
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  }
+  if (C > 1) {
+    cluster_sync_all();
+    cluster_sync_all();
+  }
+  } else {
+    tc::regs_inc<224>();
     const int t = (warp - 4) >> 2, quarter = warp & 3, r = 128 * t + 32 * quarter + lane, row = row0 + r;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
     const uint32_t ts = lane_base + 128 * t, to = lane_base + 256 + 128 * t;
@@ -919,11 +929,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
       }
     }
-  }
   __syncwarp();
   if (C > 1) {
     cluster_sync_all();
-    if (warp >= 4 && seq >= 0) {
+    if (seq >= 0) {
       // a share of the rows a CTA, HD / 4 lanes a row
       constexpr int kLanes = HD / 4;
       const int c4 = (threadIdx.x - 128) % kLanes;
@@ -958,6 +967,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
     }
     cluster_sync_all();
+  }
   }
   tc::fence_before();
   __syncthreads();
