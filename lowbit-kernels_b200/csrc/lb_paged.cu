@@ -533,24 +533,77 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnPara
 //     when one exceeds it by 8 in powers of two (weights stay below 2^8; else O would be rescaled in tensor memory every
 //     tile), writes the weights back as 16-bit pairs, and keeps their fp32 sum unrounded.
 // Masks are applied by selection and only in tiles that reach past the first row's last key. V rows past the context may
-// hold NaN, and 0 x NaN is NaN: the MMA warp zeroes them in shared memory before the last product.
+// hold NaN, and 0 x NaN is NaN: a third warp zeroes them in shared memory before the last product.
 // Weights are rounded to the 16-bit type for the second product, as tensor cores take it; scores, maxima, sums and O are
 // fp32.
 // Few tiles: a cluster of C CTAs splits the keys; each parks O, maxima and sums in its idle ring and all join their share
 // of the rows through distributed shared memory, in one fixed order.
+// two fp32 values in one 64-bit register pair
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of two values without the special-function unit: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves it
+// in the low bits), 2^f on [-1/2, 1/2] by a polynomial of least relative error (degree 3: 7.5e-5, under a bf16 weight's
+// rounding; degree 4: 2.6e-6 for fp16), n added to the exponent. x from -126; what lies below counts as 2^-126.
+template <typename T>
+__device__ __forceinline__ float2 exp2_poly(uint64_t x2) {
+  float2 x = unpair(x2);
+  x2 = pair(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const uint64_t t = add2(x2, pair(12582912.f, 12582912.f));
+  const uint64_t f = add2(x2, fma2(t, pair(-1.f, -1.f), pair(12582912.f, 12582912.f)));
+  uint64_t r;
+  if (Elem<T>::kBf16) {
+    r = fma2(f, pair(0.0551716648042202f, 0.0551716648042202f), pair(0.2426111251115799f, 0.2426111251115799f));
+    r = fma2(f, r, pair(0.6932609677314758f, 0.6932609677314758f));
+    r = fma2(f, r, pair(0.9999280571937561f, 0.9999280571937561f));
+  } else {
+    r = fma2(f, pair(0.009570101276040077f, 0.009570101276040077f), pair(0.05591785907745361f, 0.05591785907745361f));
+    r = fma2(f, r, pair(0.240247443318367f, 0.240247443318367f));
+    r = fma2(f, r, pair(0.6931217908859253f, 0.6931217908859253f));
+    r = fma2(f, r, pair(0.9999992847442627f, 0.9999992847442627f));
+  }
+  const float2 n = unpair(t), v = unpair(r);
+  return make_float2(__int_as_float(__float_as_int(v.x) + (__float_as_int(n.x) << 23)),
+                     __int_as_float(__float_as_int(v.y) + (__float_as_int(n.y) << 23)));
+}
+
 constexpr int kTileKeys = 128;
 constexpr int kTileRows = 256;
-constexpr int kChunkThreads = 12 * 32;   // loader, MMA, two idle warps (a warpgroup boundary), 8 softmax warps
+constexpr int kChunkThreads = 12 * 32;   // loader, MMA, tail and an idle warp (a warpgroup), 8 softmax warps
 constexpr int kChunkCluster = 8;
 
 template <int HD>
 struct ChunkSmem {
   static constexpr int kHalves = HD / 64;
+  static constexpr int kPoly = HD == 128 ? 5 : 7;   // of 16 weights, those by polynomial
   static constexpr int kStageBytes = kTileKeys * HD * 2;
   static constexpr int kStages = HD == 128 ? 5 : 8;
   static constexpr int kQ = kTileRows * HD * 2;
   static constexpr int kBars = kQ + kStages * kStageBytes;                  // offset of the barriers
-  static constexpr int kSlot = kBars + (2 * kStages + 8) * 8;
+  static constexpr int kSlot = kBars + (2 * kStages + 12) * 8;
   static constexpr int kTotal = kSlot + 16 + 1024;                          // + alignment
 };
 
@@ -603,9 +656,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* empty = full + St;
   uint64_t* q_ready = empty + St;
   uint64_t* s_full = q_ready + 1;
-  uint64_t* p_ready = s_full + 2;
-  uint64_t* o_done = p_ready + 2;
+  uint64_t* p_ready = s_full + 2;   // [part][tile]
+  uint64_t* o_done = p_ready + 4;
   uint64_t* drain = o_done + 2;
+  uint64_t* tail_go = drain + 1;
+  uint64_t* v_tail = drain + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kSlot);
   float* row_m = reinterpret_cast<float*>(smem);   // [256] each, over Q, which no product reads any more by then
   float* row_l = row_m + kTileRows;
@@ -620,9 +675,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     mbar_init(q_ready, 8);
     mbar_init(drain, 1);
+    mbar_init(tail_go, 1);
+    mbar_init(v_tail, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 4);
+      mbar_init(&p_ready[2 + i], 4);
       mbar_init(&o_done[i], 1);
     }
     mbar_fence_init();
@@ -708,7 +766,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (seq >= 0 && nt > 0) {
+    // one elected lane runs the whole loop: measured, eight MMAs with a wait and a commit issue in 570 clocks this way,
+    // 660 when the warp loops and elects at each group, 840 under `if (lane == 0)`; they take 512
+    if (seq >= 0 && nt > 0 && tc::elect_one()) {
       constexpr uint32_t kType = Elem<T>::kBf16 ? (1u << 7) | (1u << 10) : 0u;
       constexpr uint32_t kQK = (1u << 4) | kType | ((kTileKeys >> 3) << 17) | ((128u >> 4) << 24);
       constexpr uint32_t kPV = (1u << 4) | kType | (1u << 16) | ((HD >> 3) << 17) | ((128u >> 4) << 24);   // B MN-major
@@ -716,14 +776,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const uint64_t qd = tc::desc_sw128(smem_addr(smem), 16, 1024);
       constexpr uint32_t kStep = L::kStageBytes >> 4;
       auto qk = [&](int t, int s) {
-        if (tc::elect_one()) {
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k)
-            tc::mma_f16_ss(tmem + 128 * t, qd + ((t * kHalves * kHalfQ + (k / 4) * kHalfQ + (k % 4) * 32) >> 4),
-                           kd + s * kStep + (((k / 4) * kHalfK + (k % 4) * 32) >> 4), kQK, k > 0);
-          tc::commit(&s_full[t]);
-        }
-        __syncwarp();
+        for (int k = 0; k < HD / 16; ++k)
+          tc::mma_f16_ss(tmem + 128 * t, qd + ((t * kHalves * kHalfQ + (k / 4) * kHalfQ + (k % 4) * 32) >> 4),
+                         kd + s * kStep + (((k / 4) * kHalfK + (k % 4) * 32) >> 4), kQK, k > 0);
+        tc::commit(&s_full[t]);
       };
       bool ok = wait_bounded(q_ready, 0, &g_paged_status);
       int s = 0, phase = 0;
@@ -735,8 +792,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (ok) {
         qk(0, 0);
         qk(1, 0);
-        if (tc::elect_one()) tc::commit(&empty[0]);
-        __syncwarp();
+        tc::commit(&empty[0]);
         next();
       }
       for (int j = 0; j < nt && ok; ++j) {
@@ -746,30 +802,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const bool more = j + 1 < nt;
         if (more) next();
         ok = wait_bounded(&full[sv], pv_phase, &g_paged_status);
-        if (!ok) break;
-        const int tail = keys - (j0 + j) * kTileKeys;   // V rows of this tile that exist
-        if (tail < kTileKeys) {
-          for (int i = lane; i < (kTileKeys - tail) * 8 * kHalves; i += 32) {
-            const int half = i / ((kTileKeys - tail) * 8), e = i - half * (kTileKeys - tail) * 8;
-            *reinterpret_cast<uint4*>(ring + sv * L::kStageBytes + half * kHalfK + tail * 128 + e * 16) = make_uint4(0, 0, 0, 0);
-          }
-          tc::fence_async();
-          __syncwarp();
+        if (ok && keys - (j0 + j) * kTileKeys < kTileKeys) {   // the third warp's turn
+          mbar_arrive(tail_go);
+          ok = wait_bounded(v_tail, 0, &g_paged_status);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          ok = wait_bounded(&p_ready[t], j & 1, &g_paged_status);
-          if (!ok) break;
-          tc::fence_after();
-          if (tc::elect_one()) {
+        for (int t = 0; t < 2 && ok; ++t) {
 #pragma unroll
-            for (int k = 0; k < kTileKeys / 16; ++k)
+          for (int part = 0; part < 2 && ok; ++part) {
+            ok = wait_bounded(&p_ready[2 * part + t], j & 1, &g_paged_status);
+            if (!ok) break;
+            tc::fence_after();
+#pragma unroll
+            for (int k = part ? 6 : 0; k < (part ? 8 : 6); ++k)
               tc::mma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, vd + sv * kStep + ((k * 2048) >> 4), kPV,
                              j > 0 || k > 0);
-            tc::commit(&o_done[t]);
-            if (t == 1) tc::commit(&empty[sv]);
           }
-          __syncwarp();
+          if (!ok) break;
+          tc::commit(&o_done[t]);
+          if (t == 1) tc::commit(&empty[sv]);
           if (more) {
             if (t == 0) {
               ok = wait_bounded(&full[sk], k_phase, &g_paged_status);
@@ -777,17 +828,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               tc::fence_after();
             }
             qk(t, sk);
-            if (t == 1) {
-              if (tc::elect_one()) tc::commit(&empty[sk]);
-              __syncwarp();
-            }
+            if (t == 1) tc::commit(&empty[sk]);
           }
         }
       }
       // no MMA in flight past this point
-      if (tc::elect_one()) tc::commit(drain);
-      __syncwarp();
+      tc::commit(drain);
       wait_bounded(drain, 0, &g_paged_status);
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // the V rows behind the context in the last tile, zeroed once the tile has arrived
+    const int tail = keys - (j0 + nt - 1) * kTileKeys;
+    if (seq >= 0 && nt > 0 && tail < kTileKeys) {
+      const int fill = 2 * nt - 1;
+      wait_bounded(tail_go, 0, &g_paged_status);
+      uint8_t* tile = ring + (fill % St) * L::kStageBytes;
+      for (int half = 0; half < kHalves; ++half)
+        for (int i = lane; i < (kTileKeys - tail) * 8; i += 32)
+          *reinterpret_cast<uint4*>(tile + half * kHalfK + tail * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+      tc::fence_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_tail);
     }
     __syncwarp();
   }
@@ -837,11 +899,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         float mx[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          mx[c] = __uint_as_float(v[c][0]);
+          mx[c] = fmaxf(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
 #pragma unroll
-          for (int i = 1; i < 32; ++i) mx[c] = fmaxf(mx[c], __uint_as_float(v[c][i]));
+          for (int i = 2; i < 32; i += 2) mx[c] = max3(mx[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
         }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+        const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale;
         if (__any_sync(0xffffffffu, top > m + 8.f)) {
           const float mn = fmaxf(m, top);
           const float c = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
@@ -863,24 +925,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t w[64];
+        const uint64_t scale2 = pair(scale, scale), base2 = pair(-base, -base);
+        uint64_t sum = pair(0.f, 0.f);
+        // handed over in two parts: the products with the first 96 keys' V begin under the last weights
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float a = exp2_fast(fmaf(__uint_as_float(v[c][i]), scale, -base));
-            const float b = exp2_fast(fmaf(__uint_as_float(v[c][i + 1]), scale, -base));
-            sum[c] += a + b;
-            w[16 * c + i / 2] = Elem<T>::pack(a, b);
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t x = fma2(pair(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), scale2, base2);
+            float2 e;
+            if ((i * L::kPoly) % 16 < L::kPoly) {
+              e = exp2_poly<T>(x);
+            } else {
+              e = unpair(x);
+              e.x = exp2_fast(e.x), e.y = exp2_fast(e.y);
+            }
+            sum = add2(sum, pair(e.x, e.y));
+            w[i] = Elem<T>::pack(e.x, e.y);
           }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tc::st32(ts, w);
-        tc::st32(ts + 32, w + 32);
-        tc::wait_st();
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[t]);
+          tc::st16(ts + 16 * c, w);
+          if (c >= 2) {
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[2 * (c - 2) + t]);
+          }
+        }
+        const float2 both = unpair(sum);
+        l += both.x + both.y;
       }
       wait_bounded(&o_done[t], (nt - 1) & 1, &g_paged_status);
       __syncwarp();

@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   pdl_launch_dependents();
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (tc::elect_one()) {
       tma_prefetch_map(&wmap);
       tma_prefetch_map(&qmap);
       // counters instead of quotients: with the integer divisions of a running index this one thread took some 450
@@ -408,67 +408,52 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    // the whole warp runs the loop and one lane issues: in a loop of a single thread the descriptors' way into uniform
-    // registers made four MMAs and their waits cost 560 clocks, more than the 512 that they take at 256 tokens
-    if (!PAIR || rank == 0) {
+    // one elected lane runs the whole loop (measured, four MMAs with their wait and commit: under `if (lane == 0)` 560
+    // clocks, more than the 512 that they take at 256 tokens)
+    if ((!PAIR || rank == 0) && tc::elect_one()) {
       // int32 accumulator, signed 8-bit A and B, both K-major
       const uint32_t idesc =
           (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(acc_bn >> 3) << 17) | ((uint32_t)(kTileN >> 4) << 24);
       const uint64_t desc0 = tc::desc_sw128(smem_addr(ring), 16, 1024);   // the address field counts 16 bytes
-      const uint32_t hi = (uint32_t)(desc0 >> 32), lo0 = (uint32_t)desc0, half_step = (uint32_t)(box * kChunk) >> 4;
-      uint32_t lo = lo0;
+      const uint32_t half_step = (uint32_t)(box * kChunk) >> 4, stage_step = (uint32_t)stage_bytes >> 4;
       int s = 0, phase = 0, a = 0;   // stage, its parity, accumulators used so far
       bool ok = true;
       for (int tile = first; tile < p.tiles && ok; tile += step, a += H) {
         for (int c = 0; c < nc && ok; ++c) {
           ok = wait_bounded(&full[s], phase, &g_w8_status);
+          const uint64_t ad = desc0 + s * stage_step;
           for (int h = 0; h < H && ok; ++h) {
             const int u = a + h;
             if (c == 0 && u >= 2) ok = wait_bounded(&acc_empty[u & 1], ((u >> 1) - 1) & 1, &g_w8_status);
             if (!ok) break;
             tc::fence_after();
-            const uint32_t d = tmem + (u & 1) * p.acc_stride, lo_b = lo + (kWBytes >> 4) + h * half_step;
-            if (tc::elect_one()) {
+            const uint32_t d = tmem + (u & 1) * p.acc_stride;
+            const uint64_t bd = ad + (kWBytes >> 4) + h * half_step;
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint64_t ad = (uint64_t)hi << 32 | (lo + 2 * k), bd = (uint64_t)hi << 32 | (lo_b + 2 * k);
-                if (PAIR)
-                  tc::mma_i8_ss_pair(d, ad, bd, idesc, c > 0 || k > 0);
-                else
-                  tc::mma_i8_ss(d, ad, bd, idesc, c > 0 || k > 0);
-              }
-              if (h == H - 1) {
-                if (PAIR)
-                  tc::commit_pair(&empty[s]);
-                else
-                  tc::commit(&empty[s]);
-                if (c == nc - 1)
-                  for (int e = 0; e < H; ++e) {
-                    if (PAIR)
-                      tc::commit_pair(&acc_full[(a + e) & 1]);
-                    else
-                      tc::commit(&acc_full[(a + e) & 1]);
-                  }
-              }
+            for (int k = 0; k < 4; ++k) {
+              if (PAIR)
+                tc::mma_i8_ss_pair(d, ad + 2 * k, bd + 2 * k, idesc, c > 0 || k > 0);
+              else
+                tc::mma_i8_ss(d, ad + 2 * k, bd + 2 * k, idesc, c > 0 || k > 0);
             }
-            __syncwarp();
           }
-          lo += (uint32_t)stage_bytes >> 4;
-          if (++s == St) s = 0, phase ^= 1, lo = lo0;
+          if (!ok) break;
+          if (PAIR)
+            tc::commit_pair(&empty[s]);
+          else
+            tc::commit(&empty[s]);
+          if (++s == St) s = 0, phase ^= 1;
+        }
+        // (after a wait that gave up: what has been issued hands its tile over as it is)
+        for (int h = 0; h < H; ++h) {
+          if (PAIR)
+            tc::commit_pair(&acc_full[(a + h) & 1]);
+          else
+            tc::commit(&acc_full[(a + h) & 1]);
         }
       }
       // no MMA in flight past this point
-      if (!ok) {   // a wait gave up: what has been issued hands its tile over as it is
-        if (tc::elect_one()) {
-          if (PAIR)
-            tc::commit_pair(&acc_full[a & 1]);
-          else
-            tc::commit(&acc_full[a & 1]);
-        }
-        __syncwarp();
-        wait_bounded(&acc_full[a & 1], (a >> 1) & 1, &g_w8_status);
-      } else
-        for (int b = max(0, a - 2); b < a; ++b) wait_bounded(&acc_full[b & 1], (b >> 1) & 1, &g_w8_status);
+      for (int b = max(0, a - 2); b < a; ++b) wait_bounded(&acc_full[b & 1], (b >> 1) & 1, &g_w8_status);
     }
     __syncwarp();
   } else {
