@@ -600,7 +600,8 @@ struct ChunkSmem {
   static constexpr int kHalves = HD / 64;
   static constexpr int kPoly = HD == 128 ? 5 : 7;   // of 16 weights, those by polynomial
   static constexpr int kStageBytes = kTileKeys * HD * 2;
-  static constexpr int kStages = HD == 128 ? 5 : 8;
+  static constexpr int kDepth = HD == 128 ? 2 : 4;     // K and V tiles each in the ring
+  static constexpr int kStages = 2 * kDepth;
   static constexpr int kQ = kTileRows * HD * 2;
   static constexpr int kBars = kQ + kStages * kStageBytes;                  // offset of the barriers
   static constexpr int kSlot = kBars + (2 * kStages + 12) * 8;
@@ -685,11 +686,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     mbar_fence_init();
   }
-  if (warp == 1) tc::alloc(slot, 512);
+  if (warp == 1) tc::alloc(slot, 512);   // all there is: it starts at column 0
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const uint32_t tmem = *slot;
+  constexpr uint32_t tmem = 0;
   pdl_launch_dependents();
   pdl_wait();
 
@@ -766,75 +767,77 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    // one elected lane runs the whole loop: measured, eight MMAs with a wait and a commit issue in 570 clocks this way,
-    // 660 when the warp loops and elects at each group, 840 under `if (lane == 0)`; they take 512
+    // One elected lane runs the whole loop (measured, eight MMAs with a wait and a commit: 570 clocks this way, 660 when the
+    // warp loops and elects at each group, 840 under `if (lane == 0)`; they take 512). It shares its scheduler with two
+    // softmax warps, so an instruction costs it ten clocks: the ring is unrolled and every address a constant offset.
     if (seq >= 0 && nt > 0 && tc::elect_one()) {
       constexpr uint32_t kType = Elem<T>::kBf16 ? (1u << 7) | (1u << 10) : 0u;
       constexpr uint32_t kQK = (1u << 4) | kType | ((kTileKeys >> 3) << 17) | ((128u >> 4) << 24);
       constexpr uint32_t kPV = (1u << 4) | kType | (1u << 16) | ((HD >> 3) << 17) | ((128u >> 4) << 24);   // B MN-major
-      const uint64_t kd = tc::desc_sw128(smem_addr(ring), 16, 1024), vd = tc::desc_sw128(smem_addr(ring), kHalfK, 1024);
-      const uint64_t qd = tc::desc_sw128(smem_addr(smem), 16, 1024);
+      constexpr int D = L::kDepth;
       constexpr uint32_t kStep = L::kStageBytes >> 4;
-      auto qk = [&](int t, int s) {
+      uint32_t kd = (uint32_t)tc::desc_sw128(smem_addr(ring), 16, 1024);
+      uint32_t vd = (uint32_t)tc::desc_sw128(smem_addr(ring) + L::kStageBytes, kHalfK, 1024);
+      uint32_t qd = (uint32_t)tc::desc_sw128(smem_addr(smem), 16, 1024);
+      const uint32_t bars = smem_addr(full);
+      constexpr uint32_t kEmpty = 8 * St, kQReady = 16 * St, kSFull = kQReady + 8, kPReady = kSFull + 16, kODone = kPReady + 32,
+                         kDrain = kODone + 16, kTailGo = kDrain + 8, kVTail = kDrain + 16;
+      auto wait = [&](uint32_t off, uint32_t parity) { return wait_ready(bars + off, parity, &g_paged_status); };
+      auto qk = [&](int t, int d) {   // S_t = Q_t K^T with K stage d
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
           tc::mma_f16_ss(tmem + 128 * t, qd + ((t * kHalves * kHalfQ + (k / 4) * kHalfQ + (k % 4) * 32) >> 4),
-                         kd + s * kStep + (((k / 4) * kHalfK + (k % 4) * 32) >> 4), kQK, k > 0);
-        tc::commit(&s_full[t]);
+                         kd + 2 * d * kStep + (((k / 4) * kHalfK + (k % 4) * 32) >> 4), kQK, k > 0);
+        tc::commit_at(bars + kSFull + 8 * t);
       };
-      bool ok = wait_bounded(q_ready, 0, &g_paged_status);
-      int s = 0, phase = 0;
-      auto next = [&] {
-        if (++s == St) s = 0, phase ^= 1;
+      // tile j with V stage u, the next scores with K stage (u + 1) % D; false when a wait gave up
+      auto step = [&](int j, int u, uint32_t ring_parity, bool first, bool more) {
+        asm volatile("" : "+r"(kd), "+r"(vd), "+r"(qd));   // (or the compiler keeps every sum in a register of its own)
+        if (!wait(8 * (2 * u + 1), ring_parity)) return false;
+        if (!more && keys - (j0 + j) * kTileKeys < kTileKeys) {   // the third warp's turn
+          mbar_arrive(tail_go);
+          if (!wait(kVTail, 0)) return false;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            if (!wait(kPReady + 8 * (2 * part + t), u & 1)) return false;
+            tc::fence_after();
+#pragma unroll
+            for (int k = part ? 6 : 0; k < (part ? 8 : 6); ++k)
+              tc::mma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, vd + 2 * u * kStep + ((k * 2048) >> 4), kPV,
+                             !first || k > 0);
+          }
+          tc::commit_at(bars + kODone + 8 * t);
+          if (t == 1) tc::commit_at(bars + kEmpty + 8 * (2 * u + 1));
+          if (more) {
+            if (t == 0) {
+              if (!wait(8 * (2 * ((u + 1) % D)), u + 1 < D ? ring_parity : ring_parity ^ 1)) return false;
+              tc::fence_after();
+            }
+            qk(t, (u + 1) % D);
+            if (t == 1) tc::commit_at(bars + kEmpty + 8 * (2 * ((u + 1) % D)));
+          }
+        }
+        return true;
       };
-      if (ok) ok = wait_bounded(&full[0], 0, &g_paged_status);
+      bool ok = wait(kQReady, 0) && wait(0, 0);
       tc::fence_after();
       if (ok) {
         qk(0, 0);
         qk(1, 0);
-        tc::commit(&empty[0]);
-        next();
+        tc::commit_at(bars + kEmpty);
       }
-      for (int j = 0; j < nt && ok; ++j) {
-        const int sv = s, pv_phase = phase;
-        next();
-        const int sk = s, k_phase = phase;
-        const bool more = j + 1 < nt;
-        if (more) next();
-        ok = wait_bounded(&full[sv], pv_phase, &g_paged_status);
-        if (ok && keys - (j0 + j) * kTileKeys < kTileKeys) {   // the third warp's turn
-          mbar_arrive(tail_go);
-          ok = wait_bounded(v_tail, 0, &g_paged_status);
-        }
+      uint32_t parity = 0;
+      for (int j = 0; j < nt && ok; j += D, parity ^= 1) {
 #pragma unroll
-        for (int t = 0; t < 2 && ok; ++t) {
-#pragma unroll
-          for (int part = 0; part < 2 && ok; ++part) {
-            ok = wait_bounded(&p_ready[2 * part + t], j & 1, &g_paged_status);
-            if (!ok) break;
-            tc::fence_after();
-#pragma unroll
-            for (int k = part ? 6 : 0; k < (part ? 8 : 6); ++k)
-              tc::mma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, vd + sv * kStep + ((k * 2048) >> 4), kPV,
-                             j > 0 || k > 0);
-          }
-          if (!ok) break;
-          tc::commit(&o_done[t]);
-          if (t == 1) tc::commit(&empty[sv]);
-          if (more) {
-            if (t == 0) {
-              ok = wait_bounded(&full[sk], k_phase, &g_paged_status);
-              if (!ok) break;
-              tc::fence_after();
-            }
-            qk(t, sk);
-            if (t == 1) tc::commit(&empty[sk]);
-          }
-        }
+        for (int u = 0; u < D; ++u)
+          if (ok && j + u < nt) ok = step(j + u, u, parity, j + u == 0, j + u + 1 < nt);
       }
       // no MMA in flight past this point
-      tc::commit(drain);
-      wait_bounded(drain, 0, &g_paged_status);
+      tc::commit_at(bars + kDrain);
+      wait(kDrain, 0);
     }
     __syncwarp();
   } else if (warp == 2) {

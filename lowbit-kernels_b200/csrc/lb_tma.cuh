@@ -69,6 +69,23 @@ __device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, int
   return false;
 }
 
+// The same on a shared-memory address, for a thread whose instructions count: a completed barrier costs one test.
+__device__ __forceinline__ bool wait_ready(uint32_t bar, uint32_t parity, int* status) {
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  atomicExch(status, kErrBarrierTimeout);
+  return false;
+}
+
 // One loader thread streaming chunks 0..nc-1 through a stage ring: refills stage s once its consumers released it
 // (empty[s]), then waits for its own last copies so that none is in flight when the CTA exits.
 template <typename Issue>
