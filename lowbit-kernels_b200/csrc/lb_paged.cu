@@ -615,18 +615,19 @@ struct ChunkParams {
   int C;
 };
 
-// The grid's row tile x, counted over the sequences: its sequence and the tile in it (seq = -1: past the last). All
-// lanes of a warp call it.
-__device__ __forceinline__ int2 find_tile(const PagedAttnParams& p, int x, int grp) {
+// The grid's row tile x, counted over the sequences: its sequence (-1: past the last), the tile in it and the sequence's
+// tokens. All lanes of a warp call it.
+struct TilePlace {
+  int seq, tile;
+  SeqSpan span;
+};
+__device__ __forceinline__ TilePlace find_tile(const PagedAttnParams& p, int x, int grp) {
   const int lane = threadIdx.x & 31;
   for (int s0 = 0; s0 < p.seqs; s0 += 32) {
     const int s = s0 + lane;
-    int n = 0;
-    if (s < p.seqs) {
-      const int t0 = max(0, p.cu_new[s]);
-      n = max(0, min(p.cu_new[s + 1], p.tokens) - t0);
-    }
-    const int mine = (int)(((int64_t)n * grp + kTileRows - 1) / kTileRows);
+    SeqSpan sp = {0, 0, 0};
+    if (s < p.seqs) sp = seq_span(p, s);
+    const int mine = sp.n > 0 ? (int)(((int64_t)sp.n * grp + kTileRows - 1) / kTileRows) : 0;
     int sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -636,11 +637,18 @@ __device__ __forceinline__ int2 find_tile(const PagedAttnParams& p, int x, int g
     const uint32_t past = __ballot_sync(0xffffffffu, sum > x);
     if (past) {
       const int at = __ffs(past) - 1;
-      return make_int2(s0 + at, x - __shfl_sync(0xffffffffu, sum - mine, at));
+      return {s0 + at, x - __shfl_sync(0xffffffffu, sum - mine, at),
+              {__shfl_sync(0xffffffffu, sp.t0, at), __shfl_sync(0xffffffffu, sp.n, at), __shfl_sync(0xffffffffu, sp.len, at)}};
     }
     x -= __shfl_sync(0xffffffffu, sum, 31);
   }
-  return make_int2(-1, 0);
+  return {-1, 0, {0, 0, 0}};
+}
+
+// a lane's pointer, as every lane sees it
+template <typename T>
+__device__ __forceinline__ T* shfl_ptr(T* v, int lane) {
+  return reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), lane));
 }
 
 template <typename T, int HD>
@@ -697,12 +705,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   // heaviest tiles first: a sequence's later rows see more keys
   const int grp = p.nh / p.nkv, item = blockIdx.x / C;
   const int kvh = item % p.nkv;
-  const int2 at = find_tile(p, cp.tiles - 1 - item / p.nkv, grp);
-  const int seq = at.x, row0 = at.y * kTileRows;
-  SeqSpan sp = {0, 0, 0};
+  const TilePlace at = find_tile(p, cp.tiles - 1 - item / p.nkv, grp);
+  const int seq = at.seq, row0 = at.tile * kTileRows;
+  const SeqSpan sp = at.span;
   int rows = 0, keys = 0;
   if (seq >= 0) {
-    sp = seq_span(p, seq);
     rows = min(kTileRows, sp.n * grp - row0);
     keys = max(0, min(sp.len, sp.len - sp.n + (row0 + rows - 1) / grp + 1));   // the last row's
   }
@@ -870,13 +877,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const float scale = p.scale * 1.44269504088896340736f;
     const int last = on ? sp.len - sp.n + row / grp : -1;
     const int64_t token = sp.t0 + row / grp, head = (int64_t)kvh * grp + row % grp;
+    uint8_t* stage = smem + t * kHalves * kHalfQ + 32 * quarter * 128;   // the warp's rows of Q, swizzled
     if (seq >= 0 && nt > 0) {
-      const T* src = static_cast<const T*>(p.q) + token * p.q_token + head * p.q_head;
-      uint8_t* dst = smem + t * kHalves * kHalfQ + (32 * quarter + lane) * 128;
+      // the warp's 32 rows, HD / 8 lanes a row at a time (a row a lane took three times as long)
+      const T* mine = on ? static_cast<const T*>(p.q) + token * p.q_token + head * p.q_head : nullptr;
 #pragma unroll
-      for (int c = 0; c < HD / 8; ++c) {
-        const uint4 v = on ? ldg_cg_u128(src + 8 * c) : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + (c / 8) * kHalfQ + (((c % 8) ^ (lane & 7)) << 4)) = v;
+      for (int i = 0; i < HD / 8; ++i) {
+        const int rr = i * (256 / HD) + lane / (HD / 8), c = lane % (HD / 8);
+        const T* src = shfl_ptr(mine, rr);
+        const uint4 v = src ? ldg_cg_u128(src + 8 * c) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(stage + rr * 128 + (c / 8) * kHalfQ + (((c % 8) ^ (rr & 7)) << 4)) = v;
       }
       tc::fence_async();
       __syncwarp();
@@ -964,7 +974,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     if (C == 1) {
       if (seq >= 0) {
-        T* dst = static_cast<T*>(p.out) + token * p.out_token + head * HD;
+        // through the warp's rows of Q, which are done with, so that HD / 8 lanes store a row at a time
         const float c = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int h = 0; h < HD / 32; ++h) {
@@ -973,15 +983,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             tc::ld32(to + 32 * h, o);
             tc::wait_ld();
           }
-          if (on)
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint32_t w[4];
+          for (int i = 0; i < 4; ++i) {
+            uint32_t w[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = l > 0.f ? Elem<T>::pack(__uint_as_float(o[i + 2 * e]) * c, __uint_as_float(o[i + 2 * e + 1]) * c) : 0u;
-              *reinterpret_cast<uint4*>(dst + 32 * h + i) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            for (int e = 0; e < 4; ++e)
+              w[e] = l > 0.f ? Elem<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * c, __uint_as_float(o[8 * i + 2 * e + 1]) * c) : 0u;
+            const int piece = 4 * h + i;
+            *reinterpret_cast<uint4*>(stage + lane * 128 + (piece / 8) * kHalfQ + (((piece % 8) ^ (lane & 7)) << 4)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        __syncwarp();
+        T* mine = on ? static_cast<T*>(p.out) + token * p.out_token + head * HD : nullptr;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          const int rr = i * (256 / HD) + lane / (HD / 8), piece = lane % (HD / 8);
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + (piece / 8) * kHalfQ + (((piece % 8) ^ (rr & 7)) << 4));
+          T* dst = shfl_ptr(mine, rr);
+          if (dst) *reinterpret_cast<uint4*>(dst + 8 * piece) = v;
         }
       }
     } else {
@@ -1012,34 +1032,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       // a share of the rows a CTA, HD / 4 lanes a row
       constexpr int kLanes = HD / 4;
       const int c4 = (threadIdx.x - 128) % kLanes;
-      for (int r = rank * (256 / kLanes) + (threadIdx.x - 128) / kLanes; r < rows; r += C * (256 / kLanes)) {
-        float mk[kChunkCluster], lk[kChunkCluster];
-        float4 x[kChunkCluster];
-        const uint32_t am = smem_addr(row_m + r), al = smem_addr(row_l + r);
-        const uint32_t ao = smem_addr(ring) + r * HD * 4 + ((c4 ^ (r & 7)) << 4);
+      constexpr int kPass = 256 / kLanes, kAtOnce = 2;   // rows a pass, and passes under way together
+      for (int r0 = rank * kPass + (threadIdx.x - 128) / kLanes; r0 < rows; r0 += kAtOnce * C * kPass) {
+        float mk[kAtOnce][kChunkCluster], lk[kAtOnce][kChunkCluster];
+        float4 x[kAtOnce][kChunkCluster];
 #pragma unroll
-        for (int k = 0; k < kChunkCluster; ++k)
-          if (k < C) {
-            mk[k] = ld_dsmem_f1(mapa_shared(am, k));
-            lk[k] = ld_dsmem_f1(mapa_shared(al, k));
-            x[k] = ld_dsmem_f4(mapa_shared(ao, k));
-          }
-        float mx = -INFINITY, sum = 0.f;
+        for (int n = 0; n < kAtOnce; ++n) {
+          const int r = min(r0 + n * C * kPass, kTileRows - 1);
+          const uint32_t am = smem_addr(row_m + r), al = smem_addr(row_l + r);
+          const uint32_t ao = smem_addr(ring) + r * HD * 4 + ((c4 ^ (r & 7)) << 4);
 #pragma unroll
-        for (int k = 0; k < kChunkCluster; ++k)
-          if (k < C) mx = fmaxf(mx, mk[k]);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int k = 0; k < kChunkCluster; ++k)
+            if (k < C) {
+              mk[n][k] = ld_dsmem_f1(mapa_shared(am, k));
+              lk[n][k] = ld_dsmem_f1(mapa_shared(al, k));
+              x[n][k] = ld_dsmem_f4(mapa_shared(ao, k));
+            }
+        }
 #pragma unroll
-        for (int k = 0; k < kChunkCluster; ++k)
-          if (k < C && mk[k] != -INFINITY) {   // (a part without keys holds whatever its ring held)
-            const float c = exp2_fast(mk[k] - mx);
-            acc.x += c * x[k].x, acc.y += c * x[k].y, acc.z += c * x[k].z, acc.w += c * x[k].w;
-            sum += c * lk[k];
-          }
-        const float c = sum > 0.f ? 1.f / sum : 0.f;
-        const int row = row0 + r;
-        T* dst = static_cast<T*>(p.out) + (int64_t)(sp.t0 + row / grp) * p.out_token + ((int64_t)kvh * grp + row % grp) * HD + 4 * c4;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * c, acc.y * c), Elem<T>::pack(acc.z * c, acc.w * c));
+        for (int n = 0; n < kAtOnce; ++n) {
+          const int r = r0 + n * C * kPass, row = row0 + r;
+          if (r >= rows) break;
+          float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int k = 0; k < kChunkCluster; ++k)
+            if (k < C) mx = fmaxf(mx, mk[n][k]);
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < kChunkCluster; ++k)
+            if (k < C && mk[n][k] != -INFINITY) {   // (a part without keys holds whatever its ring held)
+              const float c = exp2_fast(mk[n][k] - mx);
+              acc.x += c * x[n][k].x, acc.y += c * x[n][k].y, acc.z += c * x[n][k].z, acc.w += c * x[n][k].w;
+              sum += c * lk[n][k];
+            }
+          const float c = sum > 0.f ? 1.f / sum : 0.f;
+          T* dst = static_cast<T*>(p.out) + (int64_t)(sp.t0 + row / grp) * p.out_token + ((int64_t)kvh * grp + row % grp) * HD + 4 * c4;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * c, acc.y * c), Elem<T>::pack(acc.z * c, acc.w * c));
+        }
       }
     }
     cluster_sync_all();
