@@ -598,9 +598,9 @@ constexpr int kChunkCluster = 8;
 template <int HD>
 struct ChunkSmem {
   static constexpr int kHalves = HD / 64;
-  static constexpr int kPoly = HD == 128 ? 5 : 7;   // of 16 weights, those by polynomial
+  static constexpr int kPoly = HD == 128 ? 5 : 4;   // of 16 weights, those by polynomial (0, 3, 4, 5, 7, 8 tried)
   static constexpr int kStageBytes = kTileKeys * HD * 2;
-  static constexpr int kDepth = HD == 128 ? 2 : 4;     // K and V tiles each in the ring
+  static constexpr int kDepth = 2;     // K and V tiles each in the ring (4 at hd 64: a longer loop, 6 % slower)
   static constexpr int kStages = 2 * kDepth;
   static constexpr int kQ = kTileRows * HD * 2;
   static constexpr int kBars = kQ + kStages * kStageBytes;                  // offset of the barriers
@@ -615,8 +615,9 @@ struct ChunkParams {
   int C;
 };
 
-// The grid's row tile x, counted over the sequences: its sequence (-1: past the last), the tile in it and the sequence's
-// tokens. All lanes of a warp call it.
+// The grid's row tile x: its sequence (-1: past the last), the tile in it and the sequence's tokens. Tiles are counted
+// longest first, so that the last CTAs to start are short: among each 32 sequences those of longer contexts come first,
+// and a sequence's later rows, which see more keys, before its earlier ones. All lanes of a warp call it.
 struct TilePlace {
   int seq, tile;
   SeqSpan span;
@@ -624,9 +625,22 @@ struct TilePlace {
 __device__ __forceinline__ TilePlace find_tile(const PagedAttnParams& p, int x, int grp) {
   const int lane = threadIdx.x & 31;
   for (int s0 = 0; s0 < p.seqs; s0 += 32) {
-    const int s = s0 + lane;
+    int s = s0 + lane;
     SeqSpan sp = {0, 0, 0};
     if (s < p.seqs) sp = seq_span(p, s);
+    if (p.seqs > 1) {   // lane i takes the sequence of rank i
+      int rank = 0, from = lane;
+      for (int i = 0; i < 32; ++i) {
+        const int len = __shfl_sync(0xffffffffu, sp.len, i);
+        rank += len > sp.len || (len == sp.len && i < lane);
+      }
+      for (int i = 0; i < 32; ++i) {
+        const uint32_t who = __ballot_sync(0xffffffffu, rank == i);
+        if (lane == i) from = __ffs(who) - 1;
+      }
+      s = s0 + from;
+      sp = {__shfl_sync(0xffffffffu, sp.t0, from), __shfl_sync(0xffffffffu, sp.n, from), __shfl_sync(0xffffffffu, sp.len, from)};
+    }
     const int mine = sp.n > 0 ? (int)(((int64_t)sp.n * grp + kTileRows - 1) / kTileRows) : 0;
     int sum = mine;
 #pragma unroll
@@ -637,7 +651,7 @@ __device__ __forceinline__ TilePlace find_tile(const PagedAttnParams& p, int x, 
     const uint32_t past = __ballot_sync(0xffffffffu, sum > x);
     if (past) {
       const int at = __ffs(past) - 1;
-      return {s0 + at, x - __shfl_sync(0xffffffffu, sum - mine, at),
+      return {__shfl_sync(0xffffffffu, s, at), __shfl_sync(0xffffffffu, sum, at) - 1 - x,
               {__shfl_sync(0xffffffffu, sp.t0, at), __shfl_sync(0xffffffffu, sp.n, at), __shfl_sync(0xffffffffu, sp.len, at)}};
     }
     x -= __shfl_sync(0xffffffffu, sum, 31);
@@ -702,10 +716,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  // heaviest tiles first: a sequence's later rows see more keys
   const int grp = p.nh / p.nkv, item = blockIdx.x / C;
   const int kvh = item % p.nkv;
-  const TilePlace at = find_tile(p, cp.tiles - 1 - item / p.nkv, grp);
+  const TilePlace at = find_tile(p, item / p.nkv, grp);
   const int seq = at.seq, row0 = at.tile * kTileRows;
   const SeqSpan sp = at.span;
   int rows = 0, keys = 0;
