@@ -24,10 +24,12 @@ namespace {
 //
 // A group of G lanes takes one head of one token, 16 values a lane as two 16-byte vectors: lane j < F / 8 the vectors
 // j and j + F / 8 (the two halves of eight pairs, so the rotation needs no exchange), the lanes after them two
-// neighbouring vectors of the unrotated rest. A CTA holds whole tokens, whose cosines and sines it computes once in
-// shared memory: the angle in fp64 as a multiple of pi (fp32 would lose 1e-3 of a turn at position 1e5), while the
-// CTA's values are already on their way from memory.
+// neighbouring vectors of the unrotated rest. A CTA holds up to four whole tokens. Once for all their heads it puts into
+// shared memory the norm weights, each token's place in the cache and its cosines and sines -- the angle in fp64 as a
+// multiple of pi (fp32 would lose 1e-3 of a turn at position 1e5) -- while the first values are already on their way;
+// each group's next head is on its way while it works on one.
 constexpr int kAppendMaxThreads = 512;
+constexpr int kAppendTokens = 4;
 
 struct AppendParams {
   const void* qkv;
@@ -49,41 +51,49 @@ struct AppendParams {
 };
 
 template <typename T, int G>
-__global__ void __launch_bounds__(kAppendMaxThreads) append_kernel(const AppendParams p) {
-  extern __shared__ float2 turn[];   // [tpb][F]: cos, sin
+__global__ void __launch_bounds__(kAppendMaxThreads, 2) append_kernel(const AppendParams p) {
+  extern __shared__ __align__(16) uint8_t append_smem[];   // norm weights [2][hd], cache offsets [tpb][2], (cos, sin) [tpb][F]
+  T* weights = reinterpret_cast<T*>(append_smem);
+  int64_t* place = reinterpret_cast<int64_t*>(weights + 2 * p.hd);
+  float2* turn = reinterpret_cast<float2*>(place + 2 * p.tpb);
   pdl_launch_dependents();
-  const int heads = p.nh + 2 * p.nkv, lanes = p.hd / 16, f8 = p.F / 8;
-  const int t0 = blockIdx.x * p.tpb, nt = min(p.tpb, p.tokens - t0);
+  const int heads = p.nh + 2 * p.nkv, f8 = p.F / 8;
+  const int t0 = blockIdx.x * p.tpb, nt = min(p.tpb, p.tokens - t0), units = nt * heads;
   const int lane = threadIdx.x % G, per = blockDim.x / G;
   const int v0 = lane < f8 ? lane : 2 * lane, v1 = lane < f8 ? lane + f8 : 2 * lane + 1;
-  const bool on = lane < lanes;
-  float wq[16], wk[16];
-  const bool norm = p.q_norm != nullptr;
-  if (norm && on) {   // model state: read before the wait
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int d = 8 * (h ? v1 : v0) + i;
-        wq[8 * h + i] = Elem<T>::to_float(static_cast<const T*>(p.q_norm)[d]);
-        wk[8 * h + i] = Elem<T>::to_float(static_cast<const T*>(p.k_norm)[d]);
-      }
-  }
+  const bool on = lane < p.hd / 16, norm = p.q_norm != nullptr;
+  if (norm)   // model state: read before the wait
+    for (int i = threadIdx.x; i < 2 * p.hd; i += blockDim.x)
+      weights[i] = i < p.hd ? static_cast<const T*>(p.q_norm)[i] : static_cast<const T*>(p.k_norm)[i - p.hd];
   pdl_wait();
-  const T* qkv = static_cast<const T*>(p.qkv);
-  const int units = nt * heads;
-  uint4 x[2];
-  auto load = [&](int u) {
-    if (u < units && on) {
-      const T* src = qkv + (int64_t)(t0 + u / heads) * p.ld + (u % heads) * p.hd;
-      x[0] = *reinterpret_cast<const uint4*>(src + 8 * v0);
-      x[1] = *reinterpret_cast<const uint4*>(src + 8 * v1);
+  const T* qkv = static_cast<const T*>(p.qkv) + t0 * p.ld;
+  int u = threadIdx.x / G, tl = u / heads, head = u - tl * heads;
+  uint4 x[2], next[2];
+  auto load = [&](uint4 (&d)[2], int unit, int tok, int h) {
+    if (unit < units && on) {
+      const T* src = qkv + tok * p.ld + h * p.hd;
+      d[0] = ldg_cg_u128(src + 8 * v0);
+      d[1] = ldg_cg_u128(src + 8 * v1);
     }
   };
-  load(threadIdx.x / G);
+  load(x, u, tl, head);
+  for (int i = threadIdx.x; i < nt; i += blockDim.x) {
+    const int64_t slot = p.slots[t0 + i];
+    int64_t k = -1, v = -1;
+    if (slot >= p.num_slots) {
+      atomicExch(&g_paged_status, kErrBadPosition);
+    } else if (slot >= 0) {
+      const int64_t page = slot / p.page_size, row = (slot - page * p.page_size) * p.hd;
+      k = page * p.k_page + row;
+      v = page * p.v_page + row;
+    }
+    place[2 * i] = k;
+    place[2 * i + 1] = v;
+  }
   for (int i = threadIdx.x; i < nt * p.F; i += blockDim.x) {
     // angle / pi reduced to [-1, 1] in fp64
-    double a = (double)p.pos[t0 + i / p.F] * (double)p.inv_freq[i % p.F] * 0.31830988618379067154;
+    const int tok = i / p.F;
+    double a = (double)p.pos[t0 + tok] * (double)p.inv_freq[i - tok * p.F] * 0.31830988618379067154;
     a -= 2.0 * rint(a * 0.5);
     float sn, cs;
     sincospif((float)a, &sn, &cs);
@@ -91,19 +101,20 @@ __global__ void __launch_bounds__(kAppendMaxThreads) append_kernel(const AppendP
   }
   __syncthreads();
   for (int u0 = 0; u0 < units; u0 += per) {
-    const int u = u0 + threadIdx.x / G;
-    if (u0) load(u);
     const bool live = u < units && on;
-    const int tl = u / heads, head = u % heads, t = t0 + tl;
+    const int tok = tl, h = head;
+    u += per;
+    head += per;
+    while (head >= heads) head -= heads, ++tl;
+    load(next, u, tl, head);
     float f[16];
-    const uint32_t* xw = reinterpret_cast<const uint32_t*>(x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 a = live ? Elem<T>::unpack(xw[i]) : make_float2(0.f, 0.f);
+      const float2 a = live ? Elem<T>::unpack(reinterpret_cast<const uint32_t*>(x)[i]) : make_float2(0.f, 0.f);
       f[2 * i] = a.x;
       f[2 * i + 1] = a.y;
     }
-    const bool is_q = head < p.nh, is_v = head >= p.nh + p.nkv;
+    const bool is_q = h < p.nh, is_v = h >= p.nh + p.nkv;
     if (norm) {
       float ss = 0.f;
 #pragma unroll
@@ -112,18 +123,30 @@ __global__ void __launch_bounds__(kAppendMaxThreads) append_kernel(const AppendP
       for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       if (live && !is_v) {
         const float r = rsqrtf(ss / (float)p.hd + p.eps);
+        const T* w = weights + (is_q ? 0 : p.hd);
+        const uint4 w0 = *reinterpret_cast<const uint4*>(w + 8 * v0), w1 = *reinterpret_cast<const uint4*>(w + 8 * v1);
+        const uint32_t ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = f[i] * r * (is_q ? wq[i] : wk[i]);
+        for (int i = 0; i < 8; ++i) {
+          const float2 a = Elem<T>::unpack(ww[i]);
+          f[2 * i] = f[2 * i] * r * a.x;
+          f[2 * i + 1] = f[2 * i + 1] * r * a.y;
+        }
       }
     }
+    x[0] = next[0];
+    x[1] = next[1];
     if (!live) continue;
     if (!is_v && lane < f8) {
-      const float2* cs = turn + tl * p.F + 8 * lane;
+      const float4* cs = reinterpret_cast<const float4*>(turn + tok * p.F + 8 * lane);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float a = f[i], b = f[8 + i];
-        f[i] = a * cs[i].x - b * cs[i].y;
-        f[8 + i] = b * cs[i].x + a * cs[i].y;
+      for (int i = 0; i < 4; ++i) {
+        const float4 c = cs[i];
+        const float a = f[2 * i], b = f[8 + 2 * i], d = f[2 * i + 1], e = f[9 + 2 * i];
+        f[2 * i] = a * c.x - b * c.y;
+        f[8 + 2 * i] = b * c.x + a * c.y;
+        f[2 * i + 1] = d * c.z - e * c.w;
+        f[9 + 2 * i] = e * c.z + d * c.w;
       }
     }
     uint32_t w[8];
@@ -131,18 +154,11 @@ __global__ void __launch_bounds__(kAppendMaxThreads) append_kernel(const AppendP
     for (int i = 0; i < 8; ++i) w[i] = Elem<T>::pack(f[2 * i], f[2 * i + 1]);
     T* dst;
     if (is_q) {
-      dst = static_cast<T*>(p.q_out) + ((int64_t)t * p.nh + head) * p.hd;
+      dst = static_cast<T*>(p.q_out) + ((int64_t)(t0 + tok) * p.nh + h) * p.hd;
     } else {
-      const int64_t slot = p.slots[t];
-      if (slot < 0) continue;
-      if (slot >= p.num_slots) {
-        atomicExch(&g_paged_status, kErrBadPosition);
-        continue;
-      }
-      const int64_t page = slot / p.page_size, row = slot - page * p.page_size;
-      const int h = head - p.nh - (is_v ? p.nkv : 0);
-      dst = static_cast<T*>(is_v ? p.v : p.k) + page * (is_v ? p.v_page : p.k_page) +
-            ((int64_t)h * p.page_size + row) * p.hd;
+      const int64_t at = place[2 * tok + is_v];
+      if (at < 0) continue;
+      dst = static_cast<T*>(is_v ? p.v : p.k) + at + (int64_t)(h - p.nh - (is_v ? p.nkv : 0)) * p.page_size * p.hd;
     }
     *reinterpret_cast<uint4*>(dst + 8 * v0) = make_uint4(w[0], w[1], w[2], w[3]);
     *reinterpret_cast<uint4*>(dst + 8 * v1) = make_uint4(w[4], w[5], w[6], w[7]);
@@ -1115,11 +1131,13 @@ cudaError_t append_t(const AppendParams& p, bool pdl, cudaStream_t st) {
   const int lanes = p.hd / 16, G = lanes <= 4 ? 4 : lanes <= 8 ? 8 : 16;
   const int per_token = (p.nh + 2 * p.nkv) * G;
   AppendParams a = p;
-  a.tpb = per_token >= 256 ? 1 : 256 / per_token;
-  const int threads = min(kAppendMaxThreads, (a.tpb * per_token + 31) / 32 * 32);
+  // whole tokens a CTA: what fills 256 threads, and up to four where there are many
+  a.tpb = max(256 / per_token, (int)min((int64_t)kAppendTokens, (int64_t)p.tokens / (4 * sm_count())));
+  a.tpb = max(1, min(a.tpb, p.tokens));
+  const int threads = min(kAppendMaxThreads, (min(a.tpb * per_token, max(256, per_token)) + 31) / 32 * 32);
   auto kern = G == 4 ? append_kernel<T, 4> : G == 8 ? append_kernel<T, 8> : append_kernel<T, 16>;
   return launch_paged(kern, dim3((unsigned)((p.tokens + a.tpb - 1) / a.tpb)), dim3(threads),
-                      (size_t)a.tpb * p.F * sizeof(float2), pdl, st, a);
+                      (size_t)2 * p.hd * sizeof(T) + a.tpb * 16 + (size_t)a.tpb * p.F * sizeof(float2), pdl, st, a);
 }
 
 // CTAs of the few-rows kernel that can be resident at once in clusters of C, on the current device
