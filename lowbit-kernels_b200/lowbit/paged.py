@@ -172,3 +172,119 @@ def attention(q, cache, page_table, seq_lens, cu_new, max_new=None, max_len=None
     if rc:
         e._raise(rc)
     return out
+
+
+class PagedDecoder:
+    """A Qwen2-architecture decoder whose calls take chunks of new tokens of any number of sequences -- a prompt in
+    pieces, single tokens of a running batch, or both at once -- over paged caches. Takes the weights of a transformers
+    model of that architecture (fp16 or bf16; per-head q_norm / k_norm modules are used where its attention has them)
+    and keeps its projections in 8-bit integers (`weights="w8"`, ops.linear_w8) or, fp16 models only, in the INT4 format
+    (`weights="w4"`, ops.linear). Per layer: RMSNorm, the fused q|k|v product, `norm_rope_append`, `attention`, the output
+    product, RMSNorm, the fused gate|up product, SiLU * up, the down product.
+
+        dec = PagedDecoder(model, num_pages=512, page_size=64)
+        a, b = dec.open(), dec.open()
+        logits = dec.forward({a: prompt_a, b: prompt_b[:512]})      # [2, vocab]: after each chunk's last token
+        logits = dec.forward({a: [next_a], b: prompt_b[512:]})
+        dec.close(a)
+    """
+
+    def __init__(self, model, num_pages, page_size=64, weights="w8", group=128):
+        if weights not in ("w8", "w4"):
+            raise ValueError('weights is "w8" or "w4"')
+        cfg, base = model.config, model.model
+        self.embed = base.embed_tokens.weight.detach()
+        self.device, self.dtype = self.embed.device, self.embed.dtype
+        if weights == "w4" and self.dtype != torch.float16:
+            raise ValueError("INT4 weights need a float16 model")
+        self.nh, self.nkv = cfg.num_attention_heads, cfg.num_key_value_heads
+        self.hd = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.nh
+        self.eps, self.page_size, self.vocab = float(cfg.rms_norm_eps), page_size, cfg.vocab_size
+        theta = float(cfg.rope_parameters["rope_theta"])
+        half = torch.arange(0, self.hd, 2, dtype=torch.float32)
+        self.inv_freq = (1.0 / theta ** (half / self.hd)).to(self.device)
+        if weights == "w8":
+            self._make, self._linear = ops.W8Weight.from_float, ops.linear_w8
+        else:
+            self._make = lambda w: ops.W4Weight.from_float(w, group, ("mma",))
+            self._linear = ops.linear
+
+        def vector(module):
+            return None if module is None else module.weight.detach().to(self.dtype).contiguous()
+
+        def fused(*linears):
+            biases = [lin.bias for lin in linears]
+            bias = None if biases[0] is None else torch.cat([b.detach() for b in biases]).to(self.dtype).contiguous()
+            return self._make(torch.cat([lin.weight.detach() for lin in linears])), bias
+
+        self.layers = []
+        for layer in base.layers:
+            a, m = layer.self_attn, layer.mlp
+            self.layers.append({
+                "qkv": fused(a.q_proj, a.k_proj, a.v_proj), "o": fused(a.o_proj), "gate_up": fused(m.gate_proj, m.up_proj),
+                "down": fused(m.down_proj), "ln1": vector(layer.input_layernorm), "ln2": vector(layer.post_attention_layernorm),
+                "q_norm": vector(getattr(a, "q_norm", None)), "k_norm": vector(getattr(a, "k_norm", None)),
+                "cache": PagedCache(num_pages, page_size, self.nkv, self.hd, dtype=self.dtype, device=self.device)})
+        self.norm, self.head = vector(base.norm), model.lm_head.weight.detach()
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._seqs, self._next = {}, 0
+
+    def open(self):
+        """A new empty sequence's id."""
+        sid, self._next = self._next, self._next + 1
+        self._seqs[sid] = {"length": 0, "pages": []}
+        return sid
+
+    def close(self, sid):
+        """Forget a sequence; its pages are free for others."""
+        self._free += reversed(self._seqs.pop(sid)["pages"])
+
+    def _rms(self, x, w):
+        f = x.float()
+        return w * (f * torch.rsqrt(f.square().mean(-1, keepdim=True) + self.eps)).to(self.dtype)
+
+    def _plan(self, chunks):
+        """The call's host arrays: token ids, positions and slots, page table, lengths and first tokens."""
+        page = self.page_size
+        need = {s: -(-(self._seqs[s]["length"] + len(new)) // page) - len(self._seqs[s]["pages"]) for s, new in chunks.items()}
+        if sum(need.values()) > len(self._free):
+            raise RuntimeError(f"{sum(need.values())} pages are needed, {len(self._free)} are free")
+        ids, pos, slots, lens, cu = [], [], [], [], [0]
+        for s, new in chunks.items():
+            seq = self._seqs[s]
+            seq["pages"] += [self._free.pop() for _ in range(need[s])]
+            for i, tok in enumerate(new, seq["length"]):
+                ids.append(int(tok))
+                pos.append(i)
+                slots.append(seq["pages"][i // page] * page + i % page)
+            seq["length"] += len(new)
+            lens.append(seq["length"])
+            cu.append(len(ids))
+        width = max(1, max(len(self._seqs[s]["pages"]) for s in chunks))
+        table = [self._seqs[s]["pages"] + [0] * (width - len(self._seqs[s]["pages"])) for s in chunks]
+        return ids, pos, slots, table, lens, cu
+
+    @torch.no_grad()
+    def forward(self, chunks):
+        """chunks: {sequence id: its new token ids, at least one}. Appends them and returns the logits [len(chunks),
+        vocab] after each sequence's last new token, in the order of `chunks`."""
+        if not chunks or any(len(new) == 0 for new in chunks.values()):
+            raise ValueError("every sequence of a call needs a new token")
+        ids, pos, slots, table, lens, cu = self._plan(chunks)
+        dev, t = self.device, len(ids)
+        ids, pos, slots = (torch.tensor(v, dtype=torch.int64, device=dev) for v in (ids, pos, slots))
+        table, lens_d, cu_d = (torch.tensor(v, dtype=torch.int32, device=dev) for v in (table, lens, cu))
+        max_new, max_len = max(len(new) for new in chunks.values()), max(lens)
+        x = self.embed[ids]
+        for ly in self.layers:
+            def product(h, name):
+                w, bias = ly[name]
+                return self._linear(h, w, bias=bias)
+            qkv = product(self._rms(x, ly["ln1"]), "qkv")
+            q = norm_rope_append(qkv, ly["cache"], pos, slots, self.nh, self.inv_freq, ly["q_norm"], ly["k_norm"], self.eps)
+            a = attention(q, ly["cache"], table, lens_d, cu_d, max_new=max_new, max_len=max_len)
+            x = x + product(a.view(t, self.nh * self.hd), "o")
+            gate, up = product(self._rms(x, ly["ln2"]), "gate_up").chunk(2, -1)
+            x = x + product(torch.nn.functional.silu(gate) * up, "down")
+        last = torch.tensor([c - 1 for c in cu[1:]], dtype=torch.int64, device=dev)
+        return torch.nn.functional.linear(self._rms(x[last], self.norm), self.head)

@@ -1,0 +1,136 @@
+"""PagedDecoder: the chunk operators together in a small decoder, against a plain float64 decoder over the same weights
+(dequantized), and its page bookkeeping. INT4 weights leave only rounding between the two. With 8-bit integers the plain
+decoder quantizes the activations as the operator is defined, and rounds to the type where the decoder stores: a value
+that one rounding moves past the middle of a step is a whole step away, so the two have to round alike."""
+import pytest
+import torch
+
+TINY = dict(hidden_size=256, intermediate_size=640, num_hidden_layers=2, num_attention_heads=4,
+            num_key_value_heads=2, vocab_size=1024, tie_word_embeddings=True)
+
+
+class Norm(torch.nn.Module):
+    def __init__(self, n, seed):
+        super().__init__()
+        g = torch.Generator().manual_seed(seed)
+        self.weight = torch.nn.Parameter((1 + 0.2 * torch.randn(n, generator=g)).half().cuda())
+
+
+def tiny(norms=False, dtype=torch.float16, seed=4):
+    from lowbit import decode
+    m = decode.build(TINY, seed=seed).to(dtype)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    for i, layer in enumerate(m.model.layers):
+        for p in (layer.self_attn.q_proj, layer.self_attn.k_proj, layer.self_attn.v_proj):
+            p.bias.data.copy_(torch.randn(p.bias.shape, device="cuda", generator=g) * 0.1)
+        for lin in (layer.self_attn.q_proj, layer.self_attn.k_proj):
+            lin.weight.data *= 6   # scores that are not all alike
+        if norms:
+            layer.self_attn.q_norm, layer.self_attn.k_norm = Norm(64, 10 + i).to(dtype), Norm(64, 20 + i).to(dtype)
+    return m
+
+
+@torch.no_grad()
+def plain_logits(model, ids, weights):
+    """Logits after every token in float64, projections dequantized from the decoder's own format."""
+    from lowbit import ops
+    cfg, nh, nkv, hd = model.config, 4, 2, 64
+    dtype = model.lm_head.weight.dtype
+
+    def stored(v):
+        return v.to(dtype).double() if weights == "w8" else v
+
+    def weight(lin):
+        if weights == "w4":
+            return ops.dequantize_w4_gpu(*ops.quantize_w4_gpu(lin.weight)).double()
+        q, s = ops.quantize_w8_gpu(lin.weight)
+        return q.double() * s.double()[:, None]
+
+    def product(x, lin):
+        if weights == "w8":   # activations too, as the operator is defined
+            amax = x.abs().amax(-1, keepdim=True)
+            x = torch.round(x * 127 / amax) * (amax / 127)
+        y = x @ weight(lin).t()
+        return stored(y if lin.bias is None else y + lin.bias.double())
+
+    def rms(x, w):
+        return stored(stored(x * torch.rsqrt(x.square().mean(-1, keepdim=True) + cfg.rms_norm_eps)) * w.double())
+
+    t = len(ids)
+    x = model.model.embed_tokens.weight[ids].double()
+    freq = 1.0 / 1e6 ** (torch.arange(0, hd, 2, device="cuda", dtype=torch.float64) / hd)
+    angle = torch.arange(t, device="cuda", dtype=torch.float64)[:, None, None] * freq
+    mask = torch.ones(t, t, device="cuda", dtype=torch.bool).triu(1)
+
+    def rope(h):
+        a, b = h.chunk(2, -1)
+        return torch.cat((a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin()), -1)
+
+    for layer in model.model.layers:
+        a, m = layer.self_attn, layer.mlp
+        h = rms(x, layer.input_layernorm.weight)
+        q, k, v = (product(h, p).view(t, -1, hd) for p in (a.q_proj, a.k_proj, a.v_proj))
+        if hasattr(a, "q_norm"):
+            q, k = (h * torch.rsqrt(h.square().mean(-1, keepdim=True) + cfg.rms_norm_eps) * n.weight.double()
+                    for h, n in ((q, a.q_norm), (k, a.k_norm)))
+        q, k = stored(rope(q)), stored(rope(k))
+        k, v = k.repeat_interleave(nh // nkv, 1), v.repeat_interleave(nh // nkv, 1)
+        s = torch.einsum("qhd,khd->hqk", q, k) / 8
+        p = torch.softmax(s.masked_fill(mask, float("-inf")), -1)
+        x = stored(x + product(stored(torch.einsum("hqk,khd->qhd", p, v).reshape(t, nh * hd)), a.o_proj))
+        h = rms(x, layer.post_attention_layernorm.weight)
+        act = stored(stored(torch.nn.functional.silu(product(h, m.gate_proj))) * product(h, m.up_proj))
+        x = stored(x + product(act, m.down_proj))
+    return rms(x, model.model.norm.weight) @ model.lm_head.weight.double().t()
+
+
+def feed(dec, ids, pieces):
+    """The logits after each piece of ids, fed in turn."""
+    sid, rows, at = dec.open(), [], 0
+    for n in pieces:
+        rows.append(dec.forward({sid: ids[at:at + n]})[0])
+        at += n
+    dec.close(sid)
+    return torch.stack(rows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("weights,norms,dtype,bar", [("w4", False, torch.float16, 2e-2), ("w4", True, torch.float16, 2e-2),
+                                                     ("w8", True, torch.float16, 8e-2), ("w8", False, torch.bfloat16, 1.2e-1)])
+def test_paged_decoder_matches_a_plain_decoder(weights, norms, dtype, bar):
+    from lowbit import ops, paged
+    model = tiny(norms, dtype)
+    dec = paged.PagedDecoder(model, num_pages=32, page_size=16, weights=weights)
+    ids = torch.randint(0, 1024, (150,), generator=torch.Generator().manual_seed(9)).tolist()
+    want = plain_logits(model, ids, weights)
+    rms = want.square().mean().sqrt()
+    for pieces in ([150], [1] * 20 + [130], [100, 1, 49], [17, 64, 1, 68]):
+        got = feed(dec, ids, pieces)
+        ends = torch.tensor(pieces).cumsum(0) - 1
+        err = ((got.double() - want[ends]).abs().max() / rms).item()
+        assert err < bar, (pieces, err)
+    assert len(dec._free) == 32 and ops.ext().lib.lb_device_error() == 0
+
+
+@pytest.mark.gpu
+def test_sequences_of_a_batch_do_not_touch_each_other():
+    """Several sequences in one call, chunks and single tokens mixed, give what each gives alone; pages come back."""
+    from lowbit import paged
+    dec = paged.PagedDecoder(tiny(), num_pages=24, page_size=16, weights="w4")
+    g = torch.Generator().manual_seed(2)
+    texts = [torch.randint(0, 1024, (n,), generator=g).tolist() for n in (40, 7, 90)]
+    alone = [feed(dec, ids, [len(ids) - 1, 1])[-1] for ids in texts]
+    sids = [dec.open() for _ in texts]
+    dec.forward({s: ids[:-1] for s, ids in zip(sids, texts)})
+    dec.close(sids.pop(1))
+    again = dec.open()
+    out = dec.forward({sids[0]: texts[0][-1:], again: texts[1], sids[1]: texts[2][-1:]})
+    scale = torch.stack(alone).float().square().mean().sqrt()
+    for row, want in zip(out, (alone[0], alone[1], alone[2])):
+        assert ((row.float() - want.float()).abs().max() / scale).item() < 2e-2
+    with pytest.raises(RuntimeError, match="pages"):
+        dec.forward({sids[0]: list(range(400))})
+    with pytest.raises(ValueError):
+        dec.forward({})
+    with pytest.raises(ValueError):
+        paged.PagedDecoder(tiny(dtype=torch.bfloat16), 4, weights="w4")
