@@ -251,7 +251,7 @@ constexpr int kMmaThreads = (2 + kEpiWarps) * 32;   // loader, MMA, epilogue war
 constexpr int kMaxStages = 8;
 constexpr int kW8MaxSplits = 8;           // portable cluster size
 constexpr int kW8Smem = 227 * 1024;
-constexpr int kBarrierBytes = (2 * kMaxStages + 4) * 8 + 16 + 2 * 256 * 4;
+constexpr int kBarrierBytes = (2 * kMaxStages + 4) * 8 + 16 + 2 * 256 * 4 + kEpiWarps * 1024;   // + scales, + staging
 
 struct W8Gemm {
   const float* s;       // token scales
@@ -262,11 +262,13 @@ struct W8Gemm {
   int bn, halves, tiles_m, tiles, splits, stages;
   int columns;          // tensor memory: 2 accumulators (persistent), or 1 (split)
   int acc_stride;       // columns between the accumulators
-  int park;             // byte offset behind the ring: barriers and scales
+  int park;             // byte offset behind the ring: barriers, scales, staging
+  bool vec;             // output rows take 16-byte stores
 };
 
 // This CTA's share of a cluster's outputs: the int32 partial tiles [token][128 channels] at the same offset of every
-// CTA's shared memory, summed, scaled and stored. A thread's four channels are the same in every round.
+// CTA's shared memory, summed, scaled and stored. A thread's four channels are the same in every round; their scales and
+// biases are under way while the cluster meets.
 template <typename T>
 __device__ __forceinline__ void sum_partials(uint32_t red, const float* sc, const float* t, const T* bias, T* y, int n0,
                                              int N, int rows, int rank, int S) {
@@ -278,7 +280,9 @@ __device__ __forceinline__ void sum_partials(uint32_t red, const float* sc, cons
     tn[j] = on ? t[n0 + r4 + j] : 0.f;
     bn[j] = on && bias ? Elem<T>::to_float(bias[n0 + r4 + j]) : 0.f;
   }
+  cluster_sync_all();
   const int warps = blockDim.x >> 5;
+  const bool vec = n0 + r4 + 4 <= N && N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & 7u) == 0;
   for (int m = rank * warps + (threadIdx.x >> 5); m < rows; m += S * warps) {
     const uint32_t off = red + (uint32_t)(m * 128 + r4) * 4u;
     float4 f[kW8MaxSplits];
@@ -294,10 +298,17 @@ __device__ __forceinline__ void sum_partials(uint32_t red, const float* sc, cons
         v[2] += __float_as_int(f[q].z);
         v[3] += __float_as_int(f[q].w);
       }
-    T* dst = y + (int64_t)m * N + n0 + r4;
+    float o[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (n0 + r4 + j < N) dst[j] = Elem<T>::from_float(fmaf(__int2float_rn(v[j]) * sc[m], tn[j], bn[j]));
+    for (int j = 0; j < 4; ++j) o[j] = fmaf(__int2float_rn(v[j]) * sc[m], tn[j], bn[j]);
+    T* dst = y + (int64_t)m * N + n0 + r4;
+    if (vec) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(o[0], o[1]), Elem<T>::pack(o[2], o[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (n0 + r4 + j < N) dst[j] = Elem<T>::from_float(o[j]);
+    }
   }
 }
 
@@ -461,6 +472,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     const uint32_t tlane = (uint32_t)(32 * quarter) << 16;
     const T* bias = static_cast<const T*>(p.bias);
     T* y = static_cast<T*>(p.y);
+    uint16_t* turn = reinterpret_cast<uint16_t*>(sc + 512) + (warp - 2) * 512;
     pdl_wait();
     bool ok = true;
     const int mine = first < p.tiles ? (p.tiles - first + step - 1) / step : 0;
@@ -483,15 +495,32 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       if (16 * part < acc_bn) tc::ld16(acc + 16 * part, v[0]);
       auto block = [&](int j0, const uint32_t (&w)[16]) {
         if (S == 1) {
-          T* dst = y + (int64_t)(m0 + j0) * p.N + n;
-          if (on && m0 + j0 + 16 <= p.M) {
+          const int left = p.M - m0 - j0;   // tokens
+          uint32_t h[8];
 #pragma unroll
-            for (int j = 0; j < 16; ++j, dst += p.N)
-              *dst = Elem<T>::from_float(fmaf(__int2float_rn((int)w[j]) * scale[j0 + j], tn, bn));
+          for (int j = 0; j < 8; ++j)
+            h[j] = Elem<T>::pack(fmaf(__int2float_rn((int)w[2 * j]) * scale[j0 + 2 * j], tn, bn),
+                                 fmaf(__int2float_rn((int)w[2 * j + 1]) * scale[j0 + 2 * j + 1], tn, bn));
+          if (p.vec) {
+            // through the warp's 1 KB: [16 tokens][32 channels], then eight rows of 64 bytes a store
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              turn[2 * j * 32 + lane] = (uint16_t)h[j];
+              turn[(2 * j + 1) * 32 + lane] = (uint16_t)(h[j] >> 16);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int j = 8 * q + (lane >> 2), c = (lane & 3) * 8;
+              const uint4 v = *reinterpret_cast<const uint4*>(turn + j * 32 + c);
+              if (j < left && n - lane + c < p.N) *reinterpret_cast<uint4*>(y + (int64_t)(m0 + j0 + j) * p.N + n - lane + c) = v;
+            }
+            __syncwarp();
           } else if (on) {
+            uint16_t* dst = reinterpret_cast<uint16_t*>(y) + (int64_t)(m0 + j0) * p.N + n;
 #pragma unroll
             for (int j = 0; j < 16; ++j, dst += p.N)
-              if (m0 + j0 + j < p.M) *dst = Elem<T>::from_float(fmaf(__int2float_rn((int)w[j]) * scale[j0 + j], tn, bn));
+              if (j < left) *dst = (uint16_t)(h[j >> 1] >> (16 * (j & 1)));
           }
         } else {
           int* red = reinterpret_cast<int*>(ring);   // [token][128 channels]
@@ -521,7 +550,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   }
   __syncwarp();
   if (!PAIR && S > 1) {
-    cluster_sync_all();
     const int n0 = first / p.tiles_m * 128, m0 = first % p.tiles_m * p.bn;
     sum_partials<T>(smem_addr(ring), sc, p.t, static_cast<const T*>(p.bias),
                     static_cast<T*>(p.y) + (int64_t)m0 * p.N, n0, p.N, min(p.bn, p.M - m0), rank, S);
@@ -543,11 +571,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 // ------------------------------------------------------------------------------------------- the product, one to eight rows
 // A CTA takes 16 channels and all of K: mma.sync m16n8k32 with the weights' fragments loaded straight into registers,
 // 64 bytes of K of a row per four lanes and 16-byte load (the order of k inside a fragment is free as long as both
-// operands share it). The first loads -- all there are, up to 64 kGemvRound NW values of K -- are issued before the wait
+// operands share it). The first loads -- all there are, up to 64 R NW values of K -- are issued before the wait
 // on the previous kernel; the CTA quantizes the token rows while they are under way. Bound by the weights' way from
 // memory; a cluster, tensor memory or a second launch would each add about a microsecond of latency to some four.
 constexpr int kGemvRows = 8;
-constexpr int kGemvRound = 4;    // 64-byte pieces of K of a warp in flight
 
 struct W8Gemv {
   const void* x;
@@ -568,8 +595,12 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <typename T, int NW, int MR>   // MR: the most rows, 1, 4 or 8
-__global__ void __launch_bounds__(32 * NW) w8_gemv_kernel(const W8Gemv p, int guard) {
+// MR: the most rows, 1, 4 or 8. R: 64-byte pieces of K a warp has in flight. An SM holds gemv_per_sm of its CTAs.
+constexpr int gemv_per_sm(int NW, int MR, int R) {
+  return NW == 16 ? (R == 2 && MR < 8 ? 2 : 1) : (MR == 8 ? 2 : 3) + (R == 2);
+}
+template <typename T, int NW, int MR, int R>
+__global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) w8_gemv_kernel(const W8Gemv p, int guard) {
   extern __shared__ __align__(16) uint8_t rows[];   // [M][pitch] quantized tokens
   __shared__ int part[NW][128];
   __shared__ uint32_t maxima[kGemvRows];
@@ -579,14 +610,14 @@ __global__ void __launch_bounds__(32 * NW) w8_gemv_kernel(const W8Gemv p, int gu
   // rows past N repeat the last one; pieces past K read as zeros (K is padded to 16, a lane's share of a piece)
   const int8_t* w0 = p.w + (int64_t)min(n0 + g, p.N - 1) * p.ldw + 16 * t;
   const int8_t* w1 = p.w + (int64_t)min(n0 + g + 8, p.N - 1) * p.ldw + 16 * t;
-  uint4 a[kGemvRound][2];
+  uint4 a[R][2];
   auto fetch = [&](int i, int c) {
     const bool on = 64 * c + 16 * t < p.K;
     a[i][0] = on ? ldg_stream(reinterpret_cast<const uint4*>(w0 + 64 * c)) : make_uint4(0, 0, 0, 0);
     a[i][1] = on ? ldg_stream(reinterpret_cast<const uint4*>(w1 + 64 * c)) : make_uint4(0, 0, 0, 0);
   };
 #pragma unroll
-  for (int i = 0; i < kGemvRound; ++i) fetch(i, warp + i * NW);
+  for (int i = 0; i < R; ++i) fetch(i, warp + i * NW);
   const int out_n = n0 + (tid & 15), out_m = tid >> 4;   // the output this thread sums, of 16 x 8
   const bool out_on = tid < 128 && out_n < p.N && out_m < p.M;
   const float tn = out_on ? p.t[out_n] : 0.f;
@@ -635,15 +666,15 @@ __global__ void __launch_bounds__(32 * NW) w8_gemv_kernel(const W8Gemv p, int gu
   __syncthreads();
   int d[4] = {0, 0, 0, 0};
   const uint32_t own = smem_addr(rows) + (uint32_t)(min(g, p.M - 1) * p.pitch + 16 * t);   // unused columns repeat a row
-  for (int c0 = warp; c0 < p.pieces; c0 += NW * kGemvRound) {
+  for (int c0 = warp; c0 < p.pieces; c0 += NW * R) {
 #pragma unroll
-    for (int i = 0; i < kGemvRound; ++i) {
+    for (int i = 0; i < R; ++i) {
       const int c = c0 + i * NW;
       if (c < p.pieces) {
         const uint4 b = lds128(own + 64 * c);
         mma_s8(d, a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b.x, b.y);
         mma_s8(d, a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b.z, b.w);
-        fetch(i, c + NW * kGemvRound);
+        fetch(i, c + NW * R);
       }
     }
   }
@@ -779,7 +810,7 @@ W8Plan w8_plan(int64_t M, int64_t N, int chunks, int sms) {
     if (S > 1 && tiles > resident_clusters<T>(S)) return;
     const int64_t ctas = tiles * (pair ? 2 : S), waves = (ctas + sms - 1) / sms;
     const int64_t chunk = max(450, 2 * bn) + (kWBytes + (pair ? bn / 2 : bn) * kChunk) / 64;
-    const int64_t c = 4700 + waves * ((chunks + S - 1) / S) * chunk + (bn > 256 ? waves * 6 * bn : 6 * bn) + (S > 1 ? 2800 : 0);
+    const int64_t c = 4700 + waves * ((chunks + S - 1) / S) * chunk + (bn > 256 ? waves * 20 * bn : 20 * bn) + (S > 1 ? 2800 : 0);
     if (c < least) {
       least = c;
       best.bn = bn, best.pair = pair, best.splits = S, best.halves = bn > 256 ? 2 : 1;
@@ -804,11 +835,19 @@ cudaError_t gemv_t(const W8Params& p, bool pdl, cudaStream_t st) {
   const int pieces = (int)((p.K + 63) / 64), pitch = (pieces * 64 + 127) / 128 * 128 + 64;
   const W8Gemv g{p.x, p.ldx, static_cast<const int8_t*>(p.w), p.ldw, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, (int)p.K,
                  pieces, pitch};
-  const bool wide = pieces > 8 * kGemvRound || p.N < 4096;
-  auto kern = p.M == 1  ? (wide ? w8_gemv_kernel<T, 16, 1> : w8_gemv_kernel<T, 8, 1>)
-              : p.M <= 4 ? (wide ? w8_gemv_kernel<T, 16, 4> : w8_gemv_kernel<T, 8, 4>)
-                         : (wide ? w8_gemv_kernel<T, 16, 8> : w8_gemv_kernel<T, 8, 8>);
-  return launch_w8(kern, (unsigned)((p.N + 15) / 16), wide ? 512 : 256, (size_t)p.M * pitch, 1, pdl, st, g, 1);
+  // 8 warps where they hold all of K, on wide layers; else 16. R = 4, or R = 2 where the more CTAs an SM then holds save a
+  // round (cold weights, M = 2: 11008 x 2048, two rounds either way, R = 4 7.0 us, R = 2 9.1; 8960 x 1536, two rounds or
+  // one, 6.0 and 4.4; M = 1: 4608 x 3584 16 warps 6.1 and 4.4; 11008 x 2048 8 warps 5.7, 16 warps 7.7)
+  const int warps = pieces > 32 || p.N < 4096 ? 16 : 8, ctas = (int)((p.N + 15) / 16), sms = sm_count();
+  auto rounds = [&](int per) { return (ctas + per * sms - 1) / (per * sms); };
+#define LB_GEMV(MR)                                                                                                   \
+  (warps == 8 ? (rounds(gemv_per_sm(8, MR, 2)) < rounds(gemv_per_sm(8, MR, 4)) ? w8_gemv_kernel<T, 8, MR, 2>           \
+                                                                               : w8_gemv_kernel<T, 8, MR, 4>)          \
+              : (rounds(gemv_per_sm(16, MR, 2)) < rounds(gemv_per_sm(16, MR, 4)) ? w8_gemv_kernel<T, 16, MR, 2>        \
+                                                                                 : w8_gemv_kernel<T, 16, MR, 4>))
+  auto kern = p.M == 1 ? LB_GEMV(1) : p.M <= 4 ? LB_GEMV(4) : LB_GEMV(8);
+#undef LB_GEMV
+  return launch_w8(kern, (unsigned)ctas, 32 * warps, (size_t)p.M * pitch, 1, pdl, st, g, 1);
 }
 
 template <typename T>
@@ -835,7 +874,8 @@ cudaError_t linear_t(const W8Params& p, bool pdl, cudaStream_t st) {
   const int tiles_m = (int)((p.M + plan.bn - 1) / plan.bn), tiles = (int)((p.N + tile_n - 1) / tile_n) * tiles_m;
   const int stride = tmem_columns(plan.bn / plan.halves), park = plan.stages * (kWBytes + own_bn * kChunk);
   const W8Gemm g{s, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, chunks, plan.bn, plan.halves, tiles_m, tiles, plan.splits,
-                 plan.stages, plan.splits > 1 ? stride : 2 * stride, stride, park};
+                 plan.stages, plan.splits > 1 ? stride : 2 * stride, stride, park,
+                 p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0};
   if (!encode_rows(&qmap, q, kp, kp, p.M, own_bn / plan.halves)) return cudaErrorInvalidValue;
   const size_t smem = (size_t)park + kBarrierBytes + 1024;
   if (plan.pair) {
