@@ -190,7 +190,12 @@ __global__ void __launch_bounds__(kQLongThreads)
     }
     wait_bounded(&bar, 0, &g_w8_status);
   } else {
-    for (int i = tid; i < 8 * held; i += kQLongThreads) mine[i] = xr[i];
+    for (int i = tid; i < held; i += kQLongThreads) {
+      Vec8<T> v;
+      v.load(xr + 8 * i, 8, false);
+#pragma unroll
+      for (int h = 0; h < (int)sizeof(T) / 2; ++h) reinterpret_cast<uint4*>(mine + 8 * i)[h] = reinterpret_cast<const uint4*>(&v.v[0])[h];
+    }
     __syncthreads();
   }
   auto fetch = [&](int j, Vec8<T>& v) {
