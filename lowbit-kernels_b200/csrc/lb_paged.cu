@@ -353,8 +353,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
           float x = fmaxf(s[nt][e], s[nt][2 + e]);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-          x = fmaxf(x, m[nt][e]);
-          const float c = x == -INFINITY ? 1.f : exp2_fast(m[nt][e] - x);
+          if (!(x > m[nt][e] + 8.f)) x = m[nt][e];   // (each row by its own scores, whatever stands beside it)
+          const float c = x == m[nt][e] ? 1.f : exp2_fast(m[nt][e] - x);
           m[nt][e] = x;
           l[nt][e] *= c;
 #pragma unroll
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
   T* out = static_cast<T*>(p.out);
   auto store = [&](int r, int d, const float4& v, float sum) {
     const int row = row0 + r;
-    const float c = sum > 0.f ? 1.f / sum : 0.f;
+    const float c = sum != 0.f ? 1.f / sum : 0.f;
     *reinterpret_cast<uint2*>(out + (int64_t)(sp.t0 + row / grp) * p.out_token + (int64_t)(kvh * grp + row % grp) * HD + d) =
         make_uint2(Elem<T>::pack(v.x * c, v.y * c), Elem<T>::pack(v.z * c, v.w * c));
   };
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnPara
     acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
     sum += weights[k];
   }
-  const float c = sum > 0.f ? 1.f / sum : 0.f;
+  const float c = sum != 0.f ? 1.f / sum : 0.f;
   T* dst = static_cast<T*>(p.out) + (int64_t)(sp.t0 + row / grp) * p.out_token + (int64_t)(kvh * grp + row % grp) * HD + d;
   *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * c, acc.y * c), Elem<T>::pack(acc.z * c, acc.w * c));
 }
@@ -575,9 +575,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if one of them is
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -941,14 +941,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         float mx[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          mx[c] = fmaxf(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
+          mx[c] = max3(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]), __uint_as_float(v[c][2]));
 #pragma unroll
-          for (int i = 2; i < 32; i += 2) mx[c] = max3(mx[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+          for (int i = 3; i < 31; i += 2) mx[c] = max3(mx[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+          mx[c] = max3(mx[c], __uint_as_float(v[c][31]), __uint_as_float(v[c][31]));
         }
-        const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * scale;
-        if (__any_sync(0xffffffffu, top > m + 8.f)) {
-          const float mn = fmaxf(m, top);
-          const float c = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
+        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * scale;
+        // a score that is NaN or +inf makes the row NaN, as exp(inf - inf) would; the polynomial below would hide it
+        if (!(top < INFINITY)) l = NAN;
+        // (each row by its own scores alone, so that its result does not depend on the rows beside it)
+        const bool move = top > m + 8.f && top < INFINITY;
+        if (__any_sync(0xffffffffu, move)) {
+          const float mn = move ? top : m;
+          const float c = move ? exp2_fast(m - mn) : 1.f;
           m = mn;
           l *= c;
           if (j > 0) {   // the last product of this tile is complete before O is touched
@@ -997,6 +1002,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const float2 both = unpair(sum);
         l += both.x + both.y;
       }
+      // a row that saw no key: the polynomial's least value is not zero
+      if (m == -INFINITY && l == l) l = 0.f;
       wait_bounded(&o_done[t], (nt - 1) & 1, &g_paged_status);
       __syncwarp();
       tc::fence_after();
@@ -1004,7 +1011,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     if (C == 1) {
       if (seq >= 0) {
         // through the warp's rows of Q, which are done with, so that HD / 8 lanes store a row at a time
-        const float c = l > 0.f ? 1.f / l : 0.f;
+        const float c = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
         for (int h = 0; h < HD / 32; ++h) {
           uint32_t o[32];
@@ -1017,7 +1024,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             uint32_t w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              w[e] = l > 0.f ? Elem<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * c, __uint_as_float(o[8 * i + 2 * e + 1]) * c) : 0u;
+              w[e] = l != 0.f ? Elem<T>::pack(__uint_as_float(o[8 * i + 2 * e]) * c, __uint_as_float(o[8 * i + 2 * e + 1]) * c) : 0u;
             const int piece = 4 * h + i;
             *reinterpret_cast<uint4*>(stage + lane * 128 + (piece / 8) * kHalfQ + (((piece % 8) ^ (lane & 7)) << 4)) =
                 make_uint4(w[0], w[1], w[2], w[3]);
@@ -1089,12 +1096,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int k = 0; k < kChunkCluster; ++k)
-            if (k < C && mk[n][k] != -INFINITY) {   // (a part without keys holds whatever its ring held)
+            if (k < C && lk[n][k] != 0.f) {   // (a part without keys holds whatever its ring held)
               const float c = exp2_fast(mk[n][k] - mx);
               acc.x += c * x[n][k].x, acc.y += c * x[n][k].y, acc.z += c * x[n][k].z, acc.w += c * x[n][k].w;
               sum += c * lk[n][k];
             }
-          const float c = sum > 0.f ? 1.f / sum : 0.f;
+          const float c = sum != 0.f ? 1.f / sum : 0.f;
           T* dst = static_cast<T*>(p.out) + (int64_t)(sp.t0 + row / grp) * p.out_token + ((int64_t)kvh * grp + row % grp) * HD + 4 * c4;
           *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * c, acc.y * c), Elem<T>::pack(acc.z * c, acc.w * c));
         }

@@ -142,6 +142,20 @@ def test_linear_w8_extreme_sums_are_exact():
 
 
 @gpu
+@pytest.mark.parametrize("k", [8193, 20000, 50001, 100000])
+def test_linear_w8_long_rows(k):
+    """Rows longer than the registers hold, and than shared memory holds; aligned to 16 bytes or to 2."""
+    ops, _ = mods()
+    g = gen(k)
+    w8 = ops.W8Weight.from_float(randn(g, 70, k, std=0.05))
+    for m in (3, 70):
+        wide = randn(g, m, k + 9, dtype=torch.bfloat16)
+        for off in (0, 1):
+            x = wide[:, off:off + k]
+            check_linear(x, w8.q, w8.scales, None, ops.linear_w8(x, w8))
+
+
+@gpu
 def test_linear_w8_strided_inputs_out_and_streams():
     ops, _ = mods()
     g = gen(11)
@@ -379,8 +393,32 @@ def test_attention_rows_without_keys_are_zero(new, ctx):
     if sum(new) == 0:
         new = new + [1]
         ctx = ctx + [1]
-    for hd, nh, nkv in ((64, 6, 2), (128, 16, 2)):
-        run_attention(gen(sum(ctx)), new, ctx, nh, nkv, hd, 16, torch.float16)
+    for hd, nh, nkv in ((64, 6, 2), (128, 16, 2), (128, 40, 1)):
+        for dtype in DTYPES:
+            run_attention(gen(sum(ctx)), new, ctx, nh, nkv, hd, 16, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,ctx", [(1, 300), (2, 40), (100, 300), (300, 1500)])
+def test_attention_scores_that_are_not_finite_reach_the_rows_that_see_them(dtype, new, ctx):
+    """A key of NaN, or one that gives an infinite score: every row that sees it is NaN, as exp(inf - inf) is, and the
+    rows before it are untouched. Keys at every place of a block, since the exponentials are not all taken the same way."""
+    ops, paged = mods()
+    q, cache, table, lens, cu = build(gen(6), [new], [ctx], 16, 2, 128, 32, dtype)
+    q = q.abs()
+    clean = paged.attention(q, cache, table, lens, cu, max_new=new)
+    for back in {1, 2, 3, 5, 8, 12, 17, new // 2, new}:
+        key = ctx - back
+        at, row = int(table[0, key // 32]), key % 32
+        keep = cache.k[at, :, row].clone()
+        for bad in (float("nan"), float("inf")):
+            cache.k[at, :, row] = bad
+            y = paged.attention(q, cache, table, lens, cu, max_new=new)
+            first = max(0, new - back)   # the first new token that sees the key
+            assert torch.isnan(y[first:]).all(), (back, bad)
+            assert torch.equal(y[:first], clean[:first]), (back, bad)
+        cache.k[at, :, row] = keep
 
 
 @gpu
