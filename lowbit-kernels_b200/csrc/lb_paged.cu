@@ -27,7 +27,8 @@ namespace {
 // neighbouring vectors of the unrotated rest. A CTA holds up to four whole tokens. Once for all their heads it puts into
 // shared memory the norm weights, each token's place in the cache and its cosines and sines -- the angle in fp64 as a
 // multiple of pi (fp32 would lose 1e-3 of a turn at position 1e5) -- while the first values are already on their way;
-// each group's next head is on its way while it works on one.
+// each group's next head is on its way while it works on one. 8192 tokens, 28 + 2 x 4 heads of 128: 35.3 us, 4.3 TB/s
+// (75.6 with one token a CTA and the norm weights and angles fetched by every group).
 constexpr int kAppendMaxThreads = 512;
 constexpr int kAppendTokens = 4;
 
@@ -180,6 +181,9 @@ __global__ void __launch_bounds__(kAppendMaxThreads, 2) append_kernel(const Appe
 // The warps' (maximum, sum, O) are joined in shared memory, the CTAs' through distributed shared memory, in one fixed
 // order. Few long contexts leave most SMs idle even so: then Z clusters share a context, and a second kernel joins their
 // parts from a workspace.
+// Bound by memory: 96 contexts of up to 8192 tokens, 28/4 heads of 128: 133 us for 742 MB (5.6 TB/s, uneven contexts
+// included); 256 of 8192: 6.5 TB/s. One short context: 6.4 us, the chain of its loads. (Two blocks of keys a warp in
+// flight: fewer CTAs an SM, slower.)
 constexpr int kFewWarps = 4;
 constexpr int kFewRows = 64;     // rows of a key head that go this way
 constexpr int kFewCluster = 8;
@@ -553,7 +557,12 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnPara
 // Weights are rounded to the 16-bit type for the second product, as tensor cores take it; scores, maxima, sums and O are
 // fp32.
 // Few tiles: a cluster of C CTAs splits the keys; each parks O, maxima and sums in its idle ring and all join their share
-// of the rows through distributed shared memory, in one fixed order.
+// of the rows through distributed shared memory, in one fixed order. (Pushing the parts to their owners instead: 33 us
+// where this takes 29.)
+// Bound by the softmax beside the MMAs: a step of 256 rows x 128 keys takes some 3100 clocks, of which the MMAs need 2048
+// at hd 128, 1024 at hd 64. 28/4 heads of 128: 4096 new tokens 115 us (1050 TFLOP/s), over 32768 1550 us (1160); 14/2 of
+// 64: 4096 over 16384 370 us (570). Neither MMAs issued by two warps (873 for 1072), nor two softmax threads a row (3 %
+// more on long contexts, 7 % less on short ones) came out ahead.
 // two fp32 values in one 64-bit register pair
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;
@@ -748,154 +757,154 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   // 128 x 56 + 256 x 224 registers are the launch's 384 x 168: a softmax thread holds its row's 128 scores. (The
   // warpgroups' paths do not meet again before the end: what follows a meeting has the fewer registers.)
   if (warp < 4) {
-  tc::regs_dec<56>();
-  if (warp == 0) {
-    if (seq >= 0 && nt > 0) {
-      if (lane == 0) {
-        tma_prefetch_map(&kmap);
-        tma_prefetch_map(&vmap);
-      }
-      // lane -> (piece, half); table entries one tile ahead
-      const int pieces = kTileKeys / cp.piece, piece = lane / kHalves, half = lane % kHalves;
-      const bool mine = piece < pieces;
-      const int32_t* table = p.table + (int64_t)seq * p.table_stride;
-      const int per_page = p.page_size / cp.piece;
-      const uint32_t dst0 = half * kHalfK + piece * cp.piece * 128;
-      auto lookup = [&](int j, int& page, int& row) {   // this lane's piece of key tile j
-        const int key = (j0 + j) * kTileKeys + piece * cp.piece;
-        page = -1;
-        if (mine && j < nt && key < keys) {
-          const int idx = key / cp.piece, tp = idx / per_page;
-          row = kvh * p.page_size + (idx - tp * per_page) * cp.piece;
-          page = table[tp];
-          if (page < 0 || page >= p.num_pages) {
-            if (half == 0) atomicExch(&g_paged_status, kErrBadPosition);
-            page = 0;
-          }
+    tc::regs_dec<56>();
+    if (warp == 0) {
+      if (seq >= 0 && nt > 0) {
+        if (lane == 0) {
+          tma_prefetch_map(&kmap);
+          tma_prefetch_map(&vmap);
         }
-      };
-      int page, row = 0, page_next, row_next = 0;
-      lookup(0, page, row);
-      int s = 0, phase = 0, filled = 0;
-      bool ok = true;
-      for (int j = 0; j < nt && ok; ++j) {
-        lookup(j + 1, page_next, row_next);
-        const int live = __popc(__ballot_sync(0xffffffffu, page >= 0));
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (filled >= St) ok = wait_bounded(&empty[s], phase, &g_paged_status);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&full[s], live * cp.piece * 128);
-          __syncwarp();
-          if (page >= 0)
-            tc::tma_load_3d(smem_addr(ring) + s * L::kStageBytes + dst0, kv ? &vmap : &kmap, 64 * half, row, page, &full[s]);
-          ++filled;
-          if (++s == St) s = 0, phase ^= filled > St;
-        }
-        page = page_next, row = row_next;
-      }
-      // no copy in flight past this point
-      const int last = min(filled, St);
-      for (int i = 0; i < last; ++i) {
-        const int f = filled - last + i;
-        wait_bounded(&full[f % St], (f / St) & 1, &g_paged_status);
-      }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // One elected lane runs the whole loop (measured, eight MMAs with a wait and a commit: 570 clocks this way, 660 when the
-    // warp loops and elects at each group, 840 under `if (lane == 0)`; they take 512). It shares its scheduler with two
-    // softmax warps, so an instruction costs it ten clocks: the ring is unrolled and every address a constant offset.
-    if (seq >= 0 && nt > 0 && tc::elect_one()) {
-      constexpr uint32_t kType = Elem<T>::kBf16 ? (1u << 7) | (1u << 10) : 0u;
-      constexpr uint32_t kQK = (1u << 4) | kType | ((kTileKeys >> 3) << 17) | ((128u >> 4) << 24);
-      constexpr uint32_t kPV = (1u << 4) | kType | (1u << 16) | ((HD >> 3) << 17) | ((128u >> 4) << 24);   // B MN-major
-      constexpr int D = L::kDepth;
-      constexpr uint32_t kStep = L::kStageBytes >> 4;
-      uint32_t kd = (uint32_t)tc::desc_sw128(smem_addr(ring), 16, 1024);
-      uint32_t vd = (uint32_t)tc::desc_sw128(smem_addr(ring) + L::kStageBytes, kHalfK, 1024);
-      uint32_t qd = (uint32_t)tc::desc_sw128(smem_addr(smem), 16, 1024);
-      const uint32_t bars = smem_addr(full);
-      constexpr uint32_t kEmpty = 8 * St, kQReady = 16 * St, kSFull = kQReady + 8, kPReady = kSFull + 16, kODone = kPReady + 32,
-                         kDrain = kODone + 16, kTailGo = kDrain + 8, kVTail = kDrain + 16;
-      auto wait = [&](uint32_t off, uint32_t parity) { return wait_ready(bars + off, parity, &g_paged_status); };
-      auto qk = [&](int t, int d) {   // S_t = Q_t K^T with K stage d
-#pragma unroll
-        for (int k = 0; k < HD / 16; ++k)
-          tc::mma_f16_ss(tmem + 128 * t, qd + ((t * kHalves * kHalfQ + (k / 4) * kHalfQ + (k % 4) * 32) >> 4),
-                         kd + 2 * d * kStep + (((k / 4) * kHalfK + (k % 4) * 32) >> 4), kQK, k > 0);
-        tc::commit_at(bars + kSFull + 8 * t);
-      };
-      // tile j with V stage u, the next scores with K stage (u + 1) % D; false when a wait gave up
-      auto step = [&](int j, int u, uint32_t ring_parity, bool first, bool more) {
-        asm volatile("" : "+r"(kd), "+r"(vd), "+r"(qd));   // (or the compiler keeps every sum in a register of its own)
-        if (!wait(8 * (2 * u + 1), ring_parity)) return false;
-        if (!more && keys - (j0 + j) * kTileKeys < kTileKeys) {   // the third warp's turn
-          mbar_arrive(tail_go);
-          if (!wait(kVTail, 0)) return false;
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            if (!wait(kPReady + 8 * (2 * part + t), u & 1)) return false;
-            tc::fence_after();
-#pragma unroll
-            for (int k = part ? 6 : 0; k < (part ? 8 : 6); ++k)
-              tc::mma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, vd + 2 * u * kStep + ((k * 2048) >> 4), kPV,
-                             !first || k > 0);
-          }
-          tc::commit_at(bars + kODone + 8 * t);
-          if (t == 1) tc::commit_at(bars + kEmpty + 8 * (2 * u + 1));
-          if (more) {
-            if (t == 0) {
-              if (!wait(8 * (2 * ((u + 1) % D)), u + 1 < D ? ring_parity : ring_parity ^ 1)) return false;
-              tc::fence_after();
+        // lane -> (piece, half); table entries one tile ahead
+        const int pieces = kTileKeys / cp.piece, piece = lane / kHalves, half = lane % kHalves;
+        const bool mine = piece < pieces;
+        const int32_t* table = p.table + (int64_t)seq * p.table_stride;
+        const int per_page = p.page_size / cp.piece;
+        const uint32_t dst0 = half * kHalfK + piece * cp.piece * 128;
+        auto lookup = [&](int j, int& page, int& row) {   // this lane's piece of key tile j
+          const int key = (j0 + j) * kTileKeys + piece * cp.piece;
+          page = -1;
+          if (mine && j < nt && key < keys) {
+            const int idx = key / cp.piece, tp = idx / per_page;
+            row = kvh * p.page_size + (idx - tp * per_page) * cp.piece;
+            page = table[tp];
+            if (page < 0 || page >= p.num_pages) {
+              if (half == 0) atomicExch(&g_paged_status, kErrBadPosition);
+              page = 0;
             }
-            qk(t, (u + 1) % D);
-            if (t == 1) tc::commit_at(bars + kEmpty + 8 * (2 * ((u + 1) % D)));
           }
-        }
-        return true;
-      };
-      bool ok = wait(kQReady, 0) && wait(0, 0);
-      tc::fence_after();
-      if (ok) {
-        qk(0, 0);
-        qk(1, 0);
-        tc::commit_at(bars + kEmpty);
-      }
-      uint32_t parity = 0;
-      for (int j = 0; j < nt && ok; j += D, parity ^= 1) {
+        };
+        int page, row = 0, page_next, row_next = 0;
+        lookup(0, page, row);
+        int s = 0, phase = 0, filled = 0;
+        bool ok = true;
+        for (int j = 0; j < nt && ok; ++j) {
+          lookup(j + 1, page_next, row_next);
+          const int live = __popc(__ballot_sync(0xffffffffu, page >= 0));
 #pragma unroll
-        for (int u = 0; u < D; ++u)
-          if (ok && j + u < nt) ok = step(j + u, u, parity, j + u == 0, j + u + 1 < nt);
+          for (int kv = 0; kv < 2; ++kv) {
+            if (filled >= St) ok = wait_bounded(&empty[s], phase, &g_paged_status);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&full[s], live * cp.piece * 128);
+            __syncwarp();
+            if (page >= 0)
+              tc::tma_load_3d(smem_addr(ring) + s * L::kStageBytes + dst0, kv ? &vmap : &kmap, 64 * half, row, page, &full[s]);
+            ++filled;
+            if (++s == St) s = 0, phase ^= filled > St;
+          }
+          page = page_next, row = row_next;
+        }
+        // no copy in flight past this point
+        const int last = min(filled, St);
+        for (int i = 0; i < last; ++i) {
+          const int f = filled - last + i;
+          wait_bounded(&full[f % St], (f / St) & 1, &g_paged_status);
+        }
       }
-      // no MMA in flight past this point
-      tc::commit_at(bars + kDrain);
-      wait(kDrain, 0);
-    }
-    __syncwarp();
-  } else if (warp == 2) {
-    // the V rows behind the context in the last tile, zeroed once the tile has arrived
-    const int tail = keys - (j0 + nt - 1) * kTileKeys;
-    if (seq >= 0 && nt > 0 && tail < kTileKeys) {
-      const int fill = 2 * nt - 1;
-      wait_bounded(tail_go, 0, &g_paged_status);
-      uint8_t* tile = ring + (fill % St) * L::kStageBytes;
-      for (int half = 0; half < kHalves; ++half)
-        for (int i = lane; i < (kTileKeys - tail) * 8; i += 32)
-          *reinterpret_cast<uint4*>(tile + half * kHalfK + tail * 128 + i * 16) = make_uint4(0, 0, 0, 0);
-      tc::fence_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(v_tail);
+    } else if (warp == 1) {
+      // One elected lane runs the whole loop (measured, eight MMAs with a wait and a commit: 570 clocks this way, 660 when the
+      // warp loops and elects at each group, 840 under `if (lane == 0)`; they take 512). It shares its scheduler with two
+      // softmax warps, so an instruction costs it ten clocks: the ring is unrolled and every address a constant offset.
+      if (seq >= 0 && nt > 0 && tc::elect_one()) {
+        constexpr uint32_t kType = Elem<T>::kBf16 ? (1u << 7) | (1u << 10) : 0u;
+        constexpr uint32_t kQK = (1u << 4) | kType | ((kTileKeys >> 3) << 17) | ((128u >> 4) << 24);
+        constexpr uint32_t kPV = (1u << 4) | kType | (1u << 16) | ((HD >> 3) << 17) | ((128u >> 4) << 24);   // B MN-major
+        constexpr int D = L::kDepth;
+        constexpr uint32_t kStep = L::kStageBytes >> 4;
+        uint32_t kd = (uint32_t)tc::desc_sw128(smem_addr(ring), 16, 1024);
+        uint32_t vd = (uint32_t)tc::desc_sw128(smem_addr(ring) + L::kStageBytes, kHalfK, 1024);
+        uint32_t qd = (uint32_t)tc::desc_sw128(smem_addr(smem), 16, 1024);
+        const uint32_t bars = smem_addr(full);
+        constexpr uint32_t kEmpty = 8 * St, kQReady = 16 * St, kSFull = kQReady + 8, kPReady = kSFull + 16, kODone = kPReady + 32,
+                           kDrain = kODone + 16, kTailGo = kDrain + 8, kVTail = kDrain + 16;
+        auto wait = [&](uint32_t off, uint32_t parity) { return wait_ready(bars + off, parity, &g_paged_status); };
+        auto qk = [&](int t, int d) {   // S_t = Q_t K^T with K stage d
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k)
+            tc::mma_f16_ss(tmem + 128 * t, qd + ((t * kHalves * kHalfQ + (k / 4) * kHalfQ + (k % 4) * 32) >> 4),
+                           kd + 2 * d * kStep + (((k / 4) * kHalfK + (k % 4) * 32) >> 4), kQK, k > 0);
+          tc::commit_at(bars + kSFull + 8 * t);
+        };
+        // tile j with V stage u, the next scores with K stage (u + 1) % D; false when a wait gave up
+        auto step = [&](int j, int u, uint32_t ring_parity, bool first, bool more) {
+          asm volatile("" : "+r"(kd), "+r"(vd), "+r"(qd));   // (or the compiler keeps every sum in a register of its own)
+          if (!wait(8 * (2 * u + 1), ring_parity)) return false;
+          if (!more && keys - (j0 + j) * kTileKeys < kTileKeys) {   // the third warp's turn
+            mbar_arrive(tail_go);
+            if (!wait(kVTail, 0)) return false;
+          }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              if (!wait(kPReady + 8 * (2 * part + t), u & 1)) return false;
+              tc::fence_after();
+#pragma unroll
+              for (int k = part ? 6 : 0; k < (part ? 8 : 6); ++k)
+                tc::mma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, vd + 2 * u * kStep + ((k * 2048) >> 4), kPV,
+                               !first || k > 0);
+            }
+            tc::commit_at(bars + kODone + 8 * t);
+            if (t == 1) tc::commit_at(bars + kEmpty + 8 * (2 * u + 1));
+            if (more) {
+              if (t == 0) {
+                if (!wait(8 * (2 * ((u + 1) % D)), u + 1 < D ? ring_parity : ring_parity ^ 1)) return false;
+                tc::fence_after();
+              }
+              qk(t, (u + 1) % D);
+              if (t == 1) tc::commit_at(bars + kEmpty + 8 * (2 * ((u + 1) % D)));
+            }
+          }
+          return true;
+        };
+        bool ok = wait(kQReady, 0) && wait(0, 0);
+        tc::fence_after();
+        if (ok) {
+          qk(0, 0);
+          qk(1, 0);
+          tc::commit_at(bars + kEmpty);
+        }
+        uint32_t parity = 0;
+        for (int j = 0; j < nt && ok; j += D, parity ^= 1) {
+#pragma unroll
+          for (int u = 0; u < D; ++u)
+            if (ok && j + u < nt) ok = step(j + u, u, parity, j + u == 0, j + u + 1 < nt);
+        }
+        // no MMA in flight past this point
+        tc::commit_at(bars + kDrain);
+        wait(kDrain, 0);
+      }
+      __syncwarp();
+    } else if (warp == 2) {
+      // the V rows behind the context in the last tile, zeroed once the tile has arrived
+      const int tail = keys - (j0 + nt - 1) * kTileKeys;
+      if (seq >= 0 && nt > 0 && tail < kTileKeys) {
+        const int fill = 2 * nt - 1;
+        wait_bounded(tail_go, 0, &g_paged_status);
+        uint8_t* tile = ring + (fill % St) * L::kStageBytes;
+        for (int half = 0; half < kHalves; ++half)
+          for (int i = lane; i < (kTileKeys - tail) * 8; i += 32)
+            *reinterpret_cast<uint4*>(tile + half * kHalfK + tail * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+        tc::fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_tail);
+      }
+      __syncwarp();
     }
-    __syncwarp();
-  }
-  if (C > 1) {
-    cluster_sync_all();
-    cluster_sync_all();
-  }
+    if (C > 1) {
+      cluster_sync_all();
+      cluster_sync_all();
+    }
   } else {
     tc::regs_inc<224>();
     const int t = (warp - 4) >> 2, quarter = warp & 3, r = 128 * t + 32 * quarter + lane, row = row0 + r;
@@ -1061,54 +1070,54 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
       }
     }
-  __syncwarp();
-  if (C > 1) {
-    cluster_sync_all();
-    if (seq >= 0) {
-      // a share of the rows a CTA, HD / 4 lanes a row
-      constexpr int kLanes = HD / 4;
-      const int c4 = (threadIdx.x - 128) % kLanes;
-      constexpr int kPass = 256 / kLanes, kAtOnce = 2;   // rows a pass, and passes under way together
-      for (int r0 = rank * kPass + (threadIdx.x - 128) / kLanes; r0 < rows; r0 += kAtOnce * C * kPass) {
-        float mk[kAtOnce][kChunkCluster], lk[kAtOnce][kChunkCluster];
-        float4 x[kAtOnce][kChunkCluster];
+    __syncwarp();
+    if (C > 1) {
+      cluster_sync_all();
+      if (seq >= 0) {
+        // a share of the rows a CTA, HD / 4 lanes a row
+        constexpr int kLanes = HD / 4;
+        const int c4 = (threadIdx.x - 128) % kLanes;
+        constexpr int kPass = 256 / kLanes, kAtOnce = 2;   // rows a pass, and passes under way together
+        for (int r0 = rank * kPass + (threadIdx.x - 128) / kLanes; r0 < rows; r0 += kAtOnce * C * kPass) {
+          float mk[kAtOnce][kChunkCluster], lk[kAtOnce][kChunkCluster];
+          float4 x[kAtOnce][kChunkCluster];
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-          const int r = min(r0 + n * C * kPass, kTileRows - 1);
-          const uint32_t am = smem_addr(row_m + r), al = smem_addr(row_l + r);
-          const uint32_t ao = smem_addr(ring) + r * HD * 4 + ((c4 ^ (r & 7)) << 4);
+          for (int n = 0; n < kAtOnce; ++n) {
+            const int r = min(r0 + n * C * kPass, kTileRows - 1);
+            const uint32_t am = smem_addr(row_m + r), al = smem_addr(row_l + r);
+            const uint32_t ao = smem_addr(ring) + r * HD * 4 + ((c4 ^ (r & 7)) << 4);
 #pragma unroll
-          for (int k = 0; k < kChunkCluster; ++k)
-            if (k < C) {
-              mk[n][k] = ld_dsmem_f1(mapa_shared(am, k));
-              lk[n][k] = ld_dsmem_f1(mapa_shared(al, k));
-              x[n][k] = ld_dsmem_f4(mapa_shared(ao, k));
-            }
-        }
+            for (int k = 0; k < kChunkCluster; ++k)
+              if (k < C) {
+                mk[n][k] = ld_dsmem_f1(mapa_shared(am, k));
+                lk[n][k] = ld_dsmem_f1(mapa_shared(al, k));
+                x[n][k] = ld_dsmem_f4(mapa_shared(ao, k));
+              }
+          }
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-          const int r = r0 + n * C * kPass, row = row0 + r;
-          if (r >= rows) break;
-          float mx = -INFINITY, sum = 0.f;
+          for (int n = 0; n < kAtOnce; ++n) {
+            const int r = r0 + n * C * kPass, row = row0 + r;
+            if (r >= rows) break;
+            float mx = -INFINITY, sum = 0.f;
 #pragma unroll
-          for (int k = 0; k < kChunkCluster; ++k)
-            if (k < C) mx = fmaxf(mx, mk[n][k]);
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < kChunkCluster; ++k)
+              if (k < C) mx = fmaxf(mx, mk[n][k]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int k = 0; k < kChunkCluster; ++k)
-            if (k < C && lk[n][k] != 0.f) {   // (a part without keys holds whatever its ring held)
-              const float c = exp2_fast(mk[n][k] - mx);
-              acc.x += c * x[n][k].x, acc.y += c * x[n][k].y, acc.z += c * x[n][k].z, acc.w += c * x[n][k].w;
-              sum += c * lk[n][k];
-            }
-          const float c = sum != 0.f ? 1.f / sum : 0.f;
-          T* dst = static_cast<T*>(p.out) + (int64_t)(sp.t0 + row / grp) * p.out_token + ((int64_t)kvh * grp + row % grp) * HD + 4 * c4;
-          *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * c, acc.y * c), Elem<T>::pack(acc.z * c, acc.w * c));
+            for (int k = 0; k < kChunkCluster; ++k)
+              if (k < C && lk[n][k] != 0.f) {   // (a part without keys holds whatever its ring held)
+                const float c = exp2_fast(mk[n][k] - mx);
+                acc.x += c * x[n][k].x, acc.y += c * x[n][k].y, acc.z += c * x[n][k].z, acc.w += c * x[n][k].w;
+                sum += c * lk[n][k];
+              }
+            const float c = sum != 0.f ? 1.f / sum : 0.f;
+            T* dst = static_cast<T*>(p.out) + (int64_t)(sp.t0 + row / grp) * p.out_token + ((int64_t)kvh * grp + row % grp) * HD + 4 * c4;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(acc.x * c, acc.y * c), Elem<T>::pack(acc.z * c, acc.w * c));
+          }
         }
       }
+      cluster_sync_all();
     }
-    cluster_sync_all();
-  }
   }
   tc::fence_before();
   __syncthreads();
@@ -1178,8 +1187,8 @@ int few_resident(int C) {
 // How few rows are laid out: tiles of 8 or 16 rows, clusters of C CTAs, Z clusters a context -- the choice whose estimated
 // time is least, in microseconds as measured: 4 to start and end a CTA, 1 a block of keys and warp, more where memory
 // bounds all CTAs' blocks together, 1 to join a cluster, 4 for the second kernel; CTAs past those resident at once come
-// in further rounds, with a quarter of a round of tail. A warp takes at most 48 blocks where a split can help it: contexts differ,
-// and the longest ends last.
+// in further rounds, with a quarter of a round of tail. A warp takes at most 48 blocks where a split can help it:
+// contexts differ, and the longest ends last.
 struct FewPlan {
   int nt, row_tiles, C, Z;
   int64_t items;

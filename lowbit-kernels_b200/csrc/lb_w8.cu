@@ -231,22 +231,27 @@ __global__ void __launch_bounds__(kQLongThreads)
 }
 
 // ------------------------------------------------------------------------------------------- the product, many rows
-// tcgen05.mma kind::i8 with the channels as the A side (128 rows a CTA) and a tile of BN tokens as the N side, int32
-// accumulators in tensor memory.
+// y[m, n] = s_m t_n sum_k q[m, k] w[n, k] + b_n by tcgen05.mma kind::i8, the channels as the A side (128 rows a CTA) and
+// a tile of BN tokens as the N side; the int32 accumulators in tensor memory are exact.
 //   * loader warp: one thread copies each 128-byte K chunk of the tile (channels, tokens; 128-byte swizzle, rows and
 //     columns past the edge read as zeros) into a stage ring; the first stages' weights before the wait on the previous
 //     kernel (the quantization), whose rows follow after it.
-//   * MMA warp: one thread issues four K = 32 MMAs per chunk; a commit per chunk releases the stage, one per tile hands
-//     the accumulator to the epilogue. Two accumulators: the next tile's MMAs run under this tile's epilogue.
+//   * MMA warp: one elected lane runs the whole loop, four K = 32 MMAs per chunk; a commit per chunk releases the stage,
+//     one per tile hands the accumulator to the epilogue. Two accumulators: the next tile's MMAs run under this tile's
+//     epilogue.
 //   * 16 epilogue warps, four per 32-lane quarter of tensor memory: a lane holds one channel (its scale and bias in
-//     registers), a column one token; a warp stores 64 consecutive bytes of an output row at a time.
+//     registers), a column one token. 16 tokens x the warp's 32 channels are turned in shared memory, so that a lane
+//     stores 16 bytes of an output row (N % 8 == 0; else single values): 18 % off the 509-token product, whose outputs
+//     left two bytes a lane before. (Tokens as the A side and a row a lane: 22.3 us instead of 18.0.)
 // CTAs are persistent over tiles, tokens innermost, so that the CTAs of one moment share weights in L2.
 // PAIR: two CTAs work on one tile of 256 channels (cta_group::2): each loads its 128 channels and half of the tokens, and
-// the leader's MMAs read both. A chunk then costs each SM 16 + BN / 16 KB of loads instead of 16 + BN / 8, and it is the
-// L2-to-SM path that bounds the single-CTA form: at BN = 224 it wants 100 bytes a clock and SM.
+// the leader's MMAs read both, so that a chunk costs each SM 16 + BN / 16 KB of loads instead of 16 + BN / 8. The loads
+// bound the small products (some 64 bytes a clock and SM arrive from L2), and single CTAs keep the grids that pairs and
+// wide tiles would leave short of the SMs.
 // With `halves` = 2 a pair's tile is up to 512 tokens wide, in two accumulators that fill the tensor memory: 48 bytes a
-// clock and SM instead of 64 for 256 x 256, and the epilogue, which then only the next tile's loads run under, is short
-// beside a long K.
+// clock and SM instead of 64 for 256 x 256; the epilogue, which then only the next tile's loads run under, is short
+// beside a long K. 8192 tokens of 18944 values, 3584 channels: 362 us (3.07 POP/s, 0.94 of twice the measured bf16 peak,
+// under the power cap; the quantization before it takes 74); 509 tokens of 1536, 17920 channels: 20.9 us with it.
 // Few tiles and long K: a cluster of S single CTAs splits K, each parks its int32 partial tile in its (then idle) ring
 // and all sum their share through distributed shared memory -- exact, so the bits do not depend on S.
 constexpr int kChunk = 128;               // bytes of K per stage
@@ -579,6 +584,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 // operands share it). The first loads -- all there are, up to 64 R NW values of K -- are issued before the wait
 // on the previous kernel; the CTA quantizes the token rows while they are under way. Bound by the weights' way from
 // memory; a cluster, tensor memory or a second launch would each add about a microsecond of latency to some four.
+// One token, weights in L2: 4608 x 3584 (16.5 MB) 4.7 us, 12544 x 1792 (22.5 MB) 5.4 us; the many-rows product takes
+// 8.5 and 9.9 with its quantization.
 constexpr int kGemvRows = 8;
 
 struct W8Gemv {
