@@ -46,8 +46,9 @@ typedef enum lb_layout { LB_LAYOUT_CANONICAL = 0, LB_LAYOUT_V3 = 1, LB_LAYOUT_MM
 
 typedef enum lb_option {
   LB_OPT_PDL = 0,           /* 1 (default): launch with programmatic dependent launch enabled */
-  LB_OPT_EARLY_WEIGHTS = 1, /* 1: GEMV kernels fetch their first weights before waiting on the previous kernel
-                               in the stream (only for weights no in-flight kernel writes); default 0 */
+  LB_OPT_EARLY_WEIGHTS = 1, /* 1: GEMV kernels, lb_w8_linear and the norm of lb_paged_norm_rope_append fetch their
+                               first weights before waiting on the previous kernel in the stream (only for weights
+                               no in-flight kernel writes); default 0 */
   LB_OPT_GEMV_KSPLIT = 2,   /* 0 (default): automatic; 1..8 forces the GEMV's K-split cluster size */
   LB_OPT_GEMV_WARPS = 3,    /* 0 (default): automatic; 4, 8 or 16 forces the GEMV's warps per CTA */
   LB_OPT_GEMV_DEPTH = 4,    /* reserved: no effect (the copy-ring GEMV it tuned was removed) */
@@ -270,10 +271,9 @@ LB_API int lb_w8_quantize_rows(const void* x, int dtype, int64_t m, int64_t k, i
 /*
  * y[M, N] = (sum_k q[m, k] w[n, k]) s[m] w_scales[n] + bias[n], q and s the rows of x quantized as above, the sum
  * exact in int32, the rest in fp32 with one rounding. x and y fp16 or bf16 (y contiguous), bias [N] of that type or
- * NULL; w int8 [N, ldw] 16-byte aligned, ldw a multiple of 16, zeros from column K to the next multiple of 16; w and w_scales are model state: they
- * may be read before the kernel waits on the previous one in the stream. workspace: lb_w8_workspace(m, n, k) bytes on the
- * current device
- * (0: none needed), 16-byte aligned, its content undefined before and after; calls that can overlap need distinct ones.
+ * NULL; w int8 [N, ldw] 16-byte aligned, ldw a multiple of 16, zeros from column K to the next multiple
+ * of 16. workspace: lb_w8_workspace(m, n, k) bytes on the current device (0: none needed), 16-byte aligned, its content
+ * undefined before and after; calls that can overlap need distinct ones.
  */
 LB_API int64_t lb_w8_workspace(int64_t m, int64_t n, int64_t k);
 LB_API int lb_w8_linear(const void* x, int dtype, int64_t ldx, const void* w, int64_t ldw, const float* w_scales,
@@ -299,8 +299,7 @@ typedef struct lb_paged_cache {
  * first `rot` dimensions rotated (x[i], x[i + rot/2]) by positions[t] * inv_freq[i] (rot a multiple of 16 up to hd,
  * inv_freq fp32 [rot/2]; 0: no rotation); q goes to q_out [tokens, nh, hd], k and v to the cache's slot slots[t]. A
  * negative slot stores no k and v; one past the cache neither, and sets lb_device_error() to 3. Tokens of one call
- * have distinct slots. hd a multiple of 16 up to 256. The norm weights (model state) are read before the kernel waits
- * on the previous one in the stream.
+ * have distinct slots. hd a multiple of 16 up to 256.
  */
 LB_API int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens, int nh, const void* q_norm,
                                      const void* k_norm, float eps, const float* inv_freq, int rot,
@@ -308,8 +307,8 @@ LB_API int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens
                                      void* q_out, lb_stream_t stream);
 
 /*
- * out[t, h] = softmax over the visible keys j of scale * q[t, h] . K[j, h / (nh / nkv)], times V; scale > 0. Sequence s has the
- * new tokens cu_new[s] .. cu_new[s + 1] - 1 (cu_new int32 [seqs + 1], not decreasing, from 0; tokens past its last
+ * out[t, h] = softmax over the visible keys j of scale * q[t, h] . K[j, h / (nh / nkv)], times V; scale > 0. Sequence s
+ * has the new tokens cu_new[s] .. cu_new[s + 1] - 1 (cu_new int32 [seqs + 1], not decreasing, from 0; tokens past its last
  * value belong to no sequence and are left unwritten) and, them included, a context of seq_lens[s] tokens in the
  * cache; its new token i of n sees keys 0 .. seq_lens[s] - n + i. A token that sees none gets zeros. seq_lens above
  * table_width * page_size are cut to that. page_table int32 [seqs, table_width], rows table_stride apart; entries past

@@ -668,7 +668,7 @@ int lb_w8_linear(const void* x, int dtype, int64_t ldx, const void* w, int64_t l
                 (long long)need);
   if (!aligned16(workspace)) return fail(LB_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
   if ((rc = check_device())) return rc;
-  const lb::W8Params p{x, ldx, dtype, w, ldw, w_scales, bias, y, m, n, k, workspace};
+  const lb::W8Params p{x, ldx, dtype, w, ldw, w_scales, bias, y, m, n, k, workspace, g_opt[LB_OPT_EARLY_WEIGHTS].load() != 0};
   return launched(lb::launch_w8_linear(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)), "w8_linear");
 }
 
@@ -690,7 +690,8 @@ int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens, int n
   const lb::PagedCacheView c{cache->k, cache->v, cache->k_page_stride, cache->v_page_stride, cache->num_pages,
                              cache->dtype, cache->nkv, cache->hd, cache->page_size};
   return launched(lb::launch_paged_append(qkv, ld, tokens, nh, q_norm, k_norm, eps, inv_freq, rot, positions, slots, c,
-                                          q_out, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)),
+                                          q_out, g_opt[LB_OPT_EARLY_WEIGHTS].load() != 0, g_opt[LB_OPT_PDL].load() != 0,
+                                          reinterpret_cast<cudaStream_t>(stream)),
                   "paged_norm_rope_append");
 }
 

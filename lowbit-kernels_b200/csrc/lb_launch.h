@@ -147,6 +147,7 @@ struct W8Params {
   void* y;              // [M, N]
   int64_t M, N, K;
   void* workspace;
+  bool early;           // w and w_scales may be read before the wait on the previous kernel
 };
 size_t w8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 cudaError_t launch_w8_linear(const W8Params& p, bool pdl, cudaStream_t st);
@@ -165,7 +166,8 @@ struct PagedCacheView {
 };
 cudaError_t launch_paged_append(const void* qkv, int64_t ld, int64_t tokens, int nh, const void* q_norm,
                                 const void* k_norm, float eps, const float* inv_freq, int rot, const int64_t* pos,
-                                const int64_t* slots, const PagedCacheView& c, void* q_out, bool pdl, cudaStream_t st);
+                                const int64_t* slots, const PagedCacheView& c, void* q_out, bool early, bool pdl,
+                                cudaStream_t st);
 struct PagedAttnParams {
   const void* q;
   int64_t q_token, q_head;   // element strides

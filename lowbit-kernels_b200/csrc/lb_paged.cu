@@ -49,6 +49,7 @@ struct AppendParams {
   int64_t num_slots;
   int page_size;
   int tpb;          // tokens per CTA
+  bool early;       // norm weights may be read before the wait on the previous kernel
 };
 
 template <typename T, int G>
@@ -63,10 +64,11 @@ __global__ void __launch_bounds__(kAppendMaxThreads, 2) append_kernel(const Appe
   const int lane = threadIdx.x % G, per = blockDim.x / G;
   const int v0 = lane < f8 ? lane : 2 * lane, v1 = lane < f8 ? lane + f8 : 2 * lane + 1;
   const bool on = lane < p.hd / 16, norm = p.q_norm != nullptr;
-  if (norm)   // model state: read before the wait
+  if (!p.early) pdl_wait();
+  if (norm)
     for (int i = threadIdx.x; i < 2 * p.hd; i += blockDim.x)
       weights[i] = i < p.hd ? static_cast<const T*>(p.q_norm)[i] : static_cast<const T*>(p.k_norm)[i - p.hd];
-  pdl_wait();
+  if (p.early) pdl_wait();
   const T* qkv = static_cast<const T*>(p.qkv) + t0 * p.ld;
   int u = threadIdx.x / G, tl = u / heads, head = u - tl * heads;
   uint4 x[2], next[2];
@@ -1351,9 +1353,10 @@ cudaError_t attention_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
 
 cudaError_t launch_paged_append(const void* qkv, int64_t ld, int64_t tokens, int nh, const void* q_norm,
                                 const void* k_norm, float eps, const float* inv_freq, int rot, const int64_t* pos,
-                                const int64_t* slots, const PagedCacheView& c, void* q_out, bool pdl, cudaStream_t st) {
+                                const int64_t* slots, const PagedCacheView& c, void* q_out, bool early, bool pdl,
+                                cudaStream_t st) {
   AppendParams p{qkv, ld, (int)tokens, nh, c.nkv, c.hd, rot / 2, q_norm, k_norm, eps, inv_freq, pos, slots, q_out,
-                 c.k, c.v, c.k_page, c.v_page, c.num_pages * c.page_size, c.page_size, 1};
+                 c.k, c.v, c.k_page, c.v_page, c.num_pages * c.page_size, c.page_size, 1, early};
   return c.dtype == 0 ? append_t<__half>(p, pdl, st) : append_t<__nv_bfloat16>(p, pdl, st);
 }
 

@@ -112,15 +112,17 @@ struct Vec8<float> {
 // GT threads take one row of up to 64 GT values: the row goes into registers once, the maximum is reduced over the
 // group, and the bytes are written 8 at a time. Memory bound: 2 K (4 K for fp32) bytes read and K written per row.
 constexpr int kQVecs = 8;
+enum Release { kAtEnd, kAfterWait, kAtEntry };   // when a quantization lets the next kernel start
 
 template <typename T, int GT>
 __global__ void __launch_bounds__(256)
     quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int ldq, float* __restrict__ s,
-                         int M, int K, bool early) {
+                         int M, int K, int release) {
   constexpr int kRows = 256 / GT;
   __shared__ uint32_t red[kRows][GT / 32];
-  if (early) pdl_launch_dependents();
+  if (release == kAtEntry) pdl_launch_dependents();
   pdl_wait();
+  if (release == kAfterWait) pdl_launch_dependents();
   const int g = threadIdx.x / GT, tid = threadIdx.x % GT;
   const int64_t row = (int64_t)blockIdx.x * kRows + g;
   const bool on = row < M;
@@ -166,11 +168,11 @@ constexpr int kQLongBytes = 96 * 1024;
 template <typename T>
 __global__ void __launch_bounds__(kQLongThreads)
     quantize_long_kernel(const T* __restrict__ x, int64_t ldx, int8_t* __restrict__ q, int ldq, float* __restrict__ s,
-                         int K, int cap, bool early) {
+                         int K, int cap, int release) {
   extern __shared__ __align__(128) uint8_t row_bytes[];
   __shared__ uint64_t bar;
   __shared__ uint32_t red[kQLongThreads / 32];
-  if (early) pdl_launch_dependents();
+  if (release == kAtEntry) pdl_launch_dependents();
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ldx;
@@ -182,6 +184,7 @@ __global__ void __launch_bounds__(kQLongThreads)
   }
   __syncthreads();
   pdl_wait();
+  if (release == kAfterWait) pdl_launch_dependents();
   T* mine = reinterpret_cast<T*>(row_bytes);
   if (aligned) {
     if (tid == 0) {
@@ -581,8 +584,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 // ------------------------------------------------------------------------------------------- the product, one to eight rows
 // A CTA takes 16 channels and all of K: mma.sync m16n8k32 with the weights' fragments loaded straight into registers,
 // 64 bytes of K of a row per four lanes and 16-byte load (the order of k inside a fragment is free as long as both
-// operands share it). The first loads -- all there are, up to 64 R NW values of K -- are issued before the wait
-// on the previous kernel; the CTA quantizes the token rows while they are under way. Bound by the weights' way from
+// operands share it). The first loads -- all there are, up to 64 R NW values of K -- are issued at once, with
+// `early` before the wait on the previous kernel; the CTA quantizes the token rows while they are under way. Bound by the weights' way from
 // memory; a cluster, tensor memory or a second launch would each add about a microsecond of latency to some four.
 // One token, weights in L2: 4608 x 3584 (16.5 MB) 4.7 us, 12544 x 1792 (22.5 MB) 5.4 us; the many-rows product takes
 // 8.5 and 9.9 with its quantization.
@@ -612,13 +615,14 @@ constexpr int gemv_per_sm(int NW, int MR, int R) {
   return NW == 16 ? (R == 2 && MR < 8 ? 2 : 1) : (MR == 8 ? 2 : 3) + (R == 2);
 }
 template <typename T, int NW, int MR, int R>
-__global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) w8_gemv_kernel(const W8Gemv p, int guard) {
+__global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) w8_gemv_kernel(const W8Gemv p, bool early) {
   extern __shared__ __align__(16) uint8_t rows[];   // [M][pitch] quantized tokens
   __shared__ int part[NW][128];
   __shared__ uint32_t maxima[kGemvRows];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * 16;
   pdl_launch_dependents();
+  if (!early) pdl_wait();
   // rows past N repeat the last one; pieces past K read as zeros (K is padded to 16, a lane's share of a piece)
   const int8_t* w0 = p.w + (int64_t)min(n0 + g, p.N - 1) * p.ldw + 16 * t;
   const int8_t* w1 = p.w + (int64_t)min(n0 + g + 8, p.N - 1) * p.ldw + 16 * t;
@@ -636,7 +640,7 @@ __global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) w8_gemv_kerne
   const float bn = out_on && p.bias ? Elem<T>::to_float(static_cast<const T*>(p.bias)[out_n]) : 0.f;
   if (tid < kGemvRows) maxima[tid] = 0u;
   __syncthreads();
-  pdl_wait_after_loads(guard);
+  if (early) pdl_wait();
   const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * sizeof(T))) & 15u) == 0;
   const T* x = static_cast<const T*>(p.x);
   const int nv = p.pieces * 8;   // vectors of 8 values of a row
@@ -741,26 +745,27 @@ cudaError_t allow_smem(Kern kern, std::atomic<uint64_t>& done, int bytes = kW8Sm
   return e;
 }
 
-// a warp or 128 threads a row where the registers hold it, else a CTA. With few rows the next kernel is let in at once;
-// with many it would take the registers of CTAs still to come (measured at 8192 rows of 18944: the quantization ran at
+// a warp or 128 threads a row where the registers hold it, else a CTA. With few rows the next kernel, the product, is let
+// in early: it may read weights before it waits, so where they may still be in the making only once everything before the
+// quantization is complete. With many rows it would take the registers of CTAs still to come (measured at 8192 rows of 18944: the quantization ran at
 // half its speed under the product's resident CTAs).
 template <typename T>
-cudaError_t quantize_t(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* s, int64_t M, int64_t K, bool pdl,
-                       cudaStream_t st) {
+cudaError_t quantize_t(const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* s, int64_t M, int64_t K,
+                       Release few, bool pdl, cudaStream_t st) {
   const int64_t nv = ldq / 8;
-  const bool early = M <= 296;
+  const int release = M <= 296 ? few : kAtEnd;
   const T* xt = static_cast<const T*>(x);
   if (nv <= 128 * kQVecs) {
     const int GT = nv <= 32 * kQVecs && M > 512 ? 32 : 128, rows = 256 / GT;
     return launch_w8(GT == 32 ? quantize_rows_kernel<T, 32> : quantize_rows_kernel<T, 128>,
-                     (unsigned)((M + rows - 1) / rows), 256, 0, 1, pdl, st, xt, ldx, q, (int)ldq, s, (int)M, (int)K, early);
+                     (unsigned)((M + rows - 1) / rows), 256, 0, 1, pdl, st, xt, ldx, q, (int)ldq, s, (int)M, (int)K, release);
   }
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_smem(quantize_long_kernel<T>, done, kQLongBytes + 16);
   if (e != cudaSuccess) return e;
   const int cap = (int)min(K, (int64_t)(kQLongBytes / sizeof(T)));
   return launch_w8(quantize_long_kernel<T>, (unsigned)M, kQLongThreads, (size_t)cap * sizeof(T) + 16, 1, pdl, st, xt, ldx,
-                   q, (int)ldq, s, (int)K, cap, early);
+                   q, (int)ldq, s, (int)K, cap, release);
 }
 
 int64_t padded(int64_t k) { return (k + 15) / 16 * 16; }
@@ -859,7 +864,7 @@ cudaError_t gemv_t(const W8Params& p, bool pdl, cudaStream_t st) {
                                                                                  : w8_gemv_kernel<T, 16, MR, 4>))
   auto kern = p.M == 1 ? LB_GEMV(1) : p.M <= 4 ? LB_GEMV(4) : LB_GEMV(8);
 #undef LB_GEMV
-  return launch_w8(kern, (unsigned)ctas, 32 * warps, (size_t)p.M * pitch, 1, pdl, st, g, 1);
+  return launch_w8(kern, (unsigned)ctas, 32 * warps, (size_t)p.M * pitch, 1, pdl, st, g, p.early);
 }
 
 template <typename T>
@@ -872,7 +877,7 @@ cudaError_t linear_t(const W8Params& p, bool pdl, cudaStream_t st) {
   if (!encode_rows(&wmap, p.w, kp, p.ldw, p.N, 128)) return cudaErrorInvalidValue;
   int8_t* q = static_cast<int8_t*>(p.workspace);
   float* s = reinterpret_cast<float*>(q + p.M * kp);
-  cudaError_t e = quantize_t<T>(p.x, p.ldx, q, kp, s, p.M, p.K, pdl, st);
+  cudaError_t e = quantize_t<T>(p.x, p.ldx, q, kp, s, p.M, p.K, p.early ? kAtEntry : kAfterWait, pdl, st);
   if (e != cudaSuccess) return e;
   static thread_local struct {   // the last plan of this host thread: a layer's calls follow one another
     int64_t M, N, chunks;
@@ -912,9 +917,9 @@ size_t w8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
 
 cudaError_t launch_w8_quantize_rows(const void* x, int dtype, int64_t ldx, int8_t* q, int64_t ldq, float* s, int64_t M,
                                     int64_t K, bool pdl, cudaStream_t st) {
-  return dtype == 0   ? quantize_t<__half>(x, ldx, q, ldq, s, M, K, pdl, st)
-         : dtype == 1 ? quantize_t<__nv_bfloat16>(x, ldx, q, ldq, s, M, K, pdl, st)
-                      : quantize_t<float>(x, ldx, q, ldq, s, M, K, pdl, st);
+  return dtype == 0   ? quantize_t<__half>(x, ldx, q, ldq, s, M, K, kAtEnd, pdl, st)
+         : dtype == 1 ? quantize_t<__nv_bfloat16>(x, ldx, q, ldq, s, M, K, kAtEnd, pdl, st)
+                      : quantize_t<float>(x, ldx, q, ldq, s, M, K, kAtEnd, pdl, st);
 }
 
 cudaError_t launch_w8_linear(const W8Params& p, bool pdl, cudaStream_t st) {

@@ -82,7 +82,7 @@ def norm_rope_append(qkv, cache, positions, slots, nh, inv_freq, q_norm=None, k_
     apart): q and k heads times rsqrt(mean(x^2) + eps) times q_norm / k_norm ([hd], both or neither), their first
     2 * len(inv_freq) dimensions rotated (rotate-half) by positions[t] * inv_freq (int64 [T], fp32), then k and v stored
     at the cache's slots (int64 [T]; negative: not stored). Returns q [T, nh, hd] (`out`, when given). All in fp32 with
-    one rounding. The norm weights are model state: no kernel in flight on the stream may be writing them."""
+    one rounding."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc:
         q = tc.norm_rope_append(qkv, cache._ptr, cache._device, positions, slots, nh, inv_freq, q_norm, k_norm, eps, out)

@@ -156,6 +156,28 @@ def test_linear_w8_long_rows(k):
 
 
 @gpu
+@pytest.mark.parametrize("m", [1, 8, 40])
+def test_linear_w8_reads_weights_that_the_kernel_before_it_wrote(m):
+    """Weights quantized into one pair of buffers again and again, each followed at once by a product: by default no
+    weight is read before the kernel before it is done."""
+    from lowbit._lib import DTYPE_IDS
+    ops, _ = mods()
+    g, n, k = gen(m), 256, 8192
+    floats = [randn(g, n, k, std=0.01 * (i + 1)) for i in range(8)]
+    w8 = ops.W8Weight.from_float(floats[0])
+    x = randn(g, m, k, dtype=torch.float16)
+    want = [ops.linear_w8(x, ops.W8Weight.from_float(f)) for f in floats]
+    torch.cuda.synchronize()
+    got = []
+    for f in floats:
+        rc = ops.ext().lib.lb_w8_quantize_rows(f.data_ptr(), DTYPE_IDS[f.dtype], n, k, k, w8.q.data_ptr(), k,
+                                               w8.scales.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        got.append(ops.linear_w8(x, w8))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
 def test_linear_w8_strided_inputs_out_and_streams():
     ops, _ = mods()
     g = gen(11)
