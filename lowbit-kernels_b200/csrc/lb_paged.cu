@@ -629,9 +629,11 @@ struct ChunkSmem {
   static constexpr int kStageBytes = kTileKeys * HD * 2;
   static constexpr int kDepth = 2;     // K and V tiles each in the ring (4 at hd 64: a longer loop, 6 % slower)
   static constexpr int kStages = 2 * kDepth;
+  static constexpr int kScores = HD == 128 ? 2 : 3;   // score tiles beside two O in tensor memory
+  static constexpr int kRound = HD == 128 ? 2 : 6;    // jobs until a row tile meets the same score tile again
   static constexpr int kQ = kTileRows * HD * 2;
   static constexpr int kBars = kQ + kStages * kStageBytes;                  // offset of the barriers
-  static constexpr int kSlot = kBars + (2 * kStages + 12) * 8;
+  static constexpr int kSlot = kBars + (2 * kStages + kRound + 2 * kScores + 8) * 8;
   static constexpr int kTotal = kSlot + 16 + 1024;                          // + alignment
 };
 
@@ -697,7 +699,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                            const ChunkParams cp) {
   using L = ChunkSmem<HD>;
-  constexpr int kHalves = L::kHalves, St = L::kStages;
+  constexpr int kHalves = L::kHalves, St = L::kStages, B = L::kScores, R = L::kRound;
+  constexpr uint32_t kO = 128 * B;   // tensor memory: B score tiles, two O
   constexpr uint32_t kHalfK = kTileKeys * 128, kHalfQ = 128 * 128;   // bytes of a 64-dim half of a tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
@@ -706,11 +709,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* empty = full + St;
   uint64_t* q_ready = empty + St;
   uint64_t* s_full = q_ready + 1;
-  uint64_t* p_ready = s_full + 2;   // [part][tile]
-  uint64_t* o_done = p_ready + 4;
+  uint64_t* p_ready = s_full + R;   // [part][score tile]
+  uint64_t* o_done = p_ready + 2 * B;
   uint64_t* drain = o_done + 2;
   uint64_t* tail_go = drain + 1;
   uint64_t* v_tail = drain + 2;
+  uint64_t* o_last = drain + 3;     // with three score tiles a row tile's last two products may both be to come
   uint32_t* slot = reinterpret_cast<uint32_t*>(smem + L::kSlot);
   float* row_m = reinterpret_cast<float*>(smem);   // [256] each, over Q, which no product reads any more by then
   float* row_l = row_m + kTileRows;
@@ -727,11 +731,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     mbar_init(drain, 1);
     mbar_init(tail_go, 1);
     mbar_init(v_tail, 1);
+    for (int i = 0; i < R; ++i) mbar_init(&s_full[i], 1);
+    for (int i = 0; i < 2 * B; ++i) mbar_init(&p_ready[i], 4);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 4);
-      mbar_init(&p_ready[2 + i], 4);
       mbar_init(&o_done[i], 1);
+      mbar_init(&o_last[i], 1);
     }
     mbar_fence_init();
   }
@@ -827,17 +831,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         uint32_t vd = (uint32_t)tc::desc_sw128(smem_addr(ring) + L::kStageBytes, kHalfK, 1024);
         uint32_t qd = (uint32_t)tc::desc_sw128(smem_addr(smem), 16, 1024);
         const uint32_t bars = smem_addr(full);
-        constexpr uint32_t kEmpty = 8 * St, kQReady = 16 * St, kSFull = kQReady + 8, kPReady = kSFull + 16, kODone = kPReady + 32,
-                           kDrain = kODone + 16, kTailGo = kDrain + 8, kVTail = kDrain + 16;
+        constexpr uint32_t kEmpty = 8 * St, kQReady = 16 * St, kSFull = kQReady + 8, kPReady = kSFull + 8 * R, kODone = kPReady + 16 * B,
+                           kDrain = kODone + 16, kTailGo = kDrain + 8, kVTail = kDrain + 16, kOLast = kDrain + 24;
         auto wait = [&](uint32_t off, uint32_t parity) { return wait_ready(bars + off, parity, &g_paged_status); };
-        auto qk = [&](int t, int d) {   // S_t = Q_t K^T with K stage d
+        int b = 0;         // of the job at hand: its score tile, and the parity of that tile's uses
+        uint32_t bp = 0;
+        auto qk = [&](int b, int i, int t, int d) {   // the scores of a job i (mod R): row tile t with K stage d
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k)
-            tc::mma_f16_ss(tmem + 128 * t, qd + ((t * kHalves * kHalfQ + (k / 4) * kHalfQ + (k % 4) * 32) >> 4),
+            tc::mma_f16_ss(tmem + 128 * b, qd + ((t * kHalves * kHalfQ + (k / 4) * kHalfQ + (k % 4) * 32) >> 4),
                            kd + 2 * d * kStep + (((k / 4) * kHalfK + (k % 4) * 32) >> 4), kQK, k > 0);
-          tc::commit_at(bars + kSFull + 8 * t);
+          tc::commit_at(bars + kSFull + 8 * i);
         };
-        // tile j with V stage u, the next scores with K stage (u + 1) % D; false when a wait gave up
+        // tile j with V stage u, and the scores B jobs on, which take the score tile just used; false when a wait gave up
         auto step = [&](int j, int u, uint32_t ring_parity, bool first, bool more) {
           asm volatile("" : "+r"(kd), "+r"(vd), "+r"(qd));   // (or the compiler keeps every sum in a register of its own)
           if (!wait(8 * (2 * u + 1), ring_parity)) return false;
@@ -847,34 +853,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
+            const int at = B == 2 ? t : b;
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
-              if (!wait(kPReady + 8 * (2 * part + t), u & 1)) return false;
+              if (!wait(kPReady + 8 * (B * part + at), B == 2 ? u & 1 : bp)) return false;
               tc::fence_after();
 #pragma unroll
               for (int k = part ? 6 : 0; k < (part ? 8 : 6); ++k)
-                tc::mma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, vd + 2 * u * kStep + ((k * 2048) >> 4), kPV,
+                tc::mma_f16_ts(tmem + kO + HD * t, tmem + 128 * at + 8 * k, vd + 2 * u * kStep + ((k * 2048) >> 4), kPV,
                                !first || k > 0);
             }
             tc::commit_at(bars + kODone + 8 * t);
+            if (B > 2 && !more) tc::commit_at(bars + kOLast + 8 * t);
             if (t == 1) tc::commit_at(bars + kEmpty + 8 * (2 * u + 1));
-            if (more) {
-              if (t == 0) {
-                if (!wait(8 * (2 * ((u + 1) % D)), u + 1 < D ? ring_parity : ring_parity ^ 1)) return false;
+            const int tn = (t + B) & 1, un = u + (t + B) / 2;   // of job 2j + t + B
+            if (j + (t + B) / 2 < nt) {
+              if (tn == 0) {
+                if (!wait(8 * (2 * (un % D)), un / D % 2 ? ring_parity ^ 1 : ring_parity)) return false;
                 tc::fence_after();
               }
-              qk(t, (u + 1) % D);
-              if (t == 1) tc::commit_at(bars + kEmpty + 8 * (2 * ((u + 1) % D)));
+              qk(at, B == 2 ? t : bp ? b : b + B, tn, un % D);
+              if (tn == 1) tc::commit_at(bars + kEmpty + 8 * (2 * (un % D)));
             }
+            if (B > 2 && ++b == B) b = 0, bp ^= 1;
           }
           return true;
         };
         bool ok = wait(kQReady, 0) && wait(0, 0);
         tc::fence_after();
         if (ok) {
-          qk(0, 0);
-          qk(1, 0);
+          qk(0, 0, 0, 0);
+          qk(1, 1, 1, 0);
           tc::commit_at(bars + kEmpty);
+          if (B > 2 && nt > 1) {
+            ok = wait(16, 0);
+            tc::fence_after();
+            if (ok) qk(2, 2, 0, 1);
+          }
         }
         uint32_t parity = 0;
         for (int j = 0; j < nt && ok; j += D, parity ^= 1) {
@@ -911,7 +926,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     tc::regs_inc<224>();
     const int t = (warp - 4) >> 2, quarter = warp & 3, r = 128 * t + 32 * quarter + lane, row = row0 + r;
     const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
-    const uint32_t ts = lane_base + 128 * t, to = lane_base + 256 + 128 * t;
+    const uint32_t to = lane_base + kO + HD * t;
+    int job = t;                // modulo R
+    uint32_t job_parity = 0;
     const bool on = r < rows;
     float m = -INFINITY, l = 0.f;
     const float scale = p.scale * 1.44269504088896340736f;
@@ -934,7 +951,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int first_last = sp.len - sp.n + row0 / grp;   // the CTA's first row's last key
       bool ok = true;
       for (int j = 0; j < nt && ok; ++j) {
-        ok = wait_bounded(&s_full[t], j & 1, &g_paged_status);
+        const uint32_t at = B == 2 ? t : job < B ? job : job - B, ts = lane_base + 128 * at;
+        ok = wait_bounded(&s_full[B == 2 ? t : job], B == 2 ? j & 1 : job_parity, &g_paged_status);
         __syncwarp();
         tc::fence_after();
         uint32_t v[4][32];
@@ -1007,15 +1025,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             tc::wait_st();
             tc::fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_ready[2 * (c - 2) + t]);
+            if (lane == 0) mbar_arrive(&p_ready[B * (c - 2) + at]);
           }
         }
         const float2 both = unpair(sum);
         l += both.x + both.y;
+        job += 2;
+        if (job >= R) job -= R, job_parity ^= 1;
       }
       // a row that saw no key: the polynomial's least value is not zero
       if (m == -INFINITY && l == l) l = 0.f;
-      wait_bounded(&o_done[t], (nt - 1) & 1, &g_paged_status);
+      wait_bounded(B == 2 ? &o_done[t] : &o_last[t], B == 2 ? (nt - 1) & 1 : 0, &g_paged_status);
       __syncwarp();
       tc::fence_after();
     }
@@ -1053,7 +1073,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
     } else {
       // the second tile's last product is the last to read the ring
-      if (seq >= 0 && nt > 0) wait_bounded(&o_done[1], (nt - 1) & 1, &g_paged_status);
+      if (seq >= 0 && nt > 0) wait_bounded(B == 2 ? &o_done[1] : &o_last[1], B == 2 ? (nt - 1) & 1 : 0, &g_paged_status);
       __syncwarp();
       tc::fence_after();
       // parked at ring + row * HD * 4, 16-byte pieces permuted by the row so that eight lanes' stores take all banks
