@@ -27,10 +27,10 @@ namespace {
 // neighbouring vectors of the unrotated rest. A CTA holds up to four whole tokens. Once for all their heads it puts into
 // shared memory the norm weights, each token's place in the cache and its cosines and sines -- the angle in fp64 as a
 // multiple of pi (fp32 would lose 1e-3 of a turn at position 1e5) -- while the first values are already on their way;
-// each group's next head is on its way while it works on one. 8192 tokens, 28 + 2 x 4 heads of 128: 35.3 us, 4.3 TB/s
+// each group's next head is on its way while it works on one. 8192 tokens, 28 + 2 x 4 heads of 128: 33 us, 4.6 TB/s
 // (75.6 with one token a CTA and the norm weights and angles fetched by every group).
-constexpr int kAppendMaxThreads = 512;
-constexpr int kAppendTokens = 4;
+constexpr int kAppendThreads = 256;    // five CTAs an SM (4 or 6: 34.6, 37.4 us; 288 threads, a token a pass, four: 33.8)
+constexpr int kAppendTokens = 4;       // (2: 39 us, 8: 33.7)
 
 struct AppendParams {
   const void* qkv;
@@ -53,7 +53,7 @@ struct AppendParams {
 };
 
 template <typename T, int G>
-__global__ void __launch_bounds__(kAppendMaxThreads, 2) append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 5) append_kernel(const AppendParams p) {
   extern __shared__ __align__(16) uint8_t append_smem[];   // norm weights [2][hd], cache offsets [tpb][2], (cos, sin) [tpb][F]
   T* weights = reinterpret_cast<T*>(append_smem);
   int64_t* place = reinterpret_cast<int64_t*>(weights + 2 * p.hd);
@@ -1172,7 +1172,7 @@ cudaError_t append_t(const AppendParams& p, bool pdl, cudaStream_t st) {
   // whole tokens a CTA: what fills 256 threads, and up to four where there are many
   a.tpb = max(256 / per_token, (int)min((int64_t)kAppendTokens, (int64_t)p.tokens / (4 * sm_count())));
   a.tpb = max(1, min(a.tpb, p.tokens));
-  const int threads = min(kAppendMaxThreads, (min(a.tpb * per_token, max(256, per_token)) + 31) / 32 * 32);
+  const int threads = min(kAppendThreads, (a.tpb * per_token + 31) / 32 * 32);
   auto kern = G == 4 ? append_kernel<T, 4> : G == 8 ? append_kernel<T, 8> : append_kernel<T, 16>;
   return launch_paged(kern, dim3((unsigned)((p.tokens + a.tpb - 1) / a.tpb)), dim3(threads),
                       (size_t)2 * p.hd * sizeof(T) + a.tpb * 16 + (size_t)a.tpb * p.F * sizeof(float2), pdl, st, a);
