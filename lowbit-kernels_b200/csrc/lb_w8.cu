@@ -709,6 +709,101 @@ __global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) w8_gemv_kerne
   }
 }
 
+// ------------------------------------------------------------------------------------------- the product, a few tens of rows
+// The same fragments with rows quantized by a kernel before: a CTA takes 16 CT channels, all of K and up to 8 NT tokens,
+// its 16 warps the 64-byte pieces of K in turn; the tokens' fragments come straight from L2 like the weights'. Each warp's
+// first R pieces of weights are under way before the wait on the quantization (whose own wait covers what wrote the
+// weights). The warps' int32 tiles are summed in shared memory. Latency bound: what it saves is the set-up of the tcgen05
+// product's ring, tensor memory and cluster sum. (Tokens of the next piece under way under this one's MMAs: 3584 x 3584
+// M = 33 9.9 -> 9.6 us, 8960 x 1536 M = 33 13.7 -> 11.6.)
+constexpr int kRowsWarps = 16;
+
+struct W8Rows {
+  const int8_t* q;      // [M, kp]
+  const float* s;
+  const int8_t* w;
+  int64_t ldw;
+  const float* t;
+  const void* bias;
+  void* y;
+  int M, N, kp, pieces;
+};
+
+template <typename T, int CT, int NT>
+__global__ void __launch_bounds__(32 * kRowsWarps, 1) w8_rows_kernel(const W8Rows p) {
+  constexpr int R = CT * NT >= 10 ? 2 : CT * NT >= 6 ? 3 : 4, kCh = 16 * CT, kTok = 8 * NT, kPitch = kCh + 4;
+  extern __shared__ __align__(16) int rows_part[];   // [warps][kTok][kPitch]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * kCh;
+  pdl_launch_dependents();
+  const int8_t* w = p.w + 16 * t;
+  int64_t row[CT][2];   // rows past N repeat the last one
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) row[c][h] = (int64_t)min(n0 + 16 * c + 8 * h + g, p.N - 1) * p.ldw;
+  uint4 a[R][CT][2];
+  auto fetch = [&](int i, int piece) {   // shares past K as zeros (K is padded to 16, a lane's share)
+    const bool on = 64 * piece + 16 * t < p.kp;
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        a[i][c][h] = on ? ldg_stream(reinterpret_cast<const uint4*>(w + row[c][h] + 64 * piece)) : make_uint4(0, 0, 0, 0);
+  };
+#pragma unroll
+  for (int i = 0; i < R; ++i) fetch(i, warp + i * kRowsWarps);
+  int d[CT][NT][4] = {};
+  const int8_t* q = p.q + 16 * t;
+  int tok[NT];   // token rows past M repeat the last one, their columns are not stored
+#pragma unroll
+  for (int j = 0; j < NT; ++j) tok[j] = min(8 * j + g, p.M - 1) * p.kp;
+  pdl_wait();
+  uint4 b[2][NT];
+  auto tokens = [&](int k, int piece) {
+    const bool on = 64 * piece + 16 * t < p.kp;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) b[k][j] = on ? ldg_cg_u128(q + tok[j] + 64 * piece) : make_uint4(0, 0, 0, 0);
+  };
+  tokens(0, warp);
+  for (int c0 = warp; c0 < p.pieces; c0 += kRowsWarps * R) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int piece = c0 + i * kRowsWarps;
+      if (piece < p.pieces) {
+        tokens((i + 1) & 1, piece + kRowsWarps);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int c = 0; c < CT; ++c) {
+            const uint4 x = b[i & 1][j];
+            mma_s8(d[c][j], a[i][c][0].x, a[i][c][1].x, a[i][c][0].y, a[i][c][1].y, x.x, x.y);
+            mma_s8(d[c][j], a[i][c][0].z, a[i][c][1].z, a[i][c][0].w, a[i][c][1].w, x.z, x.w);
+          }
+        fetch(i, piece + kRowsWarps * R);
+      }
+    }
+  }
+  int* mine = rows_part + warp * kTok * kPitch;
+#pragma unroll
+  for (int c = 0; c < CT; ++c)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mine[(8 * j + 2 * t + (e & 1)) * kPitch + 16 * c + g + (e >> 1) * 8] = d[c][j][e];
+  __syncthreads();
+  for (int i = tid; i < kTok * kCh; i += 32 * kRowsWarps) {
+    const int m = i / kCh, c = i % kCh, n = n0 + c;
+    if (m < p.M && n < p.N) {
+      int sum = 0;
+#pragma unroll
+      for (int k = 0; k < kRowsWarps; ++k) sum += rows_part[(k * kTok + m) * kPitch + c];
+      static_cast<T*>(p.y)[(int64_t)m * p.N + n] = Elem<T>::from_float(
+          fmaf(__int2float_rn(sum) * p.s[m], p.t[n], p.bias ? Elem<T>::to_float(static_cast<const T*>(p.bias)[n]) : 0.f));
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------- launches
 template <typename Kern, typename... Args>
 cudaError_t launch_w8(Kern kern, unsigned grid, int threads, size_t smem, int cluster, bool pdl, cudaStream_t st,
@@ -867,16 +962,51 @@ cudaError_t gemv_t(const W8Params& p, bool pdl, cudaStream_t st) {
   return launch_w8(kern, (unsigned)ctas, 32 * warps, (size_t)p.M * pitch, 1, pdl, st, g, p.early);
 }
 
+// Up to 40 rows on layers of one round of 32-channel CTAs, while K is short enough for latency to count for more than the
+// tokens' second way through L2 (cold weights, tcgen05 / this, with the quantization: 3584 x 3584 M = 9 9.1 / 7.1 us,
+// M = 40 9.9 / 9.8; 4096 x 4096 M = 24 10.5 / 8.6; 4864 x 896 M = 33 9.0 / 7.8; 8960 x 1536 M = 24 10.9 / 10.1,
+// M = 40 11.1 / 11.7; 18944 x 3584 M = 9 17.9 / 23.3).
+bool rows_takes(int64_t M, int64_t N, int64_t K, int sms) {
+  return M <= 40 && N <= 32 * (int64_t)sms && K <= (M <= 24 ? 10240 : 5120);
+}
+
+template <typename T, int CT, int NT>
+cudaError_t rows_launch(const W8Rows& r, bool pdl, cudaStream_t st) {
+  constexpr size_t smem = (size_t)kRowsWarps * 8 * NT * (16 * CT + 4) * sizeof(int);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(w8_rows_kernel<T, CT, NT>, done, (int)smem);
+  if (e != cudaSuccess) return e;
+  return launch_w8(w8_rows_kernel<T, CT, NT>, (unsigned)((r.N + 16 * CT - 1) / (16 * CT)), 32 * kRowsWarps, smem, 1, pdl, st, r);
+}
+
+template <typename T>
+cudaError_t rows_t(const W8Params& p, const int8_t* q, const float* s, int kp, int sms, bool pdl, cudaStream_t st) {
+  const W8Rows r{q, s, static_cast<const int8_t*>(p.w), p.ldw, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, kp, (kp + 63) / 64};
+  if (p.N <= 16 * (int64_t)sms)
+    return p.M <= 8    ? rows_launch<T, 1, 1>(r, pdl, st)
+           : p.M <= 16 ? rows_launch<T, 1, 2>(r, pdl, st)
+           : p.M <= 24 ? rows_launch<T, 1, 3>(r, pdl, st)
+                       : rows_launch<T, 1, 5>(r, pdl, st);
+  return p.M <= 8    ? rows_launch<T, 2, 1>(r, pdl, st)
+         : p.M <= 16 ? rows_launch<T, 2, 2>(r, pdl, st)
+         : p.M <= 24 ? rows_launch<T, 2, 3>(r, pdl, st)
+                     : rows_launch<T, 2, 5>(r, pdl, st);
+}
+
 template <typename T>
 cudaError_t linear_t(const W8Params& p, bool pdl, cudaStream_t st) {
   if (gemv_takes(p.M, p.K)) return gemv_t<T>(p, pdl, st);
   const int sms = sm_count();
   const int64_t kp = padded(p.K);
   const int chunks = (int)((kp + kChunk - 1) / kChunk);
-  CUtensorMap wmap, qmap;
-  if (!encode_rows(&wmap, p.w, kp, p.ldw, p.N, 128)) return cudaErrorInvalidValue;
   int8_t* q = static_cast<int8_t*>(p.workspace);
   float* s = reinterpret_cast<float*>(q + p.M * kp);
+  if (rows_takes(p.M, p.N, p.K, sms)) {
+    const cudaError_t e = quantize_t<T>(p.x, p.ldx, q, kp, s, p.M, p.K, p.early ? kAtEntry : kAfterWait, pdl, st);
+    return e == cudaSuccess ? rows_t<T>(p, q, s, (int)kp, sms, pdl, st) : e;
+  }
+  CUtensorMap wmap, qmap;
+  if (!encode_rows(&wmap, p.w, kp, p.ldw, p.N, 128)) return cudaErrorInvalidValue;
   cudaError_t e = quantize_t<T>(p.x, p.ldx, q, kp, s, p.M, p.K, p.early ? kAtEntry : kAfterWait, pdl, st);
   if (e != cudaSuccess) return e;
   static thread_local struct {   // the last plan of this host thread: a layer's calls follow one another

@@ -142,6 +142,19 @@ def test_linear_w8_extreme_sums_are_exact():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,n", [(100, 2500), (513, 4700), (2048, 4736), (5120, 2369), (9000, 2400), (10256, 2384)])
+def test_linear_w8_up_to_forty_rows(dtype, k, n):
+    ops, _ = mods()
+    g = gen(k + n)
+    w8 = ops.W8Weight.from_float(randn(g, n, k, std=0.05))
+    bias = randn(g, n, dtype=dtype)
+    for m in (1, 3, 8, 9, 16, 17, 24, 25, 40, 41):
+        x = randn(g, m, k, dtype=dtype)
+        check_linear(x, w8.q, w8.scales, bias, ops.linear_w8(x, w8, bias=bias))
+
+
+@gpu
 @pytest.mark.parametrize("k", [8193, 20000, 50001, 100000])
 def test_linear_w8_long_rows(k):
     """Rows longer than the registers hold, and than shared memory holds; aligned to 16 bytes or to 2."""
