@@ -731,8 +731,9 @@ struct W8Rows {
 
 template <typename T, int CT, int NT>
 __global__ void __launch_bounds__(32 * kRowsWarps, 1) w8_rows_kernel(const W8Rows p) {
-  constexpr int R = CT * NT >= 10 ? 2 : CT * NT >= 6 ? 3 : 4, kCh = 16 * CT, kTok = 8 * NT, kPitch = kCh + 4;
+  constexpr int R = CT * NT >= 10 ? 2 : 4, kCh = 16 * CT, kTok = 8 * NT, kPitch = kCh + 4;
   extern __shared__ __align__(16) int rows_part[];   // [warps][kTok][kPitch]
+  static_assert(R % 2 == 0, "the two token buffers alternate from round to round");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * kCh;
   pdl_launch_dependents();
