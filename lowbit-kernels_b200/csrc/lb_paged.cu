@@ -17,6 +17,37 @@ __device__ int g_paged_status;
 
 namespace {
 
+// two fp32 values in one 64-bit register pair
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t neg2(uint64_t a) {
+  const float2 v = unpair(a);
+  return pair(-v.x, -v.y);
+}
+
 // ------------------------------------------------------------------------------------------------------- append
 // q and k heads: x <- x rsqrt(mean(x^2) + eps) w (where norm weights are given), then the pair (x_i, x_{i + F}),
 // i < F, turned by the angle pos * f_i; the dimensions from 2F on are left as they are. v heads are copied. All in
@@ -54,10 +85,11 @@ struct AppendParams {
 
 template <typename T, int G>
 __global__ void __launch_bounds__(kAppendThreads, 5) append_kernel(const AppendParams p) {
-  extern __shared__ __align__(16) uint8_t append_smem[];   // norm weights [2][hd], cache offsets [tpb][2], (cos, sin) [tpb][F]
-  T* weights = reinterpret_cast<T*>(append_smem);
+  extern __shared__ __align__(16) uint8_t append_smem[];   // norm weights [2][hd], cache offsets [tpb][2], cos, sin [tpb][F]
+  float* weights = reinterpret_cast<float*>(append_smem);
   int64_t* place = reinterpret_cast<int64_t*>(weights + 2 * p.hd);
-  float2* turn = reinterpret_cast<float2*>(place + 2 * p.tpb);
+  float* cosines = reinterpret_cast<float*>(place + 2 * p.tpb);
+  float* sines = cosines + p.tpb * p.F;
   pdl_launch_dependents();
   const int heads = p.nh + 2 * p.nkv, f8 = p.F / 8;
   const int t0 = blockIdx.x * p.tpb, nt = min(p.tpb, p.tokens - t0), units = nt * heads;
@@ -67,11 +99,12 @@ __global__ void __launch_bounds__(kAppendThreads, 5) append_kernel(const AppendP
   if (!p.early) pdl_wait();
   if (norm)
     for (int i = threadIdx.x; i < 2 * p.hd; i += blockDim.x)
-      weights[i] = i < p.hd ? static_cast<const T*>(p.q_norm)[i] : static_cast<const T*>(p.k_norm)[i - p.hd];
+      weights[i] = Elem<T>::to_float(i < p.hd ? static_cast<const T*>(p.q_norm)[i] : static_cast<const T*>(p.k_norm)[i - p.hd]);
   if (p.early) pdl_wait();
   const T* qkv = static_cast<const T*>(p.qkv) + t0 * p.ld;
+  T* q_out = static_cast<T*>(p.q_out) + (int64_t)t0 * p.nh * p.hd;
   int u = threadIdx.x / G, tl = u / heads, head = u - tl * heads;
-  uint4 x[2], next[2];
+  uint4 x[2] = {}, next[2] = {};   // lanes past the head dim hold zeros
   auto load = [&](uint4 (&d)[2], int unit, int tok, int h) {
     if (unit < units && on) {
       const T* src = qkv + tok * p.ld + h * p.hd;
@@ -100,7 +133,8 @@ __global__ void __launch_bounds__(kAppendThreads, 5) append_kernel(const AppendP
     a -= 2.0 * rint(a * 0.5);
     float sn, cs;
     sincospif((float)a, &sn, &cs);
-    turn[i] = make_float2(cs, sn);
+    cosines[i] = cs;
+    sines[i] = sn;
   }
   __syncthreads();
   for (int u0 = 0; u0 < units; u0 += per) {
@@ -110,30 +144,33 @@ __global__ void __launch_bounds__(kAppendThreads, 5) append_kernel(const AppendP
     head += per;
     while (head >= heads) head -= heads, ++tl;
     load(next, u, tl, head);
-    float f[16];
+    uint64_t f[8];   // two values each: an fp32 pair takes one instruction, and those bound this kernel beside memory
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 a = live ? Elem<T>::unpack(reinterpret_cast<const uint32_t*>(x)[i]) : make_float2(0.f, 0.f);
-      f[2 * i] = a.x;
-      f[2 * i + 1] = a.y;
+      const float2 a = Elem<T>::unpack(reinterpret_cast<const uint32_t*>(x)[i]);
+      f[i] = pair(a.x, a.y);
     }
     const bool is_q = h < p.nh, is_v = h >= p.nh + p.nkv;
     if (norm) {
-      float ss = 0.f;
+      uint64_t sq = mul2(f[0], f[0]);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) ss += f[i] * f[i];
+      for (int i = 1; i < 8; ++i) sq = fma2(f[i], f[i], sq);
+      const float2 both = unpair(sq);
+      float ss = both.x + both.y;
 #pragma unroll
       for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       if (live && !is_v) {
         const float r = rsqrtf(ss / (float)p.hd + p.eps);
-        const T* w = weights + (is_q ? 0 : p.hd);
-        const uint4 w0 = *reinterpret_cast<const uint4*>(w + 8 * v0), w1 = *reinterpret_cast<const uint4*>(w + 8 * v1);
-        const uint32_t ww[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        const ulonglong2* w0 = reinterpret_cast<const ulonglong2*>(weights + (is_q ? 0 : p.hd) + 8 * v0);
+        const ulonglong2* w1 = reinterpret_cast<const ulonglong2*>(weights + (is_q ? 0 : p.hd) + 8 * v1);
+        const uint64_t rr = pair(r, r);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 a = Elem<T>::unpack(ww[i]);
-          f[2 * i] = f[2 * i] * r * a.x;
-          f[2 * i + 1] = f[2 * i + 1] * r * a.y;
+        for (int i = 0; i < 2; ++i) {
+          const ulonglong2 a = w0[i], b = w1[i];
+          f[2 * i] = mul2(mul2(f[2 * i], rr), a.x);
+          f[2 * i + 1] = mul2(mul2(f[2 * i + 1], rr), a.y);
+          f[4 + 2 * i] = mul2(mul2(f[4 + 2 * i], rr), b.x);
+          f[5 + 2 * i] = mul2(mul2(f[5 + 2 * i], rr), b.y);
         }
       }
     }
@@ -141,23 +178,27 @@ __global__ void __launch_bounds__(kAppendThreads, 5) append_kernel(const AppendP
     x[1] = next[1];
     if (!live) continue;
     if (!is_v && lane < f8) {
-      const float4* cs = reinterpret_cast<const float4*>(turn + tok * p.F + 8 * lane);
+      const ulonglong2* cs = reinterpret_cast<const ulonglong2*>(cosines + tok * p.F + 8 * lane);
+      const ulonglong2* sn = reinterpret_cast<const ulonglong2*>(sines + tok * p.F + 8 * lane);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 c = cs[i];
-        const float a = f[2 * i], b = f[8 + 2 * i], d = f[2 * i + 1], e = f[9 + 2 * i];
-        f[2 * i] = a * c.x - b * c.y;
-        f[8 + 2 * i] = b * c.x + a * c.y;
-        f[2 * i + 1] = d * c.z - e * c.w;
-        f[9 + 2 * i] = e * c.z + d * c.w;
+      for (int i = 0; i < 2; ++i) {
+        const ulonglong2 c = cs[i], d = sn[i];
+        const uint64_t a0 = f[2 * i], a1 = f[2 * i + 1], b0 = f[4 + 2 * i], b1 = f[5 + 2 * i];
+        f[2 * i] = fma2(a0, c.x, neg2(mul2(b0, d.x)));
+        f[2 * i + 1] = fma2(a1, c.y, neg2(mul2(b1, d.y)));
+        f[4 + 2 * i] = fma2(b0, c.x, mul2(a0, d.x));
+        f[5 + 2 * i] = fma2(b1, c.y, mul2(a1, d.y));
       }
     }
     uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = Elem<T>::pack(f[2 * i], f[2 * i + 1]);
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = unpair(f[i]);
+      w[i] = Elem<T>::pack(v.x, v.y);
+    }
     T* dst;
     if (is_q) {
-      dst = static_cast<T*>(p.q_out) + ((int64_t)(t0 + tok) * p.nh + h) * p.hd;
+      dst = q_out + (tok * p.nh + h) * p.hd;
     } else {
       const int64_t at = place[2 * tok + is_v];
       if (at < 0) continue;
@@ -565,27 +606,6 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnPara
 // at hd 128, 1024 at hd 64. 28/4 heads of 128: 4096 new tokens 115 us (1050 TFLOP/s), over 32768 1550 us (1160); 14/2 of
 // 64: 4096 over 16384 370 us (570). Neither MMAs issued by two warps (873 for 1072), nor two softmax threads a row (3 %
 // more on long contexts, 7 % less on short ones) came out ahead.
-// two fp32 values in one 64-bit register pair
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if one of them is
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -1175,7 +1195,7 @@ cudaError_t append_t(const AppendParams& p, bool pdl, cudaStream_t st) {
   const int threads = min(kAppendThreads, (a.tpb * per_token + 31) / 32 * 32);
   auto kern = G == 4 ? append_kernel<T, 4> : G == 8 ? append_kernel<T, 8> : append_kernel<T, 16>;
   return launch_paged(kern, dim3((unsigned)((p.tokens + a.tpb - 1) / a.tpb)), dim3(threads),
-                      (size_t)2 * p.hd * sizeof(T) + a.tpb * 16 + (size_t)a.tpb * p.F * sizeof(float2), pdl, st, a);
+                      (size_t)2 * p.hd * sizeof(float) + a.tpb * 16 + (size_t)a.tpb * p.F * sizeof(float2), pdl, st, a);
 }
 
 // CTAs of the few-rows kernel that can be resident at once in clusters of C, on the current device
