@@ -1227,10 +1227,12 @@ int few_resident(int C) {
 }
 
 // How few rows are laid out: tiles of 8 or 16 rows, clusters of C CTAs, Z clusters a context -- the choice whose estimated
-// time is least, in microseconds as measured: 4 to start and end a CTA, 1 a block of keys and warp, more where memory
-// bounds all CTAs' blocks together, 1 to join a cluster, 4 for the second kernel; CTAs past those resident at once come
-// in further rounds, with a quarter of a round of tail. A warp takes at most 48 blocks where a split can help it:
-// contexts differ, and the longest ends last.
+// time is least, in microseconds as measured: 4 to start and end a CTA; a block of keys and warp 1.5 (hd 64: 0.95), by one
+// in a thousand CTAs more, or what memory takes for all CTAs' blocks together; 1 to join a cluster, 4 for the second
+// kernel; CTAs past those resident at once come in further rounds. A warp takes at most 36 blocks where a split can help
+// it: contexts differ, and the longest ends last. (C = 1, 2, 3, 4, 6: 32 contexts of 4096, 28/4 heads of 128 100, 60, 47,
+// 66, 53 us; 64 of 4096 110, 124, 92, 104, 104; 100 of 3000, 16/2 heads 79, 53, 68, 58, 64; 96 of up to 8192, 28/4 heads
+// 196, 146, 135, 131, 134.)
 struct FewPlan {
   int nt, row_tiles, C, Z;
   int64_t items;
@@ -1249,10 +1251,12 @@ FewPlan few_plan(int64_t rows, int64_t seqs, int nkv, int hd, int64_t max_len) {
     for (int Z = 1; Z <= (C == kFewCluster ? kFewParts : 1); ++Z) {
       if (C * Z > 1 && blocks < 2 * C * Z) break;
       const int64_t turns = (blocks + C * Z * kFewWarps - 1) / (C * Z * kFewWarps);
-      const double ctas = (double)(f.items * C * Z), full = ctas / resident;
-      const double turn = max(1.0, min(ctas, resident) * kFewWarps * 16 * hd * 4 / 6.2e6);
-      double t = (full <= 1 ? 1 : full + 0.25) * (4 + turns * turn) + (C > 1) + (Z > 1 ? 4 : 0);
-      if (turns > 48) t += turns;
+      const double ctas = (double)(f.items * C * Z), rounds = floor(ctas / resident), rest = ctas - rounds * resident;
+      auto round = [&](double n) {
+        return 4 + (C > 1) + turns * max((hd == 128 ? 1.5 : 0.95) + 0.001 * n, n * kFewWarps * 16 * hd * 4 / 6.2e6);
+      };
+      double t = rounds * round(resident) + (rest > 0 ? round(rest) : 0) + (Z > 1 ? 4 : 0);
+      if (turns > 36) t += turns;
       if (t < least) least = t, f.C = C, f.Z = Z;
     }
   }
