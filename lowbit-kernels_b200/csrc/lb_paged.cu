@@ -58,7 +58,7 @@ __device__ __forceinline__ uint64_t neg2(uint64_t a) {
 // neighbouring vectors of the unrotated rest. A CTA holds up to four whole tokens. Once for all their heads it puts into
 // shared memory the norm weights, each token's place in the cache and its cosines and sines -- the angle in fp64 as a
 // multiple of pi (fp32 would lose 1e-3 of a turn at position 1e5) -- while the first values are already on their way;
-// each group's next head is on its way while it works on one. 8192 tokens, 28 + 2 x 4 heads of 128: 33 us, 4.6 TB/s
+// each group's next head is on its way while it works on one. 8192 tokens, 28 + 2 x 4 heads of 128: 32 us, 4.7 TB/s
 // (75.6 with one token a CTA and the norm weights and angles fetched by every group).
 constexpr int kAppendThreads = 256;    // five CTAs an SM (4 or 6: 34.6, 37.4 us; 288 threads, a token a pass, four: 33.8)
 constexpr int kAppendTokens = 4;       // (2: 39 us, 8: 33.7)
@@ -592,6 +592,8 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnPara
 //   * MMA warp: S_t = Q_t K^T (K-major operands) into tensor memory, O_t += P_t V with P_t, the A operand, in tensor memory
 //     over S_t's columns and V taken as it lies (MN-major B). PV of one tile and the next QK^T of the same tile are issued
 //     together, so that while one tile's softmax runs the tensor core works for the other.
+//     At hd 64 tensor memory holds a third tile of scores: QK^T then runs three row tiles ahead, and a softmax finds its
+//     next scores there when it is done.
 //   * two softmax warpgroups, one a tile: a thread reads its row's 128 scores at once, moves its running maximum only
 //     when one exceeds it by 8 in powers of two (weights stay below 2^8; else O would be rescaled in tensor memory every
 //     tile), writes the weights back as 16-bit pairs, and keeps their fp32 sum unrounded.
@@ -602,10 +604,11 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnPara
 // Few tiles: a cluster of C CTAs splits the keys; each parks O, maxima and sums in its idle ring and all join their share
 // of the rows through distributed shared memory, in one fixed order. (Pushing the parts to their owners instead: 33 us
 // where this takes 29.)
-// Bound by the softmax beside the MMAs: a step of 256 rows x 128 keys takes some 3100 clocks, of which the MMAs need 2048
-// at hd 128, 1024 at hd 64. 28/4 heads of 128: 4096 new tokens 115 us (1050 TFLOP/s), over 32768 1550 us (1160); 14/2 of
-// 64: 4096 over 16384 370 us (570). Neither MMAs issued by two warps (873 for 1072), nor two softmax threads a row (3 %
-// more on long contexts, 7 % less on short ones) came out ahead.
+// Bound by the softmax beside the MMAs: a step of 256 rows x 128 keys takes some 3100 clocks at hd 128, of which the MMAs
+// need 2048, and 2700 at hd 64 (1024), with two warps a scheduler issuing 40 % of the time. 28/4 heads of 128: 4096 new
+// tokens 114 us (1050 TFLOP/s), over 32768 1530 us (1180); 14/2 of 64: 4096 over 16384 323 us (650; 370 with two score
+// tiles). Neither MMAs issued by two warps (873 for 1072), nor two softmax threads a row (3 % more on long contexts, 7 %
+// less on short ones) came out ahead.
 __device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if one of them is
   float r;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -1345,13 +1348,14 @@ cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   // every sequence's last tile may be partial
   cp.tiles = (int)min(p.seqs * ((p.max_new * grp + kTileRows - 1) / kTileRows), (p.tokens * grp + kTileRows - 1) / kTileRows + p.seqs);
   const int64_t items = (int64_t)cp.tiles * p.nkv, key_tiles = (p.max_len + kTileKeys - 1) / kTileKeys;
-  // The cluster that costs least: rounds of CTAs times their key tiles (1.2 us each, measured) and 6 us to start and end,
-  // 3 more to join a cluster
+  // The cluster that costs least: rounds of CTAs times their key tiles (1.4 us each, measured) and 6 us to start and end,
+  // 6 more to join a cluster (C = 1, 2, 3, 4: 300 tokens over 4096, 28/4 heads of 128 61, 44, 35, 49 us; 1000 over 1000,
+  // 16/2 heads 21, 24, 33, 32; 500 over 2000, 14/2 heads of 64 29, 23, 20, 17)
   double least = 1e30;
   cp.C = 1;
   for (int C = 1; C <= kChunkCluster && (C == 1 || key_tiles >= 2 * C); ++C) {
     const int64_t resident = C == 1 ? sm_count() : chunk_resident<HD>(C), rounds = (items + resident - 1) / resident;
-    const double t = (double)rounds * (6 + (C > 1 ? 3 : 0) + 1.2 * (double)((key_tiles + C - 1) / C));
+    const double t = (double)rounds * (6 + (C > 1 ? 6 : 0) + 1.4 * (double)((key_tiles + C - 1) / C));
     if (t < least) least = t, cp.C = C;
   }
   CUtensorMap kmap, vmap;
