@@ -312,11 +312,11 @@ LB_API int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens
  * value belong to no sequence and are left unwritten) and, them included, a context of seq_lens[s] tokens in the
  * cache; its new token i of n sees keys 0 .. seq_lens[s] - n + i. A token that sees none gets zeros. seq_lens above
  * table_width * page_size are cut to that. page_table int32 [seqs, table_width], rows table_stride apart; entries past
- * a context are not read; an entry outside the cache sets lb_device_error() to 3 (its keys count as zeros or not at
- * all). max_new / max_len: upper bounds of the new tokens and the context of any sequence (tokens and
- * table_width * page_size if unknown): a smaller value than the truth is an error that leaves outputs undefined but
- * stays inside every buffer. q's heads and tokens are strided (multiples of 8 elements), out's tokens too. hd 64 or
- * 128. Rows of the cache past a context may hold anything, NaN included. workspace:
+ * a context are not read; an entry outside the cache is not followed: its keys and values count as zeros, and
+ * lb_device_error() becomes 3. max_new / max_len: upper bounds of the new tokens and the context of any sequence
+ * (tokens and table_width * page_size if unknown): a smaller value than the truth is an error that leaves outputs
+ * undefined but stays inside every buffer. q's heads and tokens are strided (multiples of 8 elements), out's tokens
+ * too. hd 64 or 128. Rows of the cache past a context may hold anything, NaN included. workspace:
  * lb_paged_attention_workspace(...) bytes on the current device (0: none needed), 16-byte aligned, its content
  * undefined before and after; calls that can overlap need distinct ones.
  */

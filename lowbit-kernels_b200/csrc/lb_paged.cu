@@ -327,19 +327,19 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
   const int per_page = p.page_size / 16;
   const T* kbase = static_cast<const T*>(p.k) + (int64_t)kvh * p.page_size * HD;
   const T* vbase = static_cast<const T*>(p.v) + (int64_t)kvh * p.page_size * HD;
-  auto page_of = [&](int u, bool start) {   // start: the first lookups, which `pages0` may answer
+  auto page_of = [&](int u, bool start) {   // start: the first lookups, which `pages0` may answer; -1: no such page
     const int at = u / per_page;
     int pg = 0;
     if (u < u1) pg = start && at < 32 ? __shfl_sync(0xffffffffu, pages0, at) : table[at];
     if (pg < 0 || pg >= p.num_pages) {
       atomicExch(&g_paged_status, kErrBadPosition);
-      pg = 0;
+      pg = -1;
     }
     return pg;
   };
   uint4 kf[KI][2], vf[VH][4];
   auto load_k = [&](int u, int pg) {
-    const T* src = kbase + pg * p.k_page + (int64_t)(u % per_page) * 16 * HD + g * HD + 8 * t;
+    const T* src = kbase + max(pg, 0) * p.k_page + (int64_t)(u % per_page) * 16 * HD + g * HD + 8 * t;
 #pragma unroll
     for (int i = 0; i < KI; ++i) {
       kf[i][0] = ldg_cg_u128(src + 32 * i);
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
     }
   };
   auto load_v = [&](int u, int pg) {
-    const T* src = vbase + pg * p.v_page + (int64_t)(u % per_page) * 16 * HD + 2 * t * HD + 8 * g;
+    const T* src = vbase + max(pg, 0) * p.v_page + (int64_t)(u % per_page) * 16 * HD + 2 * t * HD + 8 * g;
 #pragma unroll
     for (int h = 0; h < VH; ++h) {
       vf[h][0] = ldg_cg_u128(src + 64 * h);
@@ -378,6 +378,13 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
       }
     }
     const int un = u + kFewWarps;
+    // keys and values of a page outside the cache count as zeros: what was loaded in their place is dropped here, since
+    // a branch around the loads costs every block (96 contexts of up to 8192: 134 -> 138 us)
+    const bool absent = page < 0;
+    if (absent) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+    }
     page = page_next;
     page_next = page_of(un + kFewWarps, false);
     if (un < u1) load_k(un, page);
@@ -423,10 +430,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
       b[nt][0] = transpose8(Elem<T>::pack(w[0], w[1]));
       b[nt][1] = transpose8(Elem<T>::pack(w[2], w[3]));
     }
-    if (16 * u + 16 > keys) {   // V rows that no row of the tile sees
+    if (absent || 16 * u + 16 > keys) {   // V rows that no row of the tile sees
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (16 * u + 2 * t + (j & 1) + (j >= 2 ? 8 : 0) >= keys)
+        if (absent || 16 * u + 2 * t + (j & 1) + (j >= 2 ? 8 : 0) >= keys)
 #pragma unroll
           for (int h = 0; h < VH; ++h) vf[h][j] = make_uint4(0, 0, 0, 0);
     }
@@ -808,7 +815,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             page = table[tp];
             if (page < 0 || page >= p.num_pages) {
               if (half == 0) atomicExch(&g_paged_status, kErrBadPosition);
-              page = 0;
+              page = (int)p.num_pages;   // past the tensor map's last page: the copy writes zeros
             }
           }
         };

@@ -81,7 +81,8 @@ def norm_rope_append(qkv, cache, positions, slots, nh, inv_freq, q_norm=None, k_
     """One pass over the fused projection's rows qkv [T, (nh + 2 nkv) hd] of T new tokens (rows a multiple of 8 elements
     apart): q and k heads times rsqrt(mean(x^2) + eps) times q_norm / k_norm ([hd], both or neither), their first
     2 * len(inv_freq) dimensions rotated (rotate-half) by positions[t] * inv_freq (int64 [T], fp32), then k and v stored
-    at the cache's slots (int64 [T]; negative: not stored). Returns q [T, nh, hd] (`out`, when given). All in fp32 with
+    at the cache's slots (int64 [T]; negative: not stored; past the cache: not stored, and the device status becomes 3, as in
+    `attention`). Returns q [T, nh, hd] (`out`, when given). All in fp32 with
     one rounding."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc:
@@ -128,7 +129,9 @@ def attention(q, cache, page_table, seq_lens, cu_new, max_new=None, max_len=None
 
     max_new and max_len bound the new tokens and the context of any sequence (host integers; by default T and
     W * page_size). They choose the kernel and how contexts are split, so a decode step passes max_new=1; a bound below
-    the truth is an error that leaves outputs undefined. scale defaults to 1 / sqrt(hd). Tokens past cu_new[S] (a padded
+    the truth is an error that leaves outputs undefined. A page-table entry outside the cache counts as a page of zeros and
+    sets the library's device status to 3 (`ops.ext().lib.lb_device_error()`, which synchronizes; no call reads it by
+    itself). scale defaults to 1 / sqrt(hd). Tokens past cu_new[S] (a padded
     batch's) belong to no sequence: their outputs are left unwritten."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc:

@@ -552,6 +552,34 @@ def test_attention_reports_a_page_outside_the_cache(new):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new", [1, 5, 100])
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 48), (128, 128)])
+def test_attention_keys_of_a_page_outside_the_cache_count_as_zeros(dtype, new, hd, page):
+    """Entries below and above the cache, in the middle and at the end of a context: the same as a page of zeros; no other
+    page, the first one above all, takes their place."""
+    ops, paged = mods()
+    lib = ops.ext().lib
+    q, cache, table, lens, cu = build(gen(14), [new], [700], 8, 2, hd, page, dtype, spare=3)
+    swap = table == 0   # no context holds page 0: the last spare page takes its place
+    spare = next(i for i in range(1, cache.num_pages) if not (table[0, :-(-700 // page)] == i).any())
+    cache.k[spare], cache.v[spare] = cache.k[0].clone(), cache.v[0].clone()
+    table[swap] = spare
+    cache.k[0], cache.v[0] = 3.0, float("nan")
+    last = -(-700 // page) - 1
+    table[0, 1], table[0, 3], table[0, last - 1], table[0, last] = -1, cache.num_pages, -2 ** 31, 2 ** 31 - 1
+    y = paged.attention(q, cache, table, lens, cu, max_new=new)
+    assert lib.lb_device_error() == 3
+    lib.lb_clear_device_error()
+    whole = paged.PagedCache.from_tensors(*(torch.cat((x, torch.zeros_like(x[:1]))) for x in (cache.k, cache.v)))
+    zeros = table.clone()
+    zeros[0, [1, 3, last - 1, last]] = cache.num_pages
+    check_attention(q, whole, zeros, [700], [new], y, 1 / math.sqrt(hd))
+    assert torch.equal(y, paged.attention(q, whole, zeros, lens, cu, max_new=new))
+    assert lib.lb_device_error() == 0
+
+
+@gpu
 def test_attention_refusals():
     _, paged = mods()
     q, cache, table, lens, cu = build(gen(4), [2, 1], [20, 9], 4, 2, 64, 16, torch.float16)
