@@ -458,6 +458,26 @@ def test_attention_scores_that_are_not_finite_reach_the_rows_that_see_them(dtype
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,ctx", [(2, 40), (100, 300), (300, 1500)])
+def test_attention_values_of_unseen_keys_have_no_weight(dtype, hd, new, ctx):
+    """Values at the end of the type's range: rows before the key are bit for bit what they were. Keys at every place of
+    a block, since the exponentials are not all taken the same way."""
+    _, paged = mods()
+    q, cache, table, lens, cu = build(gen(16), [new], [ctx], 16, 2, hd, 32, dtype)
+    clean = paged.attention(q, cache, table, lens, cu, max_new=new)
+    for back in sorted({b for b in (*range(1, 18), new // 2) if b < new}):
+        key = ctx - back
+        at, row = int(table[0, key // 32]), key % 32
+        keep = cache.v[at, :, row].clone()
+        cache.v[at, :, row] = -0.9 * torch.finfo(dtype).max
+        y = paged.attention(q, cache, table, lens, cu, max_new=new)
+        assert torch.equal(y[:new - back], clean[:new - back]), back
+        cache.v[at, :, row] = keep
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_large_scores_and_constant_rows(dtype):
     """Scores far apart (one key takes all the weight; the maximum found first, or last) and all alike."""
     ops, paged = mods()
