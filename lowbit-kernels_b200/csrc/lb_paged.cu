@@ -815,11 +815,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (mine && j < nt && key < keys) {
             const int idx = key / cp.piece, tp = idx / per_page;
             row = kvh * p.page_size + (idx - tp * per_page) * cp.piece;
-            page = table[tp];
-            if (page < 0 || page >= p.num_pages) {
-              if (half == 0) atomicExch(&g_paged_status, kErrBadPosition);
-              page = (int)p.num_pages;   // past the tensor map's last page: the copy writes zeros
-            }
+            // past the cache: the tensor map's first page that is not there, of which the copy writes zeros
+            const uint32_t listed = (uint32_t)table[tp], pages = (uint32_t)p.num_pages;
+            page = (int)min(listed, pages);
+            if (listed >= pages && half == 0) atomicExch(&g_paged_status, kErrBadPosition);
           }
         };
         int page, row = 0, page_next, row_next = 0;
