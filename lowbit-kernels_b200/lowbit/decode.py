@@ -33,6 +33,31 @@ def qwen2_config(arch, **overrides):
     return cfg
 
 
+def context_limit(cfg):
+    """The longest context for which the decoders of this package compute what `cfg` (a transformers config) says -- plain
+    rotary angles over whole heads, attention to every earlier token, SiLU -- or None where any length will do. Raises
+    ValueError where none does."""
+    limits = []
+    rope = cfg.rope_parameters
+    kind = rope.get("rope_type", "default")
+    if kind == "dynamic":   # the plain angles up to the length that the model was trained on
+        limits.append(cfg.max_position_embeddings)
+    elif kind != "default":
+        raise ValueError(f'rope_type "{kind}" is not supported: rotary angles are position * theta^(-2i / hd), unscaled')
+    part = rope.get("partial_rotary_factor", getattr(cfg, "partial_rotary_factor", None))
+    if part not in (None, 1):
+        raise ValueError(f"partial_rotary_factor={part} is not supported: whole heads are rotated")
+    kinds = set(getattr(cfg, "layer_types", None) or ["full_attention"])
+    if "sliding_attention" in kinds and cfg.sliding_window:   # all there is, while the window holds it
+        limits.append(cfg.sliding_window)
+        kinds.remove("sliding_attention")
+    if not kinds <= {"full_attention"}:
+        raise ValueError(f"layer types {sorted(kinds)} are not supported")
+    if getattr(cfg, "hidden_act", "silu") not in ("silu", "swish"):
+        raise ValueError(f'hidden_act "{cfg.hidden_act}" is not supported: the decoders take SiLU')
+    return min(limits) if limits else None
+
+
 @torch.no_grad()
 def build(arch, seed=0, device="cuda", **overrides):
     """A random-init fp16 Qwen2ForCausalLM, initialized directly on `device`."""
@@ -142,7 +167,8 @@ class Int4Decoder:
     """Qwen2 decode step on the library's kernels: embed -> per layer [RMSNorm + q|k|v GEMV, attention (bias +
     RoPE + KV append + split attention, combine), o GEMV, residual + RMSNorm + gate|up GEMV, SiLU*up + down GEMV]
     -> final RMSNorm -> fp16 lm_head (cuBLAS) -> argmax. Takes the weights of a transformers Qwen2ForCausalLM
-    (fp16, nn.Linear projections) and frees its decoder layers.
+    (fp16, nn.Linear projections) and frees its decoder layers. A model that scales its rotary angles, whose attention
+    slides over a window shorter than max_len, with another activation or with norms of q and k is refused (ValueError).
 
     `fuse` picks kernel fusions: "norm_epilogue" ends the o and down GEMVs with the residual add + next RMSNorm
     (the last CTA of the GEMV, or the one-shot allreduce under tensor parallelism); "swiglu_epilogue" ends the
@@ -153,12 +179,19 @@ class Int4Decoder:
     SwiGLU into the GEMV's prologue where one CTA holds the row."""
 
     def __init__(self, model, max_len, group=128, world=1, rank=0, pg=None, fuse=(), allreduce="oneshot"):
-        e = ops.ext()
-        self.lib = e.lib
         cfg = model.config
+        limit = context_limit(cfg)
+        if limit is not None and max_len > limit:
+            raise ValueError(f"max_len={max_len}: the model's sliding window or rotary scaling allows {limit} tokens here")
         self.H, I = cfg.hidden_size, cfg.intermediate_size
         nh, nkv = cfg.num_attention_heads, cfg.num_key_value_heads
         self.hd = self.H // nh
+        if (getattr(cfg, "head_dim", None) or self.hd) != self.hd:
+            raise ValueError(f"head_dim={cfg.head_dim}: hidden_size / heads = {self.hd} is supported")
+        if any(hasattr(layer.self_attn, "q_norm") for layer in model.model.layers):
+            raise ValueError("per-head norms of q and k are not supported here (paged.PagedDecoder takes them)")
+        e = ops.ext()
+        self.lib = e.lib
         self.eps = float(cfg.rms_norm_eps)
         self.max_len = max_len
         self.world, self.rank, self.pg = world, rank, pg

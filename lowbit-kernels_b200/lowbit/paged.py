@@ -12,6 +12,7 @@ import math
 import torch
 
 from . import ops
+from .decode import context_limit
 from ._lib import DTYPE_IDS, PagedCacheStruct, _Device
 
 
@@ -183,7 +184,9 @@ class PagedDecoder:
     model of that architecture (fp16 or bf16; per-head q_norm / k_norm modules are used where its attention has them)
     and keeps its projections in 8-bit integers (`weights="w8"`, ops.linear_w8) or, fp16 models only, in the INT4 format
     (`weights="w4"`, ops.linear). Per layer: RMSNorm, the fused q|k|v product, `norm_rope_append`, `attention`, the output
-    product, RMSNorm, the fused gate|up product, SiLU * up, the down product.
+    product, RMSNorm, the fused gate|up product, SiLU * up, the down product. Models that scale their rotary angles, with an
+    activation other than SiLU or with head dims other than 64 and 128 are refused (ValueError); one whose attention slides
+    over a window, or whose angles are scaled only from some length on, takes contexts up to that length.
 
         dec = PagedDecoder(model, num_pages=512, page_size=64)
         a, b = dec.open(), dec.open()
@@ -196,12 +199,15 @@ class PagedDecoder:
         if weights not in ("w8", "w4"):
             raise ValueError('weights is "w8" or "w4"')
         cfg, base = model.config, model.model
+        self.limit = context_limit(cfg)
         self.embed = base.embed_tokens.weight.detach()
         self.device, self.dtype = self.embed.device, self.embed.dtype
         if weights == "w4" and self.dtype != torch.float16:
             raise ValueError("INT4 weights need a float16 model")
         self.nh, self.nkv = cfg.num_attention_heads, cfg.num_key_value_heads
         self.hd = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.nh
+        if self.hd not in (64, 128):
+            raise ValueError(f"hd={self.hd}: the attention takes head dims 64 and 128")
         self.eps, self.page_size, self.vocab = float(cfg.rms_norm_eps), page_size, cfg.vocab_size
         theta = float(cfg.rope_parameters["rope_theta"])
         half = torch.arange(0, self.hd, 2, dtype=torch.float32)
@@ -249,6 +255,9 @@ class PagedDecoder:
     def _plan(self, chunks):
         """The call's host arrays: token ids, positions and slots, page table, lengths and first tokens."""
         page = self.page_size
+        longest = max(self._seqs[s]["length"] + len(new) for s, new in chunks.items())
+        if self.limit is not None and longest > self.limit:
+            raise ValueError(f"{longest} tokens: the model's sliding window or rotary scaling allows {self.limit} here")
         need = {s: -(-(self._seqs[s]["length"] + len(new)) // page) - len(self._seqs[s]["pages"]) for s, new in chunks.items()}
         if sum(need.values()) > len(self._free):
             raise RuntimeError(f"{sum(need.values())} pages are needed, {len(self._free)} are free")

@@ -134,3 +134,67 @@ def test_sequences_of_a_batch_do_not_touch_each_other():
         dec.forward({})
     with pytest.raises(ValueError):
         paged.PagedDecoder(tiny(dtype=torch.bfloat16), 4, weights="w4")
+
+
+# ------------------------------------------------------------------------------- what the decoders refuse (no GPU)
+
+def empty_model(**kw):
+    """A model as far as the refusals look: its config, and attention modules without weights."""
+    from types import SimpleNamespace as Ns
+    from lowbit import decode
+    return Ns(config=decode.qwen2_config(TINY, **kw), model=Ns(layers=[Ns(self_attn=Ns()) for _ in range(2)]))
+
+
+REFUSED = [dict(rope_parameters={"rope_type": "linear", "factor": 4.0, "rope_theta": 1e6}),
+           dict(rope_parameters={"rope_type": "yarn", "factor": 4.0, "rope_theta": 1e6, "original_max_position_embeddings": 8192}),
+           dict(rope_parameters={"rope_type": "llama3", "factor": 8.0, "rope_theta": 5e5, "low_freq_factor": 1.0,
+                                 "high_freq_factor": 4.0, "original_max_position_embeddings": 8192}),
+           dict(hidden_act="gelu")]
+
+
+@pytest.mark.parametrize("kw", REFUSED)
+def test_decoders_refuse_models_that_they_would_compute_wrongly(kw):
+    from lowbit import decode, paged
+    with pytest.raises(ValueError, match="not supported"):
+        paged.PagedDecoder(empty_model(**kw), num_pages=4)
+    with pytest.raises(ValueError, match="not supported"):
+        decode.Int4Decoder(empty_model(**kw), 64)
+
+
+def test_int4_decoder_refuses_head_dims_and_norms_that_it_ignores():
+    from types import SimpleNamespace as Ns
+    from lowbit import decode
+    with pytest.raises(ValueError, match="head_dim"):
+        decode.Int4Decoder(empty_model(head_dim=128), 64)
+    normed = empty_model()
+    normed.model.layers[1].self_attn = Ns(q_norm=None)
+    with pytest.raises(ValueError, match="norms"):
+        decode.Int4Decoder(normed, 64)
+
+
+def test_paged_decoder_refuses_head_dims_of_the_attention():
+    from lowbit import paged
+    model = empty_model(head_dim=32)
+    model.model.embed_tokens = torch.nn.Embedding(4, 4)
+    with pytest.raises(ValueError, match="64 and 128"):
+        paged.PagedDecoder(model, num_pages=4)
+
+
+WINDOW = dict(use_sliding_window=True, sliding_window=64, max_window_layers=1)
+DYNAMIC = dict(rope_parameters={"rope_type": "dynamic", "factor": 4.0, "rope_theta": 1e6}, max_position_embeddings=64)
+
+
+@pytest.mark.parametrize("kw", [WINDOW, DYNAMIC])
+def test_decoders_stop_where_a_window_or_scaled_angles_begin(kw):
+    from lowbit import decode, paged
+    assert decode.context_limit(empty_model(**kw).config) == 64
+    assert decode.context_limit(empty_model(use_sliding_window=False, sliding_window=64).config) is None
+    with pytest.raises(ValueError, match="64 tokens"):
+        decode.Int4Decoder(empty_model(**kw), 65)
+    dec = paged.PagedDecoder.__new__(paged.PagedDecoder)
+    dec.page_size, dec.limit, dec._free, dec._seqs, dec._next = 16, 64, list(range(9, -1, -1)), {}, 0
+    sid = dec.open()
+    dec._plan({sid: [1] * 60})
+    dec._plan({sid: [1] * 4})
+    with pytest.raises(ValueError, match="65 tokens"):
+        dec._plan({sid: [1]})
