@@ -253,7 +253,8 @@ class PagedDecoder:
         return w * (f * torch.rsqrt(f.square().mean(-1, keepdim=True) + self.eps)).to(self.dtype)
 
     def _plan(self, chunks):
-        """The call's host arrays: token ids, positions and slots, page table, lengths and first tokens."""
+        """The call's host arrays -- token ids, positions and slots, page table, lengths and first tokens -- and each
+        sequence's pages after it. Changes nothing: `_commit` does, once the call's work is launched."""
         page = self.page_size
         longest = max(self._seqs[s]["length"] + len(new) for s, new in chunks.items())
         if self.limit is not None and longest > self.limit:
@@ -261,28 +262,36 @@ class PagedDecoder:
         need = {s: -(-(self._seqs[s]["length"] + len(new)) // page) - len(self._seqs[s]["pages"]) for s, new in chunks.items()}
         if sum(need.values()) > len(self._free):
             raise RuntimeError(f"{sum(need.values())} pages are needed, {len(self._free)} are free")
-        ids, pos, slots, lens, cu = [], [], [], [], [0]
+        ids, pos, slots, lens, cu, pages, taken = [], [], [], [], [0], {}, 0
         for s, new in chunks.items():
-            seq = self._seqs[s]
-            seq["pages"] += [self._free.pop() for _ in range(need[s])]
-            for i, tok in enumerate(new, seq["length"]):
+            start = self._seqs[s]["length"]
+            pages[s] = self._seqs[s]["pages"] + [self._free[-1 - taken - i] for i in range(need[s])]
+            taken += need[s]
+            for i, tok in enumerate(new, start):
                 ids.append(int(tok))
                 pos.append(i)
-                slots.append(seq["pages"][i // page] * page + i % page)
-            seq["length"] += len(new)
-            lens.append(seq["length"])
+                slots.append(pages[s][i // page] * page + i % page)
+            lens.append(start + len(new))
             cu.append(len(ids))
-        width = max(1, max(len(self._seqs[s]["pages"]) for s in chunks))
-        table = [self._seqs[s]["pages"] + [0] * (width - len(self._seqs[s]["pages"])) for s in chunks]
-        return ids, pos, slots, table, lens, cu
+        width = max(1, max(len(v) for v in pages.values()))
+        table = [v + [0] * (width - len(v)) for v in pages.values()]
+        return ids, pos, slots, table, lens, cu, pages
+
+    def _commit(self, pages, lens):
+        """The sequences hold those pages and that many tokens."""
+        taken = sum(len(v) - len(self._seqs[s]["pages"]) for s, v in pages.items())
+        del self._free[len(self._free) - taken:]
+        for (s, v), n in zip(pages.items(), lens):
+            self._seqs[s] = {"length": n, "pages": v}
 
     @torch.no_grad()
     def forward(self, chunks):
         """chunks: {sequence id: its new token ids, at least one}. Appends them and returns the logits [len(chunks),
-        vocab] after each sequence's last new token, in the order of `chunks`."""
+        vocab] after each sequence's last new token, in the order of `chunks`. A call that raises leaves every sequence and
+        the free pages as they were."""
         if not chunks or any(len(new) == 0 for new in chunks.values()):
             raise ValueError("every sequence of a call needs a new token")
-        ids, pos, slots, table, lens, cu = self._plan(chunks)
+        ids, pos, slots, table, lens, cu, pages = self._plan(chunks)
         dev, t = self.device, len(ids)
         ids, pos, slots = (torch.tensor(v, dtype=torch.int64, device=dev) for v in (ids, pos, slots))
         table, lens_d, cu_d = (torch.tensor(v, dtype=torch.int32, device=dev) for v in (table, lens, cu))
@@ -299,4 +308,6 @@ class PagedDecoder:
             gate, up = product(self._rms(x, ly["ln2"]), "gate_up").chunk(2, -1)
             x = x + product(torch.nn.functional.silu(gate) * up, "down")
         last = torch.tensor([c - 1 for c in cu[1:]], dtype=torch.int64, device=dev)
-        return torch.nn.functional.linear(self._rms(x[last], self.norm), self.head)
+        logits = torch.nn.functional.linear(self._rms(x[last], self.norm), self.head)
+        self._commit(pages, lens)
+        return logits

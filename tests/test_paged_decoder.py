@@ -2,6 +2,8 @@
 (dequantized), and its page bookkeeping. INT4 weights leave only rounding between the two. With 8-bit integers the plain
 decoder quantizes the activations as the operator is defined, and rounds to the type where the decoder stores: a value
 that one rounding moves past the middle of a step is a whole step away, so the two have to round alike."""
+import copy
+
 import pytest
 import torch
 
@@ -191,10 +193,65 @@ def test_decoders_stop_where_a_window_or_scaled_angles_begin(kw):
     assert decode.context_limit(empty_model(use_sliding_window=False, sliding_window=64).config) is None
     with pytest.raises(ValueError, match="64 tokens"):
         decode.Int4Decoder(empty_model(**kw), 65)
-    dec = paged.PagedDecoder.__new__(paged.PagedDecoder)
-    dec.page_size, dec.limit, dec._free, dec._seqs, dec._next = 16, 64, list(range(9, -1, -1)), {}, 0
+    dec = bookkeeper(limit=64)
     sid = dec.open()
-    dec._plan({sid: [1] * 60})
-    dec._plan({sid: [1] * 4})
+    for n in (60, 4):
+        dec.forward({sid: [1] * n})
     with pytest.raises(ValueError, match="65 tokens"):
-        dec._plan({sid: [1]})
+        dec.forward({sid: [1]})
+
+
+def bookkeeper(limit=None, pages=10):
+    """A PagedDecoder without layers, on the CPU: its page bookkeeping, its embedding and its head."""
+    from lowbit import paged
+    dec = paged.PagedDecoder.__new__(paged.PagedDecoder)
+    dec.page_size, dec.limit, dec.device, dec.dtype, dec.layers, dec.eps = 16, limit, torch.device("cpu"), torch.float32, [], 1e-6
+    dec.embed, dec.head, dec.norm = torch.randn(32, 8), torch.randn(32, 8), torch.ones(8)
+    dec._free, dec._seqs, dec._next = list(range(pages - 1, -1, -1)), {}, 0
+    return dec
+
+
+def test_a_call_that_raises_changes_no_sequence():
+    dec = bookkeeper()
+    a, b = dec.open(), dec.open()
+    dec.forward({a: [1] * 20, b: [2]})
+    before = copy.deepcopy((dec._free, dec._seqs))
+    with pytest.raises(ValueError):   # a token that is none, after a sequence in order
+        dec.forward({a: [1] * 40, b: [4, "x"]})
+    assert (dec._free, dec._seqs) == before
+    norm, dec.norm = dec.norm, torch.ones(5)
+    with pytest.raises(RuntimeError):   # the last of the call's products fails
+        dec.forward({a: [1] * 40, b: [4]})
+    assert (dec._free, dec._seqs) == before
+    dec.norm = norm
+    dec.forward({a: [1] * 40, b: [4] * 30})
+    assert dec._seqs == {a: {"length": 60, "pages": [0, 1, 3, 4]}, b: {"length": 31, "pages": [2, 5]}}
+    assert dec._free == [9, 8, 7, 6]
+    dec.close(a)
+    assert sorted(dec._free) == [0, 1, 3, 4, 6, 7, 8, 9]
+
+
+@pytest.mark.gpu
+def test_a_call_that_failed_in_a_layer_can_be_repeated(monkeypatch):
+    from lowbit import paged
+    dec = paged.PagedDecoder(tiny(), num_pages=16, page_size=16, weights="w8")
+    g = torch.Generator().manual_seed(3)
+    ids = torch.randint(0, 1024, (80,), generator=g).tolist()
+    want = feed(dec, ids, [50, 30])
+    sid = dec.open()
+    first = dec.forward({sid: ids[:50]})
+    state = copy.deepcopy((dec._free, dec._seqs))
+    calls, attention = [], paged.attention
+
+    def failing(*args, **kw):
+        calls.append(1)
+        if len(calls) == 2:
+            raise torch.OutOfMemoryError("no memory")
+        return attention(*args, **kw)
+
+    monkeypatch.setattr(paged, "attention", failing)
+    with pytest.raises(torch.OutOfMemoryError):
+        dec.forward({sid: ids[50:]})
+    assert (dec._free, dec._seqs) == state
+    monkeypatch.undo()
+    assert torch.equal(torch.cat((first, dec.forward({sid: ids[50:]}))), want)
