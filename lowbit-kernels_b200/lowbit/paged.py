@@ -268,7 +268,10 @@ class PagedDecoder:
             pages[s] = self._seqs[s]["pages"] + [self._free[-1 - taken - i] for i in range(need[s])]
             taken += need[s]
             for i, tok in enumerate(new, start):
-                ids.append(int(tok))
+                tok = int(tok)
+                if not 0 <= tok < self.embed.shape[0]:   # (on the GPU the lookup's own check would end the context)
+                    raise ValueError(f"token id {tok} of {self.embed.shape[0]}")
+                ids.append(tok)
                 pos.append(i)
                 slots.append(pages[s][i // page] * page + i % page)
             lens.append(start + len(new))
@@ -287,8 +290,8 @@ class PagedDecoder:
     @torch.no_grad()
     def forward(self, chunks):
         """chunks: {sequence id: its new token ids, at least one}. Appends them and returns the logits [len(chunks),
-        vocab] after each sequence's last new token, in the order of `chunks`. A call that raises leaves every sequence and
-        the free pages as they were."""
+        vocab] after each sequence's last new token, in the order of `chunks`. A call that raises (ValueError for
+        a token id outside the embedding) leaves every sequence and the free pages as they were."""
         if not chunks or any(len(new) == 0 for new in chunks.values()):
             raise ValueError("every sequence of a call needs a new token")
         ids, pos, slots, table, lens, cu, pages = self._plan(chunks)

@@ -231,6 +231,18 @@ def test_a_call_that_raises_changes_no_sequence():
     assert sorted(dec._free) == [0, 1, 3, 4, 6, 7, 8, 9]
 
 
+@pytest.mark.parametrize("tok", [-1, 32, 2 ** 40, torch.tensor(32)])
+def test_token_ids_outside_the_embedding_are_refused_before_any_work(tok):
+    """On the host: -1 would read the last row, 32 of 32 fail in the lookup on the device."""
+    dec = bookkeeper()
+    a, b = dec.open(), dec.open()
+    dec.forward({a: [0, 31]})
+    before = copy.deepcopy((dec._free, dec._seqs))
+    with pytest.raises(ValueError, match="token id"):
+        dec.forward({b: [3], a: [1, tok]})
+    assert (dec._free, dec._seqs) == before
+
+
 @pytest.mark.gpu
 def test_a_call_that_failed_in_a_layer_can_be_repeated(monkeypatch):
     from lowbit import paged
