@@ -8,7 +8,7 @@
 //   gemv(x, w_ptr, s_ptr, device, n, k, group, version, out=None, bias=None) -> Tensor | None
 //
 // and, the same way, the calls of a chunk of new tokens (ops.linear_w8, lowbit.paged):
-//   linear_w8(x, w_ptr, scales_ptr, device, n, k, ldw, out, bias) -> Tensor | None
+//   linear_w8(x, q, scales, out, bias) -> Tensor | None   (q, scales: a W8Weight's, its layout)
 //   norm_rope_append(qkv, cache_ptr, device, positions, slots, nh, inv_freq, q_norm, k_norm, eps, out) -> Tensor | None
 //   paged_attention(q, cache_ptr, device, page_table, seq_lens, cu_new, max_new, max_len, scale, out) -> Tensor | None
 #include <Python.h>
@@ -131,10 +131,15 @@ PyObject* guarded(PyObject* const* args) {
 }
 
 PyObject* linear_w8(PyObject* const* args) {
-  long long v[6];
-  if (!to_ints(args + 1, v, 6)) return nullptr;
-  const long long dev = v[2];
-  const int64_t n = v[3], k = v[4], ldw = v[5];
+  if (!THPVariable_Check(args[1])) Py_RETURN_NONE;
+  const at::Tensor& q = THPVariable_Unpack(args[1]);
+  if (!q.is_cuda() || q.scalar_type() != at::kChar || q.dim() != 2 || q.stride(1) != 1) Py_RETURN_NONE;
+  const long long dev = q.get_device();
+  const int64_t n = q.size(0), k = q.size(1), ldw = n > 1 ? q.stride(0) : (k + 15) / 16 * 16;
+  const at::Tensor* scales = tensor_on(args[2], dev);
+  if (!scales || scales->scalar_type() != at::kFloat || scales->dim() != 1 || scales->size(0) != n ||
+      !scales->is_contiguous())
+    Py_RETURN_NONE;
   const at::Tensor* x = tensor_on(args[0], dev);
   if (!x || x->dim() != 2 || x->size(1) != k || x->size(0) == 0 || c10::cuda::current_device() != dev) Py_RETURN_NONE;
   const auto type = x->scalar_type();
@@ -142,16 +147,16 @@ PyObject* linear_w8(PyObject* const* args) {
   const int64_t m = x->size(0), ldx = m > 1 ? x->stride(0) : k;
   if (x->stride(1) != 1 || ldx < k) Py_RETURN_NONE;
   const void* bias = nullptr;
-  if (args[8] != Py_None) {
-    const at::Tensor* b = tensor_on(args[8], dev);
+  if (args[4] != Py_None) {
+    const at::Tensor* b = tensor_on(args[4], dev);
     if (!b || b->scalar_type() != type || b->dim() != 1 || b->size(0) != n || !b->is_contiguous()) Py_RETURN_NONE;
     bias = b->data_ptr();
   }
   at::Tensor y;
-  if (args[7] == Py_None) {
+  if (args[3] == Py_None) {
     y = at::empty({m, n}, x->options());
   } else {
-    const at::Tensor* o = tensor_on(args[7], dev);
+    const at::Tensor* o = tensor_on(args[3], dev);
     if (!o || o->scalar_type() != type || o->dim() != 2 || o->size(0) != m || o->size(1) != n || !o->is_contiguous())
       Py_RETURN_NONE;
     y = *o;
@@ -160,10 +165,9 @@ PyObject* linear_w8(PyObject* const* args) {
   at::Tensor ws;
   if (need > 0) ws = at::empty({need}, x->options().dtype(at::kByte));
   const int rc = lb_w8_linear(x->data_ptr(), type == at::kHalf ? LB_F16 : LB_BF16, ldx,
-                              reinterpret_cast<const void*>(static_cast<uintptr_t>(v[0])), ldw,
-                              reinterpret_cast<const float*>(static_cast<uintptr_t>(v[1])), bias, y.data_ptr(), m, n, k,
+                              q.data_ptr(), ldw, scales->data_ptr<float>(), bias, y.data_ptr(), m, n, k,
                               need > 0 ? ws.data_ptr() : nullptr, need, stream_of(dev));
-  return rc ? refused(rc) : result(args[7], y);
+  return rc ? refused(rc) : result(args[3], y);
 }
 
 at::ScalarType cache_type(const lb_paged_cache* c) { return c->dtype == LB_F16 ? at::kHalf : at::kBFloat16; }
@@ -272,8 +276,8 @@ PyCFunction fastcall() {
 }
 
 PyMethodDef methods[] = {
-    {"linear_w8", fastcall<linear_w8, 9>(), METH_FASTCALL,
-     "linear_w8(x, w_ptr, scales_ptr, device, n, k, ldw, out, bias) -> Tensor, or None for the checked path"},
+    {"linear_w8", fastcall<linear_w8, 5>(), METH_FASTCALL,
+     "linear_w8(x, q, scales, out, bias) -> Tensor, or None for the checked path"},
     {"norm_rope_append", fastcall<norm_rope_append, 11>(), METH_FASTCALL,
      "norm_rope_append(qkv, cache_ptr, device, positions, slots, nh, inv_freq, q_norm, k_norm, eps, out) -> Tensor, or "
      "None for the checked path"},

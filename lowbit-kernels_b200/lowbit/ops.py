@@ -390,21 +390,27 @@ class W8Weight:
             raise RuntimeError("W8Weight takes GPU tensors")
         if q.dtype != torch.int8 or q.dim() != 2 or not q.numel():
             raise RuntimeError("q must be an int8 [N, K] tensor")
-        self.n, self.k = q.shape
+        self.n, self.k = q.shape   # no device pointer is kept: a copy or an unpickled weight has its own memory
         if scales.dtype != torch.float32 or scales.shape != (self.n,) or scales.device != q.device:
             raise RuntimeError(f"scales must be a float32 [{self.n}] tensor on {q.device}")
         if self.k > 131072:
             raise ValueError(f"K={self.k}: at most 131072, so that the int32 sums are exact")
         if (self.k % 16 == 0 and q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.stride(0) >= self.k
                 and q.data_ptr() % 16 == 0):
-            self.q = q
+            self._q = q
         else:
             pad = torch.zeros(self.n, -(-self.k // 16) * 16, dtype=torch.int8, device=q.device)
             pad[:, :self.k] = q
-            self.q = pad[:, :self.k]
-        self.scales = scales.contiguous()
-        self._args = (self.q.data_ptr(), self.scales.data_ptr(), q.get_device(), self.n, self.k,
-                      self.q.stride(0) if self.n > 1 else -(-self.k // 16) * 16)
+            self._q = pad[:, :self.k]
+        self._scales = scales.contiguous()
+
+    @property
+    def q(self):
+        return self._q
+
+    @property
+    def scales(self):
+        return self._scales
 
     @classmethod
     def from_float(cls, w):
@@ -420,8 +426,7 @@ def linear_w8(x, w8, bias=None, out=None):
     rounded once. `out`: an optional contiguous [M, N] tensor that receives the result."""
     tc = _tc if _tc is not None else _torchcall()
     if tc:
-        p = w8._args
-        y = tc.linear_w8(x, p[0], p[1], p[2], p[3], p[4], p[5], out, bias)
+        y = tc.linear_w8(x, w8._q, w8._scales, out, bias)
         if y is not None:
             return y
     if not (isinstance(x, torch.Tensor) and x.is_cuda and x.device == w8.q.device):
@@ -441,11 +446,12 @@ def linear_w8(x, w8, bias=None, out=None):
     if x.stride(1) != 1 or (m > 1 and x.stride(0) < w8.k):
         x = x.contiguous()
     e = ext()
-    w_ptr, s_ptr, _, n, k, ldw = w8._args
+    n, k, ldw = w8.n, w8.k, w8.q.stride(0) if w8.n > 1 else -(-w8.k // 16) * 16
     with _Device(x.device):
         need = e.lib.lb_w8_workspace(m, n, k)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        rc = e.lib.lb_w8_linear(x.data_ptr(), DTYPE_IDS[x.dtype], x.stride(0) if m > 1 else k, w_ptr, ldw, s_ptr,
+        rc = e.lib.lb_w8_linear(x.data_ptr(), DTYPE_IDS[x.dtype], x.stride(0) if m > 1 else k, w8.q.data_ptr(), ldw,
+                                w8.scales.data_ptr(),
                                 None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, k,
                                 ws.data_ptr() if need else None, need, torch.cuda.current_stream().cuda_stream)
     if rc:

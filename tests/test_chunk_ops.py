@@ -11,8 +11,10 @@ Tolerances, with u = 2^-11 (fp16) or 2^-8 (bf16) the relative rounding of one st
     L 2^-25 max|v|, the weights' absolute rounding below fp16's normal range.
 Every tolerance adds 2^-24, half of fp16's smallest step, twice.
 """
+import copy
 import ctypes
 import math
+import pickle
 
 import pytest
 import torch
@@ -212,6 +214,26 @@ def test_linear_w8_strided_inputs_out_and_streams():
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(a, ops.linear_w8(x, w8))
     assert ops.linear_w8(x[:0], w8).shape == (0, 200)
+
+
+@gpu
+@pytest.mark.parametrize("k", [64, 100])
+def test_a_copy_of_a_w8_weight_is_its_own(k):
+    """copy.deepcopy and pickle: the copy multiplies with its own integers and scales, whatever becomes of the first."""
+    ops, _ = mods()
+    g = gen(k)
+    for m in (3, 70):
+        w8 = ops.W8Weight.from_float(randn(g, 48, k))
+        x = randn(g, m, k, dtype=torch.float16)
+        want = ops.linear_w8(x, w8)
+        for other in (copy.deepcopy(w8), pickle.loads(pickle.dumps(w8)), copy.copy(w8)):
+            assert torch.equal(ops.linear_w8(x, other), want)
+        twin = copy.deepcopy(w8)
+        w8.q.zero_(), w8.scales.zero_()
+        assert torch.equal(ops.linear_w8(x, twin), want) and not ops.linear_w8(x, w8).any()
+    for name in ("q", "scales"):
+        with pytest.raises(AttributeError):
+            setattr(w8, name, getattr(twin, name))
 
 
 @gpu
