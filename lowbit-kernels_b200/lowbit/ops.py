@@ -77,6 +77,10 @@ class W4Weight:
         packed, scales = quantize_w4_gpu(w, group)
         return cls(packed, scales, group, layouts)
 
+    def __getstate__(self):
+        """Without the launch arguments kept for this object's memory: a copy or an unpickled weight has its own."""
+        return {name: v for name, v in self.__dict__.items() if name not in ("_launch", "_mma_launch")}
+
     def nbytes(self):
         """Bytes of one copy of the weight (packed values + scales), whatever layouts are kept."""
         return self.n * self.k // 2 + self.scales.numel() * 2

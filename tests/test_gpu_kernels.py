@@ -554,3 +554,21 @@ def test_bias_on_the_prefill_path_and_refusals():
         ops.ext().w4_linear(x[:2], wq.packed_mma, wq.scales, 128, 6, bias=bias[:299].contiguous())
     with pytest.raises(RuntimeError):
         ops.ext().w4_linear(x[:2], wq.packed_mma, wq.scales, 128, 6, bias=bias.float())
+
+
+@pytest.mark.gpu
+def test_a_copy_of_a_weight_is_its_own():
+    """copy.deepcopy and pickle of a weight that calls have used: the copy multiplies with its own memory."""
+    import copy
+    import pickle
+    from lowbit import ops
+    g = torch.Generator(device="cuda").manual_seed(0)
+    for version in (3, 5, 6):
+        wq = ops.W4Weight.from_float(torch.randn(256, 512, device="cuda", generator=g))
+        x = torch.randn(2, 512, device="cuda", generator=g).half()
+        want = ops.gemv(x, wq, version)
+        copies = copy.deepcopy(wq), pickle.loads(pickle.dumps(wq))
+        for t in (wq.packed, wq.packed_v3, wq.packed_mma, wq.scales):
+            t.zero_()
+        for other in copies:
+            assert torch.equal(ops.gemv(x, other, version), want)
