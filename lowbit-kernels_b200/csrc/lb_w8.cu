@@ -264,7 +264,11 @@ constexpr int kMmaThreads = (2 + kEpiWarps) * 32;   // loader, MMA, epilogue war
 constexpr int kMaxStages = 8;
 constexpr int kW8MaxSplits = 8;           // portable cluster size
 constexpr int kW8Smem = 227 * 1024;
-constexpr int kBarrierBytes = (2 * kMaxStages + 4) * 8 + 16 + 2 * 256 * 4 + kEpiWarps * 1024;   // + scales, + staging
+constexpr int kBarrierBytes = (2 * kMaxStages + 4) * 8 + 16 + kEpiWarps * 64 * 4 + kEpiWarps * 1024;   // + scales, + staging
+
+// A warp's token scales: an accumulator's columns 16 part + 64 i + j, i < 4, j < 16, of its four-warp part, as 16 i + j. Each
+// warp keeps its own, so that no epilogue warp waits for another: one whose bounded wait gave up can leave by itself.
+__device__ __forceinline__ int scale_at(int column) { return (column >> 6) * 16 + (column & 15); }
 
 struct W8Gemm {
   const float* s;       // token scales
@@ -298,6 +302,7 @@ __device__ __forceinline__ void sum_partials(uint32_t red, const float* sc, cons
   const bool vec = n0 + r4 + 4 <= N && N % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & 7u) == 0;
   for (int m = rank * warps + (threadIdx.x >> 5); m < rows; m += S * warps) {
     const uint32_t off = red + (uint32_t)(m * 128 + r4) * 4u;
+    const float scale = sc[(m >> 4 & 3) * 256 + scale_at(m)];   // of the first warp of the column's part
     float4 f[kW8MaxSplits];
 #pragma unroll
     for (int q = 0; q < kW8MaxSplits; ++q)
@@ -313,7 +318,7 @@ __device__ __forceinline__ void sum_partials(uint32_t red, const float* sc, cons
       }
     float o[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = fmaf(__int2float_rn(v[j]) * sc[m], tn[j], bn[j]);
+    for (int j = 0; j < 4; ++j) o[j] = fmaf(__int2float_rn(v[j]) * scale, tn[j], bn[j]);
     T* dst = y + (int64_t)m * N + n0 + r4;
     if (vec) {
       *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(o[0], o[1]), Elem<T>::pack(o[2], o[3]));
@@ -335,7 +340,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   uint64_t* acc_full = empty + kMaxStages;
   uint64_t* acc_empty = acc_full + 2;                            // PAIR: the leader's
   uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
-  float* sc = reinterpret_cast<float*>(slot + 4);   // [2][256] token scales
+  float* sc = reinterpret_cast<float*>(slot + 4);   // [epilogue warps][64] token scales
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int own_bn = PAIR ? p.bn / 2 : p.bn;        // tokens this CTA loads
   const int H = PAIR ? p.halves : 1, acc_bn = p.bn / H, box = own_bn / H;
@@ -481,11 +486,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, part = (warp - 2) >> 2, row = 32 * quarter + lane, et = threadIdx.x - 64;
+    const int quarter = warp & 3, part = (warp - 2) >> 2, row = 32 * quarter + lane;
     const uint32_t tlane = (uint32_t)(32 * quarter) << 16;
     const T* bias = static_cast<const T*>(p.bias);
     T* y = static_cast<T*>(p.y);
-    uint16_t* turn = reinterpret_cast<uint16_t*>(sc + 512) + (warp - 2) * 512;
+    float* scale = sc + (warp - 2) * 64;
+    uint16_t* turn = reinterpret_cast<uint16_t*>(sc + kEpiWarps * 64) + (warp - 2) * 512;
     pdl_wait();
     bool ok = true;
     const int mine = first < p.tiles ? (p.tiles - first + step - 1) / step : 0;
@@ -493,11 +499,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const int tile = first + a / H * step;
       const int m0 = tile % p.tiles_m * p.bn + a % H * acc_bn, n = tile / p.tiles_m * kTileN + n_off + row;
       const bool on = n < p.N;
-      float* scale = sc + (a & 1) * 256;
-      if (et < acc_bn)
-        scale[et] = m0 + et < p.M ? __uint_as_float(ldg_cg_u32(reinterpret_cast<const uint32_t*>(p.s + m0 + et))) : 0.f;
+#pragma unroll
+      for (int i = lane; i < 64; i += 32) {
+        const int j = 64 * (i >> 4) + 16 * part + (i & 15);
+        if (j < acc_bn)
+          scale[i] = m0 + j < p.M ? __uint_as_float(ldg_cg_u32(reinterpret_cast<const uint32_t*>(p.s + m0 + j))) : 0.f;
+      }
       const float tn = on ? p.t[n] : 0.f, bn = on && bias ? Elem<T>::to_float(bias[n]) : 0.f;
-      named_barrier(1, 32 * kEpiWarps);
       ok = wait_bounded(&acc_full[a & 1], (a >> 1) & 1, &g_w8_status);
       __syncwarp();
       tc::fence_after();
@@ -512,8 +520,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           uint32_t h[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            h[j] = Elem<T>::pack(fmaf(__int2float_rn((int)w[2 * j]) * scale[j0 + 2 * j], tn, bn),
-                                 fmaf(__int2float_rn((int)w[2 * j + 1]) * scale[j0 + 2 * j + 1], tn, bn));
+            h[j] = Elem<T>::pack(fmaf(__int2float_rn((int)w[2 * j]) * scale[scale_at(j0) + 2 * j], tn, bn),
+                                 fmaf(__int2float_rn((int)w[2 * j + 1]) * scale[scale_at(j0) + 2 * j + 1], tn, bn));
           if (p.vec) {
             // through the warp's 1 KB: [16 tokens][32 channels], then eight rows of 64 bytes a store
 #pragma unroll

@@ -217,6 +217,24 @@ def test_linear_w8_strided_inputs_out_and_streams():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(629, 7531, 384), (2137, 6249, 1000), (2200, 9000, 500), (2200, 9001, 500), (1552, 11256, 3000),
+                                   (1144, 15727, 3000), (973, 15400, 4096)])
+def test_linear_w8_several_tiles_a_cta(dtype, m, n, k):
+    """Large products: single CTAs with two and three tiles each, pairs with five, and pairs whose tiles are more than
+    256 tokens wide, with one to three each; the last tile partial both ways, rows of 16-byte multiples and not."""
+    ops, _ = mods()
+    g = gen(m + n)
+    w8 = ops.W8Weight.from_float(randn(g, n, k, std=0.05))
+    bias = randn(g, n, dtype=dtype)
+    x = randn(g, m, k, dtype=dtype, std=2.0)
+    y = ops.linear_w8(x, w8, bias=bias)
+    check_linear(x, w8.q, w8.scales, bias, y)
+    assert torch.equal(y, ops.linear_w8(x, w8, bias=bias))
+    assert ops.ext().lib.lb_device_error() == 0
+
+
+@gpu
 @pytest.mark.parametrize("k", [64, 100])
 def test_a_copy_of_a_w8_weight_is_its_own(k):
     """copy.deepcopy and pickle: the copy multiplies with its own integers and scales, whatever becomes of the first."""
@@ -644,6 +662,15 @@ A, MIS = 0x10000, 0x10001   # addresses that are never read: the checks come bef
 
 def message(lib):
     return lib.lb_last_error().decode()
+
+
+def test_no_warp_of_the_chunk_kernels_meets_others_on_the_way():
+    """Every wait is bounded, and a warp whose wait gave up leaves its loop. A barrier among some of a CTA's warps inside such
+    a loop would then hold the others for good, so these kernels have none: warps meet at the CTA's or the cluster's
+    barriers, which each reaches whatever its waits returned. (Read from the source: no valid call makes a wait give up.)"""
+    for name in ("lb_w8.cu", "lb_paged.cu"):
+        source = (_lib.LIB_PATH.parent.parent / "csrc" / name).read_text()
+        assert "named_barrier(" not in source and "bar.sync" not in source and "barrier.sync" not in source, name
 
 
 def test_w8_abi_refusals():
