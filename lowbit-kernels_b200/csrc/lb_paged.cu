@@ -823,17 +823,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         };
         int page, row = 0, page_next, row_next = 0;
         lookup(0, page, row);
+        // whole pieces, a power of two of keys each
+        const int last_keys = min(keys - (j0 + nt - 1) * kTileKeys, kTileKeys);
+        const uint32_t last_bytes = (uint32_t)((last_keys + cp.piece - 1) & -cp.piece) * (128 * kHalves);
         int s = 0, phase = 0, filled = 0;
-        bool ok = true;
+        bool ok = true;   // of this lane: nothing in the loop takes the whole warp, so that one that gave up can leave alone
         for (int j = 0; j < nt && ok; ++j) {
           lookup(j + 1, page_next, row_next);
-          const int live = __popc(__ballot_sync(0xffffffffu, page >= 0));
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             if (filled >= St) ok = wait_bounded(&empty[s], phase, &g_paged_status);
             if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(&full[s], live * cp.piece * 128);
-            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(&full[s], j + 1 < nt ? L::kStageBytes : last_bytes);
             if (page >= 0)
               tc::tma_load_3d(smem_addr(ring) + s * L::kStageBytes + dst0, kv ? &vmap : &kmap, 64 * half, row, page, &full[s]);
             ++filled;
@@ -981,10 +982,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
       const int first_last = sp.len - sp.n + row0 / grp;   // the CTA's first row's last key
-      bool ok = true;
-      for (int j = 0; j < nt && ok; ++j) {
+      bool ok = true;   // of this lane: one that gave up waits no more, but stays with its warp's collective instructions
+      for (int j = 0; j < nt; ++j) {
         const uint32_t at = B == 2 ? t : job < B ? job : job - B, ts = lane_base + 128 * at;
-        ok = wait_bounded(&s_full[B == 2 ? t : job], B == 2 ? j & 1 : job_parity, &g_paged_status);
+        if (ok) ok = wait_bounded(&s_full[B == 2 ? t : job], B == 2 ? j & 1 : job_parity, &g_paged_status);
         __syncwarp();
         tc::fence_after();
         uint32_t v[4][32];
@@ -1018,7 +1019,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           m = mn;
           l *= c;
           if (j > 0) {   // the last product of this tile is complete before O is touched
-            wait_bounded(&o_done[t], (j - 1) & 1, &g_paged_status);
+            if (ok) ok = wait_bounded(&o_done[t], (j - 1) & 1, &g_paged_status);
             __syncwarp();
             tc::fence_after();
 #pragma unroll

@@ -493,9 +493,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     float* scale = sc + (warp - 2) * 64;
     uint16_t* turn = reinterpret_cast<uint16_t*>(sc + kEpiWarps * 64) + (warp - 2) * 512;
     pdl_wait();
-    bool ok = true;
+    bool ok = true;   // of this lane: one that gave up waits no more, but stays with its warp's collective instructions
     const int mine = first < p.tiles ? (p.tiles - first + step - 1) / step : 0;
-    for (int a = 0; a < mine * H && ok; ++a) {
+    for (int a = 0; a < mine * H; ++a) {
       const int tile = first + a / H * step;
       const int m0 = tile % p.tiles_m * p.bn + a % H * acc_bn, n = tile / p.tiles_m * kTileN + n_off + row;
       const bool on = n < p.N;
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           scale[i] = m0 + j < p.M ? __uint_as_float(ldg_cg_u32(reinterpret_cast<const uint32_t*>(p.s + m0 + j))) : 0.f;
       }
       const float tn = on ? p.t[n] : 0.f, bn = on && bias ? Elem<T>::to_float(bias[n]) : 0.f;
-      ok = wait_bounded(&acc_full[a & 1], (a >> 1) & 1, &g_w8_status);
+      if (ok) ok = wait_bounded(&acc_full[a & 1], (a >> 1) & 1, &g_w8_status);
       __syncwarp();
       tc::fence_after();
       // 16 columns at a time, the next ones on their way from tensor memory under this block's stores

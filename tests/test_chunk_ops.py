@@ -15,6 +15,7 @@ import copy
 import ctypes
 import math
 import pickle
+import random
 
 import pytest
 import torch
@@ -534,6 +535,29 @@ def test_attention_large_scores_and_constant_rows(dtype):
         check_attention(zero, cache, table, ctx, new, paged.attention(zero, cache, table, lens, cu, max_new=max(new)), 1 / math.sqrt(128))
         y = paged.attention(q, cache, table, lens, cu, max_new=max(new), scale=0.5)
         check_attention(q, cache, table, ctx, new, y, 0.5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nh,nkv,hd", [(28, 4, 128), (16, 2, 128), (14, 2, 64), (8, 8, 64)])
+def test_attention_many_ragged_sequences(dtype, nh, nkv, hd):
+    """More sequences than a warp has lanes, of long and empty contexts, more row tiles than SMs, and dozens of key tiles
+    one after another in a CTA."""
+    rng = random.Random(nh + hd)
+    for seqs, most_new, most_ctx in ((33, 60, 700), (70, 90, 5000)):
+        new = [rng.choice((0, 1, rng.randint(1, most_new), most_new)) for _ in range(seqs)]
+        new[seqs // 2] = most_new
+        ctx = [rng.choice((0, n, n + rng.randint(0, most_ctx), most_ctx)) for n in new]
+        ctx[0] = most_ctx
+        run_attention(gen(seqs), new, ctx, nh, nkv, hd, 48, dtype, max_new=most_new)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nh,nkv,hd", [(28, 4, 128), (14, 2, 64)])
+def test_attention_long_chunk(dtype, nh, nkv, hd):
+    """Row tiles for every SM over a long context, which no cluster splits: 95 key tiles in each CTA's ring."""
+    run_attention(gen(hd), [2700], [12150], nh, nkv, hd, 64, dtype)
 
 
 @gpu
