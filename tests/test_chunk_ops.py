@@ -223,7 +223,7 @@ def test_linear_w8_strided_inputs_out_and_streams():
                                    (1144, 15727, 3000), (973, 15400, 4096)])
 def test_linear_w8_several_tiles_a_cta(dtype, m, n, k):
     """Large products: single CTAs with two and three tiles each, pairs with five, and pairs whose tiles are more than
-    256 tokens wide, with one to three each; the last tile partial both ways, rows of 16-byte multiples and not."""
+    256 tokens wide, with two and three each; the last tile partial both ways, rows of 16-byte multiples and not."""
     ops, _ = mods()
     g = gen(m + n)
     w8 = ops.W8Weight.from_float(randn(g, n, k, std=0.05))
@@ -233,6 +233,50 @@ def test_linear_w8_several_tiles_a_cta(dtype, m, n, k):
     check_linear(x, w8.q, w8.scales, bias, y)
     assert torch.equal(y, ops.linear_w8(x, w8, bias=bias))
     assert ops.ext().lib.lb_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_chunk_operators_give_the_same_bits_under_every_launch_option(dtype):
+    """Programmatic launch off and on, static weights read before the wait and not: each operator several times in a row,
+    over products of every kernel."""
+    ops, paged = mods()
+    e = ops.ext()
+    g = gen(31)
+    shapes = [(1, 2048, 512), (8, 512, 1536), (16, 1024, 4096), (40, 2048, 2048), (100, 896, 1536), (700, 2500, 1000)]
+    weights = [(randn(g, m, k, dtype=dtype), ops.W8Weight.from_float(randn(g, n, k, std=0.05)), randn(g, n, dtype=dtype))
+               for m, n, k in shapes]
+    nh, nkv, hd = 14, 2, 64
+    norms = [(1 + randn(g, hd, std=0.1)).to(dtype) for _ in range(2)]
+    freq = 1.0 / 1e6 ** (torch.arange(0, hd, 2, device="cuda", dtype=torch.float32) / hd)
+
+    def once():
+        out = [ops.linear_w8(x, w8, bias=b) for _ in range(3) for x, w8, b in weights]
+        for new, ctx in (([1, 1], [300, 70]), ([40, 5], [300, 70])):
+            q, cache, table, lens, cu = build(gen(32), new, ctx, nh, nkv, hd, 16, dtype, poison=False)
+            pos = torch.cat([torch.arange(c - n, c, device="cuda") for n, c in zip(new, ctx)])
+            seq = torch.repeat_interleave(torch.arange(2, device="cuda"), torch.tensor(new, device="cuda"))
+            slots = table[seq, pos // 16].long() * 16 + pos % 16
+            qkv = randn(gen(33), sum(new), (nh + 2 * nkv) * hd, dtype=dtype)
+            q = paged.norm_rope_append(qkv, cache, pos, slots, nh, freq, *norms)
+            out += [q, cache.k, cache.v, paged.attention(q, cache, table, lens, cu, max_new=max(new))]
+        return out
+
+    prev = {o: e.get_option(o) for o in ("pdl", "early_weights")}
+    try:
+        runs = []
+        for pdl, early in ((0, 0), (1, 0), (1, 1)):
+            e.set_option("pdl", pdl)
+            e.set_option("early_weights", early)
+            torch.cuda.synchronize()   # what wrote the weights is done
+            runs.append(once())
+        for other in runs[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+    finally:
+        torch.cuda.synchronize()
+        for o, v in prev.items():
+            e.set_option(o, v)
+    assert e.lib.lb_device_error() == 0
 
 
 @gpu
