@@ -39,9 +39,4 @@ struct Elem<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 };
 
-template <>
-struct Elem<float> {
-  static __device__ __forceinline__ float to_float(float v) { return v; }
-};
-
 }  // namespace lb
