@@ -316,7 +316,8 @@ LB_API int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens
  * lb_device_error() becomes 3. max_new / max_len: upper bounds of the new tokens and the context of any sequence
  * (tokens and table_width * page_size if unknown): a smaller value than the truth is an error that leaves outputs
  * undefined but stays inside every buffer. q's heads and tokens are strided (multiples of 8 elements), out's tokens
- * too. hd 64 or 128. Rows of the cache past a context may hold anything, NaN included. workspace:
+ * too. hd 64 or 128. Rows of the cache past a context may hold anything, NaN included; inside a context a V row with
+ * an infinity or NaN can make earlier new tokens of the call NaN too, as 0 times it does. workspace:
  * lb_paged_attention_workspace(...) bytes on the current device (0: none needed), 16-byte aligned, its content
  * undefined before and after; calls that can overlap need distinct ones.
  */

@@ -613,8 +613,8 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnPara
 // where this takes 29.)
 // Bound by the softmax beside the MMAs: a step of 256 rows x 128 keys takes some 3100 clocks at hd 128, of which the MMAs
 // need 2048, and 2700 at hd 64 (1024), with two warps a scheduler issuing 40 % of the time. 28/4 heads of 128: 4096 new
-// tokens 114 us (1050 TFLOP/s), over 32768 1530 us (1180); 14/2 of 64: 4096 over 16384 323 us (650; 370 with two score
-// tiles). Neither MMAs issued by two warps (873 for 1072), nor two softmax threads a row (3 % more on long contexts, 7 %
+// tokens 117 us (1025 TFLOP/s), over 32768 1625 us (1110) in a first second of calls and 1760 (1025) once the power cap
+// holds the clock; 14/2 of 64: 4096 over 16384 327 to 350 us (600 to 640; 370 with two score tiles). Neither MMAs issued by two warps (873 for 1072), nor two softmax threads a row (3 % more on long contexts, 7 %
 // less on short ones) came out ahead.
 __device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if one of them is
   float r;
@@ -1240,8 +1240,9 @@ int few_resident(int C) {
 // How few rows are laid out: tiles of 8 or 16 rows, clusters of C CTAs, Z clusters a context -- the choice whose estimated
 // time is least, in microseconds as measured: 4 to start and end a CTA; a block of keys and warp 1.5 (hd 64: 0.95), by one
 // in a thousand CTAs more, or what memory takes for all CTAs' blocks together; 1 to join a cluster, 4 for the second
-// kernel; CTAs past those resident at once come in further rounds. A warp takes at most 36 blocks where a split can help
-// it: contexts differ, and the longest ends last. (C = 1, 2, 3, 4, 6: 32 contexts of 4096, 28/4 heads of 128 100, 60, 47,
+// kernel; CTAs past those resident at once come in further rounds. Where a warp has more than 36 blocks each costs 1
+// more, since contexts differ and the longest ends last (36 and 1 fit contexts spread evenly up to 8192, the last line below;
+// they are not derived). (C = 1, 2, 3, 4, 6: 32 contexts of 4096, 28/4 heads of 128 100, 60, 47,
 // 66, 53 us; 64 of 4096 110, 124, 92, 104, 104; 100 of 3000, 16/2 heads 79, 53, 68, 58, 64; 96 of up to 8192, 28/4 heads
 // 196, 146, 135, 131, 134.)
 struct FewPlan {

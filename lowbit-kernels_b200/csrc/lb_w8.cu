@@ -253,8 +253,9 @@ __global__ void __launch_bounds__(kQLongThreads)
 // wide tiles would leave short of the SMs.
 // With `halves` = 2 a pair's tile is up to 512 tokens wide, in two accumulators that fill the tensor memory: 48 bytes a
 // clock and SM instead of 64 for 256 x 256; the epilogue, which then only the next tile's loads run under, is short
-// beside a long K. 8192 tokens of 18944 values, 3584 channels: 362 us (3.07 POP/s, 0.94 of twice the measured bf16 peak,
-// under the power cap; the quantization before it takes 74); 509 tokens of 1536, 17920 channels: 20.9 us with it.
+// beside a long K. 8192 tokens of 18944 values, 3584 channels: 352 us (3.16 POP/s, 0.96 of twice the measured bf16 peak) and
+// 77 for the quantization before it, 431 a call, while a burst lasts; 498 a call once the power cap holds the clock, after
+// a tenth of a second. 4096 tokens: the tensor pipe works 88 % of the time. 509 tokens of 1536, 17920 channels: 21.3 us.
 // Few tiles and long K: a cluster of S single CTAs splits K, each parks its int32 partial tile in its (then idle) ring
 // and all sum their share through distributed shared memory -- exact, so the bits do not depend on S.
 constexpr int kChunk = 128;               // bytes of K per stage
@@ -1018,7 +1019,7 @@ cudaError_t linear_t(const W8Params& p, bool pdl, cudaStream_t st) {
   if (!encode_rows(&wmap, p.w, kp, p.ldw, p.N, 128)) return cudaErrorInvalidValue;
   cudaError_t e = quantize_t<T>(p.x, p.ldx, q, kp, s, p.M, p.K, p.early ? kAtEntry : kAfterWait, pdl, st);
   if (e != cudaSuccess) return e;
-  static thread_local struct {   // the last plan of this host thread: a layer's calls follow one another
+  static thread_local struct {   // the last plan of this host thread, for calls of one shape that follow one another
     int64_t M, N, chunks;
     int sms;
     W8Plan plan;

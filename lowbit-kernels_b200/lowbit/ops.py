@@ -427,7 +427,8 @@ class W8Weight:
 def linear_w8(x, w8, bias=None, out=None):
     """x [M, K] fp16 or bf16 (rows any stride apart) -> [M, N] of the same type: each row quantized to 8-bit integers
     with its own scale, the product with w8 (W8Weight) exact in int32, then scaled, `bias` ([N], x's type) added and
-    rounded once. `out`: an optional contiguous [M, N] tensor that receives the result."""
+    rounded once. `out`: an optional contiguous [M, N] tensor that receives the result. A serving operator: the result
+    carries no autograd graph."""
     tc = _tc if _tc is not None else _torchcall()
     if tc:
         y = tc.linear_w8(x, w8._q, w8._scales, out, bias)

@@ -3,8 +3,9 @@ q and k, rotary rotation, append to the cache in one pass) and `attention` (the 
 their cached contexts; one new token per sequence is a decode step). `PagedDecoder` runs them together with the 8-bit
 products of ops.linear_w8. No counterpart in the reference, which feeds transformers' own cache (bench/e2e.py:84-147).
 
-Every call launches on the current torch stream of the tensors' device and never synchronizes. There is no fallback:
-without the library or a CUDA device the first call raises.
+Every call launches on the current torch stream of the tensors' device and never synchronizes. Serving operators: their
+outputs carry no autograd graph, whatever their inputs require. There is no fallback: without the library or a CUDA device
+the first call raises.
 """
 import ctypes
 import math
@@ -132,7 +133,8 @@ def attention(q, cache, page_table, seq_lens, cu_new, max_new=None, max_len=None
     W * page_size). They choose the kernel and how contexts are split, so a decode step passes max_new=1; a bound below
     the truth is an error that leaves outputs undefined. A page-table entry outside the cache counts as a page of zeros and
     sets the library's device status to 3 (`ops.ext().lib.lb_device_error()`, which synchronizes; no call reads it by
-    itself). scale defaults to 1 / sqrt(hd). Tokens past cu_new[S] (a padded
+    itself). scale defaults to 1 / sqrt(hd). Cache rows past a context may hold anything; inside one, a V row with an
+    infinity or NaN can make earlier new tokens of the call NaN too, as 0 times it does. Tokens past cu_new[S] (a padded
     batch's) belong to no sequence: their outputs are left unwritten."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc:
