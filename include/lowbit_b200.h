@@ -46,7 +46,7 @@ typedef enum lb_layout { LB_LAYOUT_CANONICAL = 0, LB_LAYOUT_V3 = 1, LB_LAYOUT_MM
 
 typedef enum lb_option {
   LB_OPT_PDL = 0,           /* 1 (default): launch with programmatic dependent launch enabled */
-  LB_OPT_EARLY_WEIGHTS = 1, /* 1: GEMV kernels, lb_w8_linear and the norm of lb_paged_norm_rope_append fetch their
+  LB_OPT_EARLY_WEIGHTS = 1, /* 1: GEMV kernels, lb_w8_linear, lb_f8_linear and the norm of lb_paged_norm_rope_append fetch their
                                first weights before waiting on the previous kernel in the stream (only for weights
                                no in-flight kernel writes); default 0 */
   LB_OPT_GEMV_KSPLIT = 2,   /* 0 (default): automatic; 1..8 forces the GEMV's K-split cluster size */
@@ -281,6 +281,29 @@ LB_API int lb_w8_linear(const void* x, int dtype, int64_t ldx, const void* w, in
                         int64_t workspace_bytes, lb_stream_t stream);
 
 /*
+ * The linear layer in 8-bit floating point (e4m3: 4 exponent and 3 fraction bits, largest value 448) with a scale for each
+ * block of 128. Weights q e4m3 [N, ldq] and one fp32 scale per 128 x 128 block, t [ceil(N / 128), ceil(K / 128)]; with a =
+ * max(max |w| of the block, 2^-100), t = a / 448 and q = w * (448 / a) rounded to nearest even, columns K.. zeroed.
+ * lb_f8_quantize_weight makes both from w [N, K] in fp16, bf16 or fp32, rows ldw elements apart; ldq a multiple of 16.
+ * K <= 131072.
+ */
+LB_API int lb_f8_quantize_weight(const void* w, int dtype, int64_t n, int64_t k, int64_t ldw, void* q, int64_t ldq, float* t,
+                                 lb_stream_t stream);
+
+/*
+ * y[m, n] = sum over blocks b of K of s[m, b] t[n / 128, b] (sum over k in b of q[m, k] w[n, k]) + bias[n]: q and s are the rows of
+ * x quantized by the same rule, a scale per row and 128 values. Sums in fp32, one rounding. A row whose block holds an
+ * infinity or a NaN gives NaN; other rows do not see it. x and y fp16 or bf16 (y contiguous, rows of x ldx elements apart), bias
+ * [N] of that type or NULL; w e4m3 [N, ldw] 16-byte aligned, ldw a multiple of 16, zeros from column K to the next
+ * multiple of 16. workspace: lb_f8_workspace(m, n, k) bytes on the current device (0: none needed), 16-byte aligned, its
+ * content undefined before and after; calls that can overlap need distinct ones.
+ */
+LB_API int64_t lb_f8_workspace(int64_t m, int64_t n, int64_t k);
+LB_API int lb_f8_linear(const void* x, int dtype, int64_t ldx, const void* w, int64_t ldw, const float* w_scales,
+                        const void* bias, void* y, int64_t m, int64_t n, int64_t k, void* workspace,
+                        int64_t workspace_bytes, lb_stream_t stream);
+
+/*
  * A paged KV cache: k and v [num_pages, nkv, page_size, hd], each page's block contiguous, pages k_page_stride /
  * v_page_stride elements apart. page_size a multiple of 16. Token j of a sequence lies in row j % page_size of page
  * table[j / page_size]; its slot is page * page_size + row.
@@ -328,6 +351,70 @@ LB_API int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_h
                               int64_t table_width, const int32_t* seq_lens, const int32_t* cu_new, int seqs,
                               int64_t max_new, int64_t max_len, float scale, void* out, int64_t out_token_stride,
                               void* workspace, int64_t workspace_bytes, lb_stream_t stream);
+
+/*
+ * lb_paged_attention for drafted tokens that form trees: sequence s's new token i sees its cached context, the keys
+ * 0 .. seq_lens[s] - n - 1, and those of its n new tokens j whose bit is set, bit j % 32 of mask[(cu_new[s] + i) *
+ * mask_words + j / 32] (itself among them only where its own bit is). Any pattern of bits will do; new tokens past 32 *
+ * mask_words are seen by none. The rest, the workspace too, is as in lb_paged_attention.
+ */
+LB_API int lb_paged_tree_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
+                                   const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride,
+                                   int64_t table_width, const int32_t* seq_lens, const int32_t* cu_new, int seqs,
+                                   const uint32_t* mask, int64_t mask_words, int64_t max_new, int64_t max_len, float scale,
+                                   void* out, int64_t out_token_stride, void* workspace, int64_t workspace_bytes,
+                                   lb_stream_t stream);
+
+/*
+ * What a call on new tokens needs, from request lengths on the device: sequence s of `seqs` (at most 8192) has seq_lens[s] tokens
+ * in the cache and gets new_lens[s] more (negative lengths count as 0). Written are cu_out [seqs + 1], the first new token
+ * of each; lens_out [seqs], the tokens with the new ones; and for `tokens` rows the positions and the slots of the paged
+ * cache (int64; slot = page * page_size + row). Rows past the last sequence get position 0 and slot -1.
+ * held / free_pages / free_count (all or none): pages are given out too. A row of page_table int32 [seqs, table_width] holds
+ * held[s] pages; what it lacks is taken from free_pages [num_free], of which the first *free_count are free, the last first,
+ * by the sequences in their order, and written behind them; held_out and free_count_out say what there is then. The
+ * outputs of both, and lens_out, may be the inputs themselves. Without them the table is complete as it is.
+ * A sequence is refused where the rows, the table's width or the free pages do not suffice (from the first that lacks pages
+ * on, all that need some): its lens_out is 0, its slots are -1, and it takes no pages; its rows stay its own.
+ * parents int32 [tokens] or NULL: the new tokens of a sequence form a tree, parents[t] being the place of the token's parent
+ * among them, an earlier one; anything else makes it a root. A token's position is then seq_lens[s] + its depth, and mask
+ * uint32 [tokens, words] receives its ancestors and itself, as lb_paged_tree_attention takes them. words <= 32: trees of
+ * up to 1024 tokens; ancestors further back than 32 * words tokens from a sequence's first are not recorded.
+ */
+LB_API int lb_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int seqs, int32_t* page_table, int64_t table_stride,
+                         int64_t table_width, int page_size, int64_t tokens, const int32_t* held, const int32_t* free_pages,
+                         int64_t num_free, const int32_t* free_count, const int32_t* parents, int64_t words, int32_t* cu_out,
+                         int32_t* lens_out, int32_t* held_out, int32_t* free_count_out, int64_t* positions, int64_t* slots,
+                         uint32_t* mask, lb_stream_t stream);
+
+/*
+ * Greedy acceptance of drafted trees. logits [tokens, vocab] (fp16, bf16 or fp32, rows ld elements apart) follow the new tokens
+ * `drafted` (int64) of the sequences cu_new; targets int64 [tokens] receives each row's first largest value's index (a NaN
+ * counts as larger than all). A sequence's first token is its last certain one; from there the path goes to the
+ * first later token whose parent (parents, as in lb_paged_plan) is the token at hand and which is its target, until there is none
+ * or the path has max_path tokens. path int32 [seqs, max_path]: the places of its tokens among the new ones, -1 behind
+ * them; accepted int32 [seqs]: how many; next int64 [seqs]: the target after the last. A sequence without new tokens gets 0
+ * and -1. Rows past cu_new[seqs] are not read, their targets not written. max_new (1 to 1024) bounds the new tokens of any
+ * sequence, those behind it are ignored. workspace: lb_draft_verify_workspace(tokens, vocab) bytes, 16-byte aligned, distinct for calls that
+ * can overlap.
+ */
+LB_API int64_t lb_draft_verify_workspace(int64_t tokens, int64_t vocab);
+LB_API int lb_draft_verify(const void* logits, int dtype, int64_t ld, int64_t tokens, int64_t vocab, const int64_t* drafted,
+                           const int32_t* parents, const int32_t* cu_new, int seqs, int64_t max_new, int64_t max_path,
+                           int32_t* accepted, int32_t* path, int64_t* next, int64_t* targets, void* workspace,
+                           int64_t workspace_bytes, lb_stream_t stream);
+
+/*
+ * Moves the K and V rows of accepted tokens to where a sequence without the others has them, in `layers` (at most 128) caches of one
+ * shape, type and page strides: row seq_lens[s] - n + path[s][d] to seq_lens[s] - n + d for d < accepted[s] (n the new tokens, seq_lens
+ * with them). A path rises; an entry outside the new tokens or below its place, or a row outside the cache, is left out and
+ * sets lb_device_error() to 3. lens_out [seqs], not seq_lens itself, receives seq_lens[s] - n + accepted[s]; for a sequence
+ * that lb_paged_plan refused (seq_lens[s] < n) it is left as it is (keep) or 0, and nothing moves.
+ */
+LB_API int lb_paged_compact(const lb_paged_cache* const* caches, int layers, const int32_t* page_table, int64_t table_stride,
+                            int64_t table_width, const int32_t* seq_lens, const int32_t* cu_new, const int32_t* path,
+                            const int32_t* accepted, int seqs, int64_t max_path, int32_t* lens_out, int keep,
+                            lb_stream_t stream);
 
 #ifdef __cplusplus
 }

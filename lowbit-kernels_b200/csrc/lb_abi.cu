@@ -203,6 +203,8 @@ int lb_device_error(void) {
   if (!a) a = lb::allreduce_device_error();
   if (!a) a = lb::w8_device_error();
   if (!a) a = lb::paged_device_error();
+  if (!a) a = lb::f8_device_error();
+  if (!a) a = lb::draft_device_error();
   return a ? a : lb::decode_device_error();
 }
 
@@ -213,6 +215,8 @@ void lb_clear_device_error(void) {
   lb::allreduce_clear_device_error();
   lb::w8_clear_device_error();
   lb::paged_clear_device_error();
+  lb::f8_clear_device_error();
+  lb::draft_clear_device_error();
   lb::decode_clear_device_error();
 }
 
@@ -705,11 +709,14 @@ int64_t lb_paged_attention_workspace(int64_t tokens, int nh, const lb_paged_cach
                                                 max_len < width ? max_len : width);
 }
 
-int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
-                       const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride, int64_t table_width,
-                       const int32_t* seq_lens, const int32_t* cu_new, int seqs, int64_t max_new, int64_t max_len,
-                       float scale, void* out, int64_t out_token_stride, void* workspace,
-                       int64_t workspace_bytes, lb_stream_t stream) {
+}  // extern "C"
+
+// both forms of the attention over the cache; mask: a tree's, or null
+static int attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
+                  const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride, int64_t table_width,
+                  const int32_t* seq_lens, const int32_t* cu_new, int seqs, int64_t max_new, int64_t max_len,
+                  float scale, const uint32_t* mask, int64_t mask_words, const char* what, void* out, int64_t out_token_stride, void* workspace,
+                  int64_t workspace_bytes, lb_stream_t stream) {
   int rc = check_cache(cache);
   if (rc) return rc;
   if (!q || !page_table || !seq_lens || !cu_new || !out) return fail(LB_ERR_ARGUMENT, "null pointer argument");
@@ -731,12 +738,194 @@ int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_str
   if ((rc = check_device())) return rc;
   const int64_t width = table_width * cache->page_size;
   const lb::PagedAttnParams p{q, q_token_stride, q_head_stride, (int)tokens, nh, cache->nkv, cache->hd, cache->dtype,
-                              cache->k, cache->v, cache->k_page_stride, cache->v_page_stride, cache->page_size,
-                              cache->num_pages, page_table, table_stride, (int)table_width, seq_lens, cu_new, seqs,
-                              (int)(max_new < tokens ? max_new : tokens), (int)(max_len < width ? max_len : width), scale,
-                              out, out_token_stride, workspace};
+                         cache->k, cache->v, cache->k_page_stride, cache->v_page_stride, cache->page_size,
+                         cache->num_pages, page_table, table_stride, (int)table_width, seq_lens, cu_new, seqs,
+                         (int)(max_new < tokens ? max_new : tokens), (int)(max_len < width ? max_len : width), scale,
+                         out, out_token_stride, workspace, nullptr, nullptr, mask, (int)mask_words};
   return launched(lb::launch_paged_attention(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)),
-                  "paged_attention");
+                  what);
+}
+
+extern "C" {
+
+int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
+                       const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride, int64_t table_width,
+                       const int32_t* seq_lens, const int32_t* cu_new, int seqs, int64_t max_new, int64_t max_len,
+                       float scale, void* out, int64_t out_token_stride, void* workspace,
+                       int64_t workspace_bytes, lb_stream_t stream) {
+  return attend(q, q_token_stride, q_head_stride, tokens, nh, cache, page_table, table_stride, table_width, seq_lens, cu_new, seqs,
+                max_new, max_len, scale, nullptr, 0, "paged_attention", out, out_token_stride, workspace, workspace_bytes, stream);
+}
+
+int lb_paged_tree_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
+                            const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride,
+                            int64_t table_width, const int32_t* seq_lens, const int32_t* cu_new, int seqs,
+                            const uint32_t* mask, int64_t mask_words, int64_t max_new, int64_t max_len, float scale,
+                            void* out, int64_t out_token_stride, void* workspace, int64_t workspace_bytes,
+                            lb_stream_t stream) {
+  if (!mask) return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if (mask_words < 1 || mask_words > INT32_MAX / 32) return fail(LB_ERR_ARGUMENT, "mask_words=%lld: at least one", (long long)mask_words);
+  if (reinterpret_cast<uintptr_t>(mask) & 3u) return fail(LB_ERR_ALIGNMENT, "the mask must be 4-byte aligned");
+  return attend(q, q_token_stride, q_head_stride, tokens, nh, cache, page_table, table_stride, table_width, seq_lens, cu_new, seqs,
+                max_new, max_len, scale, mask, mask_words, "paged_tree_attention", out, out_token_stride, workspace, workspace_bytes,
+                stream);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------- 8-bit floating point
+
+static int check_f8_rows(const void* x, int dtype, int64_t rows, int64_t k, int64_t ldx, const void* q, int64_t ldq, const void* scales) {
+  if (!x || !q || !scales) return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if (rows < 1 || k < 1 || rows > (1 << 30)) return fail(LB_ERR_ARGUMENT, "shape mismatch: %lld rows, K=%lld", (long long)rows, (long long)k);
+  if (k > 131072) return fail(LB_ERR_ARGUMENT, "K=%lld: at most 131072", (long long)k);
+  if (ldx < k) return fail(LB_ERR_ARGUMENT, "rows overlap: K=%lld, stride %lld", (long long)k, (long long)ldx);
+  if (ldq < k || ldq % 16) return fail(LB_ERR_ARGUMENT, "the 8-bit rows' stride must be a multiple of 16, at least K");
+  if ((reinterpret_cast<uintptr_t>(x) & (dtype == LB_F32 ? 3u : 1u)) || !aligned16(q) || (reinterpret_cast<uintptr_t>(scales) & 3u))
+    return fail(LB_ERR_ALIGNMENT, "rows must be aligned to their type, 8-bit values to 16 bytes, scales to 4");
+  return LB_OK;
+}
+
+extern "C" {
+
+int lb_f8_quantize_weight(const void* w, int dtype, int64_t n, int64_t k, int64_t ldw, void* q, int64_t ldq, float* t,
+                          lb_stream_t stream) {
+  if (dtype < LB_F16 || dtype > LB_F32) return fail(LB_ERR_ARGUMENT, "dtype is 0 (fp16), 1 (bf16) or 2 (fp32)");
+  int rc = check_f8_rows(w, dtype, n, k, ldw, q, ldq, t);
+  if (rc) return rc;
+  if (n > 65535 * 128) return fail(LB_ERR_ARGUMENT, "N=%lld is too large", (long long)n);
+  if ((rc = check_device())) return rc;
+  return launched(lb::launch_f8_quantize_weight(w, dtype, ldw, q, ldq, t, n, k, g_opt[LB_OPT_PDL].load() != 0,
+                                                reinterpret_cast<cudaStream_t>(stream)),
+                  "f8_quantize_weight");
+}
+
+int64_t lb_f8_workspace(int64_t m, int64_t n, int64_t k) {
+  return m < 1 || n < 1 || k < 1 ? 0 : (int64_t)lb::f8_workspace_bytes(m, n, k);
+}
+
+int lb_f8_linear(const void* x, int dtype, int64_t ldx, const void* w, int64_t ldw, const float* w_scales, const void* bias,
+                 void* y, int64_t m, int64_t n, int64_t k, void* workspace, int64_t workspace_bytes, lb_stream_t stream) {
+  if (!w || !w_scales || !y) return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if (dtype != LB_F16 && dtype != LB_BF16) return fail(LB_ERR_ARGUMENT, "dtype is 0 (fp16) or 1 (bf16)");
+  int rc = check_f8_rows(x, dtype, m, k, ldx, w, ldw, w_scales);
+  if (rc) return rc;
+  if (m > 65535 * 16) return fail(LB_ERR_ARGUMENT, "M=%lld: at most %d rows a call", (long long)m, 65535 * 16);
+  if (n < 1 || n > (1 << 30)) return fail(LB_ERR_ARGUMENT, "shape mismatch: N=%lld", (long long)n);
+  if (!aligned2(bias) || !aligned2(y)) return fail(LB_ERR_ALIGNMENT, "bias and y must be 2-byte aligned");
+  const int64_t need = (int64_t)lb::f8_workspace_bytes(m, n, k);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(LB_ERR_ARGUMENT, "the workspace holds %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0),
+                (long long)need);
+  if (!aligned16(workspace)) return fail(LB_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
+  if ((rc = check_device())) return rc;
+  const lb::F8Params p{x, ldx, dtype, w, ldw, w_scales, bias, y, m, n, k, workspace, g_opt[LB_OPT_EARLY_WEIGHTS].load() != 0};
+  return launched(lb::launch_f8_linear(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)), "f8_linear");
+}
+
+// ------------------------------------------------------------------------------- a step of drafted tokens
+
+int lb_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int seqs, int32_t* page_table, int64_t table_stride,
+                  int64_t table_width, int page_size, int64_t tokens, const int32_t* held, const int32_t* free_pages,
+                  int64_t num_free, const int32_t* free_count, const int32_t* parents, int64_t words, int32_t* cu_out,
+                  int32_t* lens_out, int32_t* held_out, int32_t* free_count_out, int64_t* positions, int64_t* slots,
+                  uint32_t* mask, lb_stream_t stream) {
+  if (!seq_lens || !new_lens || !page_table || !cu_out || !lens_out || (tokens > 0 && (!positions || !slots)))
+    return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if ((held == nullptr) != (free_pages == nullptr) || (held == nullptr) != (free_count == nullptr) ||
+      (held == nullptr) != (held_out == nullptr) || (held == nullptr) != (free_count_out == nullptr))
+    return fail(LB_ERR_ARGUMENT, "held, free_pages and free_count go together, with their outputs");
+  if ((parents == nullptr) != (mask == nullptr)) return fail(LB_ERR_ARGUMENT, "parents and mask go together");
+  if (seqs < 1 || seqs > lb::kMaxPlanSeqs) return fail(LB_ERR_ARGUMENT, "seqs=%d: 1 to %d", seqs, lb::kMaxPlanSeqs);
+  if (tokens < 0 || tokens > INT32_MAX / 64) return fail(LB_ERR_ARGUMENT, "tokens=%lld out of range", (long long)tokens);
+  if (page_size < 16 || page_size % 16 || page_size > 65536)
+    return fail(LB_ERR_ARGUMENT, "page_size=%d: a multiple of 16 up to 65536", page_size);
+  if (table_width < 1 || table_stride < table_width || table_width * page_size > INT32_MAX)
+    return fail(LB_ERR_ARGUMENT, "page table: at least one page a row, contexts below 2^31");
+  if (held && (num_free < 0 || num_free > INT32_MAX)) return fail(LB_ERR_ARGUMENT, "num_free=%lld out of range", (long long)num_free);
+  if (parents && (words < 1 || words > lb::kMaxTree / 32))
+    return fail(LB_ERR_ARGUMENT, "words=%lld: trees hold up to %d tokens", (long long)words, lb::kMaxTree);
+  int rc = check_device();
+  if (rc) return rc;
+  const lb::PlanParams p{seq_lens, new_lens, held, free_pages, free_count, (int)num_free, page_table, table_stride, (int)table_width,
+                         page_size, seqs, (int)tokens, parents, (int)words, cu_out, lens_out, held_out, free_count_out, positions,
+                         slots, mask};
+  return launched(lb::launch_plan(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)), "paged_plan");
+}
+
+int64_t lb_draft_verify_workspace(int64_t tokens, int64_t vocab) {
+  return tokens < 1 || vocab < 1 ? 0 : (int64_t)lb::verify_workspace_bytes(tokens, vocab);
+}
+
+int lb_draft_verify(const void* logits, int dtype, int64_t ld, int64_t tokens, int64_t vocab, const int64_t* drafted,
+                    const int32_t* parents, const int32_t* cu_new, int seqs, int64_t max_new, int64_t max_path,
+                    int32_t* accepted, int32_t* path, int64_t* next, int64_t* targets, void* workspace,
+                    int64_t workspace_bytes, lb_stream_t stream) {
+  if (!logits || !drafted || !parents || !cu_new || !accepted || !path || !next || !targets)
+    return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if (dtype < LB_F16 || dtype > LB_F32) return fail(LB_ERR_ARGUMENT, "dtype is 0 (fp16), 1 (bf16) or 2 (fp32)");
+  if (tokens < 1 || tokens > (1 << 20) || vocab < 1 || vocab > (1 << 30) || seqs < 1)
+    return fail(LB_ERR_ARGUMENT, "shape mismatch: %lld tokens, vocabulary of %lld, %d sequences", (long long)tokens, (long long)vocab, seqs);
+  if (ld < vocab) return fail(LB_ERR_ARGUMENT, "rows of the logits overlap: %lld values, stride %lld", (long long)vocab, (long long)ld);
+  if (max_new < 1 || max_new > lb::kMaxTree) return fail(LB_ERR_ARGUMENT, "max_new=%lld: trees hold 1 to %d tokens", (long long)max_new, lb::kMaxTree);
+  if (max_path < 1 || max_path > lb::kMaxTree) return fail(LB_ERR_ARGUMENT, "max_path=%lld: 1 to %d", (long long)max_path, lb::kMaxTree);
+  if (reinterpret_cast<uintptr_t>(logits) & (dtype == LB_F32 ? 3u : 1u)) return fail(LB_ERR_ALIGNMENT, "logits must be aligned to their type");
+  const int64_t need = (int64_t)lb::verify_workspace_bytes(tokens, vocab);
+  if (!workspace || workspace_bytes < need)
+    return fail(LB_ERR_ARGUMENT, "the workspace holds %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
+  if (!aligned16(workspace)) return fail(LB_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
+  int rc = check_device();
+  if (rc) return rc;
+  const lb::VerifyParams p{logits, ld, dtype, (int)tokens, (int)vocab, drafted, parents, cu_new, seqs, (int)max_new, (int)max_path,
+                           accepted, path, next, targets, static_cast<uint64_t*>(workspace)};
+  return launched(lb::launch_verify(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)), "draft_verify");
+}
+
+int lb_paged_compact(const lb_paged_cache* const* caches, int layers, const int32_t* page_table, int64_t table_stride,
+                     int64_t table_width, const int32_t* seq_lens, const int32_t* cu_new, const int32_t* path,
+                     const int32_t* accepted, int seqs, int64_t max_path, int32_t* lens_out, int keep, lb_stream_t stream) {
+  if (!caches || !page_table || !seq_lens || !cu_new || !path || !accepted || !lens_out) return fail(LB_ERR_ARGUMENT, "null pointer argument");
+  if (layers < 1 || layers > lb::kMaxLayers) return fail(LB_ERR_ARGUMENT, "layers=%d: 1 to %d caches a call", layers, lb::kMaxLayers);
+  if (seqs < 1 || seqs > 65535) return fail(LB_ERR_ARGUMENT, "seqs=%d: 1 to 65535", seqs);
+  if (max_path < 1 || max_path > lb::kMaxTree) return fail(LB_ERR_ARGUMENT, "max_path=%lld: 1 to %d", (long long)max_path, lb::kMaxTree);
+  if (lens_out == seq_lens) return fail(LB_ERR_ARGUMENT, "lens_out must not be seq_lens itself");
+  lb::CompactParams p;
+  for (int i = 0; i < layers; ++i) {
+    const lb_paged_cache* c = caches[i];
+    int rc = check_cache(c);
+    if (rc) return rc;
+    const lb_paged_cache* a = caches[0];
+    if (c->dtype != a->dtype || c->nkv != a->nkv || c->hd != a->hd || c->page_size != a->page_size || c->num_pages != a->num_pages ||
+        c->k_page_stride != a->k_page_stride || c->v_page_stride != a->v_page_stride)
+      return fail(LB_ERR_ARGUMENT, "cache %d is not laid out as the first", i);
+    p.k[i] = c->k;
+    p.v[i] = c->v;
+  }
+  const lb_paged_cache* a = caches[0];
+  if (table_width < 1 || table_stride < table_width || table_width * a->page_size > INT32_MAX)
+    return fail(LB_ERR_ARGUMENT, "page table: at least one page a row, contexts below 2^31");
+  if (a->nkv > 65536) return fail(LB_ERR_ARGUMENT, "nkv=%d: at most 65536", a->nkv);
+  int rc = check_device();
+  if (rc) return rc;
+  p.k_page = a->k_page_stride;
+  p.v_page = a->v_page_stride;
+  p.num_pages = a->num_pages;
+  p.layers = layers;
+  p.nkv = a->nkv;
+  p.hd = a->hd;
+  p.page_size = a->page_size;
+  p.table = page_table;
+  p.table_stride = table_stride;
+  p.table_width = (int)table_width;
+  p.seq_lens = seq_lens;
+  p.cu_new = cu_new;
+  p.path = path;
+  p.accepted = accepted;
+  p.seqs = seqs;
+  p.max_path = (int)max_path;
+  p.lens_out = lens_out;
+  p.keep = keep != 0;
+  return launched(lb::launch_compact(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)), "paged_compact");
 }
 
 }  // extern "C"

@@ -156,6 +156,27 @@ cudaError_t launch_w8_quantize_rows(const void* x, int dtype, int64_t ldx, int8_
 int w8_device_error();   // synchronizes
 void w8_clear_device_error();
 
+// linear layer in 8-bit floating point with a scale for each block of 128 (lb_f8.cu); dtype as above
+struct F8Params {
+  const void* x;        // [M, K], rows ldx elements apart
+  int64_t ldx;
+  int dtype;
+  const void* w;        // e4m3 [N, ldw], zeros from K to the next multiple of 16
+  int64_t ldw;
+  const float* w_scales;   // [blocks of N][blocks of K]
+  const void* bias;     // [N] or null
+  void* y;              // [M, N]
+  int64_t M, N, K;
+  void* workspace;
+  bool early;           // w and w_scales may be read before the wait on the previous kernel
+};
+size_t f8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+cudaError_t launch_f8_linear(const F8Params& p, bool pdl, cudaStream_t st);
+cudaError_t launch_f8_quantize_weight(const void* w, int dtype, int64_t ldw, void* q, int64_t ldq, float* t, int64_t N, int64_t K,
+                                      bool pdl, cudaStream_t st);
+int f8_device_error();   // synchronizes
+void f8_clear_device_error();
+
 // paged KV cache (lb_paged.cu): K and V [num_pages, nkv, page_size, hd], pages k_page / v_page elements apart
 struct PagedCacheView {
   void* k;
@@ -189,10 +210,76 @@ struct PagedAttnParams {
   void* workspace;
   float* work_ml = nullptr;  // parts of the workspace (lb_paged.cu)
   float* work_o = nullptr;
+  const uint32_t* mask = nullptr;   // a tree's new tokens: [tokens, mask_words], bit j: the token sees its sequence's new token j
+  int mask_words = 0;
 };
 size_t paged_attention_workspace(int64_t seqs, int nh, int nkv, int hd, int64_t max_new, int64_t max_len);
 cudaError_t launch_paged_attention(const PagedAttnParams& p, bool pdl, cudaStream_t st);
 int paged_device_error();   // synchronizes
 void paged_clear_device_error();
+
+// a step of drafted tokens (lb_draft.cu)
+constexpr int kMaxTree = 1024;     // new tokens of a tree
+constexpr int kMaxPlanSeqs = 8192;
+constexpr int kMaxLayers = 128;
+struct PlanParams {
+  const int32_t* seq_lens;   // [seqs] tokens cached
+  const int32_t* new_lens;
+  const int32_t* held;       // pages held, or null: the table is complete
+  const int32_t* free_pages; // [num_free], the first *free_count of them free, the last taken first
+  const int32_t* free_count;
+  int num_free;
+  int32_t* table;
+  int64_t table_stride;
+  int table_width, page_size, seqs, tokens;
+  const int32_t* parents;    // [tokens] or null
+  int words;                 // of a row of the mask
+  int32_t* cu_out;           // [seqs + 1]
+  int32_t* lens_out;
+  int32_t* held_out;
+  int32_t* free_count_out;
+  int64_t* positions;        // [tokens]
+  int64_t* slots;
+  uint32_t* mask;            // [tokens, words]
+};
+cudaError_t launch_plan(const PlanParams& p, bool pdl, cudaStream_t st);
+
+struct VerifyParams {
+  const void* logits;        // [tokens, vocab], rows ld elements apart
+  int64_t ld;
+  int dtype, tokens, vocab;
+  const int64_t* drafted;    // [tokens]
+  const int32_t* parents;
+  const int32_t* cu_new;     // [seqs + 1]
+  int seqs, max_new, max_path;
+  int32_t* accepted;         // [seqs]
+  int32_t* path;             // [seqs, max_path]
+  int64_t* next;             // [seqs]
+  int64_t* targets;          // [tokens]
+  uint64_t* parts;           // workspace
+};
+size_t verify_workspace_bytes(int64_t tokens, int64_t vocab);
+cudaError_t launch_verify(const VerifyParams& p, bool pdl, cudaStream_t st);
+
+struct CompactParams {
+  void* k[kMaxLayers];
+  void* v[kMaxLayers];
+  int64_t k_page, v_page;    // elements between pages, alike in all layers
+  int64_t num_pages;
+  int layers, nkv, hd, page_size;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_width;
+  const int32_t* seq_lens;   // the new tokens included
+  const int32_t* cu_new;
+  const int32_t* path;       // [seqs, max_path]
+  const int32_t* accepted;
+  int seqs, max_path;
+  int32_t* lens_out;
+  bool keep;                 // lens_out of a sequence that the plan refused stays as it is, else it is 0
+};
+cudaError_t launch_compact(const CompactParams& p, bool pdl, cudaStream_t st);
+int draft_device_error();   // synchronizes
+void draft_clear_device_error();
 
 }  // namespace lb

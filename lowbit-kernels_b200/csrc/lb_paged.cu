@@ -273,7 +273,14 @@ __device__ __forceinline__ SeqSpan seq_span(const PagedAttnParams& p, int seq) {
   return v;
 }
 
-template <typename T, int HD, int NT>   // NT: n-tiles of 8 query rows
+// A word of a new token's row of bits, `at` the row's first: word -1 stands for the context, which every new token sees,
+// words past the row for nothing.
+__device__ __forceinline__ uint32_t tree_word(const PagedAttnParams& p, int64_t at, int w) {
+  return w < 0 ? 0xFFFFFFFFu : w < p.mask_words ? ldg_cg_u32(p.mask + at + w) : 0u;
+}
+
+// TREE: a new token sees the context and the new tokens whose bits its row of the mask holds, else all up to itself
+template <typename T, int HD, int NT, bool TREE>   // NT: n-tiles of 8 query rows
 __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const PagedAttnParams p, int row_tiles, int C, int Z) {
   constexpr int kRows = 8 * NT, KI = HD / 32, VH = HD / 64;
   __shared__ __align__(16) float part[kFewWarps][kRows][HD + 4];
@@ -295,12 +302,13 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
   const int rows = min(kRows, sp.n * grp - rt * kRows);   // of this tile (all the CTAs of a cluster agree)
   if (rows <= 0) return;
   const int row0 = rt * kRows;
-  const int keys = min(sp.len, sp.len - sp.n + (row0 + rows - 1) / grp + 1);   // the last row's
+  const int keys = TREE ? sp.len : min(sp.len, sp.len - sp.n + (row0 + rows - 1) / grp + 1);   // the last row's
   const int blocks = keys > 0 ? (keys + 15) / 16 : 0;
   const int share = z * C + rank, shares = Z * C;
   const int u0 = (int)((int64_t)blocks * share / shares), u1 = (int)((int64_t)blocks * (share + 1) / shares);
 
-  // Q as the n-side operand, rows past the tile as zeros; the last key each of this lane's two rows per n-tile sees
+  // Q as the n-side operand, rows past the tile as zeros; the last key each of this lane's two rows per n-tile sees (TREE:
+  // its token, -1 for none)
   uint4 q[NT][KI];
   int last[NT][2];
   int first_masked = INT_MAX;   // blocks from this key on need the mask
@@ -318,10 +326,10 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int rr = 8 * nt + 2 * t + e;
-      last[nt][e] = rr < rows ? sp.len - sp.n + (row0 + rr) / grp : -1;
+      last[nt][e] = rr < rows ? (TREE ? sp.t0 : sp.len - sp.n) + (row0 + rr) / grp : -1;
     }
   }
-  first_masked = sp.len - sp.n + row0 / grp + 1;   // the first row's count of keys
+  first_masked = TREE ? sp.len - sp.n : sp.len - sp.n + row0 / grp + 1;   // the first row's count of keys
   const float scale = p.scale * 1.44269504088896340736f;   // scores in powers of two
 
   const int per_page = p.page_size / 16;
@@ -396,7 +404,17 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         s[nt][e] *= scale;
-        if (masked && 16 * u + g + (e >= 2 ? 8 : 0) > last[nt][e & 1]) s[nt][e] = -INFINITY;
+        if (masked) {
+          const int key = 16 * u + g + (e >= 2 ? 8 : 0);
+          if (TREE) {
+            const int j = key - (sp.len - sp.n);   // of the new tokens; below 0 the context's
+            if (last[nt][e & 1] < 0 || key >= sp.len ||
+                !(tree_word(p, (int64_t)last[nt][e & 1] * p.mask_words, j >> 5) >> (j & 31) & 1u))
+              s[nt][e] = -INFINITY;
+          } else if (key > last[nt][e & 1]) {
+            s[nt][e] = -INFINITY;
+          }
+        }
         move |= s[nt][e] > m[nt][e & 1] + 8.f;
       }
     if (__any_sync(0xffffffffu, move)) {
@@ -727,7 +745,7 @@ __device__ __forceinline__ T* shfl_ptr(T* v, int lane) {
   return reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), lane));
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool TREE>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                            const ChunkParams cp) {
@@ -788,7 +806,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   int rows = 0, keys = 0;
   if (seq >= 0) {
     rows = min(kTileRows, sp.n * grp - row0);
-    keys = max(0, min(sp.len, sp.len - sp.n + (row0 + rows - 1) / grp + 1));   // the last row's
+    keys = max(0, TREE ? sp.len : min(sp.len, sp.len - sp.n + (row0 + rows - 1) / grp + 1));   // the last row's
   }
   const int key_tiles = (keys + kTileKeys - 1) / kTileKeys;
   const int j0 = (int)((int64_t)key_tiles * rank / C), nt = (int)((int64_t)key_tiles * (rank + 1) / C) - j0;
@@ -981,10 +999,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       tc::fence_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
-      const int first_last = sp.len - sp.n + row0 / grp;   // the CTA's first row's last key
+      const int first_last = TREE ? sp.len - sp.n - 1 : sp.len - sp.n + row0 / grp;   // the CTA's first row's last key
       bool ok = true;   // of this lane: one that gave up waits no more, but stays with its warp's collective instructions
       for (int j = 0; j < nt; ++j) {
         const uint32_t at = B == 2 ? t : job < B ? job : job - B, ts = lane_base + 128 * at;
+        const int k0 = (j0 + j) * kTileKeys;
+        const bool masked = k0 + kTileKeys - 1 > first_last;
+        uint32_t sees[4];   // TREE: a bit for each of the row's keys
+        if (TREE && masked) {
+          const int rel = k0 - (sp.len - sp.n), w0 = rel >> 5;   // the first key's place among the new tokens
+          uint32_t word[5];
+#pragma unroll
+          for (int i = 0; i < 5; ++i) {
+            word[i] = on ? tree_word(p, token * p.mask_words, w0 + i) : 0u;
+            const int left = sp.n - 32 * (w0 + i);   // (bits past the new tokens stand for none)
+            if (left < 32) word[i] &= left > 0 ? (1u << left) - 1u : 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sees[i] = __funnelshift_r(word[i], word[i + 1], rel & 31);
+        }
         if (ok) ok = wait_bounded(&s_full[B == 2 ? t : job], B == 2 ? j & 1 : job_parity, &g_paged_status);
         __syncwarp();
         tc::fence_after();
@@ -992,13 +1025,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tc::ld32(ts + 32 * c, v[c]);
         tc::wait_ld();
-        const int k0 = (j0 + j) * kTileKeys;
-        if (k0 + kTileKeys - 1 > first_last) {
+        if (masked) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (k0 + 32 * c + i > last) v[c][i] = 0xFF800000u;   // -inf
+              if (TREE ? !(sees[c] >> i & 1u) : k0 + 32 * c + i > last) v[c][i] = 0xFF800000u;   // -inf
         }
         float mx[4];
 #pragma unroll
@@ -1227,7 +1259,7 @@ int few_resident(int C) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, attention_few_kernel<__half, HD, NT>, &cfg) != cudaSuccess || n < 1) {
+    if (cudaOccupancyMaxActiveClusters(&n, attention_few_kernel<__half, HD, NT, false>, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = 2 * sm_count() / C;
     }
@@ -1275,7 +1307,7 @@ FewPlan few_plan(int64_t rows, int64_t seqs, int nkv, int hd, int64_t max_len) {
   return f;
 }
 
-template <typename T, int HD, int NT>
+template <typename T, int HD, int NT, bool TREE>
 cudaError_t few_t(PagedAttnParams p, const FewPlan& f, bool pdl, cudaStream_t st) {
   const int64_t rows = f.items * 8 * NT;
   p.work_ml = static_cast<float*>(p.workspace);
@@ -1297,7 +1329,7 @@ cudaError_t few_t(PagedAttnParams p, const FewPlan& f, bool pdl, cudaStream_t st
     ++cfg.numAttrs;
   }
   cfg.attrs = attr;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, attention_few_kernel<T, HD, NT>, (const PagedAttnParams)p, f.row_tiles, f.C, f.Z);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attention_few_kernel<T, HD, NT, TREE>, (const PagedAttnParams)p, f.row_tiles, f.C, f.Z);
   if (e != cudaSuccess || f.Z == 1) return e;
   cfg.gridDim = dim3((unsigned)rows);
   cfg.blockDim = dim3(128);
@@ -1326,7 +1358,7 @@ int chunk_resident(int C) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, attention_chunk_kernel<__half, HD>, &cfg) != cudaSuccess || n < 1) {
+    if (cudaOccupancyMaxActiveClusters(&n, attention_chunk_kernel<__half, HD, false>, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = max(1, (sm_count() - 16) / C);
     }
@@ -1336,17 +1368,17 @@ int chunk_resident(int C) {
   return v;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool TREE>
 cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   using L = ChunkSmem<HD>;
-  auto kern = attention_chunk_kernel<T, HD>;
+  auto kern = attention_chunk_kernel<T, HD, TREE>;
   static std::atomic<uint64_t> done{0};
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
   if (!(done.load(std::memory_order_relaxed) & bit)) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_chunk_kernel<__half, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_chunk_kernel<__half, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
     if (e != cudaSuccess) return e;
     done.fetch_or(bit, std::memory_order_relaxed);
   }
@@ -1395,15 +1427,15 @@ cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, kern, kmap, vmap, cp);
 }
 
-template <typename T>
+template <typename T, bool TREE>
 cudaError_t attention_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   const int64_t most_rows = (int64_t)p.max_new * (p.nh / p.nkv);
   if (most_rows <= kFewRows) {
     const FewPlan f = few_plan(most_rows, p.seqs, p.nkv, p.hd, p.max_len);
-    return p.hd == 128 ? (f.nt == 1 ? few_t<T, 128, 1>(p, f, pdl, st) : few_t<T, 128, 2>(p, f, pdl, st))
-                       : (f.nt == 1 ? few_t<T, 64, 1>(p, f, pdl, st) : few_t<T, 64, 2>(p, f, pdl, st));
+    return p.hd == 128 ? (f.nt == 1 ? few_t<T, 128, 1, TREE>(p, f, pdl, st) : few_t<T, 128, 2, TREE>(p, f, pdl, st))
+                       : (f.nt == 1 ? few_t<T, 64, 1, TREE>(p, f, pdl, st) : few_t<T, 64, 2, TREE>(p, f, pdl, st));
   }
-  return p.hd == 128 ? chunk_t<T, 128>(p, pdl, st) : chunk_t<T, 64>(p, pdl, st);
+  return p.hd == 128 ? chunk_t<T, 128, TREE>(p, pdl, st) : chunk_t<T, 64, TREE>(p, pdl, st);
 }
 
 }  // namespace
@@ -1426,7 +1458,8 @@ size_t paged_attention_workspace(int64_t seqs, int nh, int nkv, int hd, int64_t 
 }
 
 cudaError_t launch_paged_attention(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
-  return p.dtype == 0 ? attention_t<__half>(p, pdl, st) : attention_t<__nv_bfloat16>(p, pdl, st);
+  if (p.mask) return p.dtype == 0 ? attention_t<__half, true>(p, pdl, st) : attention_t<__nv_bfloat16, true>(p, pdl, st);
+  return p.dtype == 0 ? attention_t<__half, false>(p, pdl, st) : attention_t<__nv_bfloat16, false>(p, pdl, st);
 }
 
 int paged_device_error() {

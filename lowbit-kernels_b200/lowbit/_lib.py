@@ -56,6 +56,15 @@ SIGNATURES = {
     "lb_paged_attention_workspace": ([_I64, _I, _P, _I64, _I, _I64, _I64], _I64),
     "lb_paged_attention": ([_P, _I64, _I64, _I64, _I, _P, _P, _I64, _I64, _P, _P, _I, _I64, _I64, ctypes.c_float, _P,
                             _I64, _P, _I64, _P], _I),
+    "lb_f8_quantize_weight": ([_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P], _I),
+    "lb_f8_workspace": ([_I64, _I64, _I64], _I64),
+    "lb_f8_linear": ([_P, _I, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P], _I),
+    "lb_paged_tree_attention": ([_P, _I64, _I64, _I64, _I, _P, _P, _I64, _I64, _P, _P, _I, _P, _I64, _I64, _I64,
+                                 ctypes.c_float, _P, _I64, _P, _I64, _P], _I),
+    "lb_paged_plan": ([_P, _P, _I, _P, _I64, _I64, _I, _I64, _P, _P, _I64, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P], _I),
+    "lb_draft_verify_workspace": ([_I64, _I64], _I64),
+    "lb_draft_verify": ([_P, _I, _I64, _I64, _I64, _P, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P], _I),
+    "lb_paged_compact": ([_P, _I, _P, _I64, _I64, _P, _P, _P, _P, _I, _I64, _P, _I, _P], _I),
 }
 
 

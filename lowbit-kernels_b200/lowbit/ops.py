@@ -462,3 +462,114 @@ def linear_w8(x, w8, bias=None, out=None):
     if rc:
         e._raise(rc)
     return out
+
+
+# ------------------------------------------------------------------------------------------ 8-bit floating point
+#
+# Weights in e4m3 with one fp32 scale per 128 x 128 block, activations quantized per token and 128 values on the way into
+# the product (lb_f8_linear): the format of block-scaled 8-bit checkpoints. No counterpart in the reference.
+
+F8_BLOCK = 128
+
+
+def _f8_blocks(n):
+    return -(-n // F8_BLOCK)
+
+
+def quantize_f8_gpu(w):
+    """(float8_e4m3fn [N, K], scales fp32 [ceil(N / 128), ceil(K / 128)]) of a float weight [N, K] (fp16, bf16 or fp32, on the
+    GPU): per 128 x 128 block a = max(max|w|, 2^-100), scale = a / 448 and q = w * (448 / a) rounded to nearest even. The
+    same rule per token and 128 values is what linear_f8 applies to its activations."""
+    if not (isinstance(w, torch.Tensor) and w.is_cuda):
+        raise RuntimeError("quantize_f8_gpu takes GPU tensors")
+    if w.dim() != 2 or w.dtype not in DTYPE_IDS:
+        raise RuntimeError("w must be a float16, bfloat16 or float32 [N, K] tensor")
+    n, k = w.shape
+    if w.stride(1) != 1 or w.stride(0) < k:
+        w = w.contiguous()
+    q = torch.empty(n, -(-k // 16) * 16, dtype=torch.float8_e4m3fn, device=w.device)
+    scales = torch.empty(_f8_blocks(n), _f8_blocks(k), dtype=torch.float32, device=w.device)
+    e = ext()
+    if n and k:
+        with _Device(w.device):
+            rc = e.lib.lb_f8_quantize_weight(w.data_ptr(), DTYPE_IDS[w.dtype], n, k, w.stride(0) if n > 1 else k, q.data_ptr(),
+                                             q.shape[1], scales.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        if rc:
+            e._raise(rc)
+    return q[:, :k], scales
+
+
+class F8Weight:
+    """One linear layer's weight in 8-bit floating point on the GPU: q float8_e4m3fn [N, K], scales fp32 [ceil(N / 128),
+    ceil(K / 128)] (W = q * its block's scale). A q whose K and row stride are multiples of 16 is kept without a copy, any other
+    is laid out once with zeros behind K."""
+
+    def __init__(self, q, scales):
+        if not (isinstance(q, torch.Tensor) and isinstance(scales, torch.Tensor) and q.is_cuda):
+            raise RuntimeError("F8Weight takes GPU tensors")
+        if q.dtype != torch.float8_e4m3fn or q.dim() != 2 or not q.numel():
+            raise RuntimeError("q must be a float8_e4m3fn [N, K] tensor")
+        self.n, self.k = q.shape   # no device pointer is kept: a copy or an unpickled weight has its own memory
+        blocks = (_f8_blocks(self.n), _f8_blocks(self.k))
+        if scales.dtype != torch.float32 or scales.shape != blocks or scales.device != q.device:
+            raise RuntimeError(f"scales must be a float32 {list(blocks)} tensor on {q.device}")
+        if self.k > 131072:
+            raise ValueError(f"K={self.k}: at most 131072")
+        if (self.k % 16 == 0 and q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.stride(0) >= self.k
+                and q.data_ptr() % 16 == 0):
+            self._q = q.view(torch.uint8)   # as bytes: torch does not pickle tensors of this type
+        else:
+            pad = torch.zeros(self.n, -(-self.k // 16) * 16, dtype=torch.uint8, device=q.device)
+            pad[:, :self.k] = q.view(torch.uint8)
+            self._q = pad[:, :self.k]
+        self._scales = scales.contiguous()
+
+    @property
+    def q(self):
+        return self._q.view(torch.float8_e4m3fn)
+
+    @property
+    def scales(self):
+        return self._scales
+
+    @classmethod
+    def from_float(cls, w):
+        return cls(*quantize_f8_gpu(w))
+
+    def nbytes(self):
+        return self.n * self.k + 4 * self._scales.numel()
+
+
+def linear_f8(x, f8, bias=None, out=None):
+    """x [M, K] fp16 or bf16 (rows any stride apart) -> [M, N] of the same type: each row quantized to e4m3 with a scale per 128
+    values, the product with f8 (F8Weight) summed in fp32, each block times its two scales, `bias` ([N], x's type) added and
+    rounded once. `out`: an optional contiguous [M, N] tensor that receives the result. A serving operator: the result
+    carries no autograd graph."""
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.device == f8._q.device):
+        raise RuntimeError(f"x must be on the weight's GPU, {f8._q.device}")
+    if x.dtype not in (torch.float16, torch.bfloat16) or x.dim() != 2 or x.shape[1] != f8.k:
+        raise RuntimeError(f"x must be a float16 or bfloat16 [M, {f8.k}] tensor")
+    m = x.shape[0]
+    if bias is not None and (not bias.is_cuda or bias.device != x.device or bias.dtype != x.dtype
+                             or bias.shape != (f8.n,) or not bias.is_contiguous()):
+        raise RuntimeError(f"bias must be a contiguous {x.dtype} [{f8.n}] tensor on {x.device}")
+    if out is None:
+        out = torch.empty(m, f8.n, dtype=x.dtype, device=x.device)
+    elif out.shape != (m, f8.n) or out.dtype != x.dtype or out.device != x.device or not out.is_contiguous():
+        raise RuntimeError(f"out must be a contiguous {x.dtype} [{m}, {f8.n}] tensor on {x.device}")
+    if m == 0:
+        return out
+    if x.stride(1) != 1 or (m > 1 and x.stride(0) < f8.k):
+        x = x.contiguous()
+    e = ext()
+    n, k, ldw = f8.n, f8.k, f8._q.stride(0) if f8.n > 1 else -(-f8.k // 16) * 16
+    with _Device(x.device):
+        need = e.lib.lb_f8_workspace(m, n, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+        rc = e.lib.lb_f8_linear(x.data_ptr(), DTYPE_IDS[x.dtype], x.stride(0) if m > 1 else k, f8._q.data_ptr(), ldw,
+                                f8._scales.data_ptr(),
+                                None if bias is None else bias.data_ptr(), out.data_ptr(), m, n, k,
+                                ws.data_ptr() if need else None, need, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        e._raise(rc)
+    return out

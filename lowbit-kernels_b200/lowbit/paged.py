@@ -7,6 +7,7 @@ Every call launches on the current torch stream of the tensors' device and never
 outputs carry no autograd graph, whatever their inputs require. There is no fallback: without the library or a CUDA device
 the first call raises.
 """
+import collections
 import ctypes
 import math
 
@@ -141,6 +142,21 @@ def attention(q, cache, page_table, seq_lens, cu_new, max_new=None, max_len=None
         y = tc.paged_attention(q, cache._ptr, cache._device, page_table, seq_lens, cu_new, max_new, max_len, scale, out)
         if y is not None:
             return y
+    return _attend(q, cache, page_table, seq_lens, cu_new, None, max_new, max_len, scale, out)
+
+
+def tree_attention(q, cache, page_table, seq_lens, cu_new, mask, max_new=None, max_len=None, scale=None, out=None):
+    """`attention` for drafted tokens that form trees. mask int32 [T, words]: bit j % 32 of word j / 32 of a token's row says
+    whether it sees its sequence's new token j (`plan` makes it from the tokens' parents; any pattern will do, a row of zeros
+    too). Every new token sees the whole cached context, the keys before the sequence's new ones, which lie in the cache in the
+    order of the call; new tokens past 32 * words are seen by none. The rest is as in `attention`."""
+    if mask is None:
+        raise RuntimeError("mask must be an int32 [T, words] tensor on the cache's GPU")
+    return _attend(q, cache, page_table, seq_lens, cu_new, mask, max_new, max_len, scale, out)
+
+
+def _attend(q, cache, page_table, seq_lens, cu_new, mask, max_new, max_len, scale, out):
+    """The checked path of both attentions; mask: a tree's, or None."""
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() == cache._device):
         raise RuntimeError(f"q must be on the cache's GPU, {cache.k.device}")
     if q.dtype != cache.dtype or q.dim() != 3 or q.shape[2] != cache.hd:
@@ -162,6 +178,10 @@ def attention(q, cache, page_table, seq_lens, cu_new, max_new=None, max_len=None
     if out is None:
         out = torch.empty(t, nh, hd, dtype=q.dtype, device=q.device)
     _on(cache, "out", out, cache.dtype, t, nh, hd)
+    if mask is not None:
+        bits = _on(cache, "mask", mask, torch.int32, t, None)
+        if mask.shape[1] < 1:
+            raise RuntimeError("mask must have a word a row at least")
     max_new = t if max_new is None else int(max_new)
     max_len = width * cache.page_size if max_len is None else int(max_len)
     if t == 0 or s == 0:
@@ -170,11 +190,180 @@ def attention(q, cache, page_table, seq_lens, cu_new, max_new=None, max_len=None
     with _Device(q.device):
         need = e.lib.lb_paged_attention_workspace(t, nh, cache._ptr, width, s, max_new, max_len)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        rc = e.lib.lb_paged_attention(q.data_ptr(), t_stride, h_stride, t, nh, cache._ptr, page_table.data_ptr(),
-                                      page_table.stride(0) if s > 1 else width, width, lens, cu, s, max_new, max_len,
-                                      1 / math.sqrt(hd) if scale is None else scale, out.data_ptr(), nh * hd,
-                                      ws.data_ptr() if need else None, need,
-                                      torch.cuda.current_stream().cuda_stream)
+        head = (q.data_ptr(), t_stride, h_stride, t, nh, cache._ptr, page_table.data_ptr(),
+                page_table.stride(0) if s > 1 else width, width, lens, cu, s)
+        tail = (max_new, max_len, 1 / math.sqrt(hd) if scale is None else scale, out.data_ptr(), nh * hd,
+                ws.data_ptr() if need else None, need, torch.cuda.current_stream().cuda_stream)
+        if mask is None:
+            rc = e.lib.lb_paged_attention(*head, *tail)
+        else:
+            rc = e.lib.lb_paged_tree_attention(*head, bits, mask.shape[1], *tail)
+    if rc:
+        e._raise(rc)
+    return out
+
+
+Plan = collections.namedtuple("Plan", "cu_new seq_lens positions slots held free_count mask")
+Plan.__doc__ = """What `plan` gives: cu_new int32 [S + 1], seq_lens int32 [S] (the tokens with the new ones; 0: refused), positions and
+slots int64 [tokens], held int32 [S] and free_count int32 [1] (None without pages to give out), mask int32 [tokens, words] (None
+without parents)."""
+Verified = collections.namedtuple("Verified", "accepted path next targets")
+Verified.__doc__ = """What `verify` gives: accepted int32 [S], path int32 [S, max_path], next int64 [S], targets int64 [T]."""
+
+
+def _vector(name, t, dtype, device, *shape):
+    """Raise unless t is a contiguous tensor of that type and shape (None: any) on that GPU; its address."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.device == device):
+        raise RuntimeError(f"{name} must be on {device}")
+    if t.dtype != dtype or t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise RuntimeError(f"{name} must be a {dtype} {list(shape)} tensor, got {t.dtype} {list(t.shape)}")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _page_table(t):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] > 0
+            and t.shape[1] > 0 and t.stride(1) == 1):
+        raise RuntimeError("page_table must be an int32 [S, W] tensor on the GPU, its rows contiguous")
+    s, width = t.shape
+    if s > 1 and t.stride(0) < width:
+        raise RuntimeError("page_table's rows overlap")
+    return s, width, t.stride(0) if s > 1 else width
+
+
+def plan(page_table, seq_lens, new_lens, page_size, tokens, held=None, free_pages=None, free_count=None, parents=None,
+         max_new=None, out=None):
+    """What a call on new tokens needs, built on the GPU: sequence s has seq_lens[s] tokens in the cache and gets new_lens[s]
+    more (int32 [S] each, S up to 8192). Returns a `Plan` whose rows are the sequences' new tokens one after another, `tokens`
+    of them (a host integer, at least their sum); rows past the last sequence get position 0 and slot -1, so that
+    `norm_rope_append` stores nothing for them and `attention` leaves them out.
+
+    held int32 [S], free_pages int32 [P] and free_count int32 [1], all or none, let it give out pages: row s of page_table int32
+    [S, W] holds held[s] pages, and what the new tokens need beyond them is taken from the first free_count[0] entries of free_pages,
+    the last first, by the sequences in their order, and written into page_table behind them; the plan's held and free_count say
+    what there is then. Without them page_table is complete as it is. A sequence is refused where `tokens`, W or the free pages do not suffice
+    (from the first that lacks pages on, all that need some): its seq_lens is 0, so that attention gives it zeros, its
+    slots are -1, and it takes no pages.
+
+    parents int32 [tokens]: the new tokens of a sequence form a tree, parents[t] being the place among them of the token's
+    parent, an earlier one; anything else makes it a root. Positions are then seq_lens + depth, and the plan's mask is what
+    `tree_attention` takes, its rows ceil(max_new / 32) words (max_new bounds the new tokens of any sequence, 1024 at most; by default
+    tokens). out: a Plan whose tensors receive the result (fixed addresses for a captured step); its held, free_count
+    and seq_lens may be the ones passed in."""
+    s, width, stride = _page_table(page_table)
+    dev = page_table.device
+    lens, new = _vector("seq_lens", seq_lens, torch.int32, dev, s), _vector("new_lens", new_lens, torch.int32, dev, s)
+    paging = held is not None
+    if paging != (free_pages is not None) or paging != (free_count is not None):
+        raise RuntimeError("held, free_pages and free_count go together")
+    tokens = int(tokens)
+    words = 0
+    if parents is not None:
+        max_new = tokens if max_new is None else int(max_new)
+        words = -(-max(1, max_new) // 32)
+        if words > 32:
+            raise ValueError(f"max_new={max_new}: trees hold up to 1024 tokens")
+    if out is None:
+        def make(dtype, *shape):
+            return torch.empty(shape, dtype=dtype, device=dev)
+        out = Plan(make(torch.int32, s + 1), make(torch.int32, s), make(torch.int64, tokens), make(torch.int64, tokens),
+                   make(torch.int32, s) if paging else None, make(torch.int32, 1) if paging else None,
+                   make(torch.int32, tokens, words) if words else None)
+    cu, after = _vector("out.cu_new", out.cu_new, torch.int32, dev, s + 1), _vector("out.seq_lens", out.seq_lens, torch.int32, dev, s)
+    pos, slots = (_vector(f"out.{n}", t, torch.int64, dev, tokens) for n, t in (("positions", out.positions), ("slots", out.slots)))
+    pages = [None, None, 0, None, None, None]
+    if paging:
+        pages = [_vector("held", held, torch.int32, dev, s), _vector("free_pages", free_pages, torch.int32, dev, None), free_pages.numel(),
+                 _vector("free_count", free_count, torch.int32, dev, 1), _vector("out.held", out.held, torch.int32, dev, s),
+                 _vector("out.free_count", out.free_count, torch.int32, dev, 1)]
+    tree = bits = None
+    if words:
+        tree = _vector("parents", parents, torch.int32, dev, tokens)
+        bits = _vector("out.mask", out.mask, torch.int32, dev, tokens, words)
+        if not tokens:   # (an empty tensor has no address)
+            tree = bits = None
+    e = ops.ext()
+    with _Device(dev):
+        rc = e.lib.lb_paged_plan(lens, new, s, page_table.data_ptr(), stride, width, int(page_size), tokens, pages[0], pages[1] or (lens if paging else None),
+                                 pages[2], pages[3], tree, words if tree else 0, cu, after, pages[4], pages[5], pos, slots, bits,
+                                 torch.cuda.current_stream().cuda_stream)
+    if rc:
+        e._raise(rc)
+    return out
+
+
+def verify(logits, tokens, parents, cu_new, max_new=None, max_path=None):
+    """Greedy acceptance of drafted trees. logits [T, vocab] (fp16, bf16 or fp32, rows any stride apart) follow the new tokens
+    `tokens` int64 [T] of the sequences cu_new int32 [S + 1], whose parents int32 [T] are as in `plan`. Returns a `Verified`: targets,
+    the index of each row's first largest value (a NaN counts as larger than all); and for each sequence the path that starts at its first new token, the
+    last certain one, and goes on to the first later token that is a child of the one at hand and equals its target: how many tokens it has
+    (accepted), their places among the new ones (path, -1 behind them) and the target after the last (next). A sequence
+    without new tokens gets 0 and -1. max_new bounds the new tokens of any sequence (1024 at most; by default T),
+    max_path the path (by default max_new). Rows past cu_new[S] are not looked at, their targets left unwritten."""
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dim() == 2 and logits.dtype in DTYPE_IDS):
+        raise RuntimeError("logits must be a float16, bfloat16 or float32 [T, vocab] tensor on the GPU")
+    t, vocab = logits.shape
+    if not vocab:
+        raise RuntimeError("the vocabulary is empty")
+    if logits.stride(1) != 1 and vocab > 1 or t > 1 and logits.stride(0) < vocab:
+        logits = logits.contiguous()
+    dev = logits.device
+    drafted, tree = _vector("tokens", tokens, torch.int64, dev, t), _vector("parents", parents, torch.int32, dev, t)
+    cu = _vector("cu_new", cu_new, torch.int32, dev, None)
+    s = cu_new.numel() - 1
+    if s < 1:
+        raise RuntimeError("cu_new must hold a sequence at least")
+    max_new = t if max_new is None else int(max_new)
+    max_path = max_new if max_path is None else int(max_path)
+    if t and not 1 <= max_new <= 1024:
+        raise ValueError(f"max_new={max_new}: trees hold 1 to 1024 tokens")
+    if t and not 1 <= max_path <= 1024:
+        raise ValueError(f"max_path={max_path}: 1 to 1024")
+    if t == 0:
+        return Verified(torch.zeros(s, dtype=torch.int32, device=dev), torch.full((s, max(1, max_path)), -1, dtype=torch.int32, device=dev),
+                        torch.full((s,), -1, dtype=torch.int64, device=dev), torch.empty(0, dtype=torch.int64, device=dev))
+    got = Verified(torch.empty(s, dtype=torch.int32, device=dev), torch.empty(s, max_path, dtype=torch.int32, device=dev),
+                   torch.empty(s, dtype=torch.int64, device=dev), torch.empty(t, dtype=torch.int64, device=dev))
+    e = ops.ext()
+    with _Device(dev):
+        need = e.lib.lb_draft_verify_workspace(t, vocab)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = e.lib.lb_draft_verify(logits.data_ptr(), DTYPE_IDS[logits.dtype], logits.stride(0) if t > 1 else vocab, t, vocab, drafted,
+                                   tree, cu, s, max_new, max_path, got.accepted.data_ptr(), got.path.data_ptr(), got.next.data_ptr(),
+                                   got.targets.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        e._raise(rc)
+    return got
+
+
+def compact(caches, page_table, seq_lens, cu_new, path, accepted, out=None):
+    """Moves the accepted tokens' K and V rows to where a sequence without the other drafts has them, in all of `caches` (a list of
+    up to 128 PagedCache of one layout, a layer each): with n new tokens of sequence s and seq_lens[s] tokens, them included, row
+    seq_lens[s] - n + path[s, d] goes to seq_lens[s] - n + d for d < accepted[s] (path int32 [S, D] and accepted int32 [S] as `verify`
+    gives them: a path rises). Returns seq_lens[s] - n + accepted[s], int32 [S] (`out`, when given: not seq_lens itself). For a
+    sequence that `plan` refused this is 0, or what `out` held, and nothing moves: with the lengths before the plan as `out`
+    it keeps its context. A path's entry outside the new tokens, below its own place, or on a page outside the cache is left
+    out, and the device status becomes 3, as in `attention`."""
+    caches = list(caches)
+    if not caches or not all(isinstance(c, PagedCache) for c in caches):
+        raise RuntimeError("caches must be a list of PagedCache")
+    cache = caches[0]
+    if any(c._device != cache._device for c in caches):
+        raise RuntimeError("the caches must be on one GPU")
+    s, width, stride = _page_table(page_table)
+    if page_table.get_device() != cache._device:
+        raise RuntimeError(f"page_table must be on the cache's GPU, {cache.k.device}")
+    lens, cu = _on(cache, "seq_lens", seq_lens, torch.int32, s), _on(cache, "cu_new", cu_new, torch.int32, s + 1)
+    at, count = _on(cache, "path", path, torch.int32, s, None), _on(cache, "accepted", accepted, torch.int32, s)
+    keep = out is not None
+    if not keep:
+        out = torch.empty(s, dtype=torch.int32, device=page_table.device)
+    dst = _on(cache, "out", out, torch.int32, s)
+    e = ops.ext()
+    with _Device(page_table.device):
+        rc = e.lib.lb_paged_compact((ctypes.c_void_p * len(caches))(*[c._ptr for c in caches]), len(caches), page_table.data_ptr(), stride,
+                                    width, lens, cu, at, count, s, path.shape[1], dst, keep, torch.cuda.current_stream().cuda_stream)
     if rc:
         e._raise(rc)
     return out
