@@ -22,6 +22,11 @@ constexpr int kBlock = 128;               // values of a scale
 constexpr float kMost = 448.f;            // largest e4m3 value
 constexpr float kLeast = 0x1p-100f;       // blocks whose maximum is below count as if it were this
 
+__device__ __forceinline__ float lds_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 // two fp32 values in one 64-bit register pair
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;
@@ -173,14 +178,13 @@ __global__ void __launch_bounds__(256)
   if (threadIdx.x == 0) t[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = sc.s;
 }
 
-// ------------------------------------------------------------------------------------------------------- the product
+// ------------------------------------------------------------------------------------------------------- the product, few tokens
 // tcgen05.mma kind::f8f6f4 with the channels as the A side (128 a CTA, which is a row of the weights' blocks) and a tile of
 // bn tokens as the N side. A stage of the ring is 128 bytes of K, so one block of the scales: each stage's four MMAs start a
 // new accumulator, and 16 epilogue warps add it, times s t, to the sums that they hold in registers (a lane a channel, a
 // column a token) while the next stages' MMAs run into the other accumulators. The scale of a column is the same for all
 // lanes: each warp puts its columns' s t into shared memory, from where four come in one broadcast load; two columns take
 // one fp32-pair multiply-add.
-// PAIR: two CTAs work on one tile of 256 channels (cta_group::2): each loads its 128 channels and half of the tokens.
 // CTAs are persistent over tiles, tokens innermost. Few tiles and long K: a cluster of S single CTAs splits K, each parks
 // its fp32 partial tile in its idle ring, and all sum their share of the outputs through distributed shared memory in rank order.
 constexpr int kChunk = 128;               // bytes of K per stage
@@ -239,26 +243,22 @@ __device__ __forceinline__ void sum_partials(uint32_t red, const T* bias, T* y, 
   }
 }
 
-template <typename T, bool PAIR, int NB>   // NB: 16-column blocks of a tile a warp holds, bn <= 64 NB
+template <typename T, int NB>   // NB: 16-column blocks of a tile a warp holds, bn <= 64 NB
 __global__ void __launch_bounds__(kMmaThreads, 1)
-    f8_gemm_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap, const F8Gemm p) {
+    f8_cols_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap qmap, const F8Gemm p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + p.park);   // PAIR: the leader's, for both CTAs' copies
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + p.park);
   uint64_t* empty = full + kMaxStages;
   uint64_t* acc_full = empty + kMaxStages;
-  uint64_t* acc_empty = acc_full + kMaxAcc;                      // PAIR: the leader's
+  uint64_t* acc_empty = acc_full + kMaxAcc;
   uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + kMaxAcc);
   float* scales = reinterpret_cast<float*>(slot + 4);            // [epilogue warps][2][64]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int own_bn = PAIR ? p.bn / 2 : p.bn;                     // tokens this CTA loads
-  const int stage_bytes = kWBytes + own_bn * kChunk, S = PAIR ? 1 : p.splits, St = p.stages, A = p.acc;
-  const int rank = PAIR || S > 1 ? (int)cluster_rank() : 0;
-  const int group = PAIR ? 2 : S;
-  const int first = blockIdx.x / group, step = gridDim.x / group;
-  const int c0 = PAIR ? 0 : p.chunks * rank / S, nc = PAIR ? p.chunks : p.chunks * (rank + 1) / S - c0;
-  constexpr int kTileN = PAIR ? 256 : 128;
-  const int n_off = PAIR ? 128 * rank : 0;
+  const int stage_bytes = kWBytes + p.bn * kChunk, S = p.splits, St = p.stages, A = p.acc;
+  const int rank = S > 1 ? (int)cluster_rank() : 0;
+  const int first = blockIdx.x / S, step = gridDim.x / S;
+  const int c0 = p.chunks * rank / S, nc = p.chunks * (rank + 1) / S - c0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < St; ++i) {
@@ -267,22 +267,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
     for (int i = 0; i < A; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], PAIR ? 2 * kEpiWarps : kEpiWarps);
+      mbar_init(&acc_empty[i], kEpiWarps);
     }
     mbar_fence_init();
   }
   const uint32_t columns = (uint32_t)(A * p.acc_stride);
-  if (warp == 1) {
-    if (PAIR)
-      tc::alloc_pair(slot, columns);
-    else
-      tc::alloc(slot, columns);
-  }
+  if (warp == 1) tc::alloc(slot, columns);
   tc::fence_before();
-  if (PAIR)
-    cluster_sync_all();   // the peer's barriers exist before a copy or a commit reaches them
-  else
-    __syncthreads();
+  __syncthreads();
   tc::fence_after();
   const uint32_t tmem = *slot;
   pdl_launch_dependents();
@@ -296,27 +288,17 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       };
       auto at = [&](int tile) {
         const int n = tile / p.tiles_m, m = tile - n * p.tiles_m;
-        return Place{tile, 0, m * p.bn + (PAIR ? rank * own_bn : 0), n * kTileN + n_off};
+        return Place{tile, 0, m * p.bn, n * 128};
       };
       auto next = [&](Place& q) {
         if (++q.c == nc) q = at(q.tile + step);
       };
       auto weights = [&](const Place& q, int s) {
-        uint8_t* dst = ring + s * stage_bytes;
-        if (PAIR) {
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * stage_bytes);
-          tc::tma_load_2d_pair(dst, &wmap, q.c * kChunk, q.n0, mapa_shared(smem_addr(&full[s]), 0));
-        } else {
-          mbar_arrive_expect_tx(&full[s], stage_bytes);
-          tma_load_2d(dst, &wmap, (c0 + q.c) * kChunk, q.n0, &full[s]);
-        }
+        mbar_arrive_expect_tx(&full[s], stage_bytes);
+        tma_load_2d(ring + s * stage_bytes, &wmap, (c0 + q.c) * kChunk, q.n0, &full[s]);
       };
       auto tokens = [&](const Place& q, int s) {
-        uint8_t* dst = ring + s * stage_bytes + kWBytes;
-        if (PAIR)
-          tc::tma_load_2d_pair(dst, &qmap, q.c * kChunk, q.m0, mapa_shared(smem_addr(&full[s]), 0));
-        else
-          tma_load_2d(dst, &qmap, (c0 + q.c) * kChunk, q.m0, &full[s]);
+        tma_load_2d(ring + s * stage_bytes + kWBytes, &qmap, (c0 + q.c) * kChunk, q.m0, &full[s]);
       };
       Place w = at(first), q = w;
       int head = 0;
@@ -332,19 +314,18 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         tokens(q, s);
         if (++s == St) s = 0, phase ^= 1;
       }
-      // no copy in flight past this point (a pair's leader's barriers count its peer's copies too): stage s holds the
-      // oldest of the last `head` copies, its parity is that of the release before it
-      if (rank == 0 || !PAIR)
-        for (int i = 0; i < head; ++i) {
-          wait_bounded(&full[s], phase, &g_f8_status);
-          if (++s == head) s = 0, phase ^= 1;
-        }
+      // no copy in flight past this point: stage s holds the oldest of the last `head` copies, its parity is that of the
+      // release before it
+      for (int i = 0; i < head; ++i) {
+        wait_bounded(&full[s], phase, &g_f8_status);
+        if (++s == head) s = 0, phase ^= 1;
+      }
     }
     __syncwarp();
   } else if (warp == 1) {
-    if ((!PAIR || rank == 0) && tc::elect_one()) {
+    if (tc::elect_one()) {
       // fp32 accumulator, e4m3 A and B, both K-major
-      const uint32_t idesc = (1u << 4) | ((uint32_t)(p.bn >> 3) << 17) | ((uint32_t)(kTileN >> 4) << 24);
+      const uint32_t idesc = (1u << 4) | ((uint32_t)(p.bn >> 3) << 17) | ((128u >> 4) << 24);
       const uint64_t desc0 = tc::desc_sw128(smem_addr(ring), 16, 1024);   // the address field counts 16 bytes
       const uint32_t stage_step = (uint32_t)stage_bytes >> 4;
       int s = 0, phase = 0, a = 0, turn = 0;   // stage, its parity; accumulator, times round their ring
@@ -358,19 +339,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           const uint64_t ad = desc0 + s * stage_step, bd = ad + (kWBytes >> 4);
           const uint32_t d = tmem + a * p.acc_stride;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (PAIR)
-              tc::mma_f8_ss_pair(d, ad + 2 * k, bd + 2 * k, idesc, k > 0);
-            else
-              tc::mma_f8_ss(d, ad + 2 * k, bd + 2 * k, idesc, k > 0);
-          }
-          if (PAIR) {
-            tc::commit_pair(&empty[s]);
-            tc::commit_pair(&acc_full[a]);
-          } else {
-            tc::commit(&empty[s]);
-            tc::commit(&acc_full[a]);
-          }
+          for (int k = 0; k < 4; ++k) tc::mma_f8_ss(d, ad + 2 * k, bd + 2 * k, idesc, k > 0);
+          tc::commit(&empty[s]);
+          tc::commit(&acc_full[a]);
           if (++s == St) s = 0, phase ^= 1;
           if (++a == A) a = 0, ++turn;
         }
@@ -393,7 +364,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     int a = 0, phase = 0;
     const int blocks = (p.bn - 16 * part + 63) / 64;   // of this warp
     for (int tile = first; tile < p.tiles; tile += step) {
-      const int m0 = tile % p.tiles_m * p.bn, nt = tile / p.tiles_m, n = nt * kTileN + n_off + row;
+      const int m0 = tile % p.tiles_m * p.bn, nt = tile / p.tiles_m, n = nt * 128 + row;
       const bool on = n < p.N;
       // this lane's columns' scales and the tile's, one chunk ahead
       constexpr int kCols = NB > 2 ? 2 : 1;
@@ -405,7 +376,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         have[i] = at < 16 * NB && col < p.bn && m0 + col < p.M;
         sp[i] = p.s + (int64_t)c0 * p.lds + m0 + col;
       }
-      const float* tp = p.t + (int64_t)min((nt * kTileN + n_off) / kBlock, (p.N - 1) / kBlock) * p.chunks + c0;
+      const float* tp = p.t + (int64_t)nt * p.chunks + c0;
       float sv[kCols], tv;
       auto fetch = [&](int c) {
         tv = c < nc ? __ldcg(tp + c) : 0.f;
@@ -417,7 +388,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 #pragma unroll
       for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[i][j] = 0;
+        for (int j = 0; j < 16; ++j) sum[i][j] = 0;
       for (int c = 0; c < nc; ++c) {
         float* sc = scale + 64 * (c & 1);   // (a lane a chunk ahead writes the other half)
 #pragma unroll
@@ -446,12 +417,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           }
         tc::fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if (PAIR)
-            tc::arrive_cluster(mapa_shared(smem_addr(&acc_empty[a]), 0));
-          else
-            mbar_arrive(&acc_empty[a]);
-        }
+        if (lane == 0) mbar_arrive(&acc_empty[a]);
         if (++a == A) a = 0, phase ^= 1;
       }
       const float bn = on && bias && S == 1 ? Elem<T>::to_float(bias[n]) : 0.f;
@@ -501,22 +467,324 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     }
   }
   __syncwarp();
-  if (!PAIR && S > 1) {
+  if (S > 1) {
     const int n0 = first / p.tiles_m * 128, m0 = first % p.tiles_m * p.bn;
     sum_partials<T>(smem_addr(ring), static_cast<const T*>(p.bias), static_cast<T*>(p.y) + (int64_t)m0 * p.N, n0, p.N,
                     min(p.bn, p.M - m0), rank, S);
   }
   tc::fence_before();
-  if (PAIR || S > 1)
-    cluster_sync_all();   // no CTA leaves while its partner still reads, or signals, its shared memory
+  if (S > 1)
+    cluster_sync_all();   // no CTA leaves while another still reads its shared memory
   else
     __syncthreads();
   if (warp == 1) {
     tc::fence_after();
-    if (PAIR)
-      tc::dealloc_pair(tmem, columns);
-    else
-      tc::dealloc(tmem, columns);
+    tc::dealloc(tmem, columns);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------- the product, many tokens
+// The same with the tokens as the A side: a pair of CTAs (cta_group::2) works on 256 tokens, 128 a CTA, and a tile of bn
+// channels, half of them loaded by each. A lane now holds a token, so that its scale is one register: s t of a block
+// multiplies all columns, without the loads from shared memory that a scale a column takes. A stage's MMAs go into two
+// accumulators of about bn / 2 channels, each with its own four epilogue warps a CTA, and there are two of each in the ring: what
+// counts is how long an accumulator may take from its last MMA until it is free again, and in halves that is three half
+// stages' MMAs (810 clocks at bn = 256), in one piece it would be one stage's (540).
+constexpr int kRowsSmem = 2 * 1024;       // a warp's staging: 32 tokens x 32 channels
+constexpr int kRowsThreads = 12 * 32;      // two loaders and two MMA warps (a warpgroup), 8 epilogue warps
+constexpr int kRowsStages = 6;
+constexpr int kRowsBarriers = 256;          // bytes, with tensor memory's address; the scales behind them are tensor copies
+constexpr int kRowsBarrierBytes = kRowsBarriers + (kRowsStages + 2) * 512 + 8 * kRowsSmem;
+static_assert((2 * kRowsStages + 8) * 8 + 16 <= kRowsBarriers, "barriers");
+
+// the two accumulators' channels, multiples of 32 as a pair's MMA takes them
+__host__ __device__ constexpr int first_half(int bn) { return (bn + 63) / 64 * 32; }
+
+struct F8Rows {
+  const float* s;       // token scales [blocks][lds]
+  const float* t;       // weight scales [rows of blocks][blocks]
+  const void* bias;
+  void* y;
+  int M, N, chunks, lds;
+  int bn, tiles_m, tiles_n, tiles, stages;
+  int park;             // byte offset behind the ring: barriers, staging
+  bool vec;             // output rows take 16-byte stores
+};
+
+// The tile at a place of the order in which they are taken: n by n columns of tiles, so that what is worked on at one time is
+// about as many tokens as channels, and the fewest rows of both are read.
+constexpr int kTileColumns = 8;
+struct TilePlace {
+  int m, n;
+};
+__device__ __forceinline__ TilePlace tile_place(int tile, int tiles_m, int tiles_n) {
+  const int group = tile / (kTileColumns * tiles_m), rest = tile - group * kTileColumns * tiles_m;
+  const int wide = min(kTileColumns, tiles_n - group * kTileColumns), m = rest / wide;
+  return {m, group * kTileColumns + rest - m * wide};
+}
+
+struct F8Epilogue {
+  uint32_t acc_full, acc_empty, scales, tmem;   // shared-memory addresses, acc_empty the leader's
+  uint8_t* staging;
+  int rank, first, step, n_off, half;
+};
+
+// An epilogue warp's work on its B blocks of 16 channels and 32 tokens of every tile
+template <typename T, int B>
+__device__ __forceinline__ void rows_epilogue(const F8Rows& p, const F8Epilogue& w) {
+  const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, row = 32 * quarter + lane, rank = w.rank, h = w.half;
+  const uint32_t acc0 = w.tmem + ((uint32_t)(32 * quarter) << 16) + 128 * h;
+  const T* bias = static_cast<const T*>(p.bias);
+  T* y = static_cast<T*>(p.y);
+  uint8_t* stage = w.staging;
+  bool ok = true;   // of this lane: one that gave up waits no more, but stays with its warp's collective instructions
+  bool ready = false;   // the next accumulator, as asked under the work on this one
+  int slot = 0;         // of the scales' ring
+  uint32_t u = 0;
+  for (int tile = w.first; tile < p.tiles; tile += w.step) {
+    const TilePlace at = tile_place(tile, p.tiles_m, p.tiles_n);
+    const int m0 = at.m * 256 + 128 * rank, m = m0 + row, n0 = at.n * p.bn + w.n_off;
+    // up to 128 channels: the blocks from `turn` on belong to the next row of the weights' scales
+    const int nb = n0 / kBlock, most = (p.N - 1) / kBlock, turn = ((nb + 1) * kBlock - n0) / 16;
+    const float* t0 = p.t + (int64_t)min(nb, most) * p.chunks;
+    const float* t1 = p.t + (int64_t)min(nb + 1, most) * p.chunks;
+    // the weights' scales of 32 stages at a time, a lane a stage, loaded 32 stages before their use
+    float ta = 0.f, tb = 0.f, ta2 = 0.f, tb2 = 0.f;
+    auto fetch = [&](int c) {
+      if (c + lane < p.chunks) ta2 = __ldcg(t0 + c + lane), tb2 = __ldcg(t1 + c + lane);
+    };
+    fetch(0);
+    float sum[B][16];
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum[i][j] = 0.f;
+    for (int c = 0; c < p.chunks; ++c, ++u) {
+      if (c % 32 == 0) {
+        ta = ta2, tb = tb2;
+        fetch(c + 32);
+      }
+      float fa = __shfl_sync(0xffffffffu, ta, c & 31), fb = __shfl_sync(0xffffffffu, tb, c & 31);
+      const int a = 2 * (u & 1) + h;
+      if (ok && !ready) ok = wait_warp(w.acc_full + 8 * a, (u >> 1) & 1, &g_f8_status);
+      __syncwarp();
+      tc::fence_after();
+      const uint32_t acc = acc0 + 256 * (u & 1);
+      uint32_t v[16];
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        tc::ld16(acc + 16 * i, v);
+        if (i == 0) {
+          const float sv = lds_f32(w.scales + 512 * slot + 4 * row);   // there, since the MMAs have waited for it
+          ready = test_barrier(w.acc_full + 8 * (a ^ 2), (u + 1) >> 1 & 1);
+          fa *= sv, fb *= sv;
+        }
+        tc::wait_ld();
+        const float f = i < turn ? fa : fb;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          // two columns in one instruction, as one block of code: what the compiler is left to pair up it copies first
+          asm("{\n\t.reg .b64 a, b, c;\n\t"
+              "mov.b64 a, {%2, %3};\n\t"
+              "mov.b64 b, {%4, %4};\n\t"
+              "mov.b64 c, {%0, %1};\n\t"
+              "fma.rn.f32x2 c, a, b, c;\n\t"
+              "mov.b64 {%0, %1}, c;\n\t}"
+              : "+f"(sum[i][2 * j]), "+f"(sum[i][2 * j + 1])
+              : "r"(v[2 * j]), "r"(v[2 * j + 1]), "f"(f));
+      }
+      tc::fence_before();
+      __syncwarp();
+      tc::arrive_relaxed(w.acc_empty + 8 * a, lane == 0);
+      if (++slot == p.stages + 2) slot = 0;
+    }
+    // two blocks at a time through the warp's [32 tokens][32 channels], 16-byte pieces permuted by the row
+#pragma unroll
+    for (int i0 = 0; i0 < B; i0 += 2) {
+#pragma unroll
+        for (int i = i0; i < i0 + 2; ++i) {
+          const int n = n0 + 16 * i;
+          uint32_t o[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float2 v = make_float2(sum[i][2 * j], sum[i][2 * j + 1]);
+            if (bias) {
+              v.x += n + 2 * j < p.N ? Elem<T>::to_float(bias[n + 2 * j]) : 0.f;
+              v.y += n + 2 * j + 1 < p.N ? Elem<T>::to_float(bias[n + 2 * j + 1]) : 0.f;
+            }
+            o[j] = Elem<T>::pack(v.x, v.y);
+          }
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + (((2 * (i - i0) + q) ^ (lane >> 1 & 3)) << 4)) =
+                make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        }
+        __syncwarp();
+        const int n = n0 + 16 * i0;
+        if (p.vec) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int r = 8 * q + (lane >> 2), c = lane & 3, at = m0 + 32 * quarter + r;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 64 + ((c ^ (r >> 1 & 3)) << 4));
+            if (at < p.M && n + 8 * c < p.N) *reinterpret_cast<uint4*>(y + (int64_t)at * p.N + n + 8 * c) = v;
+          }
+        } else {
+          for (int r = 0; r < 32; ++r) {
+            const int at = m0 + 32 * quarter + r;
+            const uint16_t v = *reinterpret_cast<const uint16_t*>(stage + r * 64 + (((lane >> 3) ^ (r >> 1 & 3)) << 4) + 2 * (lane & 7));
+            if (at < p.M && n + lane < p.N) reinterpret_cast<uint16_t*>(y)[(int64_t)at * p.N + n + lane] = v;
+          }
+        }
+        __syncwarp();
+      }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowsThreads, 1)
+    f8_rows_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap wmap2,
+                   const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap smap, const F8Rows p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + p.park);   // the leader's, for both CTAs' copies
+  uint64_t* empty = full + kRowsStages;
+  uint64_t* acc_full = empty + kRowsStages;                      // [turn][half]
+  uint64_t* acc_empty = acc_full + 4;                            // the leader's
+  uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 4);
+  uint8_t* scales = ring + p.park + kRowsBarriers;   // [stages + 2][128 tokens]: the epilogue is up to two stages behind the MMAs
+  uint8_t* staging = scales + (kRowsStages + 2) * 512;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h0 = first_half(p.bn), h1 = p.bn - h0;               // channels of the two accumulators
+  const int stage_bytes = kWBytes + p.bn / 2 * kChunk, St = p.stages;
+  const int rank = (int)cluster_rank(), first = blockIdx.x / 2, step = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < St; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 2);   // both halves' MMAs
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 8);   // four warps of each CTA
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) tc::alloc_pair(slot, 512);
+  tc::fence_before();
+  cluster_sync_all();   // the peer's barriers exist before a copy or a commit reaches them
+  tc::fence_after();
+  const uint32_t tmem = *slot;
+  pdl_launch_dependents();
+
+  // 128 x 72 + 256 x 216 registers are the launch's 384 x 168: an epilogue thread holds 128 sums
+  if (warp < 4) {
+    tc::regs_dec<72>();
+    if (warp == 0 || warp == 3) {
+      // Two loaders, of the tokens and of the weights, as one would need longer for a stage than its MMAs take. The weights' first
+      // stages do not wait for the kernel before.
+      const bool weights = warp == 3;
+      if (tc::elect_one()) {
+        tma_prefetch_map(weights ? &wmap : &qmap);
+        tma_prefetch_map(weights ? &wmap2 : &smap);
+        const uint32_t bars = smem_addr(full), leader = mapa_shared(bars, 0);
+        constexpr uint32_t kEmpty = 8 * kRowsStages;
+        uint32_t dst = smem_addr(ring) + (weights ? kWBytes : 0), off = 0, phase = 1;   // of the stage; the ring starts out free
+        const uint32_t dst0 = dst, off_end = 8 * St, expect = 2 * (stage_bytes + 512);
+        uint32_t sdst = smem_addr(scales);
+        const uint32_t sdst0 = sdst, sdst_end = sdst + 512 * (St + 2);
+        int filled = 0;   // stages, up to the ring's
+        bool ok = true, ready = false;
+        if (!weights) pdl_wait();
+        for (int tile = first; tile < p.tiles && ok; tile += step) {
+          const TilePlace at = tile_place(tile, p.tiles_m, p.tiles_n);
+          const int row = weights ? at.n * p.bn + h0 / 2 * rank : at.m * 256 + 128 * rank, row2 = at.n * p.bn + h0 + h1 / 2 * rank;
+          for (int c = 0; c < p.chunks; ++c) {
+            if (!ready) ok = wait_ready(bars + off + kEmpty, phase, &g_f8_status);
+            if (!ok) break;
+            if (weights) {
+              tc::tma_load_2d_pair_at(dst, &wmap, c * kChunk, row, leader + off);
+              tc::tma_load_2d_pair_at(dst + h0 / 2 * kChunk, &wmap2, c * kChunk, row2, leader + off);
+            } else {
+              if (rank == 0) mbar_arrive_expect_tx(&full[off / 8], expect);
+              tc::tma_load_2d_pair_at(dst, &qmap, c * kChunk, row, leader + off);
+              tc::tma_load_2d_pair_at(sdst, &smap, row, c, leader + off);
+              sdst += 512;
+              if (sdst == sdst_end) sdst = sdst0;
+            }
+            filled += filled < St;
+            dst += stage_bytes;
+            off += 8;
+            if (off == off_end) off = 0, dst = dst0, phase ^= 1;
+            ready = test_barrier(bars + off + kEmpty, phase);
+          }
+        }
+        // no copy in flight past this point (the leader's barriers count all four loaders' copies): the stage to be filled next holds
+        // the oldest of the last ones, its parity is that of its release before, and in a ring that was not filled the first does
+        if (rank == 0 && !weights) {
+          if (filled < St) off = 0, phase = 1;
+          for (int k = 0; k < filled; ++k) {
+            wait_ready(bars + off, phase ^ (filled < St), &g_f8_status);
+            off += 8;
+            if (off == off_end) off = 0, phase ^= 1;
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp < 3) {
+      // A warp a half of the channels, one lane running its whole loop. An instruction costs it some ten clocks, since it shares
+      // its scheduler with epilogue warps and descriptors go through uniform registers: one lane for both halves took 1000
+      // clocks a stage.
+      const int h = warp - 1;
+      if (rank == 0 && tc::elect_one()) {
+        const uint32_t idesc = (1u << 4) | ((uint32_t)((h ? h1 : h0) >> 3) << 17) | ((256u >> 4) << 24);   // fp32 from e4m3, both K-major
+        const uint32_t stage_step = (uint32_t)stage_bytes >> 4, b_off = (uint32_t)(kWBytes + h * (h0 / 2 * kChunk)) >> 4;
+        const uint32_t desc0 = (uint32_t)tc::desc_sw128(smem_addr(ring), 16, 1024);   // counts 16 bytes
+        const uint32_t bars = smem_addr(full), bar_end = bars + 8 * St, acc_bars = smem_addr(acc_full) + 8 * h, d0 = tmem + 128 * h;
+        constexpr uint32_t kEmpty = 8 * kRowsStages, kAccEmpty = 32;   // bytes from a stage's or an accumulator's barrier to the other
+        uint32_t ad = desc0, bar = bars, phase = 0, u = 0;            // of the stage; stages so far
+        bool ready = false, free = true;   // (the first two accumulators are)
+        const uint32_t mine = first < p.tiles ? (uint32_t)((p.tiles - first + step - 1) / step) * p.chunks : 0;
+        for (; u < mine; ++u) {
+          const uint32_t acc = acc_bars + 16 * (u & 1), d = d0 + 256 * (u & 1);
+          if (!free && !wait_ready(acc + kAccEmpty, ((u >> 1) - 1) & 1, &g_f8_status)) break;
+          if (!ready && !wait_ready(bar, phase, &g_f8_status)) break;
+          tc::fence_after();
+          const uint32_t b = ad + b_off;
+          tc::mma_f8_ss_pair<false>(d, ad, b, idesc);
+          tc::mma_f8_ss_pair<true>(d, ad + 2, b + 2, idesc);
+          tc::mma_f8_ss_pair<true>(d, ad + 4, b + 4, idesc);
+          tc::mma_f8_ss_pair<true>(d, ad + 6, b + 6, idesc);
+          tc::commit_pair_at(acc);
+          tc::commit_pair_at(bar + kEmpty);
+          ad += stage_step;
+          bar += 8;
+          if (bar == bar_end) bar = bars, ad = desc0, phase ^= 1;
+          // the next accumulator and stage, asked together
+          free = u == 0 || test_barrier(acc_bars + kAccEmpty + 16 * (~u & 1), ((u + 1) / 2 - 1) & 1);
+          ready = test_barrier(bar, phase);
+        }
+        // no MMA in flight past this point
+        for (uint32_t i = 0; i < 2; ++i) {
+          const uint32_t uses = (u + 1 - i) >> 1;
+          if (uses > 0) wait_ready(acc_bars + 16 * i, (uses - 1) & 1, &g_f8_status);
+        }
+      }
+      __syncwarp();
+    }
+  } else {
+    tc::regs_inc<216>();
+    const int e = warp - 4, h = e >> 2;
+    const F8Epilogue w{smem_addr(acc_full), mapa_shared(smem_addr(acc_empty), 0), smem_addr(scales), tmem, staging + e * kRowsSmem, rank, first, step, h0 * h, h};
+    const int blocks = (h ? h1 : h0) / 16;
+    pdl_wait();
+    blocks == 8 ? rows_epilogue<T, 8>(p, w) : blocks == 6 ? rows_epilogue<T, 6>(p, w) : blocks == 4 ? rows_epilogue<T, 4>(p, w) : rows_epilogue<T, 2>(p, w);
+  }
+  __syncwarp();
+  tc::fence_before();
+  cluster_sync_all();   // neither CTA leaves while its partner still signals its shared memory
+  if (warp == 1) {
+    tc::fence_after();
+    tc::dealloc_pair(tmem, 512);
   }
 }
 
@@ -564,13 +832,13 @@ bool encode_rows(CUtensorMap* map, const void* base, int64_t width, int64_t ld, 
                               (uint32_t)box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-int tmem_columns(int bn) { return bn <= 32 ? 32 : bn <= 64 ? 64 : bn <= 128 ? 128 : 256; }
+int tmem_columns(int bn) { return bn <= 32 ? 32 : bn <= 64 ? 64 : 128; }
 
-// Tokens per tile, pairs or single CTAs, K split and stages: the candidate whose estimated time is least, in clocks per
-// CTA.
+// Which side the tokens are, the other side's width, K split and stages: the candidate whose estimated time is least, in clocks
+// per CTA.
 struct F8Plan {
   int bn, splits, stages;
-  bool pair;
+  bool rows;   // tokens as the A side, a pair of CTAs a tile
 };
 
 template <typename T, int NB>
@@ -593,8 +861,8 @@ int resident_clusters(int S) {   // of S single CTAs with the whole shared memor
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (allow_smem(f8_gemm_kernel<T, false, NB>, done) != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, f8_gemm_kernel<T, false, NB>, &cfg) != cudaSuccess) {
+    if (allow_smem(f8_cols_kernel<T, NB>, done) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, f8_cols_kernel<T, NB>, &cfg) != cudaSuccess) {
       cudaGetLastError();
       n = 0;
     }
@@ -608,23 +876,24 @@ template <typename T>
 F8Plan f8_plan(int64_t M, int64_t N, int chunks, int sms) {
   F8Plan best{0, 1, 0, false};
   int64_t least = INT64_MAX;
-  auto consider = [&](int bn, bool pair, int S) {
-    const int64_t tiles = (M + bn - 1) / bn * (pair ? (N + 255) / 256 : (N + 127) / 128);
-    if (S > 1 && tiles > resident_clusters<T, 4>(S)) return;
-    const int64_t ctas = tiles * (pair ? 2 : S), waves = (ctas + sms - 1) / sms;
-    const int64_t chunk = max(450, 2 * bn) + (kWBytes + (pair ? bn / 2 : bn) * kChunk) / 64;
+  auto consider = [&](int bn, bool rows, int S) {
+    const int64_t tiles = rows ? (M + 255) / 256 * ((N + bn - 1) / bn) : (M + bn - 1) / bn * ((N + 127) / 128);
+    if (S > 1 && tiles > resident_clusters<T, 2>(S)) return;
+    const int64_t ctas = tiles * (rows ? 2 : S), waves = (ctas + sms - 1) / sms;
+    const int64_t chunk = rows ? max(450, 2 * bn + 60) : max(450, 4 * bn) + (kWBytes + bn * kChunk) / 64;
     const int64_t c = 4700 + waves * ((chunks + S - 1) / S) * chunk + waves * 8 * bn + (S > 1 ? 2800 : 0);
     if (c < least) {
       least = c;
-      best.bn = bn, best.pair = pair, best.splits = S;
+      best.bn = bn, best.rows = rows, best.splits = S;
     }
   };
   for (int bn = 256; bn >= 64; bn -= 32) consider(bn, true, 1);
-  for (int bn = 256; bn >= 16; bn -= 16) {
+  for (int bn = 128; bn >= 16; bn -= 16) {
     if (bn - 16 >= M) continue;   // wider than the tokens
     for (int S = 1; S <= kMaxSplits && (S == 1 || chunks >= 2 * S); ++S) consider(bn, false, S);
   }
-  best.stages = min(kMaxStages, (kSmem - 1024 - kBarrierBytes) / (kWBytes + (best.pair ? best.bn / 2 : best.bn) * kChunk));
+  best.stages = min(best.rows ? kRowsStages : kMaxStages, (kSmem - 1024 - (best.rows ? kRowsBarrierBytes : kBarrierBytes)) /
+                                    (kWBytes + (best.rows ? best.bn / 2 : best.bn) * kChunk));
   return best;
 }
 
@@ -636,13 +905,13 @@ cudaError_t tokens_t(const void* x, int64_t ldx, uint8_t* q, int64_t ldq, float*
                    (int)K, release);
 }
 
-template <typename T, bool PAIR, int NB>
-cudaError_t gemm_t(const CUtensorMap& wmap, const CUtensorMap& qmap, const F8Gemm& g, unsigned ctas, size_t smem, bool pdl,
-                   cudaStream_t st) {
+template <typename T, int NB>
+cudaError_t cols_t(const CUtensorMap& wmap, const CUtensorMap& qmap, const F8Gemm& g, size_t smem, int sms, bool pdl, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = allow_smem(f8_gemm_kernel<T, PAIR, NB>, done);
+  const cudaError_t e = allow_smem(f8_cols_kernel<T, NB>, done);
   if (e != cudaSuccess) return e;
-  return launch_f8(f8_gemm_kernel<T, PAIR, NB>, dim3(ctas), kMmaThreads, smem, PAIR ? 2 : g.splits, pdl, st, wmap, qmap, g);
+  return launch_f8(f8_cols_kernel<T, NB>, dim3((unsigned)(g.splits > 1 ? g.tiles * g.splits : min(g.tiles, sms))), kMmaThreads, smem,
+                   g.splits, pdl, st, wmap, qmap, g);
 }
 
 template <typename T>
@@ -652,8 +921,6 @@ cudaError_t linear_t(const F8Params& p, bool pdl, cudaStream_t st) {
   const int chunks = (int)blocks_of(p.K);
   uint8_t* q = static_cast<uint8_t*>(p.workspace);
   float* s = reinterpret_cast<float*>(q + p.M * kp);
-  CUtensorMap wmap, qmap;
-  if (!encode_rows(&wmap, p.w, kp, p.ldw, p.N, 128)) return cudaErrorInvalidValue;
   // with few rows the product is let in early, see lb_w8.cu: it may read weights before it waits, so where they may still be
   // in the making only once everything before the quantization is complete
   const Release release = p.M > 296 ? kAtEnd : p.early ? kAtEntry : kAfterWait;
@@ -667,21 +934,30 @@ cudaError_t linear_t(const F8Params& p, bool pdl, cudaStream_t st) {
   if (last.M != p.M || last.N != p.N || last.chunks != chunks || last.sms != sms)
     last = {p.M, p.N, chunks, sms, f8_plan<T>(p.M, p.N, chunks, sms)};
   const F8Plan plan = last.plan;
-  const int own_bn = plan.pair ? plan.bn / 2 : plan.bn, tile_n = plan.pair ? 256 : 128;
-  const int tiles_m = (int)((p.M + plan.bn - 1) / plan.bn), tiles = (int)((p.N + tile_n - 1) / tile_n) * tiles_m;
-  const int stride = tmem_columns(plan.bn), park = plan.stages * (kWBytes + own_bn * kChunk);
-  const F8Gemm g{s, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, chunks, (int)lds, plan.bn, tiles_m, tiles, plan.splits, plan.stages,
-                 min(kMaxAcc, 512 / stride), stride, park, p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0};
-  if (!encode_rows(&qmap, q, kp, kp, p.M, own_bn)) return cudaErrorInvalidValue;
-  const size_t smem = (size_t)park + kBarrierBytes + 1024;
-  if (plan.pair) {
-    const unsigned ctas = (unsigned)(2 * min(tiles, sms / 2));
-    return plan.bn <= 128 ? gemm_t<T, true, 2>(wmap, qmap, g, ctas, smem, pdl, st) : gemm_t<T, true, 4>(wmap, qmap, g, ctas, smem, pdl, st);
+  CUtensorMap wmap, qmap;
+  const bool vec = p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
+  const int tile_m = plan.rows ? 256 : plan.bn, tile_n = plan.rows ? plan.bn : 128;
+  const int tiles_m = (int)((p.M + tile_m - 1) / tile_m), tiles = (int)((p.N + tile_n - 1) / tile_n) * tiles_m;
+  if (plan.rows) {
+    CUtensorMap wmap2, smap;
+    const int h0 = first_half(plan.bn);
+    if (!encode_rows(&wmap, p.w, kp, p.ldw, p.N, h0 / 2) || !encode_rows(&wmap2, p.w, kp, p.ldw, p.N, (plan.bn - h0) / 2) ||
+        !encode_rows(&qmap, q, kp, kp, p.M, 128) ||
+        !encode_tensor_map_2d(&smap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, s, (uint64_t)lds, (uint64_t)chunks, (uint64_t)lds * 4, 128, 1, CU_TENSOR_MAP_SWIZZLE_NONE))
+      return cudaErrorInvalidValue;
+    const int park = plan.stages * (kWBytes + plan.bn / 2 * kChunk);
+    const F8Rows g{s, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, chunks, (int)lds, plan.bn, tiles_m, tiles / tiles_m, tiles, plan.stages, park, vec};
+    static std::atomic<uint64_t> done{0};
+    if ((e = allow_smem(f8_rows_kernel<T>, done)) != cudaSuccess) return e;
+    return launch_f8(f8_rows_kernel<T>, dim3((unsigned)(2 * min(tiles, sms / 2))), kRowsThreads, (size_t)park + kRowsBarrierBytes + 1024, 2, pdl,
+                     st, wmap, wmap2, qmap, smap, g);
   }
-  const unsigned ctas = (unsigned)(plan.splits > 1 ? tiles * plan.splits : min(tiles, sms));
-  return plan.bn <= 64    ? gemm_t<T, false, 1>(wmap, qmap, g, ctas, smem, pdl, st)
-         : plan.bn <= 128 ? gemm_t<T, false, 2>(wmap, qmap, g, ctas, smem, pdl, st)
-                          : gemm_t<T, false, 4>(wmap, qmap, g, ctas, smem, pdl, st);
+  if (!encode_rows(&wmap, p.w, kp, p.ldw, p.N, 128) || !encode_rows(&qmap, q, kp, kp, p.M, plan.bn)) return cudaErrorInvalidValue;
+  const int stride = tmem_columns(plan.bn), park = plan.stages * (kWBytes + plan.bn * kChunk);
+  const F8Gemm g{s, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, chunks, (int)lds, plan.bn, tiles_m, tiles, plan.splits, plan.stages,
+                 min(kMaxAcc, 512 / stride), stride, park, vec};
+  const size_t smem = (size_t)park + kBarrierBytes + 1024;
+  return plan.bn <= 64 ? cols_t<T, 1>(wmap, qmap, g, smem, sms, pdl, st) : cols_t<T, 2>(wmap, qmap, g, smem, sms, pdl, st);
 }
 
 }  // namespace

@@ -86,6 +86,13 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_2d_pair_at(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -99,18 +106,38 @@ __device__ __forceinline__ void mma_f8_ss(uint32_t d, uint64_t a, uint64_t b, ui
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void mma_f8_ss_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// the same by a pair of CTAs (see mma_i8_ss_pair), the descriptors by their low words as below
+constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;   // the high word of desc_sw128 with sbo = 1024
+template <bool ACCUMULATE>
+__device__ __forceinline__ void mma_f8_ss_pair(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(ACCUMULATE ? 1 : 0), "n"(kDescHi)
+      : "memory");
+}
+__device__ __forceinline__ void commit_pair_at(uint32_t bar) {   // commit_pair on a shared-memory address
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+      : "memory");
+}
+
+// One lane's arrival, on a barrier of any CTA of the cluster, that hands an accumulator back: all that stands before it are
+// reads of tensor memory that have completed (tcgen05.wait::ld), so it needs no release, which would wait for the warp's
+// loads in flight.
+__device__ __forceinline__ void arrive_relaxed(uint32_t bar, bool on) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar), "r"((uint32_t)on)
       : "memory");
 }
 
 // fp16 or bf16 operands and an fp32 accumulator, A in shared or in tensor memory. The descriptors by their low words
-// (address and `lbo`): the high word is kDescHi, that of desc_sw128 with sbo = 1024.
-constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
+// (address and `lbo`): the high word is kDescHi.
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"

@@ -82,6 +82,40 @@ __device__ __forceinline__ bool wait_ready(uint32_t bar, uint32_t parity, int* s
   return false;
 }
 
+// The same for a whole warp in a loop that its instructions bound: one block of code without branches for the compiler, so
+// that nothing is inserted to bring lanes together again.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, %3;\n\t"
+      "LB_AGAIN_%=:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.eq.or.u32 q, n, 0, p;\n\t"
+      "@!q bra.uni LB_AGAIN_%=;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity), "r"(kSpinLimit)
+      : "memory");
+  if (!done) atomicExch(status, kErrBarrierTimeout);
+  return done;
+}
+
+// Whether a phase has completed, without waiting: asked ahead of the work before a wait, it hides what a wait costs even
+// when there is nothing to wait for (some 200 clocks).
+__device__ __forceinline__ bool test_barrier(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
 // One loader thread streaming chunks 0..nc-1 through a stage ring: refills stage s once its consumers released it
 // (empty[s]), then waits for its own last copies so that none is in flight when the CTA exits.
 template <typename Issue>
