@@ -98,6 +98,14 @@ __device__ __forceinline__ uint32_t amax8(const float (&f)[8]) {
   return a;
 }
 
+// max |x| of eight 16-bit values as fp32 bits: the values' bits without the sign order like the magnitudes, NaN above all
+template <typename T>
+__device__ __forceinline__ uint32_t amax_packed(const uint4& v) {
+  const uint32_t m = 0x7FFF7FFFu;
+  const uint32_t a = __vmaxu2(__vmaxu2(v.x & m, v.y & m), __vmaxu2(v.z & m, v.w & m));
+  return __float_as_uint(Elem<T>::unpack(max(a & 0xFFFFu, a >> 16)).x);
+}
+
 // Tokens: 16 lanes take a block of 128 values, a warp two tokens, a CTA 16 tokens x kQBlocks blocks, all of whose loads are
 // under way at once. The scales go to [block][token], as the product reads them, 16 tokens a run. Bound by memory.
 constexpr int kQBlocks = 4;
@@ -125,7 +133,7 @@ __global__ void __launch_bounds__(256)
     const int b = b0 + i, k = b * kBlock + 8 * lane;
     float f[8];
     floats8<T>(v[i], f);
-    uint32_t a = amax8(f);
+    uint32_t a = amax_packed<T>(v[i]);
 #pragma unroll
     for (int d = 8; d > 0; d >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, d));
     const BlockScale sc = block_scale(a);
@@ -788,6 +796,123 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   }
 }
 
+// ------------------------------------------------------------------------------------------------------- the product, one to eight tokens
+// A CTA takes 16 channels and all of K: mma.sync m16n8k32 with the weights' fragments loaded straight into registers, 64 bytes
+// of K (half a block) of a row per four lanes and 16-byte load (the order of k inside a fragment is free as long as both
+// operands share it); each piece's sums are scaled into fp32 registers. The first loads are issued at once, with `early` before
+// the wait on the previous kernel; the CTA quantizes the token rows while they are under way. Bound by the weights' way from
+// memory.
+constexpr int kGemvRows = 8;
+
+struct F8Gemv {
+  const void* x;
+  int64_t ldx;
+  const uint8_t* w;
+  int64_t ldw;
+  const float* t;
+  const void* bias;
+  void* y;
+  int M, N, K, blocks;
+  int pitch;             // bytes between the quantized rows: 64 modulo 128, so that two rows' reads do not share banks
+};
+
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// MR: the most rows, 1, 4 or 8. R: 64-byte pieces of K a warp has in flight. An SM holds gemv_per_sm of its CTAs.
+constexpr int gemv_per_sm(int NW, int MR, int R) {
+  return NW == 16 ? (R == 2 && MR < 8 ? 2 : 1) : (MR == 8 ? 2 : 3) + (R == 2);
+}
+template <typename T, int NW, int MR, int R>
+__global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) f8_gemv_kernel(const F8Gemv p, bool early) {
+  extern __shared__ __align__(16) uint8_t rows[];   // [M][pitch] quantized tokens, then the scales s t [blocks][MR]
+  __shared__ float part[NW][128];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16, pieces = 2 * p.blocks;
+  float* scales = reinterpret_cast<float*>(rows + p.M * p.pitch);
+  pdl_launch_dependents();
+  if (!early) pdl_wait();
+  // rows past N repeat the last one; pieces past K read as zeros (K is padded to 16, a lane's share of a piece)
+  const uint8_t* w0 = p.w + (int64_t)min(n0 + g, p.N - 1) * p.ldw + 16 * t;
+  const uint8_t* w1 = p.w + (int64_t)min(n0 + g + 8, p.N - 1) * p.ldw + 16 * t;
+  const float* tb = p.t + (int64_t)(n0 / kBlock) * p.blocks;
+  uint4 a[R][2];
+  auto fetch = [&](int i, int c) {
+    const bool on = 64 * c + 16 * t < p.K;
+    a[i][0] = on ? ldg_stream(reinterpret_cast<const uint4*>(w0 + 64 * c)) : make_uint4(0, 0, 0, 0);
+    a[i][1] = on ? ldg_stream(reinterpret_cast<const uint4*>(w1 + 64 * c)) : make_uint4(0, 0, 0, 0);
+  };
+#pragma unroll
+  for (int i = 0; i < R; ++i) fetch(i, warp + i * NW);
+  const int out_n = n0 + (tid & 15), out_m = tid >> 4;   // the output this thread sums, of 16 x 8
+  const bool out_on = tid < 128 && out_n < p.N && out_m < p.M;
+  const float bn = out_on && p.bias ? Elem<T>::to_float(static_cast<const T*>(p.bias)[out_n]) : 0.f;
+  if (early) pdl_wait();
+  const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * sizeof(T))) & 15u) == 0;
+  const T* x = static_cast<const T*>(p.x);
+  // 16 lanes a block of 128 values; all rows' loads of a round under way together
+  for (int j0 = 0; j0 < 16 * p.blocks; j0 += 32 * NW) {
+    const int j = j0 + tid;
+    const float t128 = (j & 15) == 0 && j < 16 * p.blocks ? __ldg(tb + (j >> 4)) : 0.f;
+    uint4 v[MR];
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+      v[m] = m < p.M && 8 * j < p.K ? load8(x + m * p.ldx + 8 * j, p.K - 8 * j, aligned) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+      if (m < p.M) {
+        float f[8];
+        floats8<T>(v[m], f);
+        uint32_t am = amax_packed<T>(v[m]);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) am = max(am, __shfl_xor_sync(0xffffffffu, am, d));
+        const BlockScale sc = block_scale(am);
+        if (j < 16 * p.blocks) {
+          *reinterpret_cast<uint2*>(rows + m * p.pitch + 8 * j) = e4m3x8(f, sc.up);
+          if ((j & 15) == 0) scales[(j >> 4) * MR + m] = sc.s * t128;
+        }
+      }
+  }
+  __syncthreads();
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const uint32_t own = smem_addr(rows) + (uint32_t)(min(g, p.M - 1) * p.pitch + 16 * t);   // unused columns repeat a row
+  const int m0 = min(2 * t, p.M - 1), m1 = min(2 * t + 1, p.M - 1);
+  for (int c0 = warp; c0 < pieces; c0 += NW * R) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int c = c0 + i * NW;
+      if (c < pieces) {
+        const uint4 b = lds128(own + 64 * c);
+        const float s0 = scales[(c >> 1) * MR + m0], s1 = scales[(c >> 1) * MR + m1];
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_e4m3(d, a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b.x, b.y);
+        mma_e4m3(d, a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b.z, b.w);
+        fetch(i, c + NW * R);
+        sum[0] = fmaf(d[0], s0, sum[0]);
+        sum[1] = fmaf(d[1], s1, sum[1]);
+        sum[2] = fmaf(d[2], s0, sum[2]);
+        sum[3] = fmaf(d[3], s1, sum[3]);
+      }
+    }
+  }
+  // D[g][2t], D[g][2t + 1], D[g + 8][..]: channel x token
+  part[warp][(2 * t) * 16 + g] = sum[0];
+  part[warp][(2 * t + 1) * 16 + g] = sum[1];
+  part[warp][(2 * t) * 16 + g + 8] = sum[2];
+  part[warp][(2 * t + 1) * 16 + g + 8] = sum[3];
+  __syncthreads();
+  if (out_on) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += part[w][tid];
+    static_cast<T*>(p.y)[(int64_t)out_m * p.N + out_n] = Elem<T>::from_float(v + bn);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------- launches
 template <typename Kern, typename... Args>
 cudaError_t launch_f8(Kern kern, dim3 grid, int threads, size_t smem, int cluster, bool pdl, cudaStream_t st, Args... args) {
@@ -835,7 +960,9 @@ bool encode_rows(CUtensorMap* map, const void* base, int64_t width, int64_t ld, 
 int tmem_columns(int bn) { return bn <= 32 ? 32 : bn <= 64 ? 64 : 128; }
 
 // Which side the tokens are, the other side's width, K split and stages: the candidate whose estimated time is least, in clocks
-// per CTA.
+// per CTA: a start and an end; per wave and stage what the way of an accumulator costs beside its columns (fitted to the
+// product at bn = 128 to 256: 8192 x 18944 x 3584, 4096 x 4096 x 3584; and 61 to 300 tokens of 3584, both sides' kernels: 129
+// tokens of 4608 channels 16.7 / 18.0 us, 257 22.4 / 20.1); stores; and a cluster's sum where all its CTAs can be resident.
 struct F8Plan {
   int bn, splits, stages;
   bool rows;   // tokens as the A side, a pair of CTAs a tile
@@ -880,7 +1007,7 @@ F8Plan f8_plan(int64_t M, int64_t N, int chunks, int sms) {
     const int64_t tiles = rows ? (M + 255) / 256 * ((N + bn - 1) / bn) : (M + bn - 1) / bn * ((N + 127) / 128);
     if (S > 1 && tiles > resident_clusters<T, 2>(S)) return;
     const int64_t ctas = tiles * (rows ? 2 : S), waves = (ctas + sms - 1) / sms;
-    const int64_t chunk = rows ? max(450, 2 * bn + 60) : max(450, 4 * bn) + (kWBytes + bn * kChunk) / 64;
+    const int64_t chunk = rows ? 600 + 2 * bn : 700 + 3 * bn;
     const int64_t c = 4700 + waves * ((chunks + S - 1) / S) * chunk + waves * 8 * bn + (S > 1 ? 2800 : 0);
     if (c < least) {
       least = c;
@@ -914,8 +1041,29 @@ cudaError_t cols_t(const CUtensorMap& wmap, const CUtensorMap& qmap, const F8Gem
                    g.splits, pdl, st, wmap, qmap, g);
 }
 
+// One to eight tokens, while their values are few: every CTA quantizes all of them.
+bool gemv_takes(int64_t M, int64_t K) { return M <= kGemvRows && M * K <= 12288; }
+
+template <typename T>
+cudaError_t gemv_t(const F8Params& p, bool pdl, cudaStream_t st) {
+  const int blocks = (int)blocks_of(p.K), pitch = blocks * kBlock + 64, mr = p.M == 1 ? 1 : p.M <= 4 ? 4 : 8;
+  const F8Gemv g{p.x, p.ldx, static_cast<const uint8_t*>(p.w), p.ldw, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, (int)p.K, blocks, pitch};
+  // 8 warps where they hold all of K, on wide layers; else 16. R = 4, or R = 2 where the more CTAs an SM then holds save a round
+  const int warps = blocks > 16 || p.N < 4096 ? 16 : 8, ctas = (int)((p.N + 15) / 16), sms = sm_count();
+  auto rounds = [&](int per) { return (ctas + per * sms - 1) / (per * sms); };
+#define LB_GEMV(MR)                                                                                                   \
+  (warps == 8 ? (rounds(gemv_per_sm(8, MR, 2)) < rounds(gemv_per_sm(8, MR, 4)) ? f8_gemv_kernel<T, 8, MR, 2>           \
+                                                                               : f8_gemv_kernel<T, 8, MR, 4>)          \
+              : (rounds(gemv_per_sm(16, MR, 2)) < rounds(gemv_per_sm(16, MR, 4)) ? f8_gemv_kernel<T, 16, MR, 2>        \
+                                                                                 : f8_gemv_kernel<T, 16, MR, 4>))
+  auto kern = p.M == 1 ? LB_GEMV(1) : p.M <= 4 ? LB_GEMV(4) : LB_GEMV(8);
+#undef LB_GEMV
+  return launch_f8(kern, dim3((unsigned)ctas), 32 * warps, (size_t)p.M * pitch + (size_t)blocks * mr * 4, 1, pdl, st, g, p.early);
+}
+
 template <typename T>
 cudaError_t linear_t(const F8Params& p, bool pdl, cudaStream_t st) {
+  if (gemv_takes(p.M, p.K)) return gemv_t<T>(p, pdl, st);
   const int sms = sm_count();
   const int64_t kp = padded(p.K), lds = scale_rows(p.M);
   const int chunks = (int)blocks_of(p.K);
@@ -962,7 +1110,9 @@ cudaError_t linear_t(const F8Params& p, bool pdl, cudaStream_t st) {
 
 }  // namespace
 
+// none where the product quantizes by itself
 size_t f8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (gemv_takes(M, K)) return 0;
   return (size_t)M * (size_t)padded(K) + (size_t)scale_rows(M) * blocks_of(K) * 4;
 }
 
