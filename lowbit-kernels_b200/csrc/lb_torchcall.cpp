@@ -11,6 +11,13 @@
 //   linear_w8(x, q, scales, out, bias) -> Tensor | None   (q, scales: a W8Weight's, its layout)
 //   norm_rope_append(qkv, cache_ptr, device, positions, slots, nh, inv_freq, q_norm, k_norm, eps, out) -> Tensor | None
 //   paged_attention(q, cache_ptr, device, page_table, seq_lens, cu_new, max_new, max_len, scale, out) -> Tensor | None
+//
+// and of a step of drafted tokens:
+//   linear_f8(x, q, scales, out, bias) -> Tensor | None   (q as bytes, scales: an F8Weight's)
+//   paged_tree_attention(q, cache_ptr, device, page_table, seq_lens, cu_new, mask, max_new, max_len, scale, out) -> Tensor | None
+//   plan(page_table, seq_lens, new_lens, page_size, tokens, held, free_pages, free_count, parents, max_new) -> tuple | None
+//   verify(logits, tokens, parents, cu_new, max_new, max_path) -> tuple | None
+//   compact(cache_ptrs, device, page_table, seq_lens, cu_new, path, accepted, out) -> Tensor | None
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
@@ -170,6 +177,45 @@ PyObject* linear_w8(PyObject* const* args) {
   return rc ? refused(rc) : result(args[3], y);
 }
 
+PyObject* linear_f8(PyObject* const* args) {
+  if (!THPVariable_Check(args[1])) Py_RETURN_NONE;
+  const at::Tensor& q = THPVariable_Unpack(args[1]);
+  if (!q.is_cuda() || q.scalar_type() != at::kByte || q.dim() != 2 || q.stride(1) != 1) Py_RETURN_NONE;
+  const long long dev = q.get_device();
+  const int64_t n = q.size(0), k = q.size(1), ldw = n > 1 ? q.stride(0) : (k + 15) / 16 * 16;
+  const at::Tensor* scales = tensor_on(args[2], dev);
+  if (!scales || scales->scalar_type() != at::kFloat || scales->dim() != 2 || scales->size(0) != (n + 127) / 128 ||
+      scales->size(1) != (k + 127) / 128 || !scales->is_contiguous())
+    Py_RETURN_NONE;
+  const at::Tensor* x = tensor_on(args[0], dev);
+  if (!x || x->dim() != 2 || x->size(1) != k || x->size(0) == 0 || c10::cuda::current_device() != dev) Py_RETURN_NONE;
+  const auto type = x->scalar_type();
+  if (type != at::kHalf && type != at::kBFloat16) Py_RETURN_NONE;
+  const int64_t m = x->size(0), ldx = m > 1 ? x->stride(0) : k;
+  if (x->stride(1) != 1 || ldx < k) Py_RETURN_NONE;
+  const void* bias = nullptr;
+  if (args[4] != Py_None) {
+    const at::Tensor* b = tensor_on(args[4], dev);
+    if (!b || b->scalar_type() != type || b->dim() != 1 || b->size(0) != n || !b->is_contiguous()) Py_RETURN_NONE;
+    bias = b->data_ptr();
+  }
+  at::Tensor y;
+  if (args[3] == Py_None) {
+    y = at::empty({m, n}, x->options());
+  } else {
+    const at::Tensor* o = tensor_on(args[3], dev);
+    if (!o || o->scalar_type() != type || o->dim() != 2 || o->size(0) != m || o->size(1) != n || !o->is_contiguous())
+      Py_RETURN_NONE;
+    y = *o;
+  }
+  const int64_t need = lb_f8_workspace(m, n, k);
+  at::Tensor ws;
+  if (need > 0) ws = at::empty({need}, x->options().dtype(at::kByte));
+  const int rc = lb_f8_linear(x->data_ptr(), type == at::kHalf ? LB_F16 : LB_BF16, ldx, q.data_ptr(), ldw, scales->data_ptr<float>(),
+                              bias, y.data_ptr(), m, n, k, need > 0 ? ws.data_ptr() : nullptr, need, stream_of(dev));
+  return rc ? refused(rc) : result(args[3], y);
+}
+
 at::ScalarType cache_type(const lb_paged_cache* c) { return c->dtype == LB_F16 ? at::kHalf : at::kBFloat16; }
 
 // a contiguous vector of that type and length on the device
@@ -225,7 +271,10 @@ PyObject* norm_rope_append(PyObject* const* args) {
   return rc ? refused(rc) : result(args[10], y);
 }
 
-PyObject* paged_attention(PyObject* const* args) {
+// both attentions; the arguments behind cu_new start at args[more], a tree's mask stands before them
+template <bool TREE>
+PyObject* attend(PyObject* const* args) {
+  constexpr int more = TREE ? 7 : 6;
   long long v[2];
   if (!to_ints(args + 1, v, 2)) return nullptr;
   const auto* c = reinterpret_cast<const lb_paged_cache*>(static_cast<uintptr_t>(v[0]));
@@ -241,24 +290,171 @@ PyObject* paged_attention(PyObject* const* args) {
     Py_RETURN_NONE;
   const int64_t t = q->size(0), nh = q->size(1), s = table->size(0), w = table->size(1);
   if (s > INT32_MAX || !vector_of(lens, at::kInt, s) || !vector_of(cu, at::kInt, s + 1)) Py_RETURN_NONE;
+  const at::Tensor* mask = nullptr;
+  if (TREE) {
+    mask = tensor_on(args[6], dev);
+    if (!mask || mask->scalar_type() != at::kInt || mask->dim() != 2 || mask->size(0) != t || mask->size(1) == 0 || !mask->is_contiguous())
+      Py_RETURN_NONE;
+  }
   long long bound[2] = {t, w * c->page_size};
   for (int i = 0; i < 2; ++i)
-    if (args[6 + i] != Py_None && !to_ints(args + 6 + i, bound + i, 1)) return nullptr;
+    if (args[more + i] != Py_None && !to_ints(args + more + i, bound + i, 1)) return nullptr;
   double scale = c->hd == 64 ? 0.125 : 0.08838834764831845;   // 1 / sqrt(hd) of the head dims the kernel takes
-  if (args[8] != Py_None) {
-    scale = PyFloat_AsDouble(args[8]);
+  if (args[more + 2] != Py_None) {
+    scale = PyFloat_AsDouble(args[more + 2]);
     if (scale == -1.0 && PyErr_Occurred()) return nullptr;
   }
   at::Tensor y;
-  if (!heads_out(args[9], dev, *q, t, nh, c->hd, &y)) Py_RETURN_NONE;
+  if (!heads_out(args[more + 3], dev, *q, t, nh, c->hd, &y)) Py_RETURN_NONE;
   const int64_t need = lb_paged_attention_workspace(t, (int)nh, c, w, (int)s, bound[0], bound[1]);
   at::Tensor ws;
   if (need > 0) ws = at::empty({need}, q->options().dtype(at::kByte));
-  const int rc = lb_paged_attention(q->data_ptr(), t > 1 ? q->stride(0) : 0, nh > 1 ? q->stride(1) : 0, t, (int)nh, c, table->data_ptr<int32_t>(),
-                                    s > 1 ? table->stride(0) : w, w, lens->data_ptr<int32_t>(), cu->data_ptr<int32_t>(),
-                                    (int)s, bound[0], bound[1], (float)scale, y.data_ptr(), nh * c->hd,
-                                    need > 0 ? ws.data_ptr() : nullptr, need, stream_of(dev));
-  return rc ? refused(rc) : result(args[9], y);
+  const int64_t ts = t > 1 ? q->stride(0) : 0, hs = nh > 1 ? q->stride(1) : 0, table_stride = s > 1 ? table->stride(0) : w;
+  void* const work = need > 0 ? ws.data_ptr() : nullptr;
+  const int rc =
+      TREE ? lb_paged_tree_attention(q->data_ptr(), ts, hs, t, (int)nh, c, table->data_ptr<int32_t>(), table_stride, w,
+                                     lens->data_ptr<int32_t>(), cu->data_ptr<int32_t>(), (int)s,
+                                     reinterpret_cast<const uint32_t*>(mask->data_ptr<int32_t>()), mask->size(1), bound[0], bound[1],
+                                     (float)scale, y.data_ptr(), nh * c->hd, work, need, stream_of(dev))
+           : lb_paged_attention(q->data_ptr(), ts, hs, t, (int)nh, c, table->data_ptr<int32_t>(), table_stride, w,
+                                lens->data_ptr<int32_t>(), cu->data_ptr<int32_t>(), (int)s, bound[0], bound[1], (float)scale,
+                                y.data_ptr(), nh * c->hd, work, need, stream_of(dev));
+  return rc ? refused(rc) : result(args[more + 3], y);
+}
+
+PyObject* tuple_of(std::initializer_list<at::Tensor*> tensors) {   // null or undefined: None
+  PyObject* r = PyTuple_New((Py_ssize_t)tensors.size());
+  if (!r) return nullptr;
+  Py_ssize_t i = 0;
+  for (at::Tensor* t : tensors) {
+    PyObject* o;
+    if (t && t->defined()) {
+      o = THPVariable_Wrap(std::move(*t));
+    } else {
+      Py_INCREF(Py_None);
+      o = Py_None;
+    }
+    if (!o) {
+      Py_DECREF(r);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(r, i++, o);
+  }
+  return r;
+}
+
+// an int32 page table with contiguous rows that do not overlap
+bool page_table_of(const at::Tensor* t) {
+  return t && t->scalar_type() == at::kInt && t->dim() == 2 && t->size(0) > 0 && t->size(0) <= INT32_MAX && t->size(1) > 0 &&
+         t->stride(1) == 1 && (t->size(0) == 1 || t->stride(0) >= t->size(1));
+}
+
+PyObject* plan(PyObject* const* args) {
+  if (!THPVariable_Check(args[0])) Py_RETURN_NONE;
+  const at::Tensor& table = THPVariable_Unpack(args[0]);
+  if (!table.is_cuda() || !page_table_of(&table)) Py_RETURN_NONE;
+  const long long dev = table.get_device();
+  if (c10::cuda::current_device() != dev) Py_RETURN_NONE;
+  const int64_t s = table.size(0), w = table.size(1);
+  const at::Tensor *lens = tensor_on(args[1], dev), *fresh = tensor_on(args[2], dev);
+  if (!vector_of(lens, at::kInt, s) || !vector_of(fresh, at::kInt, s)) Py_RETURN_NONE;
+  long long v[2], most = 0;
+  if (!to_ints(args + 3, v, 2)) return nullptr;
+  const long long page = v[0], tokens = v[1];
+  if (tokens < 1 || page < 1 || page > 65536) Py_RETURN_NONE;
+  const at::Tensor *held = nullptr, *list = nullptr, *count = nullptr, *parents = nullptr;
+  const bool paging = args[5] != Py_None;
+  if (paging != (args[6] != Py_None) || paging != (args[7] != Py_None)) Py_RETURN_NONE;
+  if (paging) {
+    held = tensor_on(args[5], dev), list = tensor_on(args[6], dev), count = tensor_on(args[7], dev);
+    if (!list || list->numel() == 0 || !vector_of(held, at::kInt, s) || !vector_of(list, at::kInt, list->numel()) || !vector_of(count, at::kInt, 1))
+      Py_RETURN_NONE;
+  }
+  int64_t words = 0;
+  if (args[8] != Py_None) {
+    parents = tensor_on(args[8], dev);
+    if (!vector_of(parents, at::kInt, tokens)) Py_RETURN_NONE;
+    most = tokens;
+    if (args[9] != Py_None && !to_ints(args + 9, &most, 1)) return nullptr;
+    if (most < 1 || most > 1024) Py_RETURN_NONE;
+    words = (most + 31) / 32;
+  }
+  const auto ints = lens->options(), longs = lens->options().dtype(at::kLong);
+  at::Tensor cu = at::empty({s + 1}, ints), after = at::empty({s}, ints), pos = at::empty({tokens}, longs), slots = at::empty({tokens}, longs);
+  at::Tensor held_out, count_out, mask;
+  if (paging) held_out = at::empty({s}, ints), count_out = at::empty({1}, ints);
+  if (parents) mask = at::empty({tokens, words}, ints);
+  const int rc = lb_paged_plan(lens->data_ptr<int32_t>(), fresh->data_ptr<int32_t>(), (int)s, table.data_ptr<int32_t>(),
+                               s > 1 ? table.stride(0) : w, w, (int)page, tokens, paging ? held->data_ptr<int32_t>() : nullptr,
+                               paging ? list->data_ptr<int32_t>() : nullptr, paging ? list->numel() : 0,
+                               paging ? count->data_ptr<int32_t>() : nullptr, parents ? parents->data_ptr<int32_t>() : nullptr, words,
+                               cu.data_ptr<int32_t>(), after.data_ptr<int32_t>(), paging ? held_out.data_ptr<int32_t>() : nullptr,
+                               paging ? count_out.data_ptr<int32_t>() : nullptr, pos.data_ptr<int64_t>(), slots.data_ptr<int64_t>(),
+                               parents ? reinterpret_cast<uint32_t*>(mask.data_ptr<int32_t>()) : nullptr, stream_of(dev));
+  return rc ? refused(rc) : tuple_of({&cu, &after, &pos, &slots, &held_out, &count_out, &mask});
+}
+
+PyObject* verify(PyObject* const* args) {
+  if (!THPVariable_Check(args[0])) Py_RETURN_NONE;
+  const at::Tensor& x = THPVariable_Unpack(args[0]);
+  if (!x.is_cuda() || x.dim() != 2 || x.size(0) == 0 || x.size(1) == 0 || x.stride(1) != 1) Py_RETURN_NONE;
+  const auto type = x.scalar_type();
+  if (type != at::kHalf && type != at::kBFloat16 && type != at::kFloat) Py_RETURN_NONE;
+  const long long dev = x.get_device();
+  if (c10::cuda::current_device() != dev) Py_RETURN_NONE;
+  const int64_t t = x.size(0), vocab = x.size(1), ld = t > 1 ? x.stride(0) : vocab;
+  const at::Tensor *tokens = tensor_on(args[1], dev), *parents = tensor_on(args[2], dev), *cu = tensor_on(args[3], dev);
+  if (ld < vocab || !vector_of(tokens, at::kLong, t) || !vector_of(parents, at::kInt, t) || !cu || !vector_of(cu, at::kInt, cu->numel()) || cu->numel() < 2 ||
+      cu->numel() > INT32_MAX)
+    Py_RETURN_NONE;
+  long long bound[2] = {t, 0};
+  if (args[4] != Py_None && !to_ints(args + 4, bound, 1)) return nullptr;
+  bound[1] = bound[0];
+  if (args[5] != Py_None && !to_ints(args + 5, bound + 1, 1)) return nullptr;
+  if (bound[0] < 1 || bound[0] > 1024 || bound[1] < 1 || bound[1] > 1024) Py_RETURN_NONE;
+  const int64_t s = cu->numel() - 1, need = lb_draft_verify_workspace(t, vocab);
+  const auto ints = cu->options(), longs = tokens->options();
+  at::Tensor accepted = at::empty({s}, ints), path = at::empty({s, bound[1]}, ints), next = at::empty({s}, longs), targets = at::empty({t}, longs);
+  at::Tensor ws = at::empty({need}, cu->options().dtype(at::kByte));
+  const int rc = lb_draft_verify(x.data_ptr(), type == at::kHalf ? LB_F16 : type == at::kBFloat16 ? LB_BF16 : LB_F32, ld, t, vocab,
+                                 tokens->data_ptr<int64_t>(), parents->data_ptr<int32_t>(), cu->data_ptr<int32_t>(), (int)s, bound[0], bound[1],
+                                 accepted.data_ptr<int32_t>(), path.data_ptr<int32_t>(), next.data_ptr<int64_t>(), targets.data_ptr<int64_t>(),
+                                 ws.data_ptr(), need, stream_of(dev));
+  return rc ? refused(rc) : tuple_of({&accepted, &path, &next, &targets});
+}
+
+PyObject* compact(PyObject* const* args) {
+  if (!PyList_Check(args[0])) Py_RETURN_NONE;
+  const Py_ssize_t layers = PyList_GET_SIZE(args[0]);
+  if (layers < 1 || layers > 128) Py_RETURN_NONE;
+  const lb_paged_cache* caches[128];
+  for (Py_ssize_t i = 0; i < layers; ++i) {
+    long long v;
+    PyObject* const one = PyList_GET_ITEM(args[0], i);
+    if (!to_ints(&one, &v, 1)) return nullptr;
+    caches[i] = reinterpret_cast<const lb_paged_cache*>(static_cast<uintptr_t>(v));
+  }
+  long long dev;
+  if (!to_ints(args + 1, &dev, 1)) return nullptr;
+  const at::Tensor *table = tensor_on(args[2], dev), *lens = tensor_on(args[3], dev), *cu = tensor_on(args[4], dev), *path = tensor_on(args[5], dev),
+                   *accepted = tensor_on(args[6], dev);
+  if (!page_table_of(table) || c10::cuda::current_device() != dev) Py_RETURN_NONE;
+  const int64_t s = table->size(0), w = table->size(1);
+  if (!vector_of(lens, at::kInt, s) || !vector_of(cu, at::kInt, s + 1) || !vector_of(accepted, at::kInt, s) || !path ||
+      path->scalar_type() != at::kInt || path->dim() != 2 || path->size(0) != s || path->size(1) == 0 || !path->is_contiguous())
+    Py_RETURN_NONE;
+  at::Tensor y;
+  if (args[7] == Py_None) {
+    y = at::empty({s}, lens->options());
+  } else {
+    const at::Tensor* o = tensor_on(args[7], dev);
+    if (!vector_of(o, at::kInt, s)) Py_RETURN_NONE;
+    y = *o;
+  }
+  const int rc = lb_paged_compact(caches, (int)layers, table->data_ptr<int32_t>(), s > 1 ? table->stride(0) : w, w, lens->data_ptr<int32_t>(),
+                                  cu->data_ptr<int32_t>(), path->data_ptr<int32_t>(), accepted->data_ptr<int32_t>(), (int)s, path->size(1),
+                                  y.data_ptr<int32_t>(), args[7] != Py_None, stream_of(dev));
+  return rc ? refused(rc) : result(args[7], y);
 }
 
 template <PyObject* (*F)(PyObject* const*), int N>
@@ -281,7 +477,19 @@ PyMethodDef methods[] = {
     {"norm_rope_append", fastcall<norm_rope_append, 11>(), METH_FASTCALL,
      "norm_rope_append(qkv, cache_ptr, device, positions, slots, nh, inv_freq, q_norm, k_norm, eps, out) -> Tensor, or "
      "None for the checked path"},
-    {"paged_attention", fastcall<paged_attention, 10>(), METH_FASTCALL,
+    {"linear_f8", fastcall<linear_f8, 5>(), METH_FASTCALL,
+     "linear_f8(x, q, scales, out, bias) -> Tensor, or None for the checked path"},
+    {"paged_tree_attention", fastcall<attend<true>, 11>(), METH_FASTCALL,
+     "paged_tree_attention(q, cache_ptr, device, page_table, seq_lens, cu_new, mask, max_new, max_len, scale, out) -> Tensor, or "
+     "None for the checked path"},
+    {"plan", fastcall<plan, 10>(), METH_FASTCALL,
+     "plan(page_table, seq_lens, new_lens, page_size, tokens, held, free_pages, free_count, parents, max_new) -> tuple, or None "
+     "for the checked path"},
+    {"verify", fastcall<verify, 6>(), METH_FASTCALL,
+     "verify(logits, tokens, parents, cu_new, max_new, max_path) -> tuple, or None for the checked path"},
+    {"compact", fastcall<compact, 8>(), METH_FASTCALL,
+     "compact(cache_ptrs, device, page_table, seq_lens, cu_new, path, accepted, out) -> Tensor, or None for the checked path"},
+    {"paged_attention", fastcall<attend<false>, 10>(), METH_FASTCALL,
      "paged_attention(q, cache_ptr, device, page_table, seq_lens, cu_new, max_new, max_len, scale, out) -> Tensor, or "
      "None for the checked path"},
     {"gemv", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(tc_gemv)), METH_FASTCALL,

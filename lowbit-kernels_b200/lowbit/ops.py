@@ -545,6 +545,11 @@ def linear_f8(x, f8, bias=None, out=None):
     values, the product with f8 (F8Weight) summed in fp32, each block times its two scales, `bias` ([N], x's type) added and
     rounded once. `out`: an optional contiguous [M, N] tensor that receives the result. A serving operator: the result
     carries no autograd graph."""
+    tc = _tc if _tc is not None else _torchcall()
+    if tc:
+        y = tc.linear_f8(x, f8._q, f8._scales, out, bias)
+        if y is not None:
+            return y
     if not (isinstance(x, torch.Tensor) and x.is_cuda and x.device == f8._q.device):
         raise RuntimeError(f"x must be on the weight's GPU, {f8._q.device}")
     if x.dtype not in (torch.float16, torch.bfloat16) or x.dim() != 2 or x.shape[1] != f8.k:

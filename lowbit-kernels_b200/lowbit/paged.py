@@ -150,6 +150,11 @@ def tree_attention(q, cache, page_table, seq_lens, cu_new, mask, max_new=None, m
     whether it sees its sequence's new token j (`plan` makes it from the tokens' parents; any pattern will do, a row of zeros
     too). Every new token sees the whole cached context, the keys before the sequence's new ones, which lie in the cache in the
     order of the call; new tokens past 32 * words are seen by none. The rest is as in `attention`."""
+    tc = ops._tc if ops._tc is not None else ops._torchcall()
+    if tc:
+        y = tc.paged_tree_attention(q, cache._ptr, cache._device, page_table, seq_lens, cu_new, mask, max_new, max_len, scale, out)
+        if y is not None:
+            return y
     if mask is None:
         raise RuntimeError("mask must be an int32 [T, words] tensor on the cache's GPU")
     return _attend(q, cache, page_table, seq_lens, cu_new, mask, max_new, max_len, scale, out)
@@ -251,6 +256,11 @@ def plan(page_table, seq_lens, new_lens, page_size, tokens, held=None, free_page
     `tree_attention` takes, its rows ceil(max_new / 32) words (max_new bounds the new tokens of any sequence, 1024 at most; by default
     tokens). out: a Plan whose tensors receive the result (fixed addresses for a captured step); its held, free_count
     and seq_lens may be the ones passed in."""
+    tc = ops._tc if ops._tc is not None else ops._torchcall()
+    if tc and out is None:
+        got = tc.plan(page_table, seq_lens, new_lens, page_size, tokens, held, free_pages, free_count, parents, max_new)
+        if got is not None:
+            return Plan._make(got)
     s, width, stride = _page_table(page_table)
     dev = page_table.device
     lens, new = _vector("seq_lens", seq_lens, torch.int32, dev, s), _vector("new_lens", new_lens, torch.int32, dev, s)
@@ -301,6 +311,11 @@ def verify(logits, tokens, parents, cu_new, max_new=None, max_path=None):
     (accepted), their places among the new ones (path, -1 behind them) and the target after the last (next). A sequence
     without new tokens gets 0 and -1. max_new bounds the new tokens of any sequence (1024 at most; by default T),
     max_path the path (by default max_new). Rows past cu_new[S] are not looked at, their targets left unwritten."""
+    tc = ops._tc if ops._tc is not None else ops._torchcall()
+    if tc:
+        got = tc.verify(logits, tokens, parents, cu_new, max_new, max_path)
+        if got is not None:
+            return Verified._make(got)
     if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dim() == 2 and logits.dtype in DTYPE_IDS):
         raise RuntimeError("logits must be a float16, bfloat16 or float32 [T, vocab] tensor on the GPU")
     t, vocab = logits.shape
@@ -351,6 +366,11 @@ def compact(caches, page_table, seq_lens, cu_new, path, accepted, out=None):
     cache = caches[0]
     if any(c._device != cache._device for c in caches):
         raise RuntimeError("the caches must be on one GPU")
+    tc = ops._tc if ops._tc is not None else ops._torchcall()
+    if tc:
+        got = tc.compact([c._ptr for c in caches], cache._device, page_table, seq_lens, cu_new, path, accepted, out)
+        if got is not None:
+            return got
     s, width, stride = _page_table(page_table)
     if page_table.get_device() != cache._device:
         raise RuntimeError(f"page_table must be on the cache's GPU, {cache.k.device}")
