@@ -1396,7 +1396,13 @@ cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   cp.C = 1;
   for (int C = 1; C <= kChunkCluster && (C == 1 || key_tiles >= 2 * C); ++C) {
     const int64_t resident = C == 1 ? sm_count() : chunk_resident<HD>(C), rounds = (items + resident - 1) / resident;
-    const double t = (double)rounds * (6 + (C > 1 ? 6 : 0) + 1.4 * (double)((key_tiles + C - 1) / C));
+    const double ends = 6 + (C > 1 ? 6 : 0), steps = 1.4 * (double)((key_tiles + C - 1) / C);
+    double t = (double)rounds * (ends + steps);
+    // Trees of several sequences all start at the end of their contexts, and those differ: the longest one, or the work of contexts
+    // spread evenly up to it, over what can be resident (32 trees of 25 tokens, 28/4 heads: contexts spread to 8192, C = 1, 2, 3,
+    // 4: 121, 74, 89, 99 us, all of 8192 121, 135, 149, 156; 64 of 16 to 4000 87, 104, 135, 157; 8 of 61 to 6000, 16/2 heads 98,
+    // 63, 46, 37)
+    if (TREE && p.seqs > 1) t = max(ends + steps, (double)items * (ends + 0.5 * steps * (p.seqs + 1) / p.seqs) / (double)resident);
     if (t < least) least = t, cp.C = C;
   }
   CUtensorMap kmap, vmap;
