@@ -1,7 +1,9 @@
 """A paged KV cache and the two operators a chunk of new tokens runs against it: `norm_rope_append` (per-head norms of
 q and k, rotary rotation, append to the cache in one pass) and `attention` (the new tokens of several sequences over
-their cached contexts; one new token per sequence is a decode step). `PagedDecoder` runs them together with the 8-bit
-products of ops.linear_w8. No counterpart in the reference, which feeds transformers' own cache (bench/e2e.py:84-147).
+their cached contexts; one new token per sequence is a decode step). For drafted tokens that form trees: `plan` (page tables,
+slots, positions and tree masks from lengths on the GPU), `tree_attention`, `verify` (which drafts are accepted) and `compact`
+(their K and V rows move together). `PagedDecoder` runs them together with the 8-bit products of ops.linear_w8 and
+ops.linear_f8. No counterpart in the reference, which feeds transformers' own cache (bench/e2e.py:84-147).
 
 Every call launches on the current torch stream of the tensors' device and never synchronizes. Serving operators: their
 outputs carry no autograd graph, whatever their inputs require. There is no fallback: without the library or a CUDA device
@@ -393,8 +395,8 @@ class PagedDecoder:
     """A Qwen2-architecture decoder whose calls take chunks of new tokens of any number of sequences -- a prompt in
     pieces, single tokens of a running batch, or both at once -- over paged caches. Takes the weights of a transformers
     model of that architecture (fp16 or bf16; per-head q_norm / k_norm modules are used where its attention has them)
-    and keeps its projections in 8-bit integers (`weights="w8"`, ops.linear_w8) or, fp16 models only, in the INT4 format
-    (`weights="w4"`, ops.linear). Per layer: RMSNorm, the fused q|k|v product, `norm_rope_append`, `attention`, the output
+    and keeps its projections in 8-bit integers (`weights="w8"`, ops.linear_w8), in 8-bit floating point with block scales
+    (`weights="f8"`, ops.linear_f8) or, fp16 models only, in the INT4 format (`weights="w4"`, ops.linear). Per layer: RMSNorm, the fused q|k|v product, `norm_rope_append`, `attention`, the output
     product, RMSNorm, the fused gate|up product, SiLU * up, the down product. Models that scale their rotary angles, with an
     activation other than SiLU or with head dims other than 64 and 128 are refused (ValueError); one whose attention slides
     over a window, or whose angles are scaled only from some length on, takes contexts up to that length.
@@ -403,12 +405,13 @@ class PagedDecoder:
         a, b = dec.open(), dec.open()
         logits = dec.forward({a: prompt_a, b: prompt_b[:512]})      # [2, vocab]: after each chunk's last token
         logits = dec.forward({a: [next_a], b: prompt_b[512:]})
+        more = dec.verify({a: ([next_a, x, y, z], [-1, 0, 0, 1])})   # drafts x and y after next_a, z after x
         dec.close(a)
     """
 
     def __init__(self, model, num_pages, page_size=64, weights="w8", group=128):
-        if weights not in ("w8", "w4"):
-            raise ValueError('weights is "w8" or "w4"')
+        if weights not in ("w8", "f8", "w4"):
+            raise ValueError('weights is "w8", "f8" or "w4"')
         cfg, base = model.config, model.model
         self.limit = context_limit(cfg)
         self.embed = base.embed_tokens.weight.detach()
@@ -425,6 +428,8 @@ class PagedDecoder:
         self.inv_freq = (1.0 / theta ** (half / self.hd)).to(self.device)
         if weights == "w8":
             self._make, self._linear = ops.W8Weight.from_float, ops.linear_w8
+        elif weights == "f8":
+            self._make, self._linear = ops.F8Weight.from_float, ops.linear_f8
         else:
             self._make = lambda w: ops.W4Weight.from_float(w, group, ("mma",))
             self._linear = ops.linear
@@ -498,6 +503,19 @@ class PagedDecoder:
         for (s, v), n in zip(pages.items(), lens):
             self._seqs[s] = {"length": n, "pages": v}
 
+    def _layers(self, x, pos, slots, attend):
+        """The residual stream x [T, hidden] after all layers; attend(q, cache) is their attention."""
+        for ly in self.layers:
+            def product(h, name):
+                w, bias = ly[name]
+                return self._linear(h, w, bias=bias)
+            qkv = product(self._rms(x, ly["ln1"]), "qkv")
+            q = norm_rope_append(qkv, ly["cache"], pos, slots, self.nh, self.inv_freq, ly["q_norm"], ly["k_norm"], self.eps)
+            x = x + product(attend(q, ly["cache"]).view(len(x), self.nh * self.hd), "o")
+            gate, up = product(self._rms(x, ly["ln2"]), "gate_up").chunk(2, -1)
+            x = x + product(torch.nn.functional.silu(gate) * up, "down")
+        return x
+
     @torch.no_grad()
     def forward(self, chunks):
         """chunks: {sequence id: its new token ids, at least one}. Appends them and returns the logits [len(chunks),
@@ -506,22 +524,53 @@ class PagedDecoder:
         if not chunks or any(len(new) == 0 for new in chunks.values()):
             raise ValueError("every sequence of a call needs a new token")
         ids, pos, slots, table, lens, cu, pages = self._plan(chunks)
-        dev, t = self.device, len(ids)
+        dev = self.device
         ids, pos, slots = (torch.tensor(v, dtype=torch.int64, device=dev) for v in (ids, pos, slots))
         table, lens_d, cu_d = (torch.tensor(v, dtype=torch.int32, device=dev) for v in (table, lens, cu))
         max_new, max_len = max(len(new) for new in chunks.values()), max(lens)
-        x = self.embed[ids]
-        for ly in self.layers:
-            def product(h, name):
-                w, bias = ly[name]
-                return self._linear(h, w, bias=bias)
-            qkv = product(self._rms(x, ly["ln1"]), "qkv")
-            q = norm_rope_append(qkv, ly["cache"], pos, slots, self.nh, self.inv_freq, ly["q_norm"], ly["k_norm"], self.eps)
-            a = attention(q, ly["cache"], table, lens_d, cu_d, max_new=max_new, max_len=max_len)
-            x = x + product(a.view(t, self.nh * self.hd), "o")
-            gate, up = product(self._rms(x, ly["ln2"]), "gate_up").chunk(2, -1)
-            x = x + product(torch.nn.functional.silu(gate) * up, "down")
+        x = self._layers(self.embed[ids], pos, slots,
+                         lambda q, cache: attention(q, cache, table, lens_d, cu_d, max_new=max_new, max_len=max_len))
         last = torch.tensor([c - 1 for c in cu[1:]], dtype=torch.int64, device=dev)
         logits = torch.nn.functional.linear(self._rms(x[last], self.norm), self.head)
         self._commit(pages, lens)
         return logits
+
+    @torch.no_grad()
+    def verify(self, trees):
+        """trees: {sequence id: (tokens, parents)}. A sequence's first token is its last certain one, not fed yet (what `forward` or
+        `verify` gave as the next), its parent -1; each further one is a draft that follows the token at its parent's place,
+        an earlier one. All of them run through the model at once. Returns {sequence id: its new certain tokens}, one at least:
+        the drafts on the path that the model's own choices (the first largest logit) take from the first token, then its choice after the
+        last of them, which is the first token of the next call. The sequences keep the first token and the accepted drafts. A call
+        that raises (ValueError for a token id outside the embedding or parents that are no tree) leaves every sequence and the
+        free pages as they were."""
+        if not trees:
+            raise ValueError("no trees")
+        for tokens, parents in trees.values():
+            if not 1 <= len(tokens) <= 1024 or len(parents) != len(tokens):
+                raise ValueError("a tree has 1 to 1024 tokens, and a parent for each")
+            if int(parents[0]) != -1 or any(not 0 <= int(p) < i for i, p in enumerate(parents[1:], 1)):
+                raise ValueError("the first token's parent is -1, any other's an earlier token's place")
+        ids, _, _, table, lens, cu, pages = self._plan({s: tokens for s, (tokens, _) in trees.items()})
+        dev, new = self.device, [b - a for a, b in zip(cu, cu[1:])]
+        drafted = torch.tensor(ids, dtype=torch.int64, device=dev)
+        ints = (table, [n - k for n, k in zip(lens, new)], new, [int(p) for _, parents in trees.values() for p in parents])
+        table_d, before, new_d, parents = (torch.tensor(v, dtype=torch.int32, device=dev) for v in ints)
+        max_new, max_len = max(new), max(lens)
+        at = plan(table_d, before, new_d, self.page_size, len(ids), parents=parents, max_new=max_new)
+        x = self._layers(self.embed[drafted], at.positions, at.slots,
+                         lambda q, cache: tree_attention(q, cache, table_d, at.seq_lens, at.cu_new, at.mask, max_new=max_new, max_len=max_len))
+        logits = torch.nn.functional.linear(self._rms(x, self.norm), self.head)
+        got = verify(logits, drafted, parents, at.cu_new, max_new=max_new)
+        if self.layers:
+            compact([ly["cache"] for ly in self.layers], table_d, at.seq_lens, at.cu_new, got.path, got.accepted)
+        accepted, path, following = got.accepted.tolist(), got.path.tolist(), got.next.tolist()
+        kept = [n - k + a for n, k, a in zip(lens, new, accepted)]
+        self._commit(pages, kept)
+        more = {}
+        for (s, (tokens, _)), a, way, nxt in zip(trees.items(), accepted, path, following):
+            mine, need = self._seqs[s]["pages"], -(-self._seqs[s]["length"] // self.page_size)
+            self._free += reversed(mine[need:])
+            del mine[need:]
+            more[s] = [int(tokens[i]) for i in way[1:a]] + [nxt]
+        return more

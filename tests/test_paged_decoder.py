@@ -267,3 +267,189 @@ def test_a_call_that_failed_in_a_layer_can_be_repeated(monkeypatch):
     assert (dec._free, dec._seqs) == state
     monkeypatch.undo()
     assert torch.equal(torch.cat((first, dec.forward({sid: ids[50:]}))), want)
+
+
+# ------------------------------------------------------------------------------------- drafted trees, 8-bit floating point
+
+@torch.no_grad()
+def plain_f8_logits(model, ids, activations=True):
+    """plain_logits with the projections of linear_f8: weights and (or not) activations quantized by blocks, as the operator is
+    defined, values rounded to the model's type where the decoder stores them."""
+    from lowbit import ops
+
+    class Blocks(torch.nn.Module):
+        def __init__(self, lin):
+            super().__init__()
+            q, s = ops.quantize_f8_gpu(lin.weight)
+            n, k = q.shape
+            self.w = q.double() * s.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+            self.bias = lin.bias
+
+    dtype = model.lm_head.weight.dtype
+
+    def product(x, b):
+        if not activations:
+            y = x @ b.w.t()
+            return (y if b.bias is None else y + b.bias.double()).to(dtype).double()
+        t, k = x.shape
+        g = torch.nn.functional.pad(x, (0, -k % 128)).view(t, -1, 128)
+        a = g.abs().amax(2, keepdim=True).clamp(min=2.0 ** -100)
+        g = (g.float() * (448.0 / a).float()).to(torch.float8_e4m3fn).double() * (a / 448)
+        y = g.reshape(t, -1)[:, :k] @ b.w.t()
+        return (y if b.bias is None else y + b.bias.double()).to(dtype).double()
+
+    def rms(x, w):
+        return (((x * torch.rsqrt(x.square().mean(-1, keepdim=True) + model.config.rms_norm_eps)).to(dtype).double()) * w.double()).to(dtype).double()
+
+    t, hd = len(ids), 64
+    x = model.model.embed_tokens.weight[ids].double()
+    freq = 1.0 / 1e6 ** (torch.arange(0, hd, 2, device="cuda", dtype=torch.float64) / hd)
+    angle = torch.arange(t, device="cuda", dtype=torch.float64)[:, None, None] * freq
+    mask = torch.ones(t, t, device="cuda", dtype=torch.bool).triu(1)
+    for layer in model.model.layers:
+        a, m = layer.self_attn, layer.mlp
+        # the decoder quantizes q, k, v and gate, up as one weight each: blocks of 128 rows do not cross them at these sizes
+        h = rms(x, layer.input_layernorm.weight)
+        q, k, v = (product(h, Blocks(p)).view(t, -1, hd) for p in (a.q_proj, a.k_proj, a.v_proj))
+
+        def rope(z):
+            c, d = z.chunk(2, -1)
+            return torch.cat((c * angle.cos() - d * angle.sin(), d * angle.cos() + c * angle.sin()), -1).to(dtype).double()
+
+        q, k = rope(q), rope(k)
+        k, v = k.repeat_interleave(2, 1), v.repeat_interleave(2, 1)
+        p = torch.softmax((torch.einsum("qhd,khd->hqk", q, k) / 8).masked_fill(mask, float("-inf")), -1)
+        x = (x + product(torch.einsum("hqk,khd->qhd", p, v).reshape(t, -1).to(dtype).double(), Blocks(a.o_proj))).to(dtype).double()
+        h = rms(x, layer.post_attention_layernorm.weight)
+        act = (torch.nn.functional.silu(product(h, Blocks(m.gate_proj))).to(dtype).double() * product(h, Blocks(m.up_proj))).to(dtype).double()
+        x = (x + product(act, Blocks(m.down_proj))).to(dtype).double()
+    return rms(x, model.model.norm.weight) @ model.lm_head.weight.double().t()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_paged_decoder_with_f8_weights_is_as_near_as_a_plain_one(dtype):
+    """An e4m3 step is up to 2^-3 of a value, and where a rounding of the stored type moves a value past the middle of a step, the
+    decoder and a plain one go a whole step apart there: after a layer the two are as good as quantized independently. So neither is the
+    other's measure; both have the same distance (root mean square, over more than 10^5 logits) from a decoder with the same
+    weights whose activations are not quantized, to a quarter for what the stored type's own roundings add."""
+    from lowbit import ops, paged
+    model = tiny(dtype=dtype)
+    dec = paged.PagedDecoder(model, num_pages=32, page_size=16, weights="f8")
+    ids = torch.randint(0, 1024, (150,), generator=torch.Generator().manual_seed(9)).tolist()
+    exact = plain_f8_logits(model, ids, activations=False)
+    plain = (plain_f8_logits(model, ids) - exact).square().mean().sqrt().item()
+    for pieces in ([1] * 150, [2] * 75):
+        got = feed(dec, ids, pieces)
+        ends = torch.tensor(pieces).cumsum(0) - 1
+        mine = (got.double() - exact[ends]).square().mean().sqrt().item()
+        assert mine < 1.25 * plain, (pieces[:2], mine, plain)
+    whole = feed(dec, ids, [150])
+    assert (whole.double() - exact[-1:]).square().mean().sqrt().item() < 2 * plain   # (1024 values of one row, not alike)
+    assert len(dec._free) == 32 and ops.ext().lib.lb_device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("weights", ["w4", "w8", "f8"])
+def test_verify_keeps_what_the_model_would_have_chosen(weights):
+    """Trees of right and wrong drafts, several sequences at once: every accepted token is, within the products' roundings, the largest
+    logit of a decoder that is fed the same text plainly; a tree's cache then continues as that decoder's does. The bars are those of the
+    tests against plain decoders; f8: an activation's error is 2^-3 / sqrt(12) / 1.44 = 2.5 % of it in the mean square (steps of 2^-4 to
+    2^-3 of a value), so each product's, and six that add up in the residual stream give at most 6 %; two decoders are sqrt(2) times
+    that apart, and of 10^4 values the largest at 4.5 times: 0.4."""
+    from lowbit import ops, paged
+    import random
+    model = tiny()
+    bar = {"w4": 2e-2, "w8": 8e-2, "f8": 4e-1}[weights]
+    dec, ref = (paged.PagedDecoder(model, num_pages=64, page_size=16, weights=weights) for _ in range(2))
+    rng = random.Random(5)
+    sids = [dec.open() for _ in range(3)]
+    texts = {s: [rng.randrange(1024) for _ in range(n)] for s, n in zip(sids, (5, 33, 16))}
+    logits = dec.forward(dict(texts))
+    nxt = {s: int(row.argmax()) for s, row in zip(sids, logits)}
+
+    def greedy(text, n):   # what a plain decoder would say next, as drafts
+        sid, out = ref.open(), []
+        last = ref.forward({sid: text})[0]
+        for _ in range(n):
+            out.append(int(last.argmax()))
+            last = ref.forward({sid: out[-1:]})[0]
+        ref.close(sid)
+        return out
+
+    taken = 0
+    for turn in range(4):
+        trees = {}
+        for s in sids:
+            good = greedy(texts[s] + [nxt[s]], 3)
+            # the right drafts among wrong ones, in levels: 1 2 3 after the first token, 4 5 after one of them, 6 after one of those
+            first, second = rng.randint(1, 3), rng.randint(4, 5)
+            tokens = [nxt[s]] + [rng.randrange(1024) for _ in range(6)]
+            parents = [-1, 0, 0, 0, first, first, second]
+            tokens[first], tokens[second], tokens[6] = good[0], good[1], good[2] if turn % 2 else (good[2] + 1) % 1024
+            trees[s] = (tokens, parents)
+        got = dec.verify(trees)
+        for s in sids:
+            new = [nxt[s]] + got[s][:-1]
+            text = texts[s] + new
+            assert dec._seqs[s]["length"] == len(text) and len(dec._seqs[s]["pages"]) == -(-len(text) // 16)
+            sid = ref.open()
+            rows = [ref.forward({sid: text[:len(texts[s]) + 1]})[0]] + [ref.forward({sid: [t]})[0] for t in new[1:]]
+            ref.close(sid)
+            for row, choice in zip(rows, got[s]):
+                assert (row.max() - row[choice]).item() <= 2 * bar * row.float().square().mean().sqrt().item()
+            texts[s], nxt[s] = text, got[s][-1]
+            taken += len(got[s])
+    assert taken > 2 * 3 * 4   # most of the right drafts were accepted
+    # the caches hold the texts: their next logits are a plain decoder's
+    out = dec.forward({s: [nxt[s]] for s in sids})
+    for row, s in zip(out, sids):
+        sid = ref.open()
+        want = ref.forward({sid: texts[s] + [nxt[s]]})[0].float()
+        ref.close(sid)
+        assert ((row.float() - want).abs().max() / want.square().mean().sqrt()).item() < bar
+    for s in sids:
+        dec.close(s)
+    assert sorted(dec._free) == list(range(64)) and ops.ext().lib.lb_device_error() == 0
+
+
+@pytest.mark.parametrize("tree", [([], []), ([1], [-1, 0]), ([1, 2], [-1, 1]), ([1, 2], [-1, -1]), ([1, 2], [0, 0]), ([1, 2, 3], [-1, 2, 0]),
+                                  ([32, 1], [-1, 0]), ([1, -1], [-1, 0]), ([1] * 1025, list(range(-1, 1024))), ([1] * 200, list(range(-1, 199)))])
+def test_verify_refuses_what_is_no_tree_and_changes_nothing(tree):
+    """Before any work: shapes, parents, token ids, and more tokens than pages."""
+    dec = bookkeeper()
+    a, b = dec.open(), dec.open()
+    dec.forward({a: [1] * 20})
+    before = copy.deepcopy((dec._free, dec._seqs))
+    with pytest.raises((ValueError, RuntimeError)):
+        dec.verify({b: ([3], [-1]), a: tree})
+    with pytest.raises(ValueError):
+        dec.verify({})
+    assert (dec._free, dec._seqs) == before
+
+
+@pytest.mark.gpu
+def test_a_verification_that_failed_in_a_layer_can_be_repeated(monkeypatch):
+    from lowbit import paged
+    dec = paged.PagedDecoder(tiny(), num_pages=16, page_size=16, weights="f8")
+    sid = dec.open()
+    logits = dec.forward({sid: list(range(30))})
+    tree = ([int(logits[0].argmax()), 5, 6, 7], [-1, 0, 1, 0])
+    state = copy.deepcopy((dec._free, dec._seqs))
+    calls, attention = [], paged.tree_attention
+
+    def failing(*args, **kw):
+        calls.append(1)
+        if len(calls) == 2:
+            raise torch.OutOfMemoryError("no memory")
+        return attention(*args, **kw)
+
+    monkeypatch.setattr(paged, "tree_attention", failing)
+    with pytest.raises(torch.OutOfMemoryError):
+        dec.verify({sid: tree})
+    assert (dec._free, dec._seqs) == state
+    monkeypatch.undo()
+    other = paged.PagedDecoder(tiny(), num_pages=16, page_size=16, weights="f8")
+    oid = other.open()
+    other.forward({oid: list(range(30))})
+    assert dec.verify({sid: tree})[sid] == other.verify({oid: tree})[oid]
