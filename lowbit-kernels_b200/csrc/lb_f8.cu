@@ -541,14 +541,16 @@ struct F8Epilogue {
 template <typename T, int B>
 __device__ __forceinline__ void rows_epilogue(const F8Rows& p, const F8Epilogue& w) {
   const int lane = threadIdx.x & 31, quarter = (threadIdx.x >> 5) & 3, row = 32 * quarter + lane, rank = w.rank, h = w.half;
-  const uint32_t acc0 = w.tmem + ((uint32_t)(32 * quarter) << 16) + 128 * h;
   const T* bias = static_cast<const T*>(p.bias);
   T* y = static_cast<T*>(p.y);
   uint8_t* stage = w.staging;
   bool ok = true;   // of this lane: one that gave up waits no more, but stays with its warp's collective instructions
   bool ready = false;   // the next accumulator, as asked under the work on this one
-  int slot = 0;         // of the scales' ring
-  uint32_t u = 0;
+  // of the accumulator: its barrier, that of its release, its columns, the parity of its uses (the turns are 16 bytes and 256
+  // columns apart, both aligned to twice that); and the place of the stage's scale
+  uint32_t bar = w.acc_full + 8 * h, empty = w.acc_empty + 8 * h, acc = w.tmem + ((uint32_t)(32 * quarter) << 16) + 128 * h, parity = 0, odd = 0;
+  const uint32_t scale0 = w.scales + 4 * row, scale_end = scale0 + 512 * (p.stages + 2);
+  uint32_t scale = scale0;
   for (int tile = w.first; tile < p.tiles; tile += w.step) {
     const TilePlace at = tile_place(tile, p.tiles_m, p.tiles_n);
     const int m0 = at.m * 256 + 128 * rank, m = m0 + row, n0 = at.n * p.bn + w.n_off;
@@ -567,25 +569,27 @@ __device__ __forceinline__ void rows_epilogue(const F8Rows& p, const F8Epilogue&
     for (int i = 0; i < B; ++i)
 #pragma unroll
       for (int j = 0; j < 16; ++j) sum[i][j] = 0.f;
-    for (int c = 0; c < p.chunks; ++c, ++u) {
+    for (int c = 0; c < p.chunks; ++c) {
       if (c % 32 == 0) {
         ta = ta2, tb = tb2;
         fetch(c + 32);
       }
-      float fa = __shfl_sync(0xffffffffu, ta, c & 31), fb = __shfl_sync(0xffffffffu, tb, c & 31);
-      const int a = 2 * (u & 1) + h;
-      if (ok && !ready) ok = wait_warp(w.acc_full + 8 * a, (u >> 1) & 1, &g_f8_status);
+      float fa, fb;
+      if (ok && !ready) ok = wait_warp(bar, parity, &g_f8_status);
       __syncwarp();
       tc::fence_after();
-      const uint32_t acc = acc0 + 256 * (u & 1);
+      bar ^= 16;
+      parity ^= odd;
+      odd ^= 1;
       uint32_t v[16];
 #pragma unroll
       for (int i = 0; i < B; ++i) {
         tc::ld16(acc + 16 * i, v);
         if (i == 0) {
-          const float sv = lds_f32(w.scales + 512 * slot + 4 * row);   // there, since the MMAs have waited for it
-          ready = test_barrier(w.acc_full + 8 * (a ^ 2), (u + 1) >> 1 & 1);
-          fa *= sv, fb *= sv;
+          const float sv = lds_f32(scale);   // there, since the MMAs have waited for it
+          ready = test_barrier(bar, parity);
+          fa = __shfl_sync(0xffffffffu, ta, c & 31) * sv;
+          fb = __shfl_sync(0xffffffffu, tb, c & 31) * sv;
         }
         tc::wait_ld();
         const float f = i < turn ? fa : fb;
@@ -603,8 +607,11 @@ __device__ __forceinline__ void rows_epilogue(const F8Rows& p, const F8Epilogue&
       }
       tc::fence_before();
       __syncwarp();
-      tc::arrive_relaxed(w.acc_empty + 8 * a, lane == 0);
-      if (++slot == p.stages + 2) slot = 0;
+      tc::arrive_relaxed(empty, lane == 0);
+      empty ^= 16;
+      acc ^= 256;
+      scale += 512;
+      if (scale == scale_end) scale = scale0;
     }
     // two blocks at a time through the warp's [32 tokens][32 channels], 16-byte pieces permuted by the row
 #pragma unroll
