@@ -15,9 +15,10 @@ __device__ __forceinline__ int ldg_cg_i32(const int32_t* p) { return (int)ldg_cg
 __device__ __forceinline__ int64_t ldg_cg_i64(const int64_t* p) { return __ldcg(reinterpret_cast<const long long*>(p)); }
 
 // --------------------------------------------------------------------------------------------------------- plan
-// A few bytes of arithmetic a token behind two prefix sums over the sequences: latency. Every CTA of one cluster sums all
-// sequences by itself (they are read once more from L2, which costs less than handing the sums over), so that the only
-// meeting is one cluster barrier before the arrays that may lie over the inputs are written; then each writes its share.
+// A few bytes of arithmetic a token behind two prefix sums over the sequences: latency. Every CTA sums all sequences by
+// itself (they are read once more from L2, which costs less than handing the sums over), then writes its share, without
+// meeting the others. Where outputs lie over the inputs the grid is one cluster of up to eight CTAs, which meet once, before
+// the first of them writes.
 // With pages to give out, sequence s takes free_pages[count - 1 - first_s - j] as its page held_s + j, first_s being the
 // sum of what the sequences before it need: the pages a loop over the sequences would pop from a stack. A token's slot on a
 // new page is taken from that list too, not from the table that another CTA is writing.
@@ -51,17 +52,22 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warps, int64_t
   return __shfl_sync(0xffffffffu, all - before, warp) + sum - v;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, int C) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, int C, bool meet) {
   extern __shared__ int plan_smem[];
   __shared__ int64_t warps[32];
+  __shared__ unsigned long long taken;   // pages of the sequences that are served
   const PlanSmem m{plan_smem, plan_smem + p.seqs + 1, plan_smem + 2 * p.seqs + 1, plan_smem + 3 * p.seqs + 1};
   int* stage = plan_smem + 4 * p.seqs + 1;
-  const int rank = C > 1 ? (int)cluster_rank() : 0;
+  const int rank = blockIdx.x;
   pdl_launch_dependents();
   pdl_wait();
+  const bool whole = p.parents && C == 1 && p.tokens <= kPlanStage;   // all parents are staged, on their way under the sums
+  if (whole)
+    for (int t = threadIdx.x; t < p.tokens; t += blockDim.x) stage[t] = ldg_cg_i32(p.parents + t);
+  if (threadIdx.x == 0) taken = 0;
   const int64_t room = (int64_t)p.table_width * p.page_size;
   const int64_t count = p.free_count ? max(0, min(ldg_cg_i32(p.free_count), p.num_free)) : 0;
-  int64_t tokens = 0, pages = 0, taken = 0;   // of the sequences so far; pages of those that are served
+  int64_t tokens = 0, pages = 0;   // of the sequences so far
   for (int s0 = 0; s0 < p.seqs; s0 += blockDim.x) {
     const int s = s0 + threadIdx.x;
     const bool on = s < p.seqs;
@@ -80,8 +86,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, 
     const int64_t first = pages + block_scan(need, warps, &sum);
     pages += sum;
     served = served && (need == 0 || first + need <= count);
-    block_scan(served ? need : 0, warps, &sum);
-    taken += sum;
+    if (served && need > 0) atomicMax(&taken, (unsigned long long)(first + need));   // those that are served come first
     if (on) {
       m.cu[s] = (int)min(at, (int64_t)p.tokens);
       m.len[s] = (int)len;
@@ -90,8 +95,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, 
     }
   }
   if (threadIdx.x == 0) m.cu[p.seqs] = (int)min(tokens, (int64_t)p.tokens);
-  if (C > 1)
-    cluster_sync_all();   // every CTA has read what the outputs may lie over
+  if (meet)
+    cluster_sync_all();   // every CTA has read what the outputs lie over
   else
     __syncthreads();
 
@@ -110,7 +115,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, 
   }
   if (rank == 0 && threadIdx.x == 0) {
     p.cu_out[p.seqs] = m.cu[p.seqs];
-    if (p.free_count) p.free_count_out[0] = (int)(count - taken);
+    if (p.free_count) p.free_count_out[0] = (int)(count - (int64_t)taken);
   }
 
   // a token's sequence: the last that starts at or before it and has tokens
@@ -155,10 +160,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, 
   const int share = (p.tokens + C - 1) / C, t1 = min(p.tokens, (rank + 1) * share);
   for (int t0 = rank * share; t0 < t1; t0 += kPlanStage) {
     const int last = min(t1, t0 + kPlanStage);
-    const int from = t0 < end ? max(m.cu[find(t0)], t0 - kMaxTree) : t0;   // a tree's parents may lie that far before
-    __syncthreads();
-    for (int t = from + threadIdx.x; t < last; t += blockDim.x) stage[t - from] = ldg_cg_i32(p.parents + t);
-    __syncthreads();
+    const int from = whole ? 0 : t0 < end ? max(m.cu[find(t0)], t0 - kMaxTree) : t0;   // a tree's parents may lie that far before
+    if (!whole) {
+      __syncthreads();
+      for (int t = from + threadIdx.x; t < last; t += blockDim.x) stage[t - from] = ldg_cg_i32(p.parents + t);
+      __syncthreads();
+    }
     for (int u = threadIdx.x; u < (last - t0) * G; u += blockDim.x) {
       const int t = t0 + u / G, w = u % G;
       uint32_t bits = 0;
@@ -365,6 +372,8 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const __grid_cons
   pdl_launch_dependents();
   pdl_wait();
   const int s = blockIdx.y;
+  const int32_t* path = p.path + (int64_t)s * p.max_path;
+  int from = (int)threadIdx.x < p.max_path ? ldg_cg_i32(path + threadIdx.x) : 0;   // on its way together with the lengths
   const int n = max(0, ldg_cg_i32(p.cu_new + s + 1) - ldg_cg_i32(p.cu_new + s));
   const int start = ldg_cg_i32(p.seq_lens + s) - n, length = min(ldg_cg_i32(p.accepted + s), min(p.max_path, n));
   if (start < 0) {   // a sequence that the plan refused
@@ -388,7 +397,7 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const __grid_cons
     __syncthreads();
     const int d = d0 + threadIdx.x;
     if (d < length) {
-      const int from = ldg_cg_i32(p.path + (int64_t)s * p.max_path + d);
+      if (d0 > 0) from = ldg_cg_i32(path + d);
       int64_t place[2] = {-1, -1};
       bool ok = from >= d && from < n;
 #pragma unroll
@@ -440,24 +449,37 @@ cudaError_t launch_draft(Kern kern, dim3 grid, int threads, size_t smem, int clu
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
+// Two CTAs an SM where rows are few, with 4096 values each at least; three CTAs a row or so where they are many, so that the last
+// round is short (990 rows of 152064: 57.9 us with one, 52.6 with three; 250 rows of 151936: 13.5 with two, 21.5 with fourteen)
 int verify_splits(int64_t tokens, int64_t vocab) {
-  // two CTAs an SM, a split of 8192 values at least
-  const int64_t want = (2 * sm_count() + tokens - 1) / tokens;
-  return (int)max((int64_t)1, min(want, vocab / 8192));
+  const int64_t sms = sm_count(), few = min((2 * sms + tokens - 1) / tokens, vocab / 4096), many = min((16 * sms + tokens - 1) / tokens, vocab / 49152);
+  return (int)max((int64_t)1, max(few, many));
 }
 
 }  // namespace
 
 cudaError_t launch_plan(const PlanParams& p, bool pdl, cudaStream_t st) {
-  // one CTA while it has work for its threads alone
+  auto over = [](const void* out, int64_t n, const void* in, int64_t k) {
+    const auto a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(in);
+    return out && in && a < b + 4 * k && b < a + 4 * n;
+  };
+  bool meet = false;
+  const void* ins[3] = {p.seq_lens, p.new_lens, p.held};
+  for (const void* in : ins)
+    meet |= over(p.lens_out, p.seqs, in, p.seqs) || over(p.held_out, p.seqs, in, p.seqs) || over(p.cu_out, p.seqs + 1, in, p.seqs) ||
+            over(p.free_count_out, 1, in, p.seqs);
+  meet |= over(p.free_count_out, 1, p.free_count, 1) || over(p.lens_out, p.seqs, p.free_count, 1) || over(p.held_out, p.seqs, p.free_count, 1);
+  // one small CTA where that holds the work, else one for each 1024 threads' worth, to all SMs
   const int64_t work = (int64_t)p.tokens * (p.parents ? p.words : 1);
-  const int C = work <= 2 * kPlanThreads ? 1 : work <= 8 * kPlanThreads ? 4 : kPlanCluster;
+  int threads = work <= 512 && p.seqs <= 256 ? 256 : kPlanThreads, C = (int)max((int64_t)1, min((work + kPlanThreads - 1) / kPlanThreads, (int64_t)sm_count()));
+  if (meet) C = work <= 2 * kPlanThreads ? 1 : work <= 8 * kPlanThreads ? 4 : kPlanCluster;
+  meet = meet && C > 1;
   const size_t smem = (size_t)(4 * p.seqs + 1 + (p.parents ? kPlanStage + kMaxTree : 0)) * sizeof(int);
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
-  return launch_draft(plan_kernel, dim3(C), kPlanThreads, smem, C, pdl, st, p, C);
+  return launch_draft(plan_kernel, dim3(C), threads, smem, meet ? C : 1, pdl, st, p, C, meet);
 }
 
 size_t verify_workspace_bytes(int64_t tokens, int64_t vocab) { return (size_t)tokens * verify_splits(tokens, vocab) * sizeof(uint64_t); }
