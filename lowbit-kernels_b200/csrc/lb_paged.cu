@@ -311,6 +311,7 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
   // its token, -1 for none)
   uint4 q[NT][KI];
   int last[NT][2];
+  uint32_t bits[NT][2][2] = {};   // TREE: what those rows see of the first 64 new tokens, on its way with Q
   int first_masked = INT_MAX;   // blocks from this key on need the mask
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -327,6 +328,11 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
     for (int e = 0; e < 2; ++e) {
       const int rr = 8 * nt + 2 * t + e;
       last[nt][e] = rr < rows ? (TREE ? sp.t0 : sp.len - sp.n) + (row0 + rr) / grp : -1;
+      if (TREE && last[nt][e] >= 0) {
+        const int64_t at = (int64_t)last[nt][e] * p.mask_words;
+        bits[nt][e][0] = tree_word(p, at, 0);
+        bits[nt][e][1] = tree_word(p, at, 1);
+      }
     }
   }
   first_masked = TREE ? sp.len - sp.n : sp.len - sp.n + row0 / grp + 1;   // the first row's count of keys
@@ -408,9 +414,8 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
           const int key = 16 * u + g + (e >= 2 ? 8 : 0);
           if (TREE) {
             const int j = key - (sp.len - sp.n);   // of the new tokens; below 0 the context's
-            if (last[nt][e & 1] < 0 || key >= sp.len ||
-                !(tree_word(p, (int64_t)last[nt][e & 1] * p.mask_words, j >> 5) >> (j & 31) & 1u))
-              s[nt][e] = -INFINITY;
+            const uint32_t word = j < 0 ? 0xFFFFFFFFu : j & 32 ? bits[nt][e & 1][1] : bits[nt][e & 1][0];   // (64 rows, 64 new tokens at most)
+            if (last[nt][e & 1] < 0 || key >= sp.len || j >= 64 || !(word >> (j & 31) & 1u)) s[nt][e] = -INFINITY;
           } else if (key > last[nt][e & 1]) {
             s[nt][e] = -INFINITY;
           }
