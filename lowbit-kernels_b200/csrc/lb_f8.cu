@@ -107,7 +107,8 @@ __device__ __forceinline__ uint32_t amax_packed(const uint4& v) {
 }
 
 // Tokens: 16 lanes take a block of 128 values, a warp two tokens, a CTA 16 tokens x kQBlocks blocks, all of whose loads are
-// under way at once. The scales go to [block][token], as the product reads them, 16 tokens a run. Bound by memory.
+// under way at once. The scales go to [block][token], as the product reads them, 16 tokens a run. Bound by memory: 8192 tokens
+// of 18944 values 92 us, 5.0 TB/s (eight blocks a CTA: 5 us less there, 1.3 more for 61 tokens of 3584, which take 2.8).
 constexpr int kQBlocks = 4;
 enum Release { kAtEnd, kAfterWait, kAtEntry };   // when the quantization lets the next kernel start
 
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(256)
 // column a token) while the next stages' MMAs run into the other accumulators. The scale of a column is the same for all
 // lanes: each warp puts its columns' s t into shared memory, from where four come in one broadcast load; two columns take
 // one fp32-pair multiply-add.
-// CTAs are persistent over tiles, tokens innermost. Few tiles and long K: a cluster of S single CTAs splits K, each parks
+// CTAs are persistent over tiles, tokens innermost. Few tiles and long K: a cluster of S CTAs splits K, each parks
 // its fp32 partial tile in its idle ring, and all sum their share of the outputs through distributed shared memory in rank order.
 constexpr int kChunk = 128;               // bytes of K per stage
 constexpr int kWBytes = 128 * kChunk;
@@ -495,32 +496,37 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 // The same with the tokens as the A side: a pair of CTAs (cta_group::2) works on 256 tokens, 128 a CTA, and a tile of bn
 // channels, half of them loaded by each. A lane now holds a token, so that its scale is one register: s t of a block
 // multiplies all columns, without the loads from shared memory that a scale a column takes. A stage's MMAs go into two
-// accumulators of about bn / 2 channels, each with its own four epilogue warps a CTA, and there are two of each in the ring: what
-// counts is how long an accumulator may take from its last MMA until it is free again, and in halves that is three half
-// stages' MMAs (810 clocks at bn = 256), in one piece it would be one stage's (540).
+// accumulators of about bn / 2 channels, each with an MMA warp and four epilogue warps a CTA of its own, and there are two of
+// each in tensor memory, which then is full: what counts is how long one is away, from its first MMA until its last column has
+// been read and the issuing thread knows, which is 1700 clocks. So a barrier is asked ahead of the work before it (a completed
+// one costs 200 clocks all the same), accumulators are handed back without a release (one at the cluster's scope waits for
+// everything in flight: 1840 us a call where this takes 615), scales come with the stage by tensor copies.
+// Bound by that way round, 890 clocks a stage of 256 x 224 x 128 for 480 of MMAs: 8192 x 18944 x 3584 615 to 650 us with the
+// quantization, 720 under the power cap after a second of calls, 4096 x 4096 x 3584 82. Without the epilogue's multiply-adds a stage
+// takes 700 clocks. Left out: four accumulators of 64 channels (700 us), sixteen epilogue warps (646: five warps a scheduler
+// slow the MMA warps down), one MMA warp for both halves (738), tiles of 256 channels where 224 fill the last round (740).
 constexpr int kRowsSmem = 2 * 1024;       // a warp's staging: 32 tokens x 32 channels
-constexpr int kRowsThreads = 12 * 32;      // two loaders and two MMA warps (a warpgroup), 8 epilogue warps
+constexpr int kRowsThreads = 12 * 32;     // two loaders and two MMA warps (a warpgroup), 8 epilogue warps
 constexpr int kRowsStages = 6;
-constexpr int kRowsBarriers = 256;          // bytes, with tensor memory's address; the scales behind them are tensor copies
+constexpr int kRowsBarriers = 256;        // bytes, with tensor memory's address; the scales behind them are tensor copies
 constexpr int kRowsBarrierBytes = kRowsBarriers + (kRowsStages + 2) * 512 + 8 * kRowsSmem;
-static_assert((2 * kRowsStages + 8) * 8 + 16 <= kRowsBarriers, "barriers");
+static_assert((2 * kRowsStages + 8) * 8 + 16 <= kRowsBarriers && kRowsStages % 2 == 0, "barriers: the accumulators' aligned to 32 bytes");
 
 // the two accumulators' channels, multiples of 32 as a pair's MMA takes them
 __host__ __device__ constexpr int first_half(int bn) { return (bn + 63) / 64 * 32; }
 
 struct F8Rows {
-  const float* s;       // token scales [blocks][lds]
   const float* t;       // weight scales [rows of blocks][blocks]
   const void* bias;
   void* y;
-  int M, N, chunks, lds;
-  int bn, tiles_m, tiles_n, tiles, stages;
+  int M, N, chunks;
+  int bn, tiles_m, tiles_n, tiles, stages;   // bn a multiple of 32
   int park;             // byte offset behind the ring: barriers, staging
   bool vec;             // output rows take 16-byte stores
 };
 
-// The tile at a place of the order in which they are taken: n by n columns of tiles, so that what is worked on at one time is
-// about as many tokens as channels, and the fewest rows of both are read.
+// The tile at a place of the order in which they are taken: eight columns of tiles at a time, so that what is worked on at one
+// moment is about as many tokens as channels, and the fewest rows of both are read.
 constexpr int kTileColumns = 8;
 struct TilePlace {
   int m, n;
@@ -553,7 +559,7 @@ __device__ __forceinline__ void rows_epilogue(const F8Rows& p, const F8Epilogue&
   uint32_t scale = scale0;
   for (int tile = w.first; tile < p.tiles; tile += w.step) {
     const TilePlace at = tile_place(tile, p.tiles_m, p.tiles_n);
-    const int m0 = at.m * 256 + 128 * rank, m = m0 + row, n0 = at.n * p.bn + w.n_off;
+    const int m0 = at.m * 256 + 128 * rank, n0 = at.n * p.bn + w.n_off;
     // up to 128 channels: the blocks from `turn` on belong to the next row of the weights' scales
     const int nb = n0 / kBlock, most = (p.N - 1) / kBlock, turn = ((nb + 1) * kBlock - n0) / 16;
     const float* t0 = p.t + (int64_t)min(nb, most) * p.chunks;
@@ -668,7 +674,7 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
   uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 4);
   uint8_t* scales = ring + p.park + kRowsBarriers;   // [stages + 2][128 tokens]: the epilogue is up to two stages behind the MMAs
   uint8_t* staging = scales + (kRowsStages + 2) * 512;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
   const int h0 = first_half(p.bn), h1 = p.bn - h0;               // channels of the two accumulators
   const int stage_bytes = kWBytes + p.bn / 2 * kChunk, St = p.stages;
   const int rank = (int)cluster_rank(), first = blockIdx.x / 2, step = gridDim.x / 2;
@@ -807,8 +813,10 @@ __global__ void __launch_bounds__(kRowsThreads, 1)
 // A CTA takes 16 channels and all of K: mma.sync m16n8k32 with the weights' fragments loaded straight into registers, 64 bytes
 // of K (half a block) of a row per four lanes and 16-byte load (the order of k inside a fragment is free as long as both
 // operands share it); each piece's sums are scaled into fp32 registers. The first loads are issued at once, with `early` before
-// the wait on the previous kernel; the CTA quantizes the token rows while they are under way. Bound by the weights' way from
-// memory.
+// the wait on the previous kernel; the CTA quantizes the token rows while they are under way. On this
+// machine mma.sync takes e4m3 by converting it to fp16, which is a third of the instructions. One token, cold weights: 2048 x
+// 11008 7.8 us (6.2 without the quantization, in a graph with the call before still running 6.0), 1536 x 8960 4.7, 3584 x 3584
+// 5.2. (fp16 tokens in shared memory, converted once: 8.3, 5.4, 6.0; scales of the weights fetched with them: 8.5, 4.9, 5.5.)
 constexpr int kGemvRows = 8;
 
 struct F8Gemv {
@@ -1048,7 +1056,8 @@ cudaError_t cols_t(const CUtensorMap& wmap, const CUtensorMap& qmap, const F8Gem
                    g.splits, pdl, st, wmap, qmap, g);
 }
 
-// One to eight tokens, while their values are few: every CTA quantizes all of them.
+// One to eight tokens, while their values are few: every CTA quantizes all of them (measured against the two launches: 2048 x
+// 11008 M = 4 9.9 / 13.5 us, 1536 x 4608 M = 8 5.4 / 8.8).
 bool gemv_takes(int64_t M, int64_t K) { return M <= kGemvRows && M * K <= 12288; }
 
 template <typename T>
@@ -1101,7 +1110,7 @@ cudaError_t linear_t(const F8Params& p, bool pdl, cudaStream_t st) {
         !encode_tensor_map_2d(&smap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, s, (uint64_t)lds, (uint64_t)chunks, (uint64_t)lds * 4, 128, 1, CU_TENSOR_MAP_SWIZZLE_NONE))
       return cudaErrorInvalidValue;
     const int park = plan.stages * (kWBytes + plan.bn / 2 * kChunk);
-    const F8Rows g{s, p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, chunks, (int)lds, plan.bn, tiles_m, tiles / tiles_m, tiles, plan.stages, park, vec};
+    const F8Rows g{p.w_scales, p.bias, p.y, (int)p.M, (int)p.N, chunks, plan.bn, tiles_m, tiles / tiles_m, tiles, plan.stages, park, vec};
     static std::atomic<uint64_t> done{0};
     if ((e = allow_smem(f8_rows_kernel<T>, done)) != cudaSuccess) return e;
     return launch_f8(f8_rows_kernel<T>, dim3((unsigned)(2 * min(tiles, sms / 2))), kRowsThreads, (size_t)park + kRowsBarrierBytes + 1024, 2, pdl,
