@@ -293,8 +293,8 @@ LB_API int lb_f8_quantize_weight(const void* w, int dtype, int64_t n, int64_t k,
 /*
  * y[m, n] = sum over blocks b of K of s[m, b] t[n / 128, b] (sum over k in b of q[m, k] w[n, k]) + bias[n]: q and s are the rows of
  * x quantized by the same rule, a scale per row and 128 values. Sums in fp32, one rounding. A row whose block holds an
- * infinity or a NaN gives NaN; other rows do not see it. x and y fp16 or bf16 (y contiguous, rows of x ldx elements apart), bias
- * [N] of that type or NULL; w e4m3 [N, ldw] 16-byte aligned, ldw a multiple of 16, zeros from column K to the next
+ * infinity or a NaN gives NaN; other rows do not see it. x and y fp16 or bf16 (y contiguous, rows of x ldx elements apart, apart from each
+ * other), bias [N] of that type or NULL; w e4m3 [N, ldw] 16-byte aligned, ldw a multiple of 16, zeros from column K to the next
  * multiple of 16. workspace: lb_f8_workspace(m, n, k) bytes on the current device (0: none needed), 16-byte aligned, its
  * content undefined before and after; calls that can overlap need distinct ones.
  */
@@ -356,7 +356,8 @@ LB_API int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_h
  * lb_paged_attention for drafted tokens that form trees: sequence s's new token i sees its cached context, the keys
  * 0 .. seq_lens[s] - n - 1, and those of its n new tokens j whose bit is set, bit j % 32 of mask[(cu_new[s] + i) *
  * mask_words + j / 32] (itself among them only where its own bit is). Any pattern of bits will do; new tokens past 32 *
- * mask_words are seen by none. The rest, the workspace too, is as in lb_paged_attention.
+ * mask_words are seen by none. A V row with an infinity or NaN can make any new token of the same call NaN, whether it sees that
+ * row or not. The rest, the workspace too, is as in lb_paged_attention.
  */
 LB_API int lb_paged_tree_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
                                    const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride,
@@ -373,13 +374,15 @@ LB_API int lb_paged_tree_attention(const void* q, int64_t q_token_stride, int64_
  * held / free_pages / free_count (all or none): pages are given out too. A row of page_table int32 [seqs, table_width] holds
  * held[s] pages; what it lacks is taken from free_pages [num_free], of which the first *free_count are free, the last first,
  * by the sequences in their order, and written behind them; held_out and free_count_out say what there is then. The
- * outputs of both, and lens_out, may be the inputs themselves. Without them the table is complete as it is.
+ * outputs of both, and lens_out, may be the inputs themselves; no other output may lie over an input. Without them the table is
+ * complete as it is.
  * A sequence is refused where the rows, the table's width or the free pages do not suffice (from the first that lacks pages
- * on, all that need some): its lens_out is 0, its slots are -1, and it takes no pages; its rows stay its own.
+ * on, all that need some), or where it is a tree of more than 32 * words tokens: its lens_out is 0, its slots are -1, and it
+ * takes no pages; its rows stay its own.
  * parents int32 [tokens] or NULL: the new tokens of a sequence form a tree, parents[t] being the place of the token's parent
  * among them, an earlier one; anything else makes it a root. A token's position is then seq_lens[s] + its depth, and mask
  * uint32 [tokens, words] receives its ancestors and itself, as lb_paged_tree_attention takes them. words <= 32: trees of
- * up to 1024 tokens; ancestors further back than 32 * words tokens from a sequence's first are not recorded.
+ * up to 1024 tokens.
  */
 LB_API int lb_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int seqs, int32_t* page_table, int64_t table_stride,
                          int64_t table_width, int page_size, int64_t tokens, const int32_t* held, const int32_t* free_pages,
@@ -406,9 +409,9 @@ LB_API int lb_draft_verify(const void* logits, int dtype, int64_t ld, int64_t to
 
 /*
  * Moves the K and V rows of accepted tokens to where a sequence without the others has them, in `layers` (at most 128) caches of one
- * shape, type and page strides: row seq_lens[s] - n + path[s][d] to seq_lens[s] - n + d for d < accepted[s] (n the new tokens, seq_lens
+ * shape, type and page strides, none given twice: row seq_lens[s] - n + path[s][d] to seq_lens[s] - n + d for d < accepted[s] (n the new tokens, seq_lens
  * with them). A path rises; an entry outside the new tokens or below its place, or a row outside the cache, is left out and
- * sets lb_device_error() to 3. lens_out [seqs], not seq_lens itself, receives seq_lens[s] - n + accepted[s]; for a sequence
+ * sets lb_device_error() to 3. lens_out [seqs], over none of the inputs, receives seq_lens[s] - n + accepted[s]; for a sequence
  * that lb_paged_plan refused (seq_lens[s] < n) it is left as it is (keep) or 0, and nothing moves.
  */
 LB_API int lb_paged_compact(const lb_paged_cache* const* caches, int layers, const int32_t* page_table, int64_t table_stride,

@@ -1,9 +1,12 @@
 // The C ABI (include/lowbit_b200.h): argument validation with the reference's error contract
 // (csrc/w4_gemv.cu:312-325 and the per-op checks at :454-540), tiling heuristics, kernel launches.
+#include <algorithm>
 #include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
+#include <utility>
 
 #include "../../include/lowbit_b200.h"
 #include "lb_launch.h"
@@ -818,12 +821,24 @@ int lb_f8_linear(const void* x, int dtype, int64_t ldx, const void* w, int64_t l
     return fail(LB_ERR_ARGUMENT, "the workspace holds %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0),
                 (long long)need);
   if (!aligned16(workspace)) return fail(LB_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
+  const char *xa = static_cast<const char*>(x), *ya = static_cast<const char*>(y);
+  if (ya < xa + 2 * ((m - 1) * ldx + k) && xa < ya + 2 * m * n) return fail(LB_ERR_ARGUMENT, "x and y overlap");
   if ((rc = check_device())) return rc;
   const lb::F8Params p{x, ldx, dtype, w, ldw, w_scales, bias, y, m, n, k, workspace, g_opt[LB_OPT_EARLY_WEIGHTS].load() != 0};
   return launched(lb::launch_f8_linear(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)), "f8_linear");
 }
 
+}  // extern "C"
+
 // ------------------------------------------------------------------------------- a step of drafted tokens
+
+static bool misaligned(std::initializer_list<const void*> pointers, uintptr_t bytes) {
+  uintptr_t all = 0;
+  for (const void* p : pointers) all |= reinterpret_cast<uintptr_t>(p);
+  return all & (bytes - 1);
+}
+
+extern "C" {
 
 int lb_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int seqs, int32_t* page_table, int64_t table_stride,
                   int64_t table_width, int page_size, int64_t tokens, const int32_t* held, const int32_t* free_pages,
@@ -836,6 +851,9 @@ int lb_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int seqs, in
       (held == nullptr) != (held_out == nullptr) || (held == nullptr) != (free_count_out == nullptr))
     return fail(LB_ERR_ARGUMENT, "held, free_pages and free_count go together, with their outputs");
   if ((parents == nullptr) != (mask == nullptr)) return fail(LB_ERR_ARGUMENT, "parents and mask go together");
+  if (misaligned({seq_lens, new_lens, page_table, held, free_pages, free_count, parents, cu_out, lens_out, held_out, free_count_out, mask}, 4) ||
+      misaligned({positions, slots}, 8))
+    return fail(LB_ERR_ALIGNMENT, "arrays must be aligned to their type");
   if (seqs < 1 || seqs > lb::kMaxPlanSeqs) return fail(LB_ERR_ARGUMENT, "seqs=%d: 1 to %d", seqs, lb::kMaxPlanSeqs);
   if (tokens < 0 || tokens > INT32_MAX / 64) return fail(LB_ERR_ARGUMENT, "tokens=%lld out of range", (long long)tokens);
   if (page_size < 16 || page_size % 16 || page_size > 65536)
@@ -869,7 +887,8 @@ int lb_draft_verify(const void* logits, int dtype, int64_t ld, int64_t tokens, i
   if (ld < vocab) return fail(LB_ERR_ARGUMENT, "rows of the logits overlap: %lld values, stride %lld", (long long)vocab, (long long)ld);
   if (max_new < 1 || max_new > lb::kMaxTree) return fail(LB_ERR_ARGUMENT, "max_new=%lld: trees hold 1 to %d tokens", (long long)max_new, lb::kMaxTree);
   if (max_path < 1 || max_path > lb::kMaxTree) return fail(LB_ERR_ARGUMENT, "max_path=%lld: 1 to %d", (long long)max_path, lb::kMaxTree);
-  if (reinterpret_cast<uintptr_t>(logits) & (dtype == LB_F32 ? 3u : 1u)) return fail(LB_ERR_ALIGNMENT, "logits must be aligned to their type");
+  if (misaligned({logits}, dtype == LB_F32 ? 4 : 2) || misaligned({parents, cu_new, accepted, path}, 4) || misaligned({drafted, next, targets}, 8))
+    return fail(LB_ERR_ALIGNMENT, "arrays must be aligned to their type");
   const int64_t need = (int64_t)lb::verify_workspace_bytes(tokens, vocab);
   if (!workspace || workspace_bytes < need)
     return fail(LB_ERR_ARGUMENT, "the workspace holds %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0), (long long)need);
@@ -888,7 +907,11 @@ int lb_paged_compact(const lb_paged_cache* const* caches, int layers, const int3
   if (layers < 1 || layers > lb::kMaxLayers) return fail(LB_ERR_ARGUMENT, "layers=%d: 1 to %d caches a call", layers, lb::kMaxLayers);
   if (seqs < 1 || seqs > 65535) return fail(LB_ERR_ARGUMENT, "seqs=%d: 1 to 65535", seqs);
   if (max_path < 1 || max_path > lb::kMaxTree) return fail(LB_ERR_ARGUMENT, "max_path=%lld: 1 to %d", (long long)max_path, lb::kMaxTree);
-  if (lens_out == seq_lens) return fail(LB_ERR_ARGUMENT, "lens_out must not be seq_lens itself");
+  if (misaligned({page_table, seq_lens, cu_new, path, accepted, lens_out}, 4)) return fail(LB_ERR_ALIGNMENT, "int32 arrays must be 4-byte aligned");
+  // written by one CTA of a sequence while others read
+  for (const auto& in : {std::make_pair(seq_lens, (int64_t)seqs), std::make_pair(cu_new, (int64_t)seqs + 1), std::make_pair(accepted, (int64_t)seqs),
+                         std::make_pair(path, seqs * max_path)})
+    if (lens_out < in.first + in.second && in.first < lens_out + seqs) return fail(LB_ERR_ARGUMENT, "lens_out must not lie over an input (seq_lens itself, say)");
   lb::CompactParams p;
   for (int i = 0; i < layers; ++i) {
     const lb_paged_cache* c = caches[i];
@@ -901,6 +924,11 @@ int lb_paged_compact(const lb_paged_cache* const* caches, int layers, const int3
     p.k[i] = c->k;
     p.v[i] = c->v;
   }
+  const void* all[2 * lb::kMaxLayers];   // memory named twice would be moved twice
+  std::copy(p.k, p.k + layers, all);
+  std::copy(p.v, p.v + layers, all + layers);
+  std::sort(all, all + 2 * layers);
+  if (std::adjacent_find(all, all + 2 * layers) != all + 2 * layers) return fail(LB_ERR_ARGUMENT, "a cache is given twice");
   const lb_paged_cache* a = caches[0];
   if (table_width < 1 || table_stride < table_width || table_width * a->page_size > INT32_MAX)
     return fail(LB_ERR_ARGUMENT, "page table: at least one page a row, contexts below 2^31");

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, 
     int64_t sum;
     const int64_t at = tokens + block_scan(n, warps, &sum);
     tokens += sum;
-    bool served = (n == 0 || at + n <= p.tokens) && len + n <= room;
+    bool served = (n == 0 || at + n <= p.tokens) && len + n <= room && (!p.parents || n <= 32 * p.words);
     const int64_t need = p.held && served ? max((int64_t)0, (len + n + p.page_size - 1) / p.page_size - held) : 0;
     const int64_t first = pages + block_scan(need, warps, &sum);
     pages += sum;

@@ -872,7 +872,7 @@ __global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) f8_gemv_kerne
   // 16 lanes a block of 128 values; all rows' loads of a round under way together
   for (int j0 = 0; j0 < 16 * p.blocks; j0 += 32 * NW) {
     const int j = j0 + tid;
-    const float t128 = (j & 15) == 0 && j < 16 * p.blocks ? __ldg(tb + (j >> 4)) : 0.f;
+    const float t128 = (j & 15) == 0 && j < 16 * p.blocks ? __ldcg(tb + (j >> 4)) : 0.f;
     uint4 v[MR];
 #pragma unroll
     for (int m = 0; m < MR; ++m)

@@ -543,8 +543,8 @@ class F8Weight:
 def linear_f8(x, f8, bias=None, out=None):
     """x [M, K] fp16 or bf16 (rows any stride apart) -> [M, N] of the same type: each row quantized to e4m3 with a scale per 128
     values, the product with f8 (F8Weight) summed in fp32, each block times its two scales, `bias` ([N], x's type) added and
-    rounded once. `out`: an optional contiguous [M, N] tensor that receives the result. A serving operator: the result
-    carries no autograd graph."""
+    rounded once. `out`: an optional contiguous [M, N] tensor that receives the result, not over x. A serving operator:
+    the result carries no autograd graph."""
     tc = _tc if _tc is not None else _torchcall()
     if tc:
         y = tc.linear_f8(x, f8._q, f8._scales, out, bias)

@@ -151,7 +151,8 @@ def tree_attention(q, cache, page_table, seq_lens, cu_new, mask, max_new=None, m
     """`attention` for drafted tokens that form trees. mask int32 [T, words]: bit j % 32 of word j / 32 of a token's row says
     whether it sees its sequence's new token j (`plan` makes it from the tokens' parents; any pattern will do, a row of zeros
     too). Every new token sees the whole cached context, the keys before the sequence's new ones, which lie in the cache in the
-    order of the call; new tokens past 32 * words are seen by none. The rest is as in `attention`."""
+    order of the call; new tokens past 32 * words are seen by none. A V row with an infinity or NaN can make any new token of the same
+    call NaN, whether it sees that row or not. The rest is as in `attention`."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc:
         y = tc.paged_tree_attention(q, cache._ptr, cache._device, page_table, seq_lens, cu_new, mask, max_new, max_len, scale, out)
@@ -250,14 +251,14 @@ def plan(page_table, seq_lens, new_lens, page_size, tokens, held=None, free_page
     [S, W] holds held[s] pages, and what the new tokens need beyond them is taken from the first free_count[0] entries of free_pages,
     the last first, by the sequences in their order, and written into page_table behind them; the plan's held and free_count say
     what there is then. Without them page_table is complete as it is. A sequence is refused where `tokens`, W or the free pages do not suffice
-    (from the first that lacks pages on, all that need some): its seq_lens is 0, so that attention gives it zeros, its
-    slots are -1, and it takes no pages.
+    (from the first that lacks pages on, all that need some), or where it is a tree of more tokens than its mask has bits: its seq_lens is
+    0, so that attention gives it zeros, its slots are -1, and it takes no pages.
 
     parents int32 [tokens]: the new tokens of a sequence form a tree, parents[t] being the place among them of the token's
     parent, an earlier one; anything else makes it a root. Positions are then seq_lens + depth, and the plan's mask is what
     `tree_attention` takes, its rows ceil(max_new / 32) words (max_new bounds the new tokens of any sequence, 1024 at most; by default
     tokens). out: a Plan whose tensors receive the result (fixed addresses for a captured step); its held, free_count
-    and seq_lens may be the ones passed in."""
+    and seq_lens may be the ones passed in, nothing else of it may lie over an input."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc and out is None:
         got = tc.plan(page_table, seq_lens, new_lens, page_size, tokens, held, free_pages, free_count, parents, max_new)
@@ -311,8 +312,8 @@ def verify(logits, tokens, parents, cu_new, max_new=None, max_path=None):
     the index of each row's first largest value (a NaN counts as larger than all); and for each sequence the path that starts at its first new token, the
     last certain one, and goes on to the first later token that is a child of the one at hand and equals its target: how many tokens it has
     (accepted), their places among the new ones (path, -1 behind them) and the target after the last (next). A sequence
-    without new tokens gets 0 and -1. max_new bounds the new tokens of any sequence (1024 at most; by default T),
-    max_path the path (by default max_new). Rows past cu_new[S] are not looked at, their targets left unwritten."""
+    without new tokens gets 0 and -1. max_new bounds the new tokens of any sequence (1024 at most; by default T;
+    those past it are left out, their targets unwritten), max_path the path (by default max_new). Rows past cu_new[S] are not looked at, their targets left unwritten."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc:
         got = tc.verify(logits, tokens, parents, cu_new, max_new, max_path)
@@ -356,9 +357,9 @@ def verify(logits, tokens, parents, cu_new, max_new=None, max_path=None):
 
 def compact(caches, page_table, seq_lens, cu_new, path, accepted, out=None):
     """Moves the accepted tokens' K and V rows to where a sequence without the other drafts has them, in all of `caches` (a list of
-    up to 128 PagedCache of one layout, a layer each): with n new tokens of sequence s and seq_lens[s] tokens, them included, row
+    up to 128 PagedCache of one layout, a layer each, none twice): with n new tokens of sequence s and seq_lens[s] tokens, them included, row
     seq_lens[s] - n + path[s, d] goes to seq_lens[s] - n + d for d < accepted[s] (path int32 [S, D] and accepted int32 [S] as `verify`
-    gives them: a path rises). Returns seq_lens[s] - n + accepted[s], int32 [S] (`out`, when given: not seq_lens itself). For a
+    gives them: a path rises). Returns seq_lens[s] - n + accepted[s], int32 [S] (`out`, when given: over none of the inputs). For a
     sequence that `plan` refused this is 0, or what `out` held, and nothing moves: with the lengths before the plan as `out`
     it keeps its context. A path's entry outside the new tokens, below its own place, or on a page outside the cache is left
     out, and the device status becomes 3, as in `attention`."""

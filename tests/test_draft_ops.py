@@ -198,6 +198,32 @@ def test_plan_refuses_sequences_that_do_not_fit():
 
 
 @gpu
+def test_plan_refuses_trees_of_more_tokens_than_the_mask_has_bits():
+    """33 and 70 tokens where the rows have a word: what they need is not taken, and the others are as without them."""
+    _, paged = mods()
+    new, most = [5, 33, 32, 70, 1], 20
+    lens, table = [0, 16, 3, 0, 40], [[-1] * 8 for _ in new]
+    parents = [i - 1 for n in new for i in range(n)]
+    free, t = list(range(30)), i32(table)
+    got = paged.plan(t, i32(lens), i32(new), 16, sum(new), held=i32([0] * 5), free_pages=i32(free), free_count=i32([30]), parents=i32(parents), max_new=most)
+    served = [True, False, True, False, True]
+    assert got.cu_new.tolist() == [0, 5, 38, 70, 140, 141]
+    assert got.seq_lens.tolist() == [c + n if ok else 0 for c, n, ok in zip(lens, new, served)]
+    need = [-(-(c + n) // 16) if ok else 0 for c, n, ok in zip(lens, new, served)]
+    assert got.held.tolist() == need and got.free_count.item() == 30 - sum(need)
+    slots, cu = got.slots.tolist(), got.cu_new.tolist()
+    at = 30
+    for s, (c, n) in enumerate(zip(lens, new)):
+        pages = [free[at - 1 - j] for j in range(need[s])]
+        at -= need[s]
+        assert t[s].tolist() == pages + [-1] * (8 - need[s])
+        want = [pages[(c + i) // 16] * 16 + (c + i) % 16 for i in range(n)] if served[s] else [-1] * n
+        assert slots[cu[s]:cu[s + 1]] == want
+        if served[s]:
+            assert torch.equal(got.mask[cu[s]:cu[s + 1]], words_of(ancestors(parents[cu[s]:cu[s + 1]]), 1))
+
+
+@gpu
 def test_plan_over_its_own_inputs_captured_and_on_another_stream():
     """held, free_count and the lengths in place, step after step, as a captured loop has them."""
     _, paged = mods()
@@ -657,6 +683,14 @@ def test_compact_refusals():
             paged.compact(**{**ok, **kw})
     with pytest.raises(RuntimeError, match="itself"):
         paged.compact(**ok, out=ok["seq_lens"])
+    buf = i32([20, 0, 5, 2])   # the output over each other input
+    for kw in (dict(cu_new=buf[1:3], out=buf[2:3]), dict(accepted=buf[3:], out=buf[3:]), dict(path=buf[None, 1:3], out=buf[2:3])):
+        with pytest.raises(RuntimeError, match="over an input"):
+            paged.compact(**{**ok, **kw})
+    with pytest.raises(RuntimeError, match="twice"):
+        paged.compact(**{**ok, "caches": [caches[0], caches[1], caches[0]]})
+    paged.compact(**{**ok, "accepted": buf[3:]}, out=buf[:1])
+    assert buf.tolist() == [17, 0, 5, 2]
 
 
 # ------------------------------------------------------------------------------------------------------ linear_f8
@@ -879,6 +913,11 @@ def test_linear_f8_refusals():
                dict(out=torch.ones(3, 40, device="cuda", dtype=torch.bfloat16))):
         with pytest.raises(RuntimeError):
             ops.linear_f8(**{**dict(x=x, f8=f8), **kw})
+    square = ops.F8Weight.from_float(torch.ones(64, 64, device="cuda"))
+    with pytest.raises(RuntimeError, match="overlap"):   # other rows are still to be read when the first are written
+        ops.linear_f8(x, square, out=x)
+    both = torch.ones(7, 64, device="cuda", dtype=torch.float16)
+    ops.linear_f8(both[:3], square, out=both[3:6])
     q, s = ops.quantize_f8_gpu(w)
     for a, b in ((q.view(torch.uint8), s), (q, s.double()), (q, s[0]), (q[0], s), (q.cpu(), s), (q, s.cpu()), (q[:0], s)):
         with pytest.raises(RuntimeError):
@@ -999,6 +1038,43 @@ def test_no_warp_of_the_kernels_meets_others_on_the_way():
     for name in ("lb_f8.cu", "lb_draft.cu"):
         source = (_lib.LIB_PATH.parent.parent / "csrc" / name).read_text()
         assert "named_barrier(" not in source and "bar.sync" not in source and "barrier.sync" not in source, name
+
+
+def test_abi_refusals_of_what_lies_over_the_inputs_or_is_misaligned():
+    lib = _lib.load_library()
+
+    def cache(k, v):
+        return _lib.PagedCacheStruct(k=k, v=v, k_page_stride=2048, v_page_stride=2048, num_pages=4, dtype=0, nkv=2, hd=64, page_size=16)
+
+    def compact(caches, table=A, lens=A, cu=2 * A, path=3 * A, count=4 * A, out=5 * A, seqs=3, most=4):
+        ptrs = (ctypes.c_void_p * len(caches))(*[ctypes.addressof(c) for c in caches])
+        return lib.lb_paged_compact(ptrs, len(caches), table, 3, 3, lens, cu, path, count, seqs, most, out, 0, None)
+
+    one = [cache(A, 2 * A)]
+    for out in (A, A + 8, A - 8, 2 * A + 12, 2 * A - 8, 3 * A + 44, 4 * A + 4):
+        assert compact(one, out=out) == 1 and "over an input" in message(lib), out
+    for caches in ([cache(A, A)], one + [cache(3 * A, A)], [cache(i * A, (i + 40) * A) for i in range(1, 30)] + [cache(7 * A, 90 * A)]):
+        assert compact(caches) == 1 and "twice" in message(lib)
+    for kw in (dict(table=A + 2), dict(lens=A + 1), dict(cu=2 * A + 2), dict(path=A + 2), dict(count=A + 2), dict(out=5 * A + 2)):
+        assert compact(one, **kw) == 2, kw
+
+    def plan(lens=A, new=A, table=A, cu=A, pos=A, slots=A, parents=A, mask=A):
+        return lib.lb_paged_plan(lens, new, 2, table, 4, 4, 16, 8, None, None, 0, None, parents, 1, cu, A, None, None, pos, slots, mask, None)
+
+    for kw in (dict(lens=A + 2), dict(new=A + 1), dict(table=A + 2), dict(cu=A + 2), dict(pos=A + 4), dict(slots=A + 4), dict(parents=A + 2), dict(mask=A + 2)):
+        assert plan(**kw) == 2, kw
+
+    def verify(drafted=A, parents=A, cu=A, acc=A, path=A, after=A, targets=A):
+        return lib.lb_draft_verify(A, 0, 100, 4, 100, drafted, parents, cu, 1, 4, 4, acc, path, after, targets, A, 1 << 30, None)
+
+    for kw in (dict(drafted=A + 4), dict(parents=A + 2), dict(cu=A + 2), dict(acc=A + 2), dict(path=A + 2), dict(after=A + 4), dict(targets=A + 4)):
+        assert verify(**kw) == 2, kw
+
+    def linear(x, y, m=3, n=8, k=64, ldx=64):
+        return lib.lb_f8_linear(x, 0, ldx, A, 64, A, None, y, m, n, k, A, 1 << 40, None)
+
+    for x, y in ((A, A), (A, A + 2 * (2 * 64 + 63)), (A + 2 * 23, A)):
+        assert linear(x, y) == 1 and "overlap" in message(lib), (x, y)
 
 
 def test_f8_abi_refusals():
