@@ -357,8 +357,11 @@ LB_API int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_h
  * 0 .. seq_lens[s] - n - 1, and those of its n new tokens j whose bit is set, bit j % 32 of mask[(cu_new[s] + i) *
  * mask_words + j / 32] (itself among them only where its own bit is). Any pattern of bits will do; new tokens past 32 *
  * mask_words are seen by none. A V row with an infinity or NaN can make any new token of the same call NaN, whether it sees that
- * row or not. The rest, the workspace too, is as in lb_paged_attention.
+ * row or not. The rest is as in lb_paged_attention; workspace:
+ * lb_paged_tree_attention_workspace(...) bytes.
  */
+LB_API int64_t lb_paged_tree_attention_workspace(int64_t tokens, int nh, const lb_paged_cache* cache, int64_t table_width,
+                                                 int seqs, int64_t max_new, int64_t max_len);
 LB_API int lb_paged_tree_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
                                    const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride,
                                    int64_t table_width, const int32_t* seq_lens, const int32_t* cu_new, int seqs,

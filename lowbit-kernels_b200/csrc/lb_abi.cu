@@ -702,17 +702,17 @@ int lb_paged_norm_rope_append(const void* qkv, int64_t ld, int64_t tokens, int n
                   "paged_norm_rope_append");
 }
 
-int64_t lb_paged_attention_workspace(int64_t tokens, int nh, const lb_paged_cache* cache, int64_t table_width, int seqs,
-                                     int64_t max_new, int64_t max_len) {
+}  // extern "C"
+
+static int64_t attend_workspace(int64_t tokens, int nh, const lb_paged_cache* cache, int64_t table_width, int seqs,
+                                int64_t max_new, int64_t max_len, bool tree) {
   if (!cache || tokens < 1 || nh < 1 || cache->nkv < 1 || nh % cache->nkv || table_width < 1 || seqs < 1 || max_new < 1 ||
       max_len < 1)
     return 0;
   const int64_t width = table_width * cache->page_size;
-  return (int64_t)lb::paged_attention_workspace(seqs, nh, cache->nkv, cache->hd, max_new < tokens ? max_new : tokens,
-                                                max_len < width ? max_len : width);
+  return (int64_t)lb::paged_attention_workspace(tokens, seqs, nh, cache->nkv, cache->hd, max_new < tokens ? max_new : tokens,
+                                                max_len < width ? max_len : width, tree);
 }
-
-}  // extern "C"
 
 // both forms of the attention over the cache; mask: a tree's, or null
 static int attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
@@ -733,7 +733,7 @@ static int attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, 
   if (q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_token_stride < (int64_t)nh * cache->hd)
     return fail(LB_ERR_ARGUMENT, "q and out strides must be multiples of 8 elements");
   if (!aligned16(q) || !aligned16(out)) return fail(LB_ERR_ALIGNMENT, "q and out must be 16-byte aligned");
-  const int64_t need = lb_paged_attention_workspace(tokens, nh, cache, table_width, seqs, max_new, max_len);
+  const int64_t need = attend_workspace(tokens, nh, cache, table_width, seqs, max_new, max_len, mask != nullptr);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(LB_ERR_ARGUMENT, "the workspace holds %lld bytes, %lld are needed", (long long)(workspace ? workspace_bytes : 0),
                 (long long)need);
@@ -750,6 +750,16 @@ static int attend(const void* q, int64_t q_token_stride, int64_t q_head_stride, 
 }
 
 extern "C" {
+
+int64_t lb_paged_attention_workspace(int64_t tokens, int nh, const lb_paged_cache* cache, int64_t table_width, int seqs,
+                                     int64_t max_new, int64_t max_len) {
+  return attend_workspace(tokens, nh, cache, table_width, seqs, max_new, max_len, false);
+}
+
+int64_t lb_paged_tree_attention_workspace(int64_t tokens, int nh, const lb_paged_cache* cache, int64_t table_width, int seqs,
+                                          int64_t max_new, int64_t max_len) {
+  return attend_workspace(tokens, nh, cache, table_width, seqs, max_new, max_len, true);
+}
 
 int lb_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens, int nh,
                        const lb_paged_cache* cache, const int32_t* page_table, int64_t table_stride, int64_t table_width,

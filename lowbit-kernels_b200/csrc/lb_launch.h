@@ -213,7 +213,7 @@ struct PagedAttnParams {
   const uint32_t* mask = nullptr;   // a tree's new tokens: [tokens, mask_words], bit j: the token sees its sequence's new token j
   int mask_words = 0;
 };
-size_t paged_attention_workspace(int64_t seqs, int nh, int nkv, int hd, int64_t max_new, int64_t max_len);
+size_t paged_attention_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int hd, int64_t max_new, int64_t max_len, bool tree);
 cudaError_t launch_paged_attention(const PagedAttnParams& p, bool pdl, cudaStream_t st);
 int paged_device_error();   // synchronizes
 void paged_clear_device_error();

@@ -559,55 +559,67 @@ __global__ void __launch_bounds__(32 * kFewWarps) attention_few_kernel(const Pag
   cluster_sync_all();   // no CTA leaves while another still reads its part
 }
 
-// Joins the Z <= 32 parts of each row: work_o [item rows][Z][HD], work_ml [item rows][Z][2]. A CTA takes a row; its
-// threads hold four dims of every 512 / HD-th part, all loads under way at once.
+// Joins the Z <= 32 parts of each row: work_o [item rows][Z][HD], work_ml [item rows][Z][2]. A CTA takes `per` rows: one, whose every
+// 512 / HD-th part its threads hold, four dims each, or, where a thread can hold all parts of a row, one for each group of
+// HD / 4 threads. All loads are under way at once.
 constexpr int kFewParts = 32;
+constexpr int join_groups(int HD) { return 512 / HD; }
 
-template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnParams p, int row_tiles, int Z) {
-  constexpr int kRows = 8 * NT, kGroups = 512 / HD, kHeld = kFewParts / kGroups;
+template <typename T, int HD, int kRows>   // kRows: of a row tile
+__global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnParams p, int row_tiles, int Z, int per) {
+  constexpr int kGroups = join_groups(HD), kHeld = kFewParts / kGroups;
   __shared__ float4 sums[kGroups][HD / 4];
   __shared__ float weights[kGroups];
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t work_row = blockIdx.x;
   const int group = threadIdx.x / (HD / 4), d = threadIdx.x % (HD / 4) * 4;
+  const bool whole = per > 1;
+  const int64_t work_row = whole ? (int64_t)blockIdx.x * kGroups + group : blockIdx.x;
+  const int first = whole ? 0 : group, step = whole ? 1 : kGroups;
   float2 ml[kHeld];
   float4 x[kHeld];
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
-    const int k = group + i * kGroups;
+    const int k = first + i * step;
     if (k < Z) {
       ml[i] = __ldcg(reinterpret_cast<const float2*>(p.work_ml + 2 * (work_row * Z + k)));
       x[i] = __ldcg(reinterpret_cast<const float4*>(p.work_o + (work_row * Z + k) * HD + d));
     }
   }
-  float mx = (threadIdx.x & 31) < Z ? __ldcg(p.work_ml + 2 * (work_row * Z + (threadIdx.x & 31))) : -INFINITY;
+  float mx = !whole && (threadIdx.x & 31) < Z ? __ldcg(p.work_ml + 2 * (work_row * Z + (threadIdx.x & 31))) : -INFINITY;
   int item = (int)(work_row / kRows);
   const int row = item % row_tiles * kRows + (int)(work_row % kRows);
   item /= row_tiles;
   const int kvh = item % p.nkv, seq = item / p.nkv, grp = p.nh / p.nkv;
   const SeqSpan sp = seq_span(p, seq);
   if (row >= sp.n * grp) return;
+  if (whole) {
 #pragma unroll
-  for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+    for (int i = 0; i < kHeld; ++i)
+      if (i < Z) mx = fmaxf(mx, ml[i].x);
+  } else {
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+  }
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kHeld; ++i)
-    if (group + i * kGroups < Z) {
+    if (first + i * step < Z) {
       const float c = ml[i].x == -INFINITY ? 0.f : exp2_fast(ml[i].x - mx);
       acc.x += c * x[i].x, acc.y += c * x[i].y, acc.z += c * x[i].z, acc.w += c * x[i].w;
       sum += c * ml[i].y;
     }
-  sums[group][d / 4] = acc;
-  if (d == 0) weights[group] = sum;
-  __syncthreads();
-  if (group) return;
-  for (int k = 1; k < kGroups; ++k) {
-    const float4 v = sums[k][d / 4];
-    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-    sum += weights[k];
+  if (!whole) {
+    sums[group][d / 4] = acc;
+    if (d == 0) weights[group] = sum;
+    __syncthreads();
+    if (group) return;
+    for (int k = 1; k < kGroups; ++k) {
+      const float4 v = sums[k][d / 4];
+      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+      sum += weights[k];
+    }
   }
   const float c = sum != 0.f ? 1.f / sum : 0.f;
   T* dst = static_cast<T*>(p.out) + (int64_t)(sp.t0 + row / grp) * p.out_token + (int64_t)(kvh * grp + row % grp) * HD + d;
@@ -633,7 +645,11 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const PagedAttnPara
 // fp32.
 // Few tiles: a cluster of C CTAs splits the keys; each parks O, maxima and sums in its idle ring and all join their share
 // of the rows through distributed shared memory, in one fixed order. (Pushing the parts to their owners instead: 33 us
-// where this takes 29.)
+// where this takes 29.) A few trees' contexts are split over more CTAs than a cluster has: their parts go through the workspace
+// to attention_join_kernel.
+// TREE: a row's thread fetches the words of its mask that a tile needs while the tile's scores are being made, shifts them to the
+// tile's keys and selects by their bits. 28/4 heads of 128: 32 trees of 25 tokens over up to 8192 74 us (3.4 TB/s: a tile of 256
+// rows holds 175, and contexts differ), 255 tokens over 32255 106 (1.1 PFLOP/s).
 // Bound by the softmax beside the MMAs: a step of 256 rows x 128 keys takes some 3100 clocks at hd 128, of which the MMAs
 // need 2048, and 2700 at hd 64 (1024), with two warps a scheduler issuing 40 % of the time. 28/4 heads of 128: 4096 new
 // tokens 117 us (1025 TFLOP/s), over 32768 1625 us (1110) in a first second of calls and 1760 (1025) once the power cap
@@ -698,6 +714,7 @@ struct ChunkParams {
   int piece;     // keys of one tensor copy
   int tiles;     // row tiles of the grid per key head
   int C;
+  int Z, row_tiles;   // TREE, Z > 1: CTAs that split the keys and leave their parts in the workspace; a sequence's row tiles there
 };
 
 // The grid's row tile x: its sequence (-1: past the last), the tile in it and the sequence's tokens. Tiles are counted
@@ -776,7 +793,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   float* row_l = row_m + kTileRows;
   const PagedAttnParams& p = cp.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int C = cp.C, rank = C > 1 ? (int)cluster_rank() : 0;
+  const int C = cp.C, Z = TREE ? cp.Z : 1, shares = C * Z;   // (one of them is 1)
+  const int rank = C > 1 ? (int)cluster_rank() : Z > 1 ? (int)blockIdx.x % Z : 0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < St; ++i) {
@@ -803,7 +821,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  const int grp = p.nh / p.nkv, item = blockIdx.x / C;
+  const int grp = p.nh / p.nkv, item = blockIdx.x / shares;
   const int kvh = item % p.nkv;
   const TilePlace at = find_tile(p, item / p.nkv, grp);
   const int seq = at.seq, row0 = at.tile * kTileRows;
@@ -814,7 +832,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     keys = max(0, TREE ? sp.len : min(sp.len, sp.len - sp.n + (row0 + rows - 1) / grp + 1));   // the last row's
   }
   const int key_tiles = (keys + kTileKeys - 1) / kTileKeys;
-  const int j0 = (int)((int64_t)key_tiles * rank / C), nt = (int)((int64_t)key_tiles * (rank + 1) / C) - j0;
+  const int j0 = (int)((int64_t)key_tiles * rank / shares), nt = (int)((int64_t)key_tiles * (rank + 1) / shares) - j0;
 
   // 128 x 56 + 256 x 224 registers are the launch's 384 x 168: a softmax thread holds its row's 128 scores. (The
   // warpgroups' paths do not meet again before the end: what follows a meeting has the fewer registers.)
@@ -1107,7 +1125,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       __syncwarp();
       tc::fence_after();
     }
-    if (C == 1) {
+    if (shares == 1) {
       if (seq >= 0) {
         // through the warp's rows of Q, which are done with, so that HD / 8 lanes store a row at a time
         const float c = l != 0.f ? 1.f / l : 0.f;
@@ -1161,6 +1179,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
     }
     __syncwarp();
+    if (TREE && Z > 1 && seq >= 0 && at.tile < cp.row_tiles) {   // (tiles past max_new have no place there)
+      // the warp's rows to the workspace, as attention_join_kernel reads them
+      constexpr int kPieces = HD / 4;
+      const int64_t work_row = (((int64_t)seq * p.nkv + kvh) * cp.row_tiles + at.tile) * kTileRows + 128 * t + 32 * quarter;
+      const int piece = lane % kPieces, warp_rows = min(32, rows - 128 * t - 32 * quarter);
+      if (on) *reinterpret_cast<float2*>(p.work_ml + 2 * ((work_row + lane) * Z + rank)) = nt > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+#pragma unroll 8
+      for (int rr = lane / kPieces; rr < warp_rows; rr += 32 / kPieces) {
+        const uint4 v = nt > 0 ? *reinterpret_cast<const uint4*>(ring + (128 * t + 32 * quarter + rr) * HD * 4 + ((piece ^ (rr & 7)) << 4)) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(p.work_o + ((work_row + rr) * Z + rank) * HD + 4 * piece) = v;
+      }
+    }
     if (C > 1) {
       cluster_sync_all();
       if (seq >= 0) {
@@ -1339,7 +1369,7 @@ cudaError_t few_t(PagedAttnParams p, const FewPlan& f, bool pdl, cudaStream_t st
   cfg.gridDim = dim3((unsigned)rows);
   cfg.blockDim = dim3(128);
   cfg.numAttrs = joined_attrs;
-  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, HD, NT>, (const PagedAttnParams)p, f.row_tiles, f.Z);
+  return cudaLaunchKernelEx(&cfg, attention_join_kernel<T, HD, 8 * NT>, (const PagedAttnParams)p, f.row_tiles, f.Z, 1);
 }
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
@@ -1363,7 +1393,8 @@ int chunk_resident(int C) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, attention_chunk_kernel<__half, HD, false>, &cfg) != cudaSuccess || n < 1) {
+    if (cudaFuncSetAttribute(attention_chunk_kernel<__half, HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkSmem<HD>::kTotal) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, attention_chunk_kernel<__half, HD, false>, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
       n = max(1, (sm_count() - 16) / C);
     }
@@ -1371,6 +1402,46 @@ int chunk_resident(int C) {
     known[dev & 63][C].store(v, std::memory_order_relaxed);
   }
   return v;
+}
+
+// How a chunk call is laid out: clusters of C CTAs that split the keys, or (trees) Z CTAs that do so through the workspace
+struct ChunkPlan {
+  int C, Z, row_tiles;
+  int64_t tiles;
+};
+ChunkPlan chunk_plan(int hd, int64_t tokens, int64_t seqs, int64_t grp, int nkv, int64_t max_new, int64_t max_len, bool tree) {
+  ChunkPlan f;
+  f.row_tiles = (int)((max_new * grp + kTileRows - 1) / kTileRows);
+  // every sequence's last tile may be partial
+  f.tiles = min(seqs * f.row_tiles, (tokens * grp + kTileRows - 1) / kTileRows + seqs);
+  const int64_t items = f.tiles * nkv, key_tiles = (max_len + kTileKeys - 1) / kTileKeys;
+  // The cluster that costs least: rounds of CTAs times their key tiles (1.4 us each, measured) and 6 us to start and end,
+  // 6 more to join a cluster (C = 1, 2, 3, 4: 300 tokens over 4096, 28/4 heads of 128 61, 44, 35, 49 us; 1000 over 1000,
+  // 16/2 heads 21, 24, 33, 32; 500 over 2000, 14/2 heads of 64 29, 23, 20, 17)
+  double least = 1e30;
+  f.C = f.Z = 1;
+  for (int C = 1; C <= kChunkCluster && (C == 1 || key_tiles >= 2 * C); ++C) {
+    const int64_t resident = C == 1 ? sm_count() : hd == 128 ? chunk_resident<128>(C) : chunk_resident<64>(C), rounds = (items + resident - 1) / resident;
+    const double ends = 6 + (C > 1 ? 6 : 0), steps = 1.4 * (double)((key_tiles + C - 1) / C);
+    double t = (double)rounds * (ends + steps);
+    // Trees of several sequences all start at the end of their contexts, and those differ: the longest one, or the work of contexts
+    // spread evenly up to it, over what can be resident (32 trees of 25 tokens, 28/4 heads: contexts spread to 8192, C = 1, 2, 3,
+    // 4: 121, 74, 89, 99 us, all of 8192 121, 135, 149, 156; 64 of 16 to 4000 87, 104, 135, 157; 8 of 61 to 6000, 16/2 heads 98,
+    // 63, 46, 37)
+    if (tree && seqs > 1) t = max(ends + steps, (double)items * (ends + 0.5 * steps * (seqs + 1) / seqs) / (double)resident);
+    if (t < least) least = t, f.C = C;
+  }
+  if (!tree) return f;
+  // Few trees over long contexts leave SMs idle where a cluster ends: Z CTAs an item, while all can be resident at once, with 9 us
+  // to start, end and join them and 0.5 for each 1000 rows joined (16/2 heads of 128, 64 tokens over 1000: 16.3 us in clusters,
+  // 13.9; over 4093 20.7, 15.6; over 32000 70, 29; 28/4, 64 over 32000 72, 41, 255 over 32255 124, 106; 2 of 61 over 6000 28.1,
+  // 24.4; 255 over 500 15.3, 17.6 if they were split)
+  const int64_t all = seqs * f.row_tiles * nkv;
+  for (int Z = 2; Z <= kFewParts && all * Z <= sm_count() && key_tiles >= 2 * Z; ++Z) {
+    const double t = 9 + 0.0005 * (double)(all * kTileRows) + 1.4 * (double)((key_tiles + Z - 1) / Z);
+    if (t < least) least = t, f.C = 1, f.Z = Z;
+  }
+  return f;
 }
 
 template <typename T, int HD, bool TREE>
@@ -1391,25 +1462,14 @@ cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   cp.a = p;
   cp.piece = gcd(p.page_size, kTileKeys);
   const int64_t grp = p.nh / p.nkv;
-  // every sequence's last tile may be partial
-  cp.tiles = (int)min(p.seqs * ((p.max_new * grp + kTileRows - 1) / kTileRows), (p.tokens * grp + kTileRows - 1) / kTileRows + p.seqs);
-  const int64_t items = (int64_t)cp.tiles * p.nkv, key_tiles = (p.max_len + kTileKeys - 1) / kTileKeys;
-  // The cluster that costs least: rounds of CTAs times their key tiles (1.4 us each, measured) and 6 us to start and end,
-  // 6 more to join a cluster (C = 1, 2, 3, 4: 300 tokens over 4096, 28/4 heads of 128 61, 44, 35, 49 us; 1000 over 1000,
-  // 16/2 heads 21, 24, 33, 32; 500 over 2000, 14/2 heads of 64 29, 23, 20, 17)
-  double least = 1e30;
-  cp.C = 1;
-  for (int C = 1; C <= kChunkCluster && (C == 1 || key_tiles >= 2 * C); ++C) {
-    const int64_t resident = C == 1 ? sm_count() : chunk_resident<HD>(C), rounds = (items + resident - 1) / resident;
-    const double ends = 6 + (C > 1 ? 6 : 0), steps = 1.4 * (double)((key_tiles + C - 1) / C);
-    double t = (double)rounds * (ends + steps);
-    // Trees of several sequences all start at the end of their contexts, and those differ: the longest one, or the work of contexts
-    // spread evenly up to it, over what can be resident (32 trees of 25 tokens, 28/4 heads: contexts spread to 8192, C = 1, 2, 3,
-    // 4: 121, 74, 89, 99 us, all of 8192 121, 135, 149, 156; 64 of 16 to 4000 87, 104, 135, 157; 8 of 61 to 6000, 16/2 heads 98,
-    // 63, 46, 37)
-    if (TREE && p.seqs > 1) t = max(ends + steps, (double)items * (ends + 0.5 * steps * (p.seqs + 1) / p.seqs) / (double)resident);
-    if (t < least) least = t, cp.C = C;
-  }
+  const ChunkPlan f = chunk_plan(HD, p.tokens, p.seqs, grp, p.nkv, p.max_new, p.max_len, TREE);
+  const int64_t items = f.tiles * p.nkv, work_rows = f.Z > 1 ? (int64_t)p.seqs * f.row_tiles * p.nkv * kTileRows : 0;
+  cp.tiles = (int)f.tiles;
+  cp.C = f.C;
+  cp.Z = f.Z;
+  cp.row_tiles = f.row_tiles;
+  cp.a.work_ml = static_cast<float*>(p.workspace);
+  cp.a.work_o = cp.a.work_ml + 2 * work_rows * f.Z;
   CUtensorMap kmap, vmap;
   const CUtensorMapDataType type = Elem<T>::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const uint64_t extent[3] = {(uint64_t)HD, (uint64_t)p.nkv * p.page_size, (uint64_t)p.num_pages};
@@ -1419,7 +1479,7 @@ cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
       !encode_tensor_map_3d(&vmap, type, p.v, extent, vs, box, CU_TENSOR_MAP_SWIZZLE_128B))
     return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(items * cp.C));
+  cfg.gridDim = dim3((unsigned)(items * f.C * f.Z));
   cfg.blockDim = dim3(kChunkThreads);
   cfg.dynamicSmemBytes = L::kTotal;
   cfg.stream = st;
@@ -1428,14 +1488,25 @@ cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
-  if (cp.C > 1) {
+  const int joined_attrs = cfg.numAttrs;
+  if (f.C > 1) {
     attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[cfg.numAttrs].val.clusterDim.x = cp.C;
+    attr[cfg.numAttrs].val.clusterDim.x = f.C;
     attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
   }
   cfg.attrs = attr;
-  return cudaLaunchKernelEx(&cfg, kern, kmap, vmap, cp);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, kmap, vmap, cp);
+  if constexpr (TREE) {
+    if (e != cudaSuccess || f.Z == 1) return e;
+    const int per = f.Z <= kFewParts / join_groups(HD) ? join_groups(HD) : 1;
+    cfg.gridDim = dim3((unsigned)(work_rows / per));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = joined_attrs;
+    e = cudaLaunchKernelEx(&cfg, attention_join_kernel<T, HD, kTileRows>, (const PagedAttnParams)cp.a, f.row_tiles, f.Z, per);
+  }
+  return e;
 }
 
 template <typename T, bool TREE>
@@ -1460,9 +1531,13 @@ cudaError_t launch_paged_append(const void* qkv, int64_t ld, int64_t tokens, int
   return c.dtype == 0 ? append_t<__half>(p, pdl, st) : append_t<__nv_bfloat16>(p, pdl, st);
 }
 
-size_t paged_attention_workspace(int64_t seqs, int nh, int nkv, int hd, int64_t max_new, int64_t max_len) {
+size_t paged_attention_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int hd, int64_t max_new, int64_t max_len, bool tree) {
   const int64_t rows = max_new * (nh / nkv);
-  if (rows > kFewRows) return 0;
+  if (rows > kFewRows) {
+    if (!tree) return 0;
+    const ChunkPlan f = chunk_plan(hd, tokens, seqs, nh / nkv, nkv, max_new, max_len, true);
+    return f.Z == 1 ? 0 : (size_t)(seqs * f.row_tiles * nkv * kTileRows * f.Z * (2 + hd)) * sizeof(float);
+  }
   const FewPlan f = few_plan(rows, seqs, nkv, hd, max_len);
   if (f.Z == 1) return 0;
   return (size_t)((2 * f.items * 8 * f.nt * f.Z + 3) / 4 * 4 + f.items * 8 * f.nt * f.Z * hd) * sizeof(float);

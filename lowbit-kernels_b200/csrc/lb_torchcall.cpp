@@ -306,7 +306,7 @@ PyObject* attend(PyObject* const* args) {
   }
   at::Tensor y;
   if (!heads_out(args[more + 3], dev, *q, t, nh, c->hd, &y)) Py_RETURN_NONE;
-  const int64_t need = lb_paged_attention_workspace(t, (int)nh, c, w, (int)s, bound[0], bound[1]);
+  const int64_t need = (TREE ? lb_paged_tree_attention_workspace : lb_paged_attention_workspace)(t, (int)nh, c, w, (int)s, bound[0], bound[1]);
   at::Tensor ws;
   if (need > 0) ws = at::empty({need}, q->options().dtype(at::kByte));
   const int64_t ts = t > 1 ? q->stride(0) : 0, hs = nh > 1 ? q->stride(1) : 0, table_stride = s > 1 ? table->stride(0) : w;

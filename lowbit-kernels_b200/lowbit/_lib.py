@@ -54,6 +54,7 @@ SIGNATURES = {
     "lb_w8_linear": ([_P, _I, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P], _I),
     "lb_paged_norm_rope_append": ([_P, _I64, _I64, _I, _P, _P, ctypes.c_float, _P, _I, _P, _P, _P, _P, _P], _I),
     "lb_paged_attention_workspace": ([_I64, _I, _P, _I64, _I, _I64, _I64], _I64),
+    "lb_paged_tree_attention_workspace": ([_I64, _I, _P, _I64, _I, _I64, _I64], _I64),
     "lb_paged_attention": ([_P, _I64, _I64, _I64, _I, _P, _P, _I64, _I64, _P, _P, _I, _I64, _I64, ctypes.c_float, _P,
                             _I64, _P, _I64, _P], _I),
     "lb_f8_quantize_weight": ([_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P], _I),

@@ -196,7 +196,8 @@ def _attend(q, cache, page_table, seq_lens, cu_new, mask, max_new, max_len, scal
         return out
     e = ops.ext()
     with _Device(q.device):
-        need = e.lib.lb_paged_attention_workspace(t, nh, cache._ptr, width, s, max_new, max_len)
+        space = e.lib.lb_paged_attention_workspace if mask is None else e.lib.lb_paged_tree_attention_workspace
+        need = space(t, nh, cache._ptr, width, s, max_new, max_len)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         head = (q.data_ptr(), t_stride, h_stride, t, nh, cache._ptr, page_table.data_ptr(),
                 page_table.stride(0) if s > 1 else width, width, lens, cu, s)

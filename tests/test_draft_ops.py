@@ -376,6 +376,27 @@ def test_tree_attention_split_contexts_and_ragged_batches(dtype, nh, nkv, hd):
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("new,ctx,nh,nkv,hd", [([64], [5000], 16, 2, 128), ([200], [9001], 14, 2, 64), ([61, 10, 0, 5], [6000, 12, 70, 0], 16, 2, 128), ([33], [1000], 8, 2, 64),
+                                               ([255], [20001], 28, 4, 128), ([1000], [1000], 2, 2, 128), ([70, 3], [3, 3000], 4, 4, 64)])
+def test_tree_attention_contexts_split_through_the_workspace(dtype, new, ctx, nh, nkv, hd):
+    """More CTAs a context than a cluster has; parts without keys, rows that see nothing in any or in all of them."""
+    ops, paged = mods()
+    for kind in ("tree", "any", "none"):
+        q, cache, table, lens, cu, mask, y = run_tree(21, new, ctx, nh, nkv, hd, 16, dtype, kind, max_new=max(new), max_len=max(ctx))
+        t, w = q.shape[0], table.shape[1]
+        assert ops.ext().lib.lb_paged_tree_attention_workspace(t, nh, cache._ptr, w, len(new), max(new), max(ctx)) > 0
+        graph, out = torch.cuda.CUDAGraph(), torch.full_like(y, 5.0)
+        with torch.cuda.graph(graph):
+            paged.tree_attention(q, cache, table, lens, cu, mask, max_new=max(new), max_len=max(ctx), out=out)
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, y)
+    assert status() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,ctx", [(3, 40), (8, 300), (60, 300), (200, 900)])
 def test_tree_attention_of_a_chain_is_attention(dtype, n, ctx):
     """A chain's mask is the causal one: the same values to the roundings of two orders of the sums."""
