@@ -17,11 +17,12 @@
 //   paged_tree_attention(q, cache_ptr, device, page_table, seq_lens, cu_new, mask, max_new, max_len, scale, out) -> Tensor | None
 //   plan(page_table, seq_lens, new_lens, page_size, tokens, held, free_pages, free_count, parents, max_new) -> tuple | None
 //   verify(logits, tokens, parents, cu_new, max_new, max_path) -> tuple | None
-//   compact(cache_ptrs, device, page_table, seq_lens, cu_new, path, accepted, out) -> Tensor | None
+//   compact(caches, PagedCache, page_table, seq_lens, cu_new, path, accepted, out) -> Tensor | None
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/TensorImpl.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -349,6 +350,26 @@ bool page_table_of(const at::Tensor* t) {
          t->stride(1) == 1 && (t->size(0) == 1 || t->stride(0) >= t->size(1));
 }
 
+// Several outputs from one allocation, each on a 64-byte boundary (seven of their own cost a call's host time 5 us more)
+class Outputs {
+ public:
+  static int64_t padded(int64_t bytes) { return (bytes + 63) / 64 * 64; }
+  Outputs(int64_t bytes, const at::Tensor& like) : base_(at::empty({bytes}, like.options().dtype(at::kByte))) {}
+  at::Tensor take(at::ScalarType type, at::IntArrayRef sizes) {
+    const auto meta = c10::scalarTypeToTypeMeta(type);
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base_.storage()), base_.key_set(), meta);
+    impl->set_storage_offset(at_ / (int64_t)meta.itemsize());
+    impl->set_sizes_contiguous(sizes);
+    at_ += padded(impl->numel() * (int64_t)meta.itemsize());
+    return at::Tensor(std::move(impl));
+  }
+  void* rest() { return static_cast<uint8_t*>(base_.data_ptr()) + at_; }
+
+ private:
+  at::Tensor base_;
+  int64_t at_ = 0;
+};
+
 PyObject* plan(PyObject* const* args) {
   if (!THPVariable_Check(args[0])) Py_RETURN_NONE;
   const at::Tensor& table = THPVariable_Unpack(args[0]);
@@ -379,11 +400,14 @@ PyObject* plan(PyObject* const* args) {
     if (most < 1 || most > 1024) Py_RETURN_NONE;
     words = (most + 31) / 32;
   }
-  const auto ints = lens->options(), longs = lens->options().dtype(at::kLong);
-  at::Tensor cu = at::empty({s + 1}, ints), after = at::empty({s}, ints), pos = at::empty({tokens}, longs), slots = at::empty({tokens}, longs);
+  Outputs outs(Outputs::padded(4 * (s + 1)) + Outputs::padded(4 * s) + 2 * Outputs::padded(8 * tokens) +
+                   (paging ? Outputs::padded(4 * s) + Outputs::padded(4) : 0) + (parents ? Outputs::padded(4 * tokens * words) : 0),
+               *lens);
+  at::Tensor cu = outs.take(at::kInt, {s + 1}), after = outs.take(at::kInt, {s}), pos = outs.take(at::kLong, {tokens}),
+             slots = outs.take(at::kLong, {tokens});
   at::Tensor held_out, count_out, mask;
-  if (paging) held_out = at::empty({s}, ints), count_out = at::empty({1}, ints);
-  if (parents) mask = at::empty({tokens, words}, ints);
+  if (paging) held_out = outs.take(at::kInt, {s}), count_out = outs.take(at::kInt, {1});
+  if (parents) mask = outs.take(at::kInt, {tokens, words});
   const int rc = lb_paged_plan(lens->data_ptr<int32_t>(), fresh->data_ptr<int32_t>(), (int)s, table.data_ptr<int32_t>(),
                                s > 1 ? table.stride(0) : w, w, (int)page, tokens, paging ? held->data_ptr<int32_t>() : nullptr,
                                paging ? list->data_ptr<int32_t>() : nullptr, paging ? list->numel() : 0,
@@ -413,29 +437,40 @@ PyObject* verify(PyObject* const* args) {
   if (args[5] != Py_None && !to_ints(args + 5, bound + 1, 1)) return nullptr;
   if (bound[0] < 1 || bound[0] > 1024 || bound[1] < 1 || bound[1] > 1024) Py_RETURN_NONE;
   const int64_t s = cu->numel() - 1, need = lb_draft_verify_workspace(t, vocab);
-  const auto ints = cu->options(), longs = tokens->options();
-  at::Tensor accepted = at::empty({s}, ints), path = at::empty({s, bound[1]}, ints), next = at::empty({s}, longs), targets = at::empty({t}, longs);
-  at::Tensor ws = at::empty({need}, cu->options().dtype(at::kByte));
+  Outputs outs(Outputs::padded(4 * s) + Outputs::padded(4 * s * bound[1]) + Outputs::padded(8 * s) + Outputs::padded(8 * t) + need, *cu);
+  at::Tensor accepted = outs.take(at::kInt, {s}), path = outs.take(at::kInt, {s, bound[1]}), next = outs.take(at::kLong, {s}),
+             targets = outs.take(at::kLong, {t});
   const int rc = lb_draft_verify(x.data_ptr(), type == at::kHalf ? LB_F16 : type == at::kBFloat16 ? LB_BF16 : LB_F32, ld, t, vocab,
                                  tokens->data_ptr<int64_t>(), parents->data_ptr<int32_t>(), cu->data_ptr<int32_t>(), (int)s, bound[0], bound[1],
                                  accepted.data_ptr<int32_t>(), path.data_ptr<int32_t>(), next.data_ptr<int64_t>(), targets.data_ptr<int64_t>(),
-                                 ws.data_ptr(), need, stream_of(dev));
+                                 outs.rest(), need, stream_of(dev));
   return rc ? refused(rc) : tuple_of({&accepted, &path, &next, &targets});
 }
 
 PyObject* compact(PyObject* const* args) {
-  if (!PyList_Check(args[0])) Py_RETURN_NONE;
-  const Py_ssize_t layers = PyList_GET_SIZE(args[0]);
+  static PyObject* const name = PyUnicode_InternFromString("_place");
+  const bool list = PyList_Check(args[0]);
+  if (!list && !PyTuple_Check(args[0])) Py_RETURN_NONE;
+  const Py_ssize_t layers = list ? PyList_GET_SIZE(args[0]) : PyTuple_GET_SIZE(args[0]);
   if (layers < 1 || layers > 128) Py_RETURN_NONE;
   const lb_paged_cache* caches[128];
+  long long dev = -1;
   for (Py_ssize_t i = 0; i < layers; ++i) {
-    long long v;
-    PyObject* const one = PyList_GET_ITEM(args[0], i);
-    if (!to_ints(&one, &v, 1)) return nullptr;
-    caches[i] = reinterpret_cast<const lb_paged_cache*>(static_cast<uintptr_t>(v));
+    PyObject* const one = list ? PyList_GET_ITEM(args[0], i) : PyTuple_GET_ITEM(args[0], i);
+    if (reinterpret_cast<PyObject*>(Py_TYPE(one)) != args[1]) Py_RETURN_NONE;
+    PyObject* const place = PyObject_GetAttr(one, name);   // (address, device)
+    if (!place) return nullptr;
+    PyObject* const* v = PyTuple_Check(place) && PyTuple_GET_SIZE(place) == 2 ? &PyTuple_GET_ITEM(place, 0) : nullptr;
+    long long at[2] = {0, -1};
+    const bool ok = v && to_ints(v, at, 2);
+    Py_DECREF(place);
+    if (!ok || (i > 0 && at[1] != dev)) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    dev = at[1];
+    caches[i] = reinterpret_cast<const lb_paged_cache*>(static_cast<uintptr_t>(at[0]));
   }
-  long long dev;
-  if (!to_ints(args + 1, &dev, 1)) return nullptr;
   const at::Tensor *table = tensor_on(args[2], dev), *lens = tensor_on(args[3], dev), *cu = tensor_on(args[4], dev), *path = tensor_on(args[5], dev),
                    *accepted = tensor_on(args[6], dev);
   if (!page_table_of(table) || c10::cuda::current_device() != dev) Py_RETURN_NONE;
@@ -488,7 +523,7 @@ PyMethodDef methods[] = {
     {"verify", fastcall<verify, 6>(), METH_FASTCALL,
      "verify(logits, tokens, parents, cu_new, max_new, max_path) -> tuple, or None for the checked path"},
     {"compact", fastcall<compact, 8>(), METH_FASTCALL,
-     "compact(cache_ptrs, device, page_table, seq_lens, cu_new, path, accepted, out) -> Tensor, or None for the checked path"},
+     "compact(caches, PagedCache, page_table, seq_lens, cu_new, path, accepted, out) -> Tensor, or None for the checked path"},
     {"paged_attention", fastcall<attend<false>, 10>(), METH_FASTCALL,
      "paged_attention(q, cache_ptr, device, page_table, seq_lens, cu_new, max_new, max_len, scale, out) -> Tensor, or "
      "None for the checked path"},

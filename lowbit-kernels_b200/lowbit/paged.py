@@ -61,6 +61,7 @@ class PagedCache:
         self._struct = PagedCacheStruct(k.data_ptr(), v.data_ptr(), k.stride(0) if pages > 1 else block,
                                         v.stride(0) if pages > 1 else block, pages, DTYPE_IDS[k.dtype], nkv, hd, page_size)
         self._ptr = ctypes.addressof(self._struct)
+        self._place = self._ptr, self._device
 
     @property
     def k(self):
@@ -364,17 +365,17 @@ def compact(caches, page_table, seq_lens, cu_new, path, accepted, out=None):
     sequence that `plan` refused this is 0, or what `out` held, and nothing moves: with the lengths before the plan as `out`
     it keeps its context. A path's entry outside the new tokens, below its own place, or on a page outside the cache is left
     out, and the device status becomes 3, as in `attention`."""
+    tc = ops._tc if ops._tc is not None else ops._torchcall()
+    if tc:
+        got = tc.compact(caches, PagedCache, page_table, seq_lens, cu_new, path, accepted, out)
+        if got is not None:
+            return got
     caches = list(caches)
     if not caches or not all(isinstance(c, PagedCache) for c in caches):
         raise RuntimeError("caches must be a list of PagedCache")
     cache = caches[0]
     if any(c._device != cache._device for c in caches):
         raise RuntimeError("the caches must be on one GPU")
-    tc = ops._tc if ops._tc is not None else ops._torchcall()
-    if tc:
-        got = tc.compact([c._ptr for c in caches], cache._device, page_table, seq_lens, cu_new, path, accepted, out)
-        if got is not None:
-            return got
     s, width, stride = _page_table(page_table)
     if page_table.get_device() != cache._device:
         raise RuntimeError(f"page_table must be on the cache's GPU, {cache.k.device}")

@@ -258,6 +258,26 @@ def test_plan_over_its_own_inputs_captured_and_on_another_stream():
 
 
 @gpu
+@pytest.mark.parametrize("inference", [False, True])
+def test_outputs_of_plan_and_verify_do_not_share_values(inference):
+    """Filled one after another, each keeps its own; sizes that end off every boundary; inside inference mode too."""
+    _, paged = mods()
+    rng = random.Random(8)
+    c = plan_case(rng, 7, 40, 16, "tree", spare_tokens=3)
+    with torch.inference_mode(inference):
+        got = run_plan(c)
+        x = randn(gen(1), 13, 1001, dtype=torch.float16)
+        ok = paged.verify(x, i64([0] * 13), i32([-1] + list(range(12))), i32([0, 5, 13]), max_path=3)
+        for outs in (got, ok):
+            for i, t in enumerate(outs):
+                assert t.is_contiguous() and not t.requires_grad and t.is_inference() == inference
+                t.fill_(100 + i)
+            torch.cuda.synchronize()
+            assert all((t == 100 + i).all() for i, t in enumerate(outs))
+            assert [t.clone().numel() for t in outs] == [t.numel() for t in outs]
+
+
+@gpu
 def test_plan_refusals():
     _, paged = mods()
     table, v = torch.zeros(3, 4, dtype=torch.int32, device="cuda"), i32([1, 2, 3])
