@@ -15,7 +15,8 @@ __device__ __forceinline__ int ldg_cg_i32(const int32_t* p) { return (int)ldg_cg
 __device__ __forceinline__ int64_t ldg_cg_i64(const int64_t* p) { return __ldcg(reinterpret_cast<const long long*>(p)); }
 
 // --------------------------------------------------------------------------------------------------------- plan
-// A few bytes of arithmetic a token behind two prefix sums over the sequences: latency. Every CTA sums all sequences by
+// A few bytes of arithmetic a token behind two prefix sums over the sequences: latency. 16 trees of up to 31 tokens 6.1 us, 48
+// prompts of up to 2048 tokens 6.4 (11.3 with eight CTAs at most, which met on the way), in a graph. Every CTA sums all sequences by
 // itself (they are read once more from L2, which costs less than handing the sums over), then writes its share, without
 // meeting the others. Where outputs lie over the inputs the grid is one cluster of up to eight CTAs, which meet once, before
 // the first of them writes.
@@ -193,8 +194,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p, 
 // ------------------------------------------------------------------------------------------------------- verify
 // First each row's argmax, `splits` CTAs a row: bound by the logits' way from memory, so the loop takes only the maximum
 // of kArgVecs 16-byte vectors a thread (packed, NaN above all) and remembers the first such group that exceeded what was
-// there; the place inside the group is looked up once, by the threads whose maximum is the CTA's. 64 trees of up to 31 tokens
-// over 152064 values: see launch_verify.
+// there; the place inside the group is looked up once, by the threads whose maximum is the CTA's. 990 rows of 152064 bf16 values
+// 52.6 us with the walk behind it, 5.75 TB/s, 88 % of a copy's rate; 8 rows of 151936 6.0 (two launches, the second released while the first runs).
 constexpr int kArgThreads = 256;
 constexpr int kArgVecs = 4;
 
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(kArgThreads) argmax_kernel(const VerifyParams 
 }
 
 // A CTA a sequence: its rows' targets from the parts, then one warp walks down the tree, 32 tokens at a time looked over for
-// the next child.
+// the next child. Latency.
 constexpr int kWalkThreads = 128;
 
 __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyParams p, int splits) {
@@ -363,7 +364,8 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyParams p
 // Row ctx + path[d] of each layer's K and V moves to ctx + d. A path rises, so a source lies at or behind its destination and
 // behind every destination before it: a thread that takes one 16-byte column of a head through the whole path, eight rows
 // loaded before the first of them is stored, overwrites nothing that is still to be read. A CTA works for one sequence; its
-// first warps look up the rows once. Latency, then memory.
+// first warps look up the rows once. Latency -- lengths and path, table, rows, one after another: 25 tokens in 36 layers 2.6 us,
+// of 64 trees in 28 layers (12.6 MB read and written) 7.2, in a graph.
 constexpr int kMoveThreads = 128;    // (64 trees in 28 layers: 7.2 us; 256: 8.3, 64: 7.3)
 constexpr int kMoveBatch = 8;
 
