@@ -106,13 +106,12 @@ __device__ __forceinline__ uint32_t amax_packed(const uint4& v) {
   return __float_as_uint(Elem<T>::unpack(max(a & 0xFFFFu, a >> 16)).x);
 }
 
-// Tokens: 16 lanes take a block of 128 values, a warp two tokens, a CTA 16 tokens x kQBlocks blocks, all of whose loads are
+// Tokens: 16 lanes take a block of 128 values, a warp two tokens, a CTA 16 tokens x QB blocks, all of whose loads are
 // under way at once. The scales go to [block][token], as the product reads them, 16 tokens a run. Bound by memory: 8192 tokens
-// of 18944 values 92 us, 5.0 TB/s (eight blocks a CTA: 5 us less there, 1.3 more for 61 tokens of 3584, which take 2.8).
-constexpr int kQBlocks = 4;
+// of 18944 values 92 us, 5.0 TB/s.
 enum Release { kAtEnd, kAfterWait, kAtEntry };   // when the quantization lets the next kernel start
 
-template <typename T>
+template <typename T, int QB>
 __global__ void __launch_bounds__(256)
     f8_tokens_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, int ldq, float* __restrict__ s, int lds,
                      int M, int K, int release) {
@@ -120,17 +119,17 @@ __global__ void __launch_bounds__(256)
   pdl_wait();
   if (release == kAfterWait) pdl_launch_dependents();
   const int g = threadIdx.x >> 4, lane = threadIdx.x & 15;
-  const int m = blockIdx.y * 16 + g, b0 = blockIdx.x * kQBlocks;
+  const int m = blockIdx.y * 16 + g, b0 = blockIdx.x * QB;
   const bool aligned = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(ldx * sizeof(T))) & 15u) == 0;
   const T* row = x + (int64_t)min(m, M - 1) * ldx;
-  uint4 v[kQBlocks];
+  uint4 v[QB];
 #pragma unroll
-  for (int i = 0; i < kQBlocks; ++i) {
+  for (int i = 0; i < QB; ++i) {
     const int k = (b0 + i) * kBlock + 8 * lane;
     v[i] = k < K ? load8(row + k, K - k, aligned) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < kQBlocks; ++i) {
+  for (int i = 0; i < QB; ++i) {
     const int b = b0 + i, k = b * kBlock + 8 * lane;
     float f[8];
     floats8<T>(v[i], f);
@@ -397,7 +396,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
 #pragma unroll
       for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sum[i][j] = 0;
+        for (int j = 0; j < 8; ++j) sum[i][j] = 0;
       for (int c = 0; c < nc; ++c) {
         float* sc = scale + 64 * (c & 1);   // (a lane a chunk ahead writes the other half)
 #pragma unroll
@@ -1039,12 +1038,17 @@ F8Plan f8_plan(int64_t M, int64_t N, int chunks, int sms) {
   return best;
 }
 
+// Blocks a CTA: two where the product starts beside the quantization; behind it one, until that makes many CTAs (QB = 1, 2, 4:
+// 100 x 8960 x 1536 14.3, 13.8, 15.1 us; 61 x 18944 x 3584 24.1, 24.2, 24.7; 300 x 3584 x 4608 18.8, 19.3, 21.0; 1000 x 1536 x 2048 12.4,
+// 13.3, 15.1; 2048 x 18944 x 3584 169.6, 168.0, 167.6; 8192 x 18944 x 3584 670, 672, 636; 61 x 3584 x 4608 13.2 with each)
 template <typename T>
 cudaError_t tokens_t(const void* x, int64_t ldx, uint8_t* q, int64_t ldq, float* s, int64_t lds, int64_t M, int64_t K, int release,
                      bool pdl, cudaStream_t st) {
-  const dim3 grid((unsigned)((blocks_of(K) + kQBlocks - 1) / kQBlocks), (unsigned)((M + 15) / 16));
-  return launch_f8(f8_tokens_kernel<T>, grid, 256, 0, 1, pdl, st, static_cast<const T*>(x), ldx, q, (int)ldq, s, (int)lds, (int)M,
-                   (int)K, release);
+  const int64_t blocks = blocks_of(K), rows = (M + 15) / 16;
+  const int per = release != kAtEnd ? 2 : blocks * rows <= 8192 ? 1 : 4;
+  auto kern = per == 1 ? f8_tokens_kernel<T, 1> : per == 2 ? f8_tokens_kernel<T, 2> : f8_tokens_kernel<T, 4>;
+  return launch_f8(kern, dim3((unsigned)((blocks + per - 1) / per), (unsigned)rows), 256, 0, 1, pdl, st, static_cast<const T*>(x), ldx, q,
+                   (int)ldq, s, (int)lds, (int)M, (int)K, release);
 }
 
 template <typename T, int NB>
