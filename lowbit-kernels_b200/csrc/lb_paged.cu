@@ -5,6 +5,7 @@
 // context lies in the pages its row of the page table lists, page_size tokens each.
 #include <atomic>
 #include <climits>
+#include <cstring>
 
 #include "lb_launch.h"
 #include "lb_tc.cuh"
@@ -1315,6 +1316,7 @@ int few_resident(int C) {
 struct FewPlan {
   int nt, row_tiles, C, Z;
   int64_t items;
+  double time;   // the estimate, us
 };
 FewPlan few_plan(int64_t rows, int64_t seqs, int nkv, int hd, int64_t max_len) {
   FewPlan f;
@@ -1339,6 +1341,7 @@ FewPlan few_plan(int64_t rows, int64_t seqs, int nkv, int hd, int64_t max_len) {
       if (t < least) least = t, f.C = C, f.Z = Z;
     }
   }
+  f.time = least;
   return f;
 }
 
@@ -1408,6 +1411,7 @@ int chunk_resident(int C) {
 struct ChunkPlan {
   int C, Z, row_tiles;
   int64_t tiles;
+  double time;   // the estimate, us
 };
 ChunkPlan chunk_plan(int hd, int64_t tokens, int64_t seqs, int64_t grp, int nkv, int64_t max_new, int64_t max_len, bool tree) {
   ChunkPlan f;
@@ -1431,6 +1435,7 @@ ChunkPlan chunk_plan(int hd, int64_t tokens, int64_t seqs, int64_t grp, int nkv,
     if (tree && seqs > 1) t = max(ends + steps, (double)items * (ends + 0.5 * steps * (seqs + 1) / seqs) / (double)resident);
     if (t < least) least = t, f.C = C;
   }
+  f.time = least;
   if (!tree) return f;
   // Few trees over long contexts leave SMs idle where a cluster ends: Z CTAs an item, while all can be resident at once, with 9 us
   // to start, end and join them and 0.5 for each 1000 rows joined (16/2 heads of 128, 64 tokens over 1000: 16.3 us in clusters,
@@ -1441,7 +1446,42 @@ ChunkPlan chunk_plan(int hd, int64_t tokens, int64_t seqs, int64_t grp, int nkv,
     const double t = 9 + 0.0005 * (double)(all * kTileRows) + 1.4 * (double)((key_tiles + Z - 1) / Z);
     if (t < least) least = t, f.C = 1, f.Z = Z;
   }
+  f.time = least;
   return f;
+}
+
+// A tree call's plan, kept for calls of one shape that follow one another on a host thread. A tree has several row tiles of the
+// few-rows kernel, each of which reads the keys, where one tile of the chunk kernel may hold them all: whichever is estimated
+// to take less, with what the estimates miss -- contexts spread up to the longest, and row tiles that find each other's
+// keys in L2; for chunks a fifth, or more in several rounds of CTAs (few rows / chunks, 28/4 heads of 128: 8 tokens over 700 8.6,
+// 11.8 us, over 8000 21.6, 15.1; 4 over 8000 13.8, 15.1; 32 trees of 8 over up to 8192 124, 67, of 4 89, 72; 64 of 4 over up to 4000
+// 90, 75; 14/2 of 64: 32 of 8 over up to 4000 25.1, 27.6; a near miss: 96 of 3 over up to 3000 85, 102).
+struct TreePlan {
+  bool few;
+  FewPlan f;
+  ChunkPlan c;
+};
+const TreePlan& tree_plan(int hd, int64_t tokens, int64_t seqs, int64_t grp, int nkv, int64_t max_new, int64_t max_len) {
+  static thread_local struct {
+    int64_t key[8];
+    TreePlan plan;
+  } last = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int64_t key[8] = {hd, tokens, seqs, grp, nkv, max_new, max_len, dev + 1};
+  if (memcmp(key, last.key, sizeof(key)) != 0) {
+    TreePlan& t = last.plan;
+    const int64_t rows = max_new * grp;
+    t.c = chunk_plan(hd, tokens, seqs, grp, nkv, max_new, max_len, true);
+    t.few = rows <= kFewRows;
+    if (t.few) {
+      t.f = few_plan(rows, seqs, nkv, hd, max_len);
+      const double few = seqs == 1 ? t.f.time : 4 + 0.34 * t.f.time * (double)(seqs + 1) / (double)seqs;
+      t.few = few <= (t.c.C * t.c.Z == 1 && t.c.tiles * nkv > sm_count() ? 1.65 : 1.2) * t.c.time;
+    }
+    memcpy(last.key, key, sizeof(key));
+  }
+  return last.plan;
 }
 
 template <typename T, int HD, bool TREE>
@@ -1462,7 +1502,8 @@ cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   cp.a = p;
   cp.piece = gcd(p.page_size, kTileKeys);
   const int64_t grp = p.nh / p.nkv;
-  const ChunkPlan f = chunk_plan(HD, p.tokens, p.seqs, grp, p.nkv, p.max_new, p.max_len, TREE);
+  const ChunkPlan f = TREE ? tree_plan(HD, p.tokens, p.seqs, grp, p.nkv, p.max_new, p.max_len).c
+                           : chunk_plan(HD, p.tokens, p.seqs, grp, p.nkv, p.max_new, p.max_len, false);
   const int64_t items = f.tiles * p.nkv, work_rows = f.Z > 1 ? (int64_t)p.seqs * f.row_tiles * p.nkv * kTileRows : 0;
   cp.tiles = (int)f.tiles;
   cp.C = f.C;
@@ -1512,8 +1553,9 @@ cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
 template <typename T, bool TREE>
 cudaError_t attention_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   const int64_t most_rows = (int64_t)p.max_new * (p.nh / p.nkv);
-  if (most_rows <= kFewRows) {
-    const FewPlan f = few_plan(most_rows, p.seqs, p.nkv, p.hd, p.max_len);
+  const TreePlan* t = TREE ? &tree_plan(p.hd, p.tokens, p.seqs, p.nh / p.nkv, p.nkv, p.max_new, p.max_len) : nullptr;
+  if (t ? t->few : most_rows <= kFewRows) {
+    const FewPlan f = t ? t->f : few_plan(most_rows, p.seqs, p.nkv, p.hd, p.max_len);
     return p.hd == 128 ? (f.nt == 1 ? few_t<T, 128, 1, TREE>(p, f, pdl, st) : few_t<T, 128, 2, TREE>(p, f, pdl, st))
                        : (f.nt == 1 ? few_t<T, 64, 1, TREE>(p, f, pdl, st) : few_t<T, 64, 2, TREE>(p, f, pdl, st));
   }
@@ -1533,12 +1575,10 @@ cudaError_t launch_paged_append(const void* qkv, int64_t ld, int64_t tokens, int
 
 size_t paged_attention_workspace(int64_t tokens, int64_t seqs, int nh, int nkv, int hd, int64_t max_new, int64_t max_len, bool tree) {
   const int64_t rows = max_new * (nh / nkv);
-  if (rows > kFewRows) {
-    if (!tree) return 0;
-    const ChunkPlan f = chunk_plan(hd, tokens, seqs, nh / nkv, nkv, max_new, max_len, true);
-    return f.Z == 1 ? 0 : (size_t)(seqs * f.row_tiles * nkv * kTileRows * f.Z * (2 + hd)) * sizeof(float);
-  }
-  const FewPlan f = few_plan(rows, seqs, nkv, hd, max_len);
+  const TreePlan* t = tree ? &tree_plan(hd, tokens, seqs, nh / nkv, nkv, max_new, max_len) : nullptr;
+  if (t && !t->few) return t->c.Z == 1 ? 0 : (size_t)(seqs * t->c.row_tiles * nkv * kTileRows * t->c.Z * (2 + hd)) * sizeof(float);
+  if (rows > kFewRows) return 0;
+  const FewPlan f = t ? t->f : few_plan(rows, seqs, nkv, hd, max_len);
   if (f.Z == 1) return 0;
   return (size_t)((2 * f.items * 8 * f.nt * f.Z + 3) / 4 * 4 + f.items * 8 * f.nt * f.Z * hd) * sizeof(float);
 }

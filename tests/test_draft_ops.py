@@ -417,6 +417,22 @@ def test_tree_attention_contexts_split_through_the_workspace(dtype, new, ctx, nh
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nh,nkv,hd", [(28, 4, 128), (16, 2, 128), (14, 2, 64), (8, 8, 128)])
+def test_tree_attention_small_trees_whichever_kernel_takes_them(dtype, nh, nkv, hd):
+    """1 to 64 rows a key head, where contexts and batches decide between the kernels; single tokens and empty contexts among them."""
+    rng = random.Random(nh + hd)
+    for seqs, most, longest in ((1, 8, 9000), (1, 4, 9000), (24, 8, 3000), (24, 4, 700), (70, 3, 900), (40, 1, 2000), (5, 8, 200)):
+        new = [rng.choice((most, rng.randint(0, most))) for _ in range(seqs)]
+        ctx = [rng.choice((longest, rng.randint(n, longest), n)) for n in new]
+        new[0], ctx[0] = most, longest
+        if seqs > 2:
+            new[-1], ctx[-1] = 1, 0
+        for kind in ("tree", "any"):
+            run_tree(31, new, ctx, nh, nkv, hd, 16, dtype, kind, max_new=most, max_len=longest)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,ctx", [(3, 40), (8, 300), (60, 300), (200, 900)])
 def test_tree_attention_of_a_chain_is_attention(dtype, n, ctx):
     """A chain's mask is the causal one: the same values to the roundings of two orders of the sums."""
