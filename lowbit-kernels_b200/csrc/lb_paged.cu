@@ -768,7 +768,11 @@ __device__ __forceinline__ T* shfl_ptr(T* v, int lane) {
   return reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), lane));
 }
 
-template <typename T, int HD, bool TREE>
+// DUAL (trees at hd 128 whose rows fit half a row tile): both tiles hold the same rows and take turns at the key tiles, each with a
+// K and a V stage of its own; their sums are joined at the end (28/4 heads, 32 trees of 8 over up to 8192 67 -> 59 us, 64 of 16 over
+// up to 4000 88 -> 76, 8 of 16 over up to 16000 60 -> 52; 16/2, 8 over 32000 23.6 -> 19.1). A kernel of its own: decided inside, it
+// cost the others 7 %.
+template <typename T, int HD, bool TREE, bool DUAL = false>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     attention_chunk_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                            const ChunkParams cp) {
@@ -829,11 +833,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const SeqSpan sp = at.span;
   int rows = 0, keys = 0;
   if (seq >= 0) {
-    rows = min(kTileRows, sp.n * grp - row0);
+    rows = min(DUAL ? kTileRows / 2 : kTileRows, sp.n * grp - row0);   // (DUAL: more only where max_new is below the truth)
     keys = max(0, TREE ? sp.len : min(sp.len, sp.len - sp.n + (row0 + rows - 1) / grp + 1));   // the last row's
   }
   const int key_tiles = (keys + kTileKeys - 1) / kTileKeys;
   const int j0 = (int)((int64_t)key_tiles * rank / shares), nt = (int)((int64_t)key_tiles * (rank + 1) / shares) - j0;
+
+  constexpr bool dual = DUAL;
 
   // 128 x 56 + 256 x 224 registers are the launch's 384 x 168: a softmax thread holds its row's 128 scores. (The
   // warpgroups' paths do not meet again before the end: what follows a meeting has the fewer registers.)
@@ -954,7 +960,51 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
           return true;
         };
-        bool ok = wait(kQReady, 0) && wait(0, 0);
+        bool ok = wait(kQReady, 0);
+        if (dual) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (ok && t < nt) {
+              ok = wait(16 * t, 0);
+              tc::fence_after();
+              if (ok) {
+                qk(t, t, t, t);
+                tc::commit_at(bars + kEmpty + 16 * t);
+              }
+            }
+          for (int j = 0; 2 * j < nt && ok; ++j) {
+            asm volatile("" : "+r"(kd), "+r"(vd), "+r"(qd));
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!ok || 2 * j + t >= nt) break;
+              ok = wait(16 * t + 8, j & 1);
+              if (ok && 2 * j + t == nt - 1 && keys - (j0 + nt - 1) * kTileKeys < kTileKeys) {   // the third warp's turn
+                mbar_arrive(tail_go);
+                ok = wait(kVTail, 0);
+              }
+#pragma unroll
+              for (int part = 0; part < 2; ++part) {
+                if (ok) ok = wait(kPReady + 8 * (B * part + t), j & 1);
+                if (!ok) break;
+                tc::fence_after();
+#pragma unroll
+                for (int k = part ? 6 : 0; k < (part ? 8 : 6); ++k)
+                  tc::mma_f16_ts(tmem + kO + HD * t, tmem + 128 * t + 8 * k, vd + 2 * t * kStep + ((k * 2048) >> 4), kPV, j > 0 || k > 0);
+              }
+              if (!ok) break;
+              tc::commit_at(bars + kODone + 8 * t);
+              tc::commit_at(bars + kEmpty + 16 * t + 8);
+              if (2 * (j + 1) + t < nt) {
+                ok = wait(16 * t, (j + 1) & 1);
+                if (!ok) break;
+                tc::fence_after();
+                qk(t, t, t, t);
+                tc::commit_at(bars + kEmpty + 16 * t);
+              }
+            }
+          }
+        }
+        ok = ok && !dual && wait(0, 0);   // (the loop below is not for two tiles of the same rows)
         tc::fence_after();
         if (ok) {
           qk(0, 0, 0, 0);
@@ -993,18 +1043,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       __syncwarp();
     }
+    if (dual) cluster_sync_all();
     if (C > 1) {
       cluster_sync_all();
       cluster_sync_all();
     }
   } else {
     tc::regs_inc<224>();
-    const int t = (warp - 4) >> 2, quarter = warp & 3, r = 128 * t + 32 * quarter + lane, row = row0 + r;
+    const int t = (warp - 4) >> 2, quarter = warp & 3, r = 128 * t + 32 * quarter + lane, own = dual ? r & 127 : r, row = row0 + own;
+    const int turns = dual ? (nt + 1 - t) >> 1 : nt;   // key tiles of this row tile
     const uint32_t lane_base = tmem + ((uint32_t)(32 * quarter) << 16);
     const uint32_t to = lane_base + kO + HD * t;
     int job = t;                // modulo R
     uint32_t job_parity = 0;
-    const bool on = r < rows;
+    const bool on = own < rows;
     float m = -INFINITY, l = 0.f;
     const float scale = p.scale * 1.44269504088896340736f;
     const int last = on ? sp.len - sp.n + row / grp : -1;
@@ -1025,9 +1077,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (lane == 0) mbar_arrive(q_ready);
       const int first_last = TREE ? sp.len - sp.n - 1 : sp.len - sp.n + row0 / grp;   // the CTA's first row's last key
       bool ok = true;   // of this lane: one that gave up waits no more, but stays with its warp's collective instructions
-      for (int j = 0; j < nt; ++j) {
+      for (int j = 0; j < turns; ++j) {
         const uint32_t at = B == 2 ? t : job < B ? job : job - B, ts = lane_base + 128 * at;
-        const int k0 = (j0 + j) * kTileKeys;
+        const int k0 = (j0 + (dual ? 2 * j + t : j)) * kTileKeys;
         const bool masked = k0 + kTileKeys - 1 > first_last;
         uint32_t sees[4];   // TREE: a bit for each of the row's keys
         if (TREE && masked) {
@@ -1122,11 +1174,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         job += 2;
         if (job >= R) job -= R, job_parity ^= 1;
       }
-      wait_bounded(B == 2 ? &o_done[t] : &o_last[t], B == 2 ? (nt - 1) & 1 : 0, &g_paged_status);
+      if (turns > 0) wait_bounded(B == 2 ? &o_done[t] : &o_last[t], B == 2 ? (turns - 1) & 1 : 0, &g_paged_status);
       __syncwarp();
       tc::fence_after();
     }
-    if (shares == 1) {
+    if (shares == 1 && !dual) {
       if (seq >= 0) {
         // through the warp's rows of Q, which are done with, so that HD / 8 lanes store a row at a time
         const float c = l != 0.f ? 1.f / l : 0.f;
@@ -1160,13 +1212,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
     } else {
       // the second tile's last product is the last to read the ring
-      if (seq >= 0 && nt > 0) wait_bounded(B == 2 ? &o_done[1] : &o_last[1], B == 2 ? (nt - 1) & 1 : 0, &g_paged_status);
+      if (dual) {
+        for (int i = 0; i < 2; ++i)
+          if (i < nt) wait_bounded(&o_done[i], (((nt + 1 - i) >> 1) - 1) & 1, &g_paged_status);
+      } else if (seq >= 0 && nt > 0) {
+        wait_bounded(B == 2 ? &o_done[1] : &o_last[1], B == 2 ? (nt - 1) & 1 : 0, &g_paged_status);
+      }
       __syncwarp();
       tc::fence_after();
       // parked at ring + row * HD * 4, 16-byte pieces permuted by the row so that eight lanes' stores take all banks
-      row_m[r] = nt > 0 ? m : -INFINITY;
-      row_l[r] = nt > 0 ? l : 0.f;
-      if (seq >= 0 && nt > 0) {
+      row_m[r] = turns > 0 ? m : -INFINITY;
+      row_l[r] = turns > 0 ? l : 0.f;
+      if (seq >= 0 && turns > 0) {
 #pragma unroll
         for (int h = 0; h < HD / 32; ++h) {
           uint32_t o[32];
@@ -1180,12 +1237,43 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
     }
     __syncwarp();
-    if (TREE && Z > 1 && seq >= 0 && at.tile < cp.row_tiles) {   // (tiles past max_new have no place there)
+    if (dual) {
+      // the second tile's part joins the first's, HD / 4 lanes a row: for the cluster, the workspace or the output
+      cluster_sync_all();
+      const int64_t work_row = (((int64_t)seq * p.nkv + kvh) * cp.row_tiles + at.tile) * kTileRows;
+#pragma unroll 4
+      for (int q = warp - 4; q < rows; q += 8) {
+        const float m0 = row_m[q], m1 = row_m[q + 128], l0 = row_l[q], l1 = row_l[q + 128], mx = fmaxf(m0, m1);
+        const float c0 = l0 != 0.f ? exp2_fast(m0 - mx) : 0.f, c1 = l1 != 0.f ? exp2_fast(m1 - mx) : 0.f;
+        float4* const a = reinterpret_cast<float4*>(ring + q * HD * 4 + ((lane ^ (q & 7)) << 4));
+        const float4 x0 = *a, x1 = *reinterpret_cast<const float4*>(ring + (q + 128) * HD * 4 + ((lane ^ (q & 7)) << 4));
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+        if (l0 != 0.f) x.x = c0 * x0.x, x.y = c0 * x0.y, x.z = c0 * x0.z, x.w = c0 * x0.w, sum = c0 * l0;   // (a part without keys holds whatever its ring held)
+        if (l1 != 0.f) x.x += c1 * x1.x, x.y += c1 * x1.y, x.z += c1 * x1.z, x.w += c1 * x1.w, sum += c1 * l1;
+        if (Z > 1) {
+          const int64_t part = (work_row + q) * Z + rank;
+          if (at.tile < cp.row_tiles) {   // (tiles past max_new have no place there)
+            *reinterpret_cast<float4*>(p.work_o + part * HD + 4 * lane) = x;
+            if (lane == 0) *reinterpret_cast<float2*>(p.work_ml + 2 * part) = make_float2(mx, sum);
+          }
+        } else if (C == 1) {
+          const float c = sum != 0.f ? 1.f / sum : 0.f;
+          T* dst = static_cast<T*>(p.out) + (int64_t)(sp.t0 + (row0 + q) / grp) * p.out_token + ((int64_t)kvh * grp + (row0 + q) % grp) * HD + 4 * lane;
+          *reinterpret_cast<uint2*>(dst) = make_uint2(Elem<T>::pack(x.x * c, x.y * c), Elem<T>::pack(x.z * c, x.w * c));
+        } else {
+          *a = x;
+          __syncwarp();
+          if (lane == 0) row_m[q] = mx, row_l[q] = sum;
+        }
+      }
+    }
+    if (TREE && !dual && Z > 1 && seq >= 0 && at.tile < cp.row_tiles) {   // (tiles past max_new have no place there)
       // the warp's rows to the workspace, as attention_join_kernel reads them
       constexpr int kPieces = HD / 4;
       const int64_t work_row = (((int64_t)seq * p.nkv + kvh) * cp.row_tiles + at.tile) * kTileRows + 128 * t + 32 * quarter;
       const int piece = lane % kPieces, warp_rows = min(32, rows - 128 * t - 32 * quarter);
-      if (on) *reinterpret_cast<float2*>(p.work_ml + 2 * ((work_row + lane) * Z + rank)) = nt > 0 ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+      if (r < rows) *reinterpret_cast<float2*>(p.work_ml + 2 * ((work_row + lane) * Z + rank)) = make_float2(row_m[r], row_l[r]);
 #pragma unroll 8
       for (int rr = lane / kPieces; rr < warp_rows; rr += 32 / kPieces) {
         const uint4 v = nt > 0 ? *reinterpret_cast<const uint4*>(ring + (128 * t + 32 * quarter + rr) * HD * 4 + ((piece ^ (rr & 7)) << 4)) : make_uint4(0, 0, 0, 0);
@@ -1453,9 +1541,10 @@ ChunkPlan chunk_plan(int hd, int64_t tokens, int64_t seqs, int64_t grp, int nkv,
 // A tree call's plan, kept for calls of one shape that follow one another on a host thread. A tree has several row tiles of the
 // few-rows kernel, each of which reads the keys, where one tile of the chunk kernel may hold them all: whichever is estimated
 // to take less, with what the estimates miss -- contexts spread up to the longest, and row tiles that find each other's
-// keys in L2; for chunks a fifth, or more in several rounds of CTAs (few rows / chunks, 28/4 heads of 128: 8 tokens over 700 8.6,
-// 11.8 us, over 8000 21.6, 15.1; 4 over 8000 13.8, 15.1; 32 trees of 8 over up to 8192 124, 67, of 4 89, 72; 64 of 4 over up to 4000
-// 90, 75; 14/2 of 64: 32 of 8 over up to 4000 25.1, 27.6; a near miss: 96 of 3 over up to 3000 85, 102).
+// keys in L2; for chunks a fifth, or more in several rounds of CTAs (few rows / chunks, 28/4 heads of 128: 8 tokens over 700 8.5,
+// 11.6 us, over 8000 21.6, 14.1; 4 over 8000 14, 13.5; 32 trees of 8 over up to 8192 124, 59, of 4 89, 64; 64 of 4 over up to 4000
+// 90, 61; 128 of 4 over up to 1000 47, 63; 14/2 of 64: 32 of 8 over up to 4000 25.1, 27.6; near misses: 16/2, 64 of 2 over up to 8000
+// 76, 68, 4 of 4 over up to 16000 28, 22).
 struct TreePlan {
   bool few;
   FewPlan f;
@@ -1487,8 +1576,14 @@ const TreePlan& tree_plan(int hd, int64_t tokens, int64_t seqs, int64_t grp, int
 template <typename T, int HD, bool TREE>
 cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   using L = ChunkSmem<HD>;
-  auto kern = attention_chunk_kernel<T, HD, TREE>;
-  static std::atomic<uint64_t> done{0};
+  const int64_t grp = p.nh / p.nkv;
+  const ChunkPlan f = TREE ? tree_plan(HD, p.tokens, p.seqs, grp, p.nkv, p.max_new, p.max_len).c
+                           : chunk_plan(HD, p.tokens, p.seqs, grp, p.nkv, p.max_new, p.max_len, false);
+  // (not for one or two key tiles a CTA: 2 trees of 16 over up to 500, 16/2 heads 14.0 us, 15.4 with it)
+  const bool dual = TREE && HD == 128 && p.max_new * grp <= kTileRows / 2 && p.max_len > 2 * kTileKeys * f.C * f.Z;
+  auto kern = dual ? attention_chunk_kernel<T, HD, TREE, TREE && HD == 128> : attention_chunk_kernel<T, HD, TREE>;
+  static std::atomic<uint64_t> known[2];   // the kernel and its DUAL form
+  std::atomic<uint64_t>& done = known[dual];
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = 1ull << (dev & 63);
@@ -1501,9 +1596,6 @@ cudaError_t chunk_t(const PagedAttnParams& p, bool pdl, cudaStream_t st) {
   ChunkParams cp;
   cp.a = p;
   cp.piece = gcd(p.page_size, kTileKeys);
-  const int64_t grp = p.nh / p.nkv;
-  const ChunkPlan f = TREE ? tree_plan(HD, p.tokens, p.seqs, grp, p.nkv, p.max_new, p.max_len).c
-                           : chunk_plan(HD, p.tokens, p.seqs, grp, p.nkv, p.max_new, p.max_len, false);
   const int64_t items = f.tiles * p.nkv, work_rows = f.Z > 1 ? (int64_t)p.seqs * f.row_tiles * p.nkv * kTileRows : 0;
   cp.tiles = (int)f.tiles;
   cp.C = f.C;

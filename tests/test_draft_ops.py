@@ -417,6 +417,19 @@ def test_tree_attention_contexts_split_through_the_workspace(dtype, new, ctx, nh
 
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_tree_attention_up_to_128_rows_over_many_key_tiles(dtype):
+    """Odd and even counts of key tiles, from one CTA a context to clusters and the workspace; contexts and parts without keys, rows
+    that see nothing; 128 rows and one."""
+    rng = random.Random(3)
+    for nh, nkv, new, ctx in ((28, 4, [18] * 40, [rng.randint(18, 1100) for _ in range(40)]), (16, 2, [16, 3, 1, 0, 16, 16], [5000, 129, 0, 8, 640, 641]),
+                              (28, 4, [18], [12000]), (28, 4, [9], [129]), (8, 8, [128], [3000]), (8, 8, [100, 128, 1], [1281, 2305, 1153]),
+                              (32, 4, [16] * 70, [16 + 37 * i for i in range(70)]), (16, 2, [16] * 12, [16 + 700 * i for i in range(12)])):
+        for kind in ("tree", "any", "none"):
+            run_tree(41, new, ctx, nh, nkv, 128, 16, dtype, kind, max_new=max(new), max_len=max(ctx))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("nh,nkv,hd", [(28, 4, 128), (16, 2, 128), (14, 2, 64), (8, 8, 128)])
 def test_tree_attention_small_trees_whichever_kernel_takes_them(dtype, nh, nkv, hd):
     """1 to 64 rows a key head, where contexts and batches decide between the kernels; single tokens and empty contexts among them."""
