@@ -1029,6 +1029,37 @@ def test_the_operators_give_the_same_bits_under_every_launch_option(dtype):
 
 
 @gpu
+def test_offsets_past_32_bits():
+    """Pages, rows of logits and rows of tokens more than 2^31 elements from the first."""
+    ops, paged = mods()
+    # the attention and the move: pages 2^27 elements apart, the same bits as in a small cache
+    near, stride = make_caches(gen(2), 1, 20, 2, 16, 64, torch.bfloat16)[0], 1 << 27
+    room = torch.empty(19 * stride + 4096, dtype=torch.bfloat16, device="cuda")
+    k, v = (room[at:].as_strided((20, 2, 16, 64), (stride, 1024, 64, 1)) for at in (0, 2048))
+    k.copy_(near.k), v.copy_(near.v)
+    far = paged.PagedCache.from_tensors(k, v)
+    table, q = i32([list(range(19, -1, -1))]), randn(gen(3), 30, 8, 64, dtype=torch.bfloat16)
+    for new, ctx in ((5, 300), (30, 310)):
+        lens, cu, mask = i32([ctx]), i32([0, new]), words_of(ancestors(tree(random.Random(1), new)), 1)
+        a, b = (paged.tree_attention(q[:new], c, table, lens, cu, mask, max_new=new) for c in (near, far))
+        assert torch.equal(a, b)
+        path = i32([[0, 2, 4]])
+        a, b = (paged.compact([c], table, lens, cu, path, i32([3])) for c in (near, far))
+        assert torch.equal(a, b) and torch.equal(near.k, far.k) and torch.equal(near.v, far.v)
+    # rows 2^26 elements apart
+    x = room.as_strided((36, 1000), (1 << 26, 1))
+    x.copy_(randn(gen(4), 36, 1000, dtype=torch.bfloat16))
+    tokens, parents, cu = i64(x.argmax(1).tolist()), i32([-1] + list(range(35))), i32([0, 36])
+    for g, w in zip(paged.verify(x, tokens, parents, cu), paged.verify(x.contiguous(), tokens, parents, cu)):
+        assert torch.equal(g, w)
+    f8 = ops.F8Weight.from_float(randn(gen(5), 300, 1000, dtype=torch.bfloat16))
+    for m in (36, 8):
+        assert torch.equal(ops.linear_f8(x[36 - m:], f8), ops.linear_f8(x[36 - m:].contiguous(), f8))
+    assert torch.equal(ops.linear_f8(x[::5], f8), ops.linear_f8(x[::5].contiguous(), f8))
+    assert status() == 0
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_a_captured_step_of_drafted_tokens(dtype):
     """Plan, append, tree attention, acceptance and move as one graph over two layers, replayed step after step without the host
