@@ -415,7 +415,8 @@ LB_API int lb_draft_verify(const void* logits, int dtype, int64_t ld, int64_t to
  * shape, type and page strides, none given twice: row seq_lens[s] - n + path[s][d] to seq_lens[s] - n + d for d < accepted[s] (n the new tokens, seq_lens
  * with them). A path rises; an entry outside the new tokens or below its place, or a row outside the cache, is left out and
  * sets lb_device_error() to 3. lens_out [seqs], over none of the inputs, receives seq_lens[s] - n + accepted[s]; for a sequence
- * that lb_paged_plan refused (seq_lens[s] < n) it is left as it is (keep) or 0, and nothing moves.
+ * that lb_paged_plan refused (seq_lens[s] is 0, whether rows were left for it or not) or that is empty, and wherever seq_lens[s] < n,
+ * it is left as it is (keep) or 0, and nothing moves.
  */
 LB_API int lb_paged_compact(const lb_paged_cache* const* caches, int layers, const int32_t* page_table, int64_t table_stride,
                             int64_t table_width, const int32_t* seq_lens, const int32_t* cu_new, const int32_t* path,

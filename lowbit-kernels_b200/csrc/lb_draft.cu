@@ -377,8 +377,8 @@ __global__ void __launch_bounds__(kMoveThreads) compact_kernel(const __grid_cons
   const int32_t* path = p.path + (int64_t)s * p.max_path;
   int from = (int)threadIdx.x < p.max_path ? ldg_cg_i32(path + threadIdx.x) : 0;   // on its way together with the lengths
   const int n = max(0, ldg_cg_i32(p.cu_new + s + 1) - ldg_cg_i32(p.cu_new + s));
-  const int start = ldg_cg_i32(p.seq_lens + s) - n, length = min(ldg_cg_i32(p.accepted + s), min(p.max_path, n));
-  if (start < 0) {   // a sequence that the plan refused
+  const int len = ldg_cg_i32(p.seq_lens + s), start = len - n, length = min(ldg_cg_i32(p.accepted + s), min(p.max_path, n));
+  if (len == 0 || start < 0) {   // a sequence that the plan refused (it may have no rows), or one that is empty: nothing to move
     if (!p.keep && blockIdx.x == 0 && threadIdx.x == 0) p.lens_out[s] = 0;
     return;
   }

@@ -276,7 +276,7 @@ struct CompactParams {
   const int32_t* accepted;
   int seqs, max_path;
   int32_t* lens_out;
-  bool keep;                 // lens_out of a sequence that the plan refused stays as it is, else it is 0
+  bool keep;                 // lens_out of a sequence that the plan refused, or that is empty, stays as it is, else it is 0
 };
 cudaError_t launch_compact(const CompactParams& p, bool pdl, cudaStream_t st);
 int draft_device_error();   // synchronizes

@@ -741,6 +741,39 @@ def test_compact_leaves_refused_sequences_and_reports_bad_paths():
 
 
 @gpu
+@pytest.mark.parametrize("short", ["rows", "width", "pages"])
+def test_compact_keeps_the_lengths_of_all_sequences_that_the_plan_refused(short):
+    """Those behind the one that did not fit have no rows left, so that nothing but their length, 0, says that they were refused; served
+    ones without new tokens and empty ones are as they were."""
+    _, paged = mods()
+    caches = make_caches(gen(1), 2, 160, 2, 16, 64, torch.float16)
+    table = torch.randperm(160, device="cuda", generator=gen(2))[:140].view(7, 20).to(torch.int32)
+    before, new, kw = [100, 200, 300, 0, 5, 60, 90], [8, 8, 8, 0, 0, 3, 0], {}
+    tokens = sum(new)
+    if short == "rows":   # four for the second sequence, none for the third and the sixth
+        tokens, served = 12, [True, False, False, True, True, False, True]
+    elif short == "width":   # contexts up to 112; the second one asks for nothing
+        new[1], served = 0, [True, False, False, True, True, True, True]
+        table, tokens = table[:, :7].contiguous(), sum(new)
+    else:   # no page is free, the third and the last sequence need one
+        before[2], before[6], new[6] = 304, 95, 2
+        kw = dict(held=i32([7, 13, 19, 0, 1, 4, 6]), free_pages=i32([159]), free_count=i32([0]))
+        tokens, served = sum(new), [True, True, False, True, True, True, False]
+    lens = i32(before)
+    p = paged.plan(table, lens, i32(new), 16, tokens, **kw)
+    assert p.seq_lens.tolist() == [c + n if ok else 0 for c, n, ok in zip(before, new, served)]
+    if short == "rows":
+        assert p.cu_new.tolist() == [0, 8, 12, 12, 12, 12, 12, 12]
+    path, count = i32([[0, 1, 2] if n else [-1] * 3 for n in new]), i32([min(n, 3) for n in new])
+    kept = [(c.k.clone(), c.v.clone()) for c in caches]
+    want = [c + min(n, 3) if ok else 0 for c, n, ok in zip(before, new, served)]
+    assert paged.compact(caches, table, p.seq_lens, p.cu_new, path, count).tolist() == want
+    want = [w if ok else c for w, c, ok in zip(want, before, served)]
+    assert paged.compact(caches, table, p.seq_lens, p.cu_new, path, count, out=lens) is lens and lens.tolist() == want
+    assert all(torch.equal(c.k, k) and torch.equal(c.v, v) for c, (k, v) in zip(caches, kept)) and status() == 0
+
+
+@gpu
 def test_compact_refusals():
     _, paged = mods()
     caches = make_caches(gen(1), 2, 8, 2, 16, 64, torch.float16)
