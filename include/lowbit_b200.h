@@ -403,12 +403,19 @@ LB_API int lb_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int s
  * and -1. Rows past cu_new[seqs] are not read, their targets not written. max_new (1 to 1024) bounds the new tokens of any
  * sequence, those behind it are ignored. workspace: lb_draft_verify_workspace(tokens, vocab) bytes, 16-byte aligned, distinct for calls that
  * can overlap.
+ * lb_draft_verify knows nothing of sequences that lb_paged_plan refused: it walks down their rows too, whose logits come from tokens
+ * that saw nothing. lb_draft_verify_planned takes the plan's lens_out as seq_lens [seqs] (or NULL) and gives a sequence with fewer
+ * tokens than new ones 0 and -1, like one without new tokens; its rows' targets are written all the same.
  */
 LB_API int64_t lb_draft_verify_workspace(int64_t tokens, int64_t vocab);
 LB_API int lb_draft_verify(const void* logits, int dtype, int64_t ld, int64_t tokens, int64_t vocab, const int64_t* drafted,
                            const int32_t* parents, const int32_t* cu_new, int seqs, int64_t max_new, int64_t max_path,
                            int32_t* accepted, int32_t* path, int64_t* next, int64_t* targets, void* workspace,
                            int64_t workspace_bytes, lb_stream_t stream);
+LB_API int lb_draft_verify_planned(const void* logits, int dtype, int64_t ld, int64_t tokens, int64_t vocab, const int64_t* drafted,
+                                   const int32_t* parents, const int32_t* cu_new, const int32_t* seq_lens, int seqs, int64_t max_new,
+                                   int64_t max_path, int32_t* accepted, int32_t* path, int64_t* next, int64_t* targets, void* workspace,
+                                   int64_t workspace_bytes, lb_stream_t stream);
 
 /*
  * Moves the K and V rows of accepted tokens to where a sequence without the others has them, in `layers` (at most 128) caches of one

@@ -889,6 +889,14 @@ int lb_draft_verify(const void* logits, int dtype, int64_t ld, int64_t tokens, i
                     const int32_t* parents, const int32_t* cu_new, int seqs, int64_t max_new, int64_t max_path,
                     int32_t* accepted, int32_t* path, int64_t* next, int64_t* targets, void* workspace,
                     int64_t workspace_bytes, lb_stream_t stream) {
+  return lb_draft_verify_planned(logits, dtype, ld, tokens, vocab, drafted, parents, cu_new, nullptr, seqs, max_new, max_path, accepted, path, next,
+                                 targets, workspace, workspace_bytes, stream);
+}
+
+int lb_draft_verify_planned(const void* logits, int dtype, int64_t ld, int64_t tokens, int64_t vocab, const int64_t* drafted,
+                            const int32_t* parents, const int32_t* cu_new, const int32_t* seq_lens, int seqs, int64_t max_new, int64_t max_path,
+                            int32_t* accepted, int32_t* path, int64_t* next, int64_t* targets, void* workspace,
+                            int64_t workspace_bytes, lb_stream_t stream) {
   if (!logits || !drafted || !parents || !cu_new || !accepted || !path || !next || !targets)
     return fail(LB_ERR_ARGUMENT, "null pointer argument");
   if (dtype < LB_F16 || dtype > LB_F32) return fail(LB_ERR_ARGUMENT, "dtype is 0 (fp16), 1 (bf16) or 2 (fp32)");
@@ -897,7 +905,7 @@ int lb_draft_verify(const void* logits, int dtype, int64_t ld, int64_t tokens, i
   if (ld < vocab) return fail(LB_ERR_ARGUMENT, "rows of the logits overlap: %lld values, stride %lld", (long long)vocab, (long long)ld);
   if (max_new < 1 || max_new > lb::kMaxTree) return fail(LB_ERR_ARGUMENT, "max_new=%lld: trees hold 1 to %d tokens", (long long)max_new, lb::kMaxTree);
   if (max_path < 1 || max_path > lb::kMaxTree) return fail(LB_ERR_ARGUMENT, "max_path=%lld: 1 to %d", (long long)max_path, lb::kMaxTree);
-  if (misaligned({logits}, dtype == LB_F32 ? 4 : 2) || misaligned({parents, cu_new, accepted, path}, 4) || misaligned({drafted, next, targets}, 8))
+  if (misaligned({logits}, dtype == LB_F32 ? 4 : 2) || misaligned({parents, cu_new, seq_lens, accepted, path}, 4) || misaligned({drafted, next, targets}, 8))
     return fail(LB_ERR_ALIGNMENT, "arrays must be aligned to their type");
   const int64_t need = (int64_t)lb::verify_workspace_bytes(tokens, vocab);
   if (!workspace || workspace_bytes < need)
@@ -905,7 +913,7 @@ int lb_draft_verify(const void* logits, int dtype, int64_t ld, int64_t tokens, i
   if (!aligned16(workspace)) return fail(LB_ERR_ALIGNMENT, "the workspace must be 16-byte aligned");
   int rc = check_device();
   if (rc) return rc;
-  const lb::VerifyParams p{logits, ld, dtype, (int)tokens, (int)vocab, drafted, parents, cu_new, seqs, (int)max_new, (int)max_path,
+  const lb::VerifyParams p{logits, ld, dtype, (int)tokens, (int)vocab, drafted, parents, cu_new, seq_lens, seqs, (int)max_new, (int)max_path,
                            accepted, path, next, targets, static_cast<uint64_t*>(workspace)};
   return launched(lb::launch_verify(p, g_opt[LB_OPT_PDL].load() != 0, reinterpret_cast<cudaStream_t>(stream)), "draft_verify");
 }

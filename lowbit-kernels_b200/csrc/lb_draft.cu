@@ -314,7 +314,8 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyParams p
   pdl_launch_dependents();
   pdl_wait();
   const int s = blockIdx.x, t0 = max(0, ldg_cg_i32(p.cu_new + s));
-  const int n = max(0, min(min(ldg_cg_i32(p.cu_new + s + 1), p.tokens) - t0, p.max_new));
+  const int all = min(ldg_cg_i32(p.cu_new + s + 1), p.tokens) - t0, n = max(0, min(all, p.max_new));
+  const bool served = n > 0 && (!p.seq_lens || ldg_cg_i32(p.seq_lens + s) >= all);   // (a refused one's rows have targets, but no path)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < n; i += kWalkThreads) {
     token[i] = ldg_cg_i64(p.drafted + t0 + i);
@@ -337,9 +338,9 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyParams p
   }
   __syncthreads();
   if (warp) return;
-  int cur = 0, length = n > 0 ? 1 : 0;
+  int cur = 0, length = served ? 1 : 0;
   int32_t* path = p.path + (int64_t)s * p.max_path;
-  if (lane == 0) path[0] = n > 0 ? 0 : -1;
+  if (lane == 0) path[0] = served ? 0 : -1;
   while (length > 0 && length < p.max_path) {
     const int64_t want = target[cur];
     int child = -1;
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyParams p
   for (int d = max(1, length) + lane; d < p.max_path; d += 32) path[d] = -1;
   if (lane == 0) {
     p.accepted[s] = length;
-    p.next[s] = n > 0 ? target[cur] : -1;
+    p.next[s] = served ? target[cur] : -1;
   }
 }
 

@@ -251,6 +251,7 @@ struct VerifyParams {
   const int64_t* drafted;    // [tokens]
   const int32_t* parents;
   const int32_t* cu_new;     // [seqs + 1]
+  const int32_t* seq_lens;   // [seqs], the new tokens included, or null: fewer than the new tokens where the plan refused the sequence
   int seqs, max_new, max_path;
   int32_t* accepted;         // [seqs]
   int32_t* path;             // [seqs, max_path]

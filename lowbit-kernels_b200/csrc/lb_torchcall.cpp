@@ -16,7 +16,7 @@
 //   linear_f8(x, q, scales, out, bias) -> Tensor | None   (q as bytes, scales: an F8Weight's)
 //   paged_tree_attention(q, cache_ptr, device, page_table, seq_lens, cu_new, mask, max_new, max_len, scale, out) -> Tensor | None
 //   plan(page_table, seq_lens, new_lens, page_size, tokens, held, free_pages, free_count, parents, max_new) -> tuple | None
-//   verify(logits, tokens, parents, cu_new, max_new, max_path) -> tuple | None
+//   verify(logits, tokens, parents, cu_new, max_new, max_path, seq_lens) -> tuple | None
 //   compact(caches, PagedCache, page_table, seq_lens, cu_new, path, accepted, out) -> Tensor | None
 #include <Python.h>
 
@@ -437,13 +437,19 @@ PyObject* verify(PyObject* const* args) {
   if (args[5] != Py_None && !to_ints(args + 5, bound + 1, 1)) return nullptr;
   if (bound[0] < 1 || bound[0] > 1024 || bound[1] < 1 || bound[1] > 1024) Py_RETURN_NONE;
   const int64_t s = cu->numel() - 1, need = lb_draft_verify_workspace(t, vocab);
+  const at::Tensor* lens = nullptr;
+  if (args[6] != Py_None) {
+    lens = tensor_on(args[6], dev);
+    if (!vector_of(lens, at::kInt, s)) Py_RETURN_NONE;
+  }
   Outputs outs(Outputs::padded(4 * s) + Outputs::padded(4 * s * bound[1]) + Outputs::padded(8 * s) + Outputs::padded(8 * t) + need, *cu);
   at::Tensor accepted = outs.take(at::kInt, {s}), path = outs.take(at::kInt, {s, bound[1]}), next = outs.take(at::kLong, {s}),
              targets = outs.take(at::kLong, {t});
-  const int rc = lb_draft_verify(x.data_ptr(), type == at::kHalf ? LB_F16 : type == at::kBFloat16 ? LB_BF16 : LB_F32, ld, t, vocab,
-                                 tokens->data_ptr<int64_t>(), parents->data_ptr<int32_t>(), cu->data_ptr<int32_t>(), (int)s, bound[0], bound[1],
-                                 accepted.data_ptr<int32_t>(), path.data_ptr<int32_t>(), next.data_ptr<int64_t>(), targets.data_ptr<int64_t>(),
-                                 outs.rest(), need, stream_of(dev));
+  const int rc = lb_draft_verify_planned(x.data_ptr(), type == at::kHalf ? LB_F16 : type == at::kBFloat16 ? LB_BF16 : LB_F32, ld, t, vocab,
+                                         tokens->data_ptr<int64_t>(), parents->data_ptr<int32_t>(), cu->data_ptr<int32_t>(),
+                                         lens ? lens->data_ptr<int32_t>() : nullptr, (int)s, bound[0], bound[1], accepted.data_ptr<int32_t>(),
+                                         path.data_ptr<int32_t>(), next.data_ptr<int64_t>(), targets.data_ptr<int64_t>(), outs.rest(), need,
+                                         stream_of(dev));
   return rc ? refused(rc) : tuple_of({&accepted, &path, &next, &targets});
 }
 
@@ -520,8 +526,8 @@ PyMethodDef methods[] = {
     {"plan", fastcall<plan, 10>(), METH_FASTCALL,
      "plan(page_table, seq_lens, new_lens, page_size, tokens, held, free_pages, free_count, parents, max_new) -> tuple, or None "
      "for the checked path"},
-    {"verify", fastcall<verify, 6>(), METH_FASTCALL,
-     "verify(logits, tokens, parents, cu_new, max_new, max_path) -> tuple, or None for the checked path"},
+    {"verify", fastcall<verify, 7>(), METH_FASTCALL,
+     "verify(logits, tokens, parents, cu_new, max_new, max_path, seq_lens) -> tuple, or None for the checked path"},
     {"compact", fastcall<compact, 8>(), METH_FASTCALL,
      "compact(caches, PagedCache, page_table, seq_lens, cu_new, path, accepted, out) -> Tensor, or None for the checked path"},
     {"paged_attention", fastcall<attend<false>, 10>(), METH_FASTCALL,

@@ -65,6 +65,7 @@ SIGNATURES = {
     "lb_paged_plan": ([_P, _P, _I, _P, _I64, _I64, _I, _I64, _P, _P, _I64, _P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P], _I),
     "lb_draft_verify_workspace": ([_I64, _I64], _I64),
     "lb_draft_verify": ([_P, _I, _I64, _I64, _I64, _P, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P], _I),
+    "lb_draft_verify_planned": ([_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _I, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P], _I),
     "lb_paged_compact": ([_P, _I, _P, _I64, _I64, _P, _P, _P, _P, _I, _I64, _P, _I, _P], _I),
 }
 

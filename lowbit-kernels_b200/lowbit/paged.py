@@ -308,17 +308,21 @@ def plan(page_table, seq_lens, new_lens, page_size, tokens, held=None, free_page
     return out
 
 
-def verify(logits, tokens, parents, cu_new, max_new=None, max_path=None):
+def verify(logits, tokens, parents, cu_new, max_new=None, max_path=None, seq_lens=None):
     """Greedy acceptance of drafted trees. logits [T, vocab] (fp16, bf16 or fp32, rows any stride apart) follow the new tokens
     `tokens` int64 [T] of the sequences cu_new int32 [S + 1], whose parents int32 [T] are as in `plan`. Returns a `Verified`: targets,
     the index of each row's first largest value (a NaN counts as larger than all); and for each sequence the path that starts at its first new token, the
     last certain one, and goes on to the first later token that is a child of the one at hand and equals its target: how many tokens it has
     (accepted), their places among the new ones (path, -1 behind them) and the target after the last (next). A sequence
     without new tokens gets 0 and -1. max_new bounds the new tokens of any sequence (1024 at most; by default T;
-    those past it are left out, their targets unwritten), max_path the path (by default max_new). Rows past cu_new[S] are not looked at, their targets left unwritten."""
+    those past it are left out, their targets unwritten), max_path the path (by default max_new). Rows past cu_new[S] are not looked at, their targets left unwritten.
+
+    A sequence that `plan` refused may have rows, and the logits after them come from tokens that saw nothing. With the plan's seq_lens
+    (int32 [S]) it gets 0 and -1 too; without them its path and next mean nothing, and the caller looks at the plan's seq_lens before
+    using them."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc:
-        got = tc.verify(logits, tokens, parents, cu_new, max_new, max_path)
+        got = tc.verify(logits, tokens, parents, cu_new, max_new, max_path, seq_lens)
         if got is not None:
             return Verified._make(got)
     if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dim() == 2 and logits.dtype in DTYPE_IDS):
@@ -334,6 +338,7 @@ def verify(logits, tokens, parents, cu_new, max_new=None, max_path=None):
     s = cu_new.numel() - 1
     if s < 1:
         raise RuntimeError("cu_new must hold a sequence at least")
+    lens = None if seq_lens is None else _vector("seq_lens", seq_lens, torch.int32, dev, s)
     max_new = t if max_new is None else int(max_new)
     max_path = max_new if max_path is None else int(max_path)
     if t and not 1 <= max_new <= 1024:
@@ -349,9 +354,9 @@ def verify(logits, tokens, parents, cu_new, max_new=None, max_path=None):
     with _Device(dev):
         need = e.lib.lb_draft_verify_workspace(t, vocab)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        rc = e.lib.lb_draft_verify(logits.data_ptr(), DTYPE_IDS[logits.dtype], logits.stride(0) if t > 1 else vocab, t, vocab, drafted,
-                                   tree, cu, s, max_new, max_path, got.accepted.data_ptr(), got.path.data_ptr(), got.next.data_ptr(),
-                                   got.targets.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+        rc = e.lib.lb_draft_verify_planned(logits.data_ptr(), DTYPE_IDS[logits.dtype], logits.stride(0) if t > 1 else vocab, t, vocab, drafted,
+                                           tree, cu, lens, s, max_new, max_path, got.accepted.data_ptr(), got.path.data_ptr(), got.next.data_ptr(),
+                                           got.targets.data_ptr(), ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
     if rc:
         e._raise(rc)
     return got

@@ -626,6 +626,37 @@ def test_verify_trees():
 
 
 @gpu
+@pytest.mark.parametrize("contiguous", [True, False])
+def test_verify_accepts_nothing_for_sequences_that_the_plan_refused(contiguous):
+    """With the plan's lengths, whether the refused one has all, some or none of its rows; the others are as without them."""
+    _, paged = mods()
+    new, vocab = [6, 9, 4, 0, 7, 5], 500
+    x = randn(gen(3), 31, vocab, dtype=torch.float16)
+    if not contiguous:   # (rows that the checked path has to lay out first)
+        x = x.t().contiguous().t()
+    top = x.argmax(1).tolist()
+    tokens, parents = [t for i in range(31) for t in ([7] if i in (0, 6, 15, 19, 26) else [top[i - 1]])], [i - 1 for n in new for i in range(n)]
+    table, before = i32([[2 * i, 2 * i + 1] for i in range(6)]), i32([10, 30, 3, 0, 0, 2])
+    for rows, served in ((31, [1, 0, 1, 1, 1, 1]), (23, [1, 0, 1, 1, 0, 0]), (19, [1, 0, 1, 1, 0, 0])):
+        at = paged.plan(table, before, i32(new), 16, rows, parents=i32(parents[:rows]), max_new=9)
+        assert [int(n > 0 or i == 3) for i, n in enumerate(at.seq_lens.tolist())] == served
+        args = x[:rows], i64(tokens[:rows]), i32(parents[:rows]), at.cu_new
+        plain, got = paged.verify(*args, max_new=9), paged.verify(*args, max_new=9, seq_lens=at.seq_lens)
+        assert torch.equal(got.targets, plain.targets)
+        for s, ok in enumerate(served):
+            if ok:
+                assert torch.equal(got.path[s], plain.path[s]) and (got.accepted[s], got.next[s]) == (plain.accepted[s], plain.next[s])
+            else:
+                assert got.accepted[s] == 0 and got.next[s] == -1 and (got.path[s] == -1).all()
+    # fewer new tokens looked at than there are: refused by all of them
+    got = paged.verify(*args, max_new=2, seq_lens=i32([5, 8, 4, 0, 0, 0]))
+    assert got.accepted.tolist() == [0, 0, 2, 0, 0, 0]
+    for bad in (i32([1] * 5), i64([1] * 6), torch.zeros(6, dtype=torch.int32)):
+        with pytest.raises(RuntimeError, match="seq_lens"):
+            paged.verify(*args, seq_lens=bad)
+
+
+@gpu
 def test_verify_leaves_rows_behind_the_last_sequence_and_replays():
     _, paged = mods()
     rng = random.Random(2)
