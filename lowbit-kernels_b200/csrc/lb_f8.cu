@@ -549,8 +549,8 @@ __device__ __forceinline__ void rows_epilogue(const F8Rows& p, const F8Epilogue&
   const T* bias = static_cast<const T*>(p.bias);
   T* y = static_cast<T*>(p.y);
   uint8_t* stage = w.staging;
-  bool ok = true;   // of this lane: one that gave up waits no more, but stays with its warp's collective instructions
-  bool ready = false;   // the next accumulator, as asked under the work on this one
+  bool ok = true;   // of the warp, as are the waits' answers: having given up it waits no more, but stays with the collective instructions
+  bool ready = false;   // the next accumulator, as asked under the work on this one; all lanes found it so
   // of the accumulator: its barrier, that of its release, its columns, the parity of its uses (the turns are 16 bytes and 256
   // columns apart, both aligned to twice that); and the place of the stage's scale
   uint32_t bar = w.acc_full + 8 * h, empty = w.acc_empty + 8 * h, acc = w.tmem + ((uint32_t)(32 * quarter) << 16) + 128 * h, parity = 0, odd = 0;
@@ -592,7 +592,7 @@ __device__ __forceinline__ void rows_epilogue(const F8Rows& p, const F8Epilogue&
         tc::ld16(acc + 16 * i, v);
         if (i == 0) {
           const float sv = lds_f32(scale);   // there, since the MMAs have waited for it
-          ready = test_barrier(bar, parity);
+          ready = __all_sync(0xffffffffu, test_barrier(bar, parity));
           fa = __shfl_sync(0xffffffffu, ta, c & 31) * sv;
           fb = __shfl_sync(0xffffffffu, tb, c & 31) * sv;
         }

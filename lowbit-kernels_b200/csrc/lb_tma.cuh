@@ -82,8 +82,10 @@ __device__ __forceinline__ bool wait_ready(uint32_t bar, uint32_t parity, int* s
   return false;
 }
 
-// The same for a whole warp in a loop that its instructions bound: one block of code without branches for the compiler, so
-// that nothing is inserted to bring lanes together again.
+// The same for a whole warp in a loop that its instructions bound. All 32 lanes call it and get one answer: it asks until every lane
+// has found the phase completed. The vote makes the branch one that all lanes take alike, which .uni promises (a lane's try_wait
+// alone may answer otherwise than its neighbour's); one block of code without branches for the compiler, so that nothing is inserted
+// to bring lanes together again.
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* status) {
   uint32_t done;
   asm volatile(
@@ -91,6 +93,7 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int* st
       "mov.u32 n, %3;\n\t"
       "LB_AGAIN_%=:\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "vote.sync.all.pred p, p, 0xffffffff;\n\t"
       "sub.u32 n, n, 1;\n\t"
       "setp.eq.or.u32 q, n, 0, p;\n\t"
       "@!q bra.uni LB_AGAIN_%=;\n\t"

@@ -17,6 +17,7 @@ import ctypes
 import math
 import pickle
 import random
+import re
 
 import pytest
 import torch
@@ -1203,6 +1204,17 @@ def test_no_warp_of_the_kernels_meets_others_on_the_way():
     for name in ("lb_f8.cu", "lb_draft.cu"):
         source = (_lib.LIB_PATH.parent.parent / "csrc" / name).read_text()
         assert "named_barrier(" not in source and "bar.sync" not in source and "barrier.sync" not in source, name
+
+
+def test_branches_that_all_lanes_have_to_take_alike_are_voted():
+    """bra.uni promises that a warp's lanes agree, but each lane's wait answers for itself: the block that branches takes a vote first."""
+    found = 0
+    for path in sorted((_lib.LIB_PATH.parent.parent / "csrc").glob("*.cu*")):
+        for block in re.findall(r"asm volatile\((.*?)\);", path.read_text(), re.S):
+            if "bra.uni" in block:
+                found += 1
+                assert "vote.sync" in block[:block.index("bra.uni")], path.name
+    assert found
 
 
 def test_abi_refusals_of_what_lies_over_the_inputs_or_is_misaligned():
