@@ -592,6 +592,9 @@ __device__ __forceinline__ void rows_epilogue(const F8Rows& p, const F8Epilogue&
         tc::ld16(acc + 16 * i, v);
         if (i == 0) {
           const float sv = lds_f32(scale);   // there, since the MMAs have waited for it
+          // The arrival below hands back the scale's place too, where a tensor copy puts that of a later stage: its address hangs on a
+          // vote for which every lane has to have its scale (rank >> 1 is 0, which the compiler does not know)
+          empty += __ballot_sync(0xffffffffu, __float_as_uint(sv) != 0u) & (uint32_t)rank >> 1;
           ready = __all_sync(0xffffffffu, test_barrier(bar, parity));
           fa = __shfl_sync(0xffffffffu, ta, c & 31) * sv;
           fb = __shfl_sync(0xffffffffu, tb, c & 31) * sv;

@@ -125,9 +125,10 @@ __device__ __forceinline__ void commit_pair_at(uint32_t bar) {   // commit_pair 
       : "memory");
 }
 
-// One lane's arrival, on a barrier of any CTA of the cluster, that hands an accumulator back: all that stands before it are
-// reads of tensor memory that have completed (tcgen05.wait::ld), so it needs no release, which would wait for the warp's
-// loads in flight.
+// One lane's arrival, on a barrier of any CTA of the cluster, that hands an accumulator back, and with it all that the warp read of the
+// stage. It is no release, which would wait for the warp's loads in flight, so it stands only behind reads that have completed, whose
+// values nothing written later can change: those of tensor memory by tcgen05.wait::ld, others where their values are in registers
+// before the arrival can be issued (see its caller).
 __device__ __forceinline__ void arrive_relaxed(uint32_t bar, bool on) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"

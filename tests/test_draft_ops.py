@@ -972,6 +972,32 @@ def test_linear_f8_several_tiles_a_cta_and_long_rows(dtype, m, n, k):
 
 
 @gpu
+@pytest.mark.parametrize("m,n,k", [(512, 896, 131072), (300, 224, 40000), (2048, 1792, 4096)])
+def test_linear_f8_uses_each_stage_with_its_own_scale(m, n, k):
+    """Tokens whose scales differ by powers of two from block to block, so that another stage's scale is off by a factor of two at least;
+    small whole numbers, so that nothing is rounded before the result. Again and again, beside copies that keep memory busy."""
+    ops, _ = mods()
+    g = gen(k)
+    blocks = -(-k // 128)
+    x = torch.randint(-3, 4, (m, blocks, 128), device="cuda", generator=g).float()
+    x[:, :, 0] = 7   # (a block's largest value, 448 at its scale, as are the whole numbers below it times 64)
+    x = (x * 2.0 ** ((torch.arange(blocks, device="cuda") * 5 + torch.arange(m, device="cuda")[:, None]) % 8)[..., None]).view(m, -1)[:, :k].contiguous()
+    w = torch.zeros(n, blocks * 128, device="cuda")
+    at = torch.randint(0, blocks, (n, 40), device="cuda", generator=g) * 128 + torch.randint(0, 128, (n, 40), device="cuda", generator=g)
+    w.scatter_(1, at.clamp(max=k - 1), torch.randint(-4, 5, (n, 40), device="cuda", generator=g).float())
+    w = w[:, :k].contiguous()
+    f8 = ops.F8Weight(w.to(F8), torch.ones(-(-n // 128), blocks, device="cuda"))
+    want = x.double() @ w.double().t()   # below 2^24 in steps of 1
+    x = x.to(torch.bfloat16)
+    noise, side = torch.empty(1 << 26, device="cuda"), torch.cuda.Stream()
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            noise.mul_(0.5)
+        close(ops.linear_f8(x, f8), want, U[torch.bfloat16] * want.abs(), "a scale of another stage")
+    assert status() == 0
+
+
+@gpu
 def test_linear_f8_strided_inputs_out_streams_and_graph():
     ops, _ = mods()
     g = gen(9)
