@@ -48,7 +48,7 @@ typedef enum lb_option {
   LB_OPT_PDL = 0,           /* 1 (default): launch with programmatic dependent launch enabled */
   LB_OPT_EARLY_WEIGHTS = 1, /* 1: GEMV kernels, lb_w8_linear, lb_f8_linear and the norm of lb_paged_norm_rope_append fetch their
                                first weights before waiting on the previous kernel in the stream (only for weights
-                               no in-flight kernel writes); default 0 */
+                               no in-flight kernel writes; the products' biases are read after the wait); default 0 */
   LB_OPT_GEMV_KSPLIT = 2,   /* 0 (default): automatic; 1..8 forces the GEMV's K-split cluster size */
   LB_OPT_GEMV_WARPS = 3,    /* 0 (default): automatic; 4, 8 or 16 forces the GEMV's warps per CTA */
   LB_OPT_GEMV_DEPTH = 4,    /* reserved: no effect (the copy-ring GEMV it tuned was removed) */

@@ -867,7 +867,6 @@ __global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) f8_gemv_kerne
   for (int i = 0; i < R; ++i) fetch(i, warp + i * NW);
   const int out_n = n0 + (tid & 15), out_m = tid >> 4;   // the output this thread sums, of 16 x 8
   const bool out_on = tid < 128 && out_n < p.N && out_m < p.M;
-  const float bn = out_on && p.bias ? Elem<T>::to_float(static_cast<const T*>(p.bias)[out_n]) : 0.f;
   if (early) pdl_wait();
   const bool aligned = ((reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.ldx * sizeof(T))) & 15u) == 0;
   const T* x = static_cast<const T*>(p.x);
@@ -895,6 +894,8 @@ __global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) f8_gemv_kerne
       }
   }
   __syncthreads();
+  // behind the wait, since the kernel before may have written it, and on its way under the products
+  const uint16_t bias = out_on && p.bias ? ldg_cg_u16(static_cast<const T*>(p.bias) + out_n) : (uint16_t)0;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   const uint32_t own = smem_addr(rows) + (uint32_t)(min(g, p.M - 1) * p.pitch + 16 * t);   // unused columns repeat a row
   const int m0 = min(2 * t, p.M - 1), m1 = min(2 * t + 1, p.M - 1);
@@ -926,7 +927,7 @@ __global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) f8_gemv_kerne
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) v += part[w][tid];
-    static_cast<T*>(p.y)[(int64_t)out_m * p.N + out_n] = Elem<T>::from_float(v + bn);
+    static_cast<T*>(p.y)[(int64_t)out_m * p.N + out_n] = Elem<T>::from_float(v + Elem<T>::unpack(bias).x);
   }
 }
 

@@ -646,7 +646,6 @@ __global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) w8_gemv_kerne
   const int out_n = n0 + (tid & 15), out_m = tid >> 4;   // the output this thread sums, of 16 x 8
   const bool out_on = tid < 128 && out_n < p.N && out_m < p.M;
   const float tn = out_on ? p.t[out_n] : 0.f;
-  const float bn = out_on && p.bias ? Elem<T>::to_float(static_cast<const T*>(p.bias)[out_n]) : 0.f;
   if (tid < kGemvRows) maxima[tid] = 0u;
   __syncthreads();
   if (early) pdl_wait();
@@ -689,6 +688,8 @@ __global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) w8_gemv_kerne
       }
   }
   __syncthreads();
+  // behind the wait, since the kernel before may have written it, and on its way under the products
+  const uint16_t bias = out_on && p.bias ? ldg_cg_u16(static_cast<const T*>(p.bias) + out_n) : (uint16_t)0;
   int d[4] = {0, 0, 0, 0};
   const uint32_t own = smem_addr(rows) + (uint32_t)(min(g, p.M - 1) * p.pitch + 16 * t);   // unused columns repeat a row
   for (int c0 = warp; c0 < p.pieces; c0 += NW * R) {
@@ -714,7 +715,7 @@ __global__ void __launch_bounds__(32 * NW, gemv_per_sm(NW, MR, R)) w8_gemv_kerne
 #pragma unroll
     for (int w = 0; w < NW; ++w) sum += part[w][tid];
     static_cast<T*>(p.y)[(int64_t)out_m * p.N + out_n] = Elem<T>::from_float(
-        fmaf(__int2float_rn(sum) * row_scale(__uint_as_float(maxima[out_m])).s, tn, bn));
+        fmaf(__int2float_rn(sum) * row_scale(__uint_as_float(maxima[out_m])).s, tn, Elem<T>::unpack(bias).x));
   }
 }
 

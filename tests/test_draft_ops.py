@@ -1120,6 +1120,38 @@ def test_the_operators_give_the_same_bits_under_every_launch_option(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["f8", "w8"])
+@pytest.mark.parametrize("m", [1, 4, 8, 40, 333])
+def test_a_bias_may_come_from_the_kernel_before_under_every_launch_option(kind, m):
+    """early_weights speaks of weights alone: a bias that the product before has just written is the one that is added."""
+    ops, _ = mods()
+    e, g = ops.ext(), gen(m)
+    make, linear = (ops.F8Weight.from_float, ops.linear_f8) if kind == "f8" else (ops.W8Weight.from_float, ops.linear_w8)
+    first, second = make(randn(g, 2000, 9000, std=0.05)), make(randn(g, 2000, 1024, std=0.05))
+    xs, x = [randn(g, 1, 9000, dtype=torch.float16) for _ in range(8)], randn(g, m, 1024, dtype=torch.float16)
+    bias = torch.empty(1, 2000, device="cuda", dtype=torch.float16)
+    want = []
+    for z in xs:
+        linear(z, first, out=bias)
+        torch.cuda.synchronize()
+        want.append(linear(x, second, bias=bias[0]))
+        torch.cuda.synchronize()
+    try:
+        for pdl in (0, 1):
+            for early in (0, 1):
+                e.set_option("pdl", pdl)
+                e.set_option("early_weights", early)
+                got = []
+                for z in xs:
+                    linear(z, first, out=bias)
+                    got.append(linear(x, second, bias=bias[0]))
+                assert all(torch.equal(a, b) for a, b in zip(got, want)), (pdl, early)
+    finally:
+        e.set_option("pdl", 1)
+        e.set_option("early_weights", 0)
+
+
+@gpu
 def test_offsets_past_32_bits():
     """Pages, rows of logits and rows of tokens more than 2^31 elements from the first."""
     ops, paged = mods()
