@@ -476,11 +476,12 @@ class PagedDecoder:
         f = x.float()
         return w * (f * torch.rsqrt(f.square().mean(-1, keepdim=True) + self.eps)).to(self.dtype)
 
-    def _plan(self, chunks):
+    def _plan(self, chunks, reach=None):
         """The call's host arrays -- token ids, positions and slots, page table, lengths and first tokens -- and each
-        sequence's pages after it. Changes nothing: `_commit` does, once the call's work is launched."""
+        sequence's pages after it. reach: how many tokens each sequence's context grows by, where its new ones do not follow one another
+        (a tree's levels). Changes nothing: `_commit` does, once the call's work is launched."""
         page = self.page_size
-        longest = max(self._seqs[s]["length"] + len(new) for s, new in chunks.items())
+        longest = max(self._seqs[s]["length"] + (len(new) if reach is None else reach[s]) for s, new in chunks.items())
         if self.limit is not None and longest > self.limit:
             raise ValueError(f"{longest} tokens: the model's sliding window or rotary scaling allows {self.limit} here")
         need = {s: -(-(self._seqs[s]["length"] + len(new)) // page) - len(self._seqs[s]["pages"]) for s, new in chunks.items()}
@@ -554,12 +555,17 @@ class PagedDecoder:
         free pages as they were."""
         if not trees:
             raise ValueError("no trees")
-        for tokens, parents in trees.values():
+        levels = {}
+        for s, (tokens, parents) in trees.items():
             if not 1 <= len(tokens) <= 1024 or len(parents) != len(tokens):
                 raise ValueError("a tree has 1 to 1024 tokens, and a parent for each")
             if int(parents[0]) != -1 or any(not 0 <= int(p) < i for i, p in enumerate(parents[1:], 1)):
                 raise ValueError("the first token's parent is -1, any other's an earlier token's place")
-        ids, _, _, table, lens, cu, pages = self._plan({s: tokens for s, (tokens, _) in trees.items()})
+            depth = [1]
+            for p in parents[1:]:
+                depth.append(depth[int(p)] + 1)
+            levels[s] = max(depth)   # what the longest path adds to the context; the branches beside it see none of each other
+        ids, _, _, table, lens, cu, pages = self._plan({s: tokens for s, (tokens, _) in trees.items()}, levels)
         dev, new = self.device, [b - a for a, b in zip(cu, cu[1:])]
         drafted = torch.tensor(ids, dtype=torch.int64, device=dev)
         ints = (table, [n - k for n, k in zip(lens, new)], new, [int(p) for _, parents in trees.values() for p in parents])

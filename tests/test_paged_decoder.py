@@ -428,6 +428,45 @@ def test_verify_refuses_what_is_no_tree_and_changes_nothing(tree):
     assert (dec._free, dec._seqs) == before
 
 
+def test_the_limit_of_a_model_holds_for_a_trees_levels_not_for_its_tokens(monkeypatch):
+    """60 tokens of 64 and a tree of 30: with four levels the last token's context is 64, with five it is 65."""
+    from lowbit import paged
+
+    class Planned(Exception):
+        pass
+
+    def plan(*args, **kw):
+        raise Planned
+
+    monkeypatch.setattr(paged, "plan", plan)
+    dec = bookkeeper(limit=64)
+    sid, other = dec.open(), dec.open()
+    dec.forward({sid: [1] * 60, other: [2] * 3})
+    wide = [-1, 0, 1, 2] + [i % 3 for i in range(26)]
+    before = copy.deepcopy((dec._free, dec._seqs))
+    with pytest.raises(Planned):
+        dec.verify({sid: ([1] * 30, wide), other: ([1] * 61, list(range(-1, 60)))})
+    with pytest.raises(ValueError, match="65 tokens.*allows 64"):
+        dec.verify({sid: ([1] * 30, wide[:-1] + [3])})
+    with pytest.raises(ValueError, match="65 tokens.*allows 64"):
+        dec.verify({sid: ([1], [-1]), other: ([1] * 62, list(range(-1, 61)))})
+    assert (dec._free, dec._seqs) == before
+
+
+@pytest.mark.gpu
+def test_a_wide_tree_at_the_models_limit_gives_what_it_gives_below_it():
+    from lowbit import paged
+    model = tiny()
+    near, far = (paged.PagedDecoder(model, num_pages=16, page_size=16) for _ in range(2))
+    near.limit, text, got = 40, [int(i) for i in torch.randint(0, 1024, (36,), generator=torch.Generator().manual_seed(2))], []
+    for dec in (near, far):
+        sid = dec.open()
+        first = int(dec.forward({sid: text})[0].argmax())
+        got.append(dec.verify({sid: ([first] + list(range(20)), [-1, 0, 1, 2] + [i % 3 for i in range(17)])})[sid])
+        got[-1] += dec.forward({sid: got[-1][-1:]})[0].tolist() if dec._seqs[sid]["length"] < 40 else []
+    assert got[0] == got[1]
+
+
 @pytest.mark.gpu
 def test_a_verification_that_failed_in_a_layer_can_be_repeated(monkeypatch):
     from lowbit import paged
