@@ -576,8 +576,9 @@ class PagedDecoder:
                          lambda q, cache: tree_attention(q, cache, table_d, at.seq_lens, at.cu_new, at.mask, max_new=max_new, max_len=max_len))
         logits = torch.nn.functional.linear(self._rms(x, self.norm), self.head)
         got = verify(logits, drafted, parents, at.cu_new, max_new=max_new)
-        if self.layers:
-            compact([ly["cache"] for ly in self.layers], table_d, at.seq_lens, at.cu_new, got.path, got.accepted)
+        caches = [ly["cache"] for ly in self.layers]
+        for i in range(0, len(caches), 128):   # (as many as a call takes)
+            compact(caches[i:i + 128], table_d, at.seq_lens, at.cu_new, got.path, got.accepted)
         accepted, path, following = got.accepted.tolist(), got.path.tolist(), got.next.tolist()
         kept = [n - k + a for n, k, a in zip(lens, new, accepted)]
         self._commit(pages, kept)

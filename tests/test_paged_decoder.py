@@ -453,6 +453,21 @@ def test_the_limit_of_a_model_holds_for_a_trees_levels_not_for_its_tokens(monkey
     assert (dec._free, dec._seqs) == before
 
 
+def test_verification_moves_the_rows_of_however_many_layers(monkeypatch):
+    """compact takes up to 128 caches a call."""
+    from lowbit import paged
+    dec, moved = bookkeeper(), []
+    dec.layers = [{"cache": i} for i in range(300)]
+    dec._layers = lambda x, *args: x
+    vector = lambda *v: torch.tensor(v)
+    monkeypatch.setattr(paged, "plan", lambda *args, **kw: paged.Plan(vector(0, 2), vector(2), vector(0, 1), vector(0, 1), None, None, None))
+    monkeypatch.setattr(paged, "verify", lambda *args, **kw: paged.Verified(vector(2), vector(0, 1)[None], vector(7), vector(3, 7)))
+    monkeypatch.setattr(paged, "compact", lambda caches, *args: (len(caches) <= 128 or pytest.fail("too many")) and moved.extend(caches))
+    sid = dec.open()
+    assert dec.verify({sid: ([1, 3], [-1, 0])}) == {sid: [3, 7]}
+    assert moved == list(range(300)) and dec._seqs[sid]["length"] == 2
+
+
 @pytest.mark.gpu
 def test_a_wide_tree_at_the_models_limit_gives_what_it_gives_below_it():
     from lowbit import paged
