@@ -926,9 +926,10 @@ int lb_paged_compact(const lb_paged_cache* const* caches, int layers, const int3
   if (seqs < 1 || seqs > 65535) return fail(LB_ERR_ARGUMENT, "seqs=%d: 1 to 65535", seqs);
   if (max_path < 1 || max_path > lb::kMaxTree) return fail(LB_ERR_ARGUMENT, "max_path=%lld: 1 to %d", (long long)max_path, lb::kMaxTree);
   if (misaligned({page_table, seq_lens, cu_new, path, accepted, lens_out}, 4)) return fail(LB_ERR_ALIGNMENT, "int32 arrays must be 4-byte aligned");
+  if (table_width < 1 || table_stride < table_width) return fail(LB_ERR_ARGUMENT, "page table: at least one page a row, contexts below 2^31");
   // written by one CTA of a sequence while others read
   for (const auto& in : {std::make_pair(seq_lens, (int64_t)seqs), std::make_pair(cu_new, (int64_t)seqs + 1), std::make_pair(accepted, (int64_t)seqs),
-                         std::make_pair(path, seqs * max_path)})
+                         std::make_pair(path, seqs * max_path), std::make_pair(page_table, (seqs - 1) * table_stride + table_width)})
     if (lens_out < in.first + in.second && in.first < lens_out + seqs) return fail(LB_ERR_ARGUMENT, "lens_out must not lie over an input (seq_lens itself, say)");
   lb::CompactParams p;
   for (int i = 0; i < layers; ++i) {
@@ -948,8 +949,7 @@ int lb_paged_compact(const lb_paged_cache* const* caches, int layers, const int3
   std::sort(all, all + 2 * layers);
   if (std::adjacent_find(all, all + 2 * layers) != all + 2 * layers) return fail(LB_ERR_ARGUMENT, "a cache is given twice");
   const lb_paged_cache* a = caches[0];
-  if (table_width < 1 || table_stride < table_width || table_width * a->page_size > INT32_MAX)
-    return fail(LB_ERR_ARGUMENT, "page table: at least one page a row, contexts below 2^31");
+  if (table_width > INT32_MAX / a->page_size) return fail(LB_ERR_ARGUMENT, "page table: at least one page a row, contexts below 2^31");
   if (a->nkv > 65536) return fail(LB_ERR_ARGUMENT, "nkv=%d: at most 65536", a->nkv);
   int rc = check_device();
   if (rc) return rc;

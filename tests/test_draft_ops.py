@@ -1312,6 +1312,14 @@ def test_abi_refusals_of_what_lies_over_the_inputs_or_is_misaligned():
         assert linear(x, y) == 1 and "overlap" in message(lib), (x, y)
 
 
+def test_compact_refuses_lengths_over_the_page_table():
+    lib = _lib.load_library()
+    cache = _lib.PagedCacheStruct(k=A, v=2 * A, k_page_stride=2048, v_page_stride=2048, num_pages=4, dtype=0, nkv=2, hd=64, page_size=16)
+    ptrs = (ctypes.c_void_p * 1)(ctypes.addressof(cache))
+    for out in (8 * A, 8 * A + 68, 8 * A - 8):   # three rows of four entries, seven apart
+        assert lib.lb_paged_compact(ptrs, 1, 8 * A, 7, 4, A, 2 * A, 3 * A, 4 * A, 3, 4, out, 0, None) == 1 and "over an input" in message(lib), out
+
+
 def test_f8_abi_refusals():
     lib = _lib.load_library()
     quant = lambda w=A, t=0, n=4, k=64, ldw=64, q=A, ldq=64, s=A: lib.lb_f8_quantize_weight(w, t, n, k, ldw, q, ldq, s, None)
