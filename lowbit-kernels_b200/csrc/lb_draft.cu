@@ -1,5 +1,7 @@
 // A step of drafted tokens around the attention: the plan of a call (page tables, slots, positions and tree masks from the
 // request lengths), the acceptance of the drafts, and the move of the accepted tokens' rows in the paged cache.
+#include <atomic>
+
 #include "lb_launch.h"
 #include "lb_tma.cuh"
 #include "lb_types.cuh"
@@ -478,9 +480,17 @@ cudaError_t launch_plan(const PlanParams& p, bool pdl, cudaStream_t st) {
   if (meet) C = work <= 2 * kPlanThreads ? 1 : work <= 8 * kPlanThreads ? 4 : kPlanCluster;
   meet = meet && C > 1;
   const size_t smem = (size_t)(4 * p.seqs + 1 + (p.parents ? kPlanStage + kMaxTree : 0)) * sizeof(int);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
+  if (smem > 48 * 1024) {   // once per device, what the largest call needs: a call's own size would take from another's under way
+    static std::atomic<uint64_t> done{0};
+    constexpr int kMost = (4 * kMaxPlanSeqs + 1 + kPlanStage + kMaxTree) * (int)sizeof(int);
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(done.load(std::memory_order_relaxed) & bit)) {
+      const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+      if (e != cudaSuccess) return e;
+      done.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
   return launch_draft(plan_kernel, dim3(C), threads, smem, meet ? C : 1, pdl, st, p, C, meet);
 }

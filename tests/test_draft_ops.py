@@ -18,6 +18,7 @@ import math
 import pickle
 import random
 import re
+import threading
 
 import pytest
 import torch
@@ -256,6 +257,51 @@ def test_plan_over_its_own_inputs_captured_and_on_another_stream():
         torch.cuda.synchronize()
         want, rows = plain_plan(before[0], before[1], c["new"], 16, c["tokens"], before[2], c["free"], before[3], c["parents"], blank.mask.shape[1])
         check_plan(out, want, table, rows)
+
+
+@gpu
+def test_plans_of_different_sizes_at_once():
+    """From two host threads, of so many sequences that the kernel's shared memory is more than what it has by default: neither call
+    takes from the other what it may use."""
+    _, paged = mods()
+    faults, together = [], threading.Barrier(3)
+
+    def work(seqs):
+        try:
+            table, lens, new = torch.zeros(seqs, 1, dtype=torch.int32, device="cuda"), i32([3] * seqs), i32([1] * seqs)
+            out = paged.plan(table, lens, new, 16, seqs)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                together.wait(60)
+                for _ in range(10000):
+                    paged.plan(table, lens, new, 16, seqs, out=out)
+                torch.cuda.current_stream().synchronize()
+            assert out.cu_new.tolist() == list(range(seqs + 1)) and out.slots.tolist() == [3] * seqs
+        except Exception as e:   # (an assertion in a thread would be lost)
+            faults.append(e)
+
+    threads = [threading.Thread(target=work, args=(seqs,)) for seqs in (8192, 4000, 6000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not faults, faults
+
+
+@gpu
+def test_a_captured_plan_of_many_sequences_after_a_smaller_one():
+    _, paged = mods()
+    made = []
+    for seqs in (8192, 3500):
+        args = torch.zeros(seqs, 1, dtype=torch.int32, device="cuda"), i32([3] * seqs), i32([1] * seqs), 16, seqs
+        out, graph = paged.plan(*args), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            paged.plan(*args, out=out)
+        made.append((seqs, out, graph, args))   # (a graph keeps no inputs alive)
+    for _ in range(3):
+        for seqs, out, graph, _ in made:
+            out.slots.fill_(-9), out.cu_new.fill_(-9)
+            graph.replay()
+            assert out.cu_new.tolist() == list(range(seqs + 1)) and out.slots.tolist() == [3] * seqs
 
 
 @gpu
