@@ -1300,6 +1300,55 @@ def test_a_captured_step_of_drafted_tokens(dtype):
     assert status() == 0
 
 
+@gpu
+def test_a_captured_step_that_runs_out_of_pages_keeps_what_it_refuses():
+    """Plan, acceptance and move as one graph with lengths, pages held and the free count in place: sequences that find no pages, or no rows
+    left, have the context they had, nothing is accepted for them, and they go on once there are pages."""
+    _, paged = mods()
+    rng = random.Random(3)
+    seqs, n, page, width, vocab, rows = 6, 14, 16, 8, 30, 75   # (rows for five sequences and five tokens)
+    cache = paged.PagedCache(64, page, 2, 64)
+    cache.k.normal_(), cache.v.normal_()
+    before, held = [5, 30, 0, 47, 17, 60], [1, 2, 0, 3, 2, 4]
+    order = list(range(64))
+    rng.shuffle(order)
+    table = i32([[order.pop() for _ in range(h)] + [-1] * (width - h) for h in held])
+    free, count, lens, held = i32(order), i32([3]), i32(before), i32(held)
+    new, parents = i32([n] * seqs), i32([p for _ in range(seqs) for p in tree(rng, n)][:rows])
+    logits, tokens = torch.empty(rows, vocab, device="cuda"), torch.empty(rows, dtype=torch.int64, device="cuda")
+    args = dict(held=held, free_pages=free, free_count=count, parents=parents, max_new=n)
+    out = paged.plan(table.clone(), lens, new, page, rows, **args)._replace(held=held, free_count=count)
+
+    def step():
+        p = paged.plan(table, lens, new, page, rows, out=out, **args)
+        v = paged.verify(logits, tokens, parents, p.cu_new, max_new=n, seq_lens=p.seq_lens)
+        paged.compact([cache], table, p.seq_lens, p.cu_new, v.path, v.accepted, out=lens)
+        return v
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        v = step()
+    refused = set()
+    for turn in range(4):
+        if turn == 2:
+            count.fill_(40)   # others have given theirs back
+        logits.normal_(generator=gen(turn))
+        top, shape = logits.argmax(1).tolist(), parents.tolist()
+        tokens.copy_(i64([top[at // n * n + shape[at]] if shape[at] >= 0 and rng.random() < 0.8 else 1 for at in range(rows)]))
+        start, pages, left, was = lens.tolist(), held.tolist(), count.item(), table.tolist()
+        want, _ = plain_plan(was, start, [n] * seqs, page, rows, pages, free.tolist(), left, shape, 1)
+        path = plain_verify(logits, tokens.tolist(), shape, [n] * 5 + [5], n)
+        graph.replay()
+        torch.cuda.synchronize()
+        for s in range(seqs):
+            ok = want["seq_lens"][s] > 0
+            assert v.accepted[s].item() == (path[0][s].item() if ok else 0) and v.next[s].item() == (path[2][s].item() if ok else -1)
+            assert lens[s].item() == start[s] + v.accepted[s].item()
+            refused |= set() if ok else {(turn, s)}
+        assert held.tolist() == want["held"] and count.item() == want["free_count"][0]
+    assert {s for t, s in refused if t < 2} > {5} and {s for t, s in refused if t >= 2} == {5} and status() == 0
+
+
 # ------------------------------------------------------------------------------- refusals of the C ABI (no GPU)
 
 def test_no_warp_of_the_kernels_meets_others_on_the_way():
