@@ -852,6 +852,22 @@ def test_compact_keeps_the_lengths_of_all_sequences_that_the_plan_refused(short)
 
 
 @gpu
+def test_compact_moves_a_path_that_does_not_rise_as_it_stands():
+    """Every entry's row as it was before the call: each lies at or behind its own place, so no row is written before it is read."""
+    _, paged = mods()
+    for path in ([0, 5, 3], [0, 4, 4, 4], [0, 9, 8, 7, 6, 5], [2, 2, 2, 9, 4]):
+        cache = make_caches(gen(len(path)), 1, 4, 2, 16, 64, torch.bfloat16)[0]
+        rows = [t.transpose(1, 2).reshape(64, 2, 64).clone() for t in (cache.k, cache.v)]
+        start = 10   # the rows 10 to 19 of pages 2 and 0
+        at = lambda j: (2, 0)[(start + j) // 16] * 16 + (start + j) % 16
+        want = [r.clone() for r in rows]
+        for w, r in zip(want, rows):
+            w[i64([at(d) for d in range(len(path))])] = r[i64([at(j) for j in path])]
+        paged.compact([cache], i32([[2, 0]]), i32([20]), i32([0, 10]), i32([path]), i32([len(path)]))
+        assert all(torch.equal(t.transpose(1, 2).reshape(64, 2, 64), w) for t, w in zip((cache.k, cache.v), want)) and status() == 0
+
+
+@gpu
 def test_compact_refusals():
     _, paged = mods()
     caches = make_caches(gen(1), 2, 8, 2, 16, 64, torch.float16)
