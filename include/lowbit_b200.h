@@ -385,7 +385,8 @@ LB_API int lb_paged_tree_attention(const void* q, int64_t q_token_stride, int64_
  * parents int32 [tokens] or NULL: the new tokens of a sequence form a tree, parents[t] being the place of the token's parent
  * among them, an earlier one; anything else makes it a root. A token's position is then seq_lens[s] + its depth, and mask
  * uint32 [tokens, words] receives its ancestors and itself, as lb_paged_tree_attention takes them. words <= 32: trees of
- * up to 1024 tokens.
+ * up to 1024 tokens. A tree of up to 32 * words tokens is served, so 32 * words, or a bound that the lengths keep, is the max_new of
+ * the attention and the acceptance after it.
  */
 LB_API int lb_paged_plan(const int32_t* seq_lens, const int32_t* new_lens, int seqs, int32_t* page_table, int64_t table_stride,
                          int64_t table_width, int page_size, int64_t tokens, const int32_t* held, const int32_t* free_pages,

@@ -259,8 +259,12 @@ def plan(page_table, seq_lens, new_lens, page_size, tokens, held=None, free_page
     parents int32 [tokens]: the new tokens of a sequence form a tree, parents[t] being the place among them of the token's
     parent, an earlier one; anything else makes it a root. Positions are then seq_lens + depth, and the plan's mask is what
     `tree_attention` takes, its rows ceil(max_new / 32) words (max_new bounds the new tokens of any sequence, 1024 at most; by default
-    tokens). out: a Plan whose tensors receive the result (fixed addresses for a captured step); its held, free_count
-    and seq_lens may be the ones passed in, nothing else of it may lie over an input."""
+    tokens). A tree is refused by the mask's bits: one of more than max_new tokens that they hold is served, and then `tree_attention` and
+    `verify`, for which max_new has to be the truth, need 32 * mask.shape[1]. Where lengths may pass the bound all three take a multiple of 32.
+
+    out: a Plan whose tensors receive the result (fixed addresses for a captured step); its held, free_count and seq_lens may be the
+    ones passed in, nothing else of it may lie over an input. Without it the tensors of a result may share one allocation: one that is
+    kept or saved keeps all of it, its clone() does not."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc and out is None:
         got = tc.plan(page_table, seq_lens, new_lens, page_size, tokens, held, free_pages, free_count, parents, max_new)
@@ -319,7 +323,7 @@ def verify(logits, tokens, parents, cu_new, max_new=None, max_path=None, seq_len
 
     A sequence that `plan` refused may have rows, and the logits after them come from tokens that saw nothing. With the plan's seq_lens
     (int32 [S]) it gets 0 and -1 too; without them its path and next mean nothing, and the caller looks at the plan's seq_lens before
-    using them."""
+    using them. The four tensors, and the call's scratch memory, may share one allocation."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc:
         got = tc.verify(logits, tokens, parents, cu_new, max_new, max_path, seq_lens)

@@ -260,6 +260,35 @@ def test_plan_over_its_own_inputs_captured_and_on_another_stream():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nh,nkv,hd", [(28, 4, 128), (14, 2, 64), (4, 4, 128)])
+def test_trees_past_max_new_that_the_mask_holds(dtype, nh, nkv, hd):
+    """A plan for 20 tokens serves trees of 21 to 32; with the mask's bits as their bound attention and acceptance take them whole."""
+    _, paged = mods()
+    rng = random.Random(6)
+    new, ctx = [32, 5, 33, 21], [400, 5, 90, 1000]
+    q, cache, table, lens, cu = build(gen(4), new, ctx, nh, nkv, hd, 16, dtype)
+    parents = [p for n in new for p in tree(rng, n)]
+    p = paged.plan(table, lens - i32(new), i32(new), 16, sum(new), parents=i32(parents), max_new=20)
+    assert p.seq_lens.tolist() == [400, 5, 0, 1000] and p.mask.shape[1] == 1
+    y = paged.tree_attention(q, cache, table, p.seq_lens, p.cu_new, p.mask, max_new=32 * p.mask.shape[1])
+    at = p.cu_new.tolist()
+    sees = [see_of(ancestors(parents[a:b]) if c else [0] * (b - a), c, b - a) for a, b, c in zip(at, at[1:], p.seq_lens.tolist())]
+    check_tree(q, cache, table, p.seq_lens.tolist(), new, sees, y, 1 / math.sqrt(hd))
+    x = randn(gen(5), sum(new), 300, dtype=dtype)
+    tokens = i64([x[a + max(0, parents[a + i])].argmax().item() for a, b in zip(at, at[1:]) for i in range(b - a)])
+    got = paged.verify(x, tokens, i32(parents), p.cu_new, max_new=32, seq_lens=p.seq_lens)
+    want = plain_verify(x, tokens.tolist(), parents, new, 32)
+    for s in range(4):
+        if s == 2:
+            assert got.accepted[s] == 0 and got.next[s] == -1
+        else:
+            assert got.accepted[s] == want[0][s] and torch.equal(got.path[s], want[1][s]) and got.next[s] == want[2][s]
+    looked_at = [i for i in range(sum(new)) if i != at[2] + 32]   # (the refused tree's last row is past the bound)
+    assert torch.equal(got.targets[looked_at], want[3][looked_at]) and status() == 0
+
+
+@gpu
 def test_plans_of_different_sizes_at_once():
     """From two host threads, of so many sequences that the kernel's shared memory is more than what it has by default: neither call
     takes from the other what it may use."""
