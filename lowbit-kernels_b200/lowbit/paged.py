@@ -254,7 +254,7 @@ def plan(page_table, seq_lens, new_lens, page_size, tokens, held=None, free_page
     the last first, by the sequences in their order, and written into page_table behind them; the plan's held and free_count say
     what there is then. Without them page_table is complete as it is. A sequence is refused where `tokens`, W or the free pages do not suffice
     (from the first that lacks pages on, all that need some), or where it is a tree of more tokens than its mask has bits: its seq_lens is
-    0, so that attention gives it zeros, its slots are -1, and it takes no pages.
+    0, so that attention gives it zeros (its rows past the attention's max_new are left unwritten), its slots are -1, and it takes no pages.
 
     parents int32 [tokens]: the new tokens of a sequence form a tree, parents[t] being the place among them of the token's
     parent, an earlier one; anything else makes it a root. Positions are then seq_lens + depth, and the plan's mask is what

@@ -273,6 +273,7 @@ def test_trees_past_max_new_that_the_mask_holds(dtype, nh, nkv, hd):
     assert p.seq_lens.tolist() == [400, 5, 0, 1000] and p.mask.shape[1] == 1
     y = paged.tree_attention(q, cache, table, p.seq_lens, p.cu_new, p.mask, max_new=32 * p.mask.shape[1])
     at = p.cu_new.tolist()
+    y[at[2] + 32] = 0   # the refused tree's last row, past the bound, is left unwritten
     sees = [see_of(ancestors(parents[a:b]) if c else [0] * (b - a), c, b - a) for a, b, c in zip(at, at[1:], p.seq_lens.tolist())]
     check_tree(q, cache, table, p.seq_lens.tolist(), new, sees, y, 1 / math.sqrt(hd))
     x = randn(gen(5), sum(new), 300, dtype=dtype)
