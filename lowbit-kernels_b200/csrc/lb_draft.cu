@@ -367,8 +367,9 @@ __global__ void __launch_bounds__(kWalkThreads) walk_kernel(const VerifyParams p
 // Row ctx + path[d] of each layer's K and V moves to ctx + d. A path rises, so a source lies at or behind its destination and
 // behind every destination before it: a thread that takes one 16-byte column of a head through the whole path, eight rows
 // loaded before the first of them is stored, overwrites nothing that is still to be read. A CTA works for one sequence; its
-// first warps look up the rows once. Latency -- lengths and path, table, rows, one after another: 25 tokens in 36 layers 2.6 us,
-// of 64 trees in 28 layers (12.6 MB read and written) 7.2, in a graph.
+// first warps look up the rows once. One sequence is latency -- lengths and path, table, rows, one after another: 25 tokens in 36
+// layers 2.6 us in a graph. A batch is at no bound: 64 trees in 28 layers 7.2 us, where the 12.6 MB read and written need 1.9; its
+// 1792 CTAs each look the same up again for at most seven rows a thread.
 constexpr int kMoveThreads = 128;    // (64 trees in 28 layers: 7.2 us; 256: 8.3, 64: 7.3)
 constexpr int kMoveBatch = 8;
 

@@ -1064,8 +1064,10 @@ cudaError_t cols_t(const CUtensorMap& wmap, const CUtensorMap& qmap, const F8Gem
                    g.splits, pdl, st, wmap, qmap, g);
 }
 
-// One to eight tokens, while their values are few: every CTA quantizes all of them (measured against the two launches: 2048 x
-// 11008 M = 4 9.9 / 13.5 us, 1536 x 4608 M = 8 5.4 / 8.8).
+// One to eight tokens, while their values are few: every CTA quantizes all of them. The bound is the one of the 8-bit integer product,
+// not fitted to this one. One launch / two, us, cold weights: inside it 4 x 2048 x 11008 9.9 / 13.5, 8 x 1536 x 4608 5.4 / 8.8; outside it
+// narrow layers would still gain (4 x 3584 x 4608 6.5 / 11.0, 2 x 8960 x 1536 6.8 / 10.5, 3 x 11008 x 2048 8.8 / 12.6), others would not
+// (8 x 3584 x 3584 10.0 / 10.0, 1 x 18944 x 3584 20.4 / 20.6, 2 x 18944 x 3584 23.6 / 20.8, 4 x 3584 x 18944 25.5 / 19.4).
 bool gemv_takes(int64_t M, int64_t K) { return M <= kGemvRows && M * K <= 12288; }
 
 template <typename T>
