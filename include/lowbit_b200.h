@@ -419,12 +419,13 @@ LB_API int lb_draft_verify_planned(const void* logits, int dtype, int64_t ld, in
                                    int64_t workspace_bytes, lb_stream_t stream);
 
 /*
- * Moves the K and V rows of accepted tokens to where a sequence without the others has them, in `layers` (at most 128) caches of one
- * shape, type and page strides, none given twice: row seq_lens[s] - n + path[s][d] to seq_lens[s] - n + d for d < accepted[s] (n the new tokens, seq_lens
- * with them). A path rises (not checked: an entry that does not is moved as it stands); an entry outside the new tokens or below its place, or a row
- * outside the cache, is left out and sets lb_device_error() to 3. lens_out [seqs], over none of the inputs, receives seq_lens[s] - n + accepted[s]; for a sequence
- * that lb_paged_plan refused (seq_lens[s] is 0, whether rows were left for it or not) or that is empty, and wherever seq_lens[s] < n,
- * it is left as it is (keep) or 0, and nothing moves.
+ * Moves the K and V rows of accepted tokens to where a sequence without the others has them, in `layers` (at most 128)
+ * caches of one shape, type and page strides, none given twice: row seq_lens[s] - n + path[s][d] to seq_lens[s] - n + d for
+ * d < accepted[s] (n the new tokens, seq_lens with them). A path rises (not checked: an entry that does not is moved as it
+ * stands); an entry outside the new tokens or below its place, or a row outside the cache, is left out and sets
+ * lb_device_error() to 3. lens_out [seqs], over none of the inputs, receives seq_lens[s] - n + accepted[s]; for a sequence
+ * that lb_paged_plan refused (seq_lens[s] is 0, whether rows were left for it or not) or that is empty, and wherever
+ * seq_lens[s] < n, it is left as it is (keep) or 0, and nothing moves.
  */
 LB_API int lb_paged_compact(const lb_paged_cache* const* caches, int layers, const int32_t* page_table, int64_t table_stride,
                             int64_t table_width, const int32_t* seq_lens, const int32_t* cu_new, const int32_t* path,

@@ -367,13 +367,14 @@ def verify(logits, tokens, parents, cu_new, max_new=None, max_path=None, seq_len
 
 
 def compact(caches, page_table, seq_lens, cu_new, path, accepted, out=None):
-    """Moves the accepted tokens' K and V rows to where a sequence without the other drafts has them, in all of `caches` (a list of
-    up to 128 PagedCache of one layout, a layer each, none twice): with n new tokens of sequence s and seq_lens[s] tokens, them included, row
-    seq_lens[s] - n + path[s, d] goes to seq_lens[s] - n + d for d < accepted[s] (path int32 [S, D] and accepted int32 [S] as `verify`
-    gives them: a path rises). Returns seq_lens[s] - n + accepted[s], int32 [S] (`out`, when given: over none of the inputs). For a
-    sequence that `plan` refused (its seq_lens is 0, whether it has rows or not), and for an empty one, this is 0, or what `out` held, and
-    nothing moves: with the lengths before the plan as `out` a refused sequence keeps its context. A path's entry outside the new tokens, below its own place, or on a page outside the cache is left
-    out, and the device status becomes 3, as in `attention`; whether it rises is not looked at, an entry that does not is moved as it stands."""
+    """Moves the accepted tokens' K and V rows to where a sequence without the other drafts has them, in all of `caches` (a list
+    of up to 128 PagedCache of one layout, a layer each, none twice): with n new tokens of sequence s and seq_lens[s] tokens, them
+    included, row seq_lens[s] - n + path[s, d] goes to seq_lens[s] - n + d for d < accepted[s] (path int32 [S, D] and accepted
+    int32 [S] as `verify` gives them: a path rises). Returns seq_lens[s] - n + accepted[s], int32 [S] (`out`, when given: over
+    none of the inputs). For a sequence that `plan` refused (its seq_lens is 0, whether it has rows or not), and for an empty one,
+    this is 0, or what `out` held, and nothing moves: with the lengths before the plan as `out` a refused sequence keeps its
+    context. A path's entry outside the new tokens, below its own place, or on a page outside the cache is left out, and the
+    device status becomes 3, as in `attention`; whether it rises is not looked at, an entry that does not is moved as it stands."""
     tc = ops._tc if ops._tc is not None else ops._torchcall()
     if tc:
         got = tc.compact(caches, PagedCache, page_table, seq_lens, cu_new, path, accepted, out)
